@@ -30,7 +30,7 @@ __all__ = [
     "LRU_SERIAL", "ASSIGN_SPREAD", "ASSIGN_AFFINITY", "ATTN_AUTO", "ATTN_VALU", "ATTN_MFMA",
     "ATTN_GROUP", "MISS_DTYPE", "EMPTY", "ARRIVAL_STEADY", "ARRIVAL_BURSTY", "ARRIVAL_POISSON", "ARRIVAL_MMPP",
     "SCHED_FIFO", "SCHED_PINNED", "trace_load", "TOPK_PER_HEAD", "TOPK_LAYER_MAX", "CAP_GROUP",
-    "CAP_PER_MEMBER",
+    "CAP_PER_MEMBER", "Pages", "rope_freqs", "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_BASE", "ROPE_PARTS",
 ]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libferry_amd.so")
@@ -50,6 +50,7 @@ ARRIVAL_STEADY, ARRIVAL_BURSTY, ARRIVAL_POISSON, ARRIVAL_MMPP = 0, 1, 2, 3
 EMPTY = 0xFFFFFFFF  # selection id of an empty position (and its slot)
 SCHED_FIFO, SCHED_PINNED = 0, 1
 TOPK_PER_HEAD, TOPK_LAYER_MAX = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
 ESIZE = {F32: 4, F16: 2, BF16: 2, FP8: 1}
 MISS_DTYPE = np.dtype([("block", "<u4"), ("slot", "<u4"), ("evicted", "<u4"), ("set", "<u4")])
 
@@ -105,6 +106,37 @@ class TraceInfo(C.Structure):
 
 _vp = C.c_void_p
 _i32 = C.c_int32
+_i64x2 = C.c_int64 * 2
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [
+        ("n_layers", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("block_tokens", _i32),
+        ("dtype", _i32), ("n_pages", _i32), ("n_lanes", _i32), ("max_pages", _i32),
+        ("device", _i32), ("pad", _i32), ("pool", _vp), ("scales", _vp), ("table", _vp),
+        ("len", _vp), ("refs", _vp), ("error", _vp), ("work", _vp), ("work_bytes", C.c_uint64),
+    ]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [
+        ("n_tokens", _i32), ("q_heads", _i32), ("x_dtype", _i32), ("q_out_dtype", _i32),
+        ("rot_dim", _i32), ("pairs", _i32), ("factor", C.c_float), ("pad", _i32),
+        ("lane", _vp), ("pos", _vp), ("inv_freq", _vp), ("kv_scale", _vp), ("q", _vp), ("k", _vp),
+        ("v", _vp), ("q_out", _vp), ("q_stride", _i64x2), ("k_stride", _i64x2),
+        ("v_stride", _i64x2), ("q_out_stride", _i64x2),
+    ]
+
+
+class AttendArgs(C.Structure):
+    _fields_ = [
+        ("n_req", _i32), ("n_tokens", _i32), ("n_groups", _i32), ("q_heads", _i32),
+        ("scale", C.c_float), ("pad", _i32), ("lanes", _vp), ("q_start", _vp), ("group_start", _vp),
+        ("shared", _vp), ("q", _vp), ("out", _vp), ("lse", _vp), ("q_stride", _i64x2),
+        ("out_stride", _i64x2), ("work", _vp), ("work_bytes", C.c_uint64),
+    ]
+
+
 _PROTOS = {
     "ferry_last_error": (C.c_char_p, []),
     "ferry_version": (C.c_char_p, []),
@@ -177,6 +209,17 @@ _PROTOS = {
     "ferry_selgen_admit_member": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _i32]),
     "ferry_selgen_step": (C.c_int, [_vp, _i32, _vp]),
     "ferry_ctx_uniform": (C.c_int, [C.c_uint64, _i32, _i32, _i32, _vp]),
+    "ferry_pages_work_bytes": (C.c_int, [C.POINTER(PagesDesc), C.POINTER(C.c_uint64)]),
+    "ferry_pages_reserve": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _i32, _vp]),
+    "ferry_pages_fork": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _vp, _i32, _vp]),
+    "ferry_pages_trim": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _i32, _vp]),
+    "ferry_pages_compact": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp]),
+    "ferry_pages_append": (C.c_int, [C.POINTER(PagesDesc), _i32, C.POINTER(AppendArgs), _vp]),
+    "ferry_pages_attend_work_bytes": (C.c_int, [C.POINTER(PagesDesc), C.POINTER(AttendArgs),
+                                                C.POINTER(C.c_uint64)]),
+    "ferry_pages_attend": (C.c_int, [C.POINTER(PagesDesc), _i32, C.POINTER(AttendArgs), _vp]),
+    "ferry_rope_freqs": (C.c_int, [C.c_int, _i32, C.c_double, C.c_double, C.c_double, C.c_double,
+                                   C.c_double, _vp]),
     "ferry_refgen_selections": (C.c_int, [_i32, _i32, _i32, _i32, C.c_uint64, _vp]),
 }
 for _name, (_res, _args) in _PROTOS.items():
@@ -560,6 +603,210 @@ class Executor:
         if not s:
             return None
         return _gather_d2h(s, 8, slot_ids).view(np.float32).reshape(-1, 2)
+
+
+def rope_freqs(kind, rot_dim, base=10000.0, stretch=1.0, trained_ctx=0.0, slow=1.0, fast=32.0):
+    """Radians per token of the rot_dim / 2 rotary pairs (float64 array), plain or
+    in one of the forms for contexts `stretch` times the trained one."""
+    if not 2 <= rot_dim <= 128:
+        raise ValueError("rot_dim must be even, 2..128")
+    out = np.zeros(rot_dim // 2, np.float64)
+    _check(lib.ferry_rope_freqs(kind, rot_dim, base, stretch, trained_ctx, slow, fast,
+                                out.ctypes.data), "ferry_rope_freqs")
+    return out
+
+
+_X_DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_PAGE_TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16,
+               FP8: torch.float8_e4m3fn}
+
+
+class Pages:
+    """A paged KV cache (ferry_pages_*): whole contexts of lanes in pages of 16
+    tokens, next to the executor's cache of selected blocks.  It is made over the
+    caller's tensors and keeps them:
+
+      pool    [layers, pages, kv heads, 2 (K, V), 16, 128], float32, float16,
+              bfloat16 or float8_e4m3fn (or uint8 with dtype=FP8)
+      scales  [layers, pages, kv heads, 2] float32, fp8 pages only
+      table   [lanes, pages per lane] int32, -1 (EMPTY) where unused
+      length  [lanes] int32, tokens
+      refs    [pages] int32, table entries that name each page; None where the
+              program hands out the pages itself
+
+    Pages.empty() allocates an empty one.  Errors found on the device are kept in
+    `error` (an int32 tensor); check() reads it and raises."""
+
+    def __init__(self, pool, table, length, refs=None, scales=None, dtype=None, error=None):
+        if not isinstance(pool, torch.Tensor) or not pool.is_cuda:
+            raise ValueError("pool: expected a CUDA tensor")
+        if pool.dim() != 6 or tuple(pool.shape[3:]) != (2, 16, 128):
+            raise ValueError("pool: expected [layers, pages, kv heads, 2, 16, 128]")
+        if dtype is None:
+            dtype = {v: k for k, v in _PAGE_TORCH.items()}.get(pool.dtype)
+        if dtype not in _PAGE_TORCH:
+            raise ValueError(f"pool: dtype {pool.dtype} holds no KV element type")
+        L, P, H = pool.shape[:3]
+        if table.dim() != 2 or length.dim() != 1 or length.shape[0] != table.shape[0]:
+            raise ValueError("table and length: expected [lanes, pages per lane] and [lanes]")
+        dev = self.device = pool.device.index
+        ok = (_PAGE_TORCH[dtype], torch.uint8) if dtype == FP8 else (_PAGE_TORCH[dtype],)
+        d = PagesDesc(L, H, 128, 16, dtype, P, table.shape[0], table.shape[1], dev, 0)
+        d.pool = _dev(pool, "pool", 1, ok, dev)
+        d.table = _dev(table, "table", 1, _I32, dev)
+        d.len = _dev(length, "length", 1, _I32, dev)
+        if (scales is None) != (dtype != FP8):
+            raise ValueError("scales go with fp8 pages")
+        if scales is not None:
+            if tuple(scales.shape) != (L, P, H, 2):
+                raise ValueError("scales: expected [layers, pages, kv heads, 2]")
+            d.scales = _dev(scales, "scales", 1, _F32, dev)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=pool.device)
+        d.error = _dev(error, "error", 1, _I32, dev)
+        work = None
+        if refs is not None:
+            if tuple(refs.shape) != (P,):
+                raise ValueError("refs: expected [pages]")
+            d.refs = _dev(refs, "refs", 1, _I32, dev)
+            n = C.c_uint64()
+            _check(lib.ferry_pages_work_bytes(C.byref(d), C.byref(n)), "ferry_pages_work_bytes")
+            work = torch.empty(n.value, dtype=torch.uint8, device=pool.device)
+            d.work, d.work_bytes = work.data_ptr(), n.value
+        self.pool, self.table, self.length, self.refs = pool, table, length, refs
+        self.scales, self.error, self.dtype, self._work = scales, error, dtype, work
+        self.q_dtype = torch.bfloat16 if dtype == FP8 else _PAGE_TORCH[dtype]
+        self._d, self._r = d, C.byref(d)
+
+    @classmethod
+    def empty(cls, n_layers, kv_heads, n_pages, n_lanes, max_pages, dtype=BF16, device=0):
+        dev = torch.device("cuda", device)
+
+        def ints(shape, v):
+            return torch.full(shape, v, dtype=torch.int32, device=dev)
+
+        return cls(torch.empty((n_layers, n_pages, kv_heads, 2, 16, 128), dtype=_PAGE_TORCH[dtype],
+                               device=dev),
+                   ints((n_lanes, max_pages), -1), ints((n_lanes,), 0), refs=ints((n_pages,), 0),
+                   scales=torch.ones((n_layers, n_pages, kv_heads, 2), device=dev)
+                   if dtype == FP8 else None)
+
+    def _s(self, stream):
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return getattr(stream, "cuda_stream", stream)
+
+    def _list(self, t, name, n):
+        return None if t is None else _dev(t, name, n, _I32, self.device)
+
+    def check(self):
+        """Raise the first error the device found since the last check
+        (synchronises)."""
+        code = int(self.error.item())
+        if code:
+            self.error.zero_()
+            raise FerryError(code, "pages (found on the device)")
+
+    # ---- managing pages ---------------------------------------------------------
+    def reserve(self, lanes, tokens, stream=None):
+        """lanes[i] grows by tokens[i]; a shared last page that is begun is copied."""
+        n = lanes.numel()
+        _check(lib.ferry_pages_reserve(self._r, self._list(lanes, "lanes", n),
+                                       self._list(tokens, "tokens", n), n, self._s(stream)),
+               "ferry_pages_reserve")
+
+    def fork(self, src, dst, keep=None, stream=None):
+        """The empty lanes dst[i] share the first keep[i] tokens (all) of src[i]."""
+        n = dst.numel()
+        _check(lib.ferry_pages_fork(self._r, self._list(src, "src", n), self._list(dst, "dst", n),
+                                    self._list(keep, "keep", n), n, self._s(stream)),
+               "ferry_pages_fork")
+
+    def trim(self, lanes, keep=None, stream=None):
+        """lanes[i] keeps its first keep[i] tokens (none: the lane ends)."""
+        n = lanes.numel()
+        _check(lib.ferry_pages_trim(self._r, self._list(lanes, "lanes", n),
+                                    self._list(keep, "keep", n), n, self._s(stream)),
+               "ferry_pages_trim")
+
+    def compact(self, live=None, stream=None):
+        """Pages in use move into the lowest ids; live[0] gets their number."""
+        _check(lib.ferry_pages_compact(self._r, self._list(live, "live", 1), self._s(stream)),
+               "ferry_pages_compact")
+
+    # ---- tokens -----------------------------------------------------------------
+    def _rows(self, t, name, rows, heads, dtypes):
+        """Pointer and (token, head) strides of a [rows, heads, 128] tensor."""
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{name}: expected a CUDA tensor on cuda:{self.device}")
+        if t.dtype not in dtypes:
+            raise ValueError(f"{name}: dtype {t.dtype}, expected {' or '.join(map(str, dtypes))}")
+        if t.dim() != 3 or t.shape[0] != rows or (heads and t.shape[1] != heads) or t.shape[2] != 128:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{rows}, {heads or 'heads'}, 128]")
+        s = t.stride()
+        if s[2] != 1:
+            raise ValueError(f"{name}: a head's 128 values must be contiguous")
+        return t.data_ptr(), _i64x2(s[0], s[1])
+
+    def append(self, layer, lane, pos, k=None, v=None, q=None, q_out=None, inv_freq=None, factor=1.0,
+               pairs=False, kv_scale=None, stream=None):
+        """Rotary positions of q (into q_out) and k, and k and v into the pages:
+        token t is at place pos[t] of lane[t] (int32 tensors).  inv_freq is a
+        float64 tensor of rot_dim / 2 radians per token."""
+        n = pos.numel()
+        x = q if q is not None else k
+        if x is None:
+            raise ValueError("neither q nor k")
+        a = AppendArgs(n_tokens=n, x_dtype=_X_DTYPE.get(x.dtype, -1), rot_dim=2 * inv_freq.numel(),
+                       pairs=int(pairs), factor=factor)
+        a.pos = self._list(pos, "pos", n)
+        a.lane = self._list(lane, "lane", n)
+        a.inv_freq = _dev(inv_freq, "inv_freq", 1, (torch.float64,), self.device)
+        if q is not None:
+            a.q, a.q_stride = self._rows(q, "q", n, 0, _X_DTYPE)
+            a.q_heads = q.shape[1]
+            a.q_out, a.q_out_stride = self._rows(q_out, "q_out", n, a.q_heads, _X_DTYPE)
+            a.q_out_dtype = _X_DTYPE[q_out.dtype]
+        if k is not None or v is not None:
+            H = self._d.kv_heads
+            a.k, a.k_stride = self._rows(k, "k", n, H, (x.dtype,))
+            a.v, a.v_stride = self._rows(v, "v", n, H, (x.dtype,))
+            if self.dtype == FP8:
+                a.kv_scale = _dev(kv_scale, "kv_scale", 2 * H, _F32, self.device)
+        if n == 0 and 0 <= layer < self._d.n_layers:
+            return  # empty tensors have no address
+        _check(lib.ferry_pages_append(self._r, layer, C.byref(a), self._s(stream)),
+               "ferry_pages_append")
+
+    def attend(self, layer, q, out, lanes, q_start=None, group_start=None, shared=None, scale=0.0,
+               lse=None, stream=None):
+        """Attention of the new query rows q [rows, q heads, 128] of lanes (all rows
+        of request r are [q_start[r], q_start[r+1]); None: one row each), into
+        out; requests [group_start[g], group_start[g+1]) share their first
+        shared[g] pages."""
+        n = lanes.numel()
+        a = AttendArgs(n_req=n, n_tokens=q.shape[0], scale=scale)
+        dt = (self.q_dtype,)
+        a.q, a.q_stride = self._rows(q, "q", a.n_tokens, 0, dt)
+        a.q_heads = q.shape[1]
+        a.out, a.out_stride = self._rows(out, "out", a.n_tokens, a.q_heads, dt)
+        a.lanes = self._list(lanes, "lanes", n)
+        a.q_start = self._list(q_start, "q_start", n + 1)
+        if group_start is not None:
+            a.n_groups = group_start.numel() - 1
+            a.group_start = self._list(group_start, "group_start", 1)
+            a.shared = _dev(shared, "shared", a.n_groups, _I32, self.device)
+        if lse is not None:
+            a.lse = _dev(lse, "lse", a.n_tokens * a.q_heads, _F32, self.device)
+        b = C.c_uint64()
+        _check(lib.ferry_pages_attend_work_bytes(self._r, C.byref(a), C.byref(b)),
+               "ferry_pages_attend_work_bytes")
+        work = torch.empty(b.value, dtype=torch.uint8, device=self.pool.device)
+        a.work, a.work_bytes = work.data_ptr(), b.value
+        s = self._s(stream)
+        if stream is not None and s != torch.cuda.current_stream(self.device).cuda_stream:
+            work.record_stream(torch.cuda.ExternalStream(s, device=self.device))
+        _check(lib.ferry_pages_attend(self._r, layer, C.byref(a), s), "ferry_pages_attend")
 
 
 _hip = None

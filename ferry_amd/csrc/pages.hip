@@ -1,0 +1,685 @@
+// pages.hip -- the paged KV cache: managing pages (reserve, fork, trim,
+// compact), rotary positions and the write of new tokens into pages.
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+#include <mutex>
+
+#include "pages.hpp"
+
+using namespace ferry_amd;
+
+namespace ferry_amd {
+
+int page_geometry(const ferry_pages* p, PageView* v) {
+  if (!p) return report(FERRY_EINVAL, "null pages");
+  if (p->dtype < FERRY_F32 || p->dtype > FERRY_FP8_E4M3)
+    return report(FERRY_EINVAL, "unknown dtype");
+  if (p->head_dim != kPageDim || p->block_tokens != kPageTokens)
+    return report(FERRY_EINVAL, "head_dim must be 128 and block_tokens 16");
+  if (p->n_layers < 1 || p->kv_heads < 1 || p->n_pages < 1 || p->n_lanes < 1 || p->max_pages < 1)
+    return report(FERRY_EINVAL, "layers, kv heads, pages, lanes and pages per lane must be positive");
+  if (p->n_lanes > kMaxLanes || p->max_pages > kMaxLanePages)
+    return report(FERRY_EINVAL, "at most 65536 lanes of 2^20 pages");
+  if (p->kv_heads > 4096 || p->n_layers > 65536) return report(FERRY_EINVAL, "at most 4096 kv heads, 65536 layers");
+  const uint32_t es = p->dtype == FERRY_F32 ? 4 : p->dtype == FERRY_FP8_E4M3 ? 1 : 2;
+  *v = PageView{p->n_layers, p->kv_heads, p->n_pages, p->n_lanes, p->max_pages,
+                2u * kPageTokens * kPageDim * es,
+                static_cast<uint8_t*>(p->pool), p->scales, p->table, p->len, p->refs, p->error};
+  return FERRY_OK;
+}
+
+int page_buffers(const ferry_pages* p, bool manage) {
+  if (int rc = check_all({{p->pool, "pool"}, {p->table, "table"}, {p->len, "len"}, {p->error, "error"}},
+                         p->device))
+    return rc;
+  if (reinterpret_cast<uintptr_t>(p->pool) % 16)
+    return report(FERRY_EINVAL, "pool must be 16-byte aligned");
+  if (p->dtype == FERRY_FP8_E4M3) {
+    if (int rc = check_on(p->scales, "scales", p->device)) return rc;
+    if (reinterpret_cast<uintptr_t>(p->scales) % 8)
+      return report(FERRY_EINVAL, "scales must be 8-byte aligned");
+  } else if (p->scales) {
+    return report(FERRY_EINVAL, "scales go with fp8 pages only");
+  }
+  if (manage) {
+    if (int rc = check_all({{p->refs, "refs"}, {p->work, "work"}}, p->device)) return rc;
+    uint64_t need = 0;
+    if (int rc = ferry_pages_work_bytes(p, &need)) return rc;
+    if (p->work_bytes < need) return report(FERRY_EINVAL, "work is smaller than ferry_pages_work_bytes");
+    if (reinterpret_cast<uintptr_t>(p->work) % 16)
+      return report(FERRY_EINVAL, "work must be 16-byte aligned");
+  } else if (p->refs) {
+    if (int rc = check_on(p->refs, "refs", p->device)) return rc;
+  }
+  return FERRY_OK;
+}
+
+int gpu_cus(int device) {
+  static std::mutex mu;
+  static int cus[64] = {};
+  if (device < 0 || device >= 64) return 256;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!cus[device]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1) {
+      (void)hipGetLastError();
+      return 256;
+    }
+    cus[device] = n;
+  }
+  return cus[device];
+}
+
+}  // namespace ferry_amd
+
+namespace {
+
+constexpr int kPlan = 1024;  // threads of the one-workgroup kernels that plan a call
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Scratch of the managing calls: a header, then arrays sized by the cache.
+struct Plan {
+  int ok;         // the call is made
+  uint32_t need;  // pages taken (reserve)
+  uint32_t copies;  // pages copied (reserve) or moved (compact)
+  uint32_t pad;
+};
+struct Work {
+  Plan* plan;
+  uint32_t* free_ids;  // [n_pages] pages taken, in order (reserve); new id of each page (compact)
+  uint32_t* uses;      // [n_pages] listed lanes whose last page this is (reserve)
+  uint32_t* last;      // [n_pages] the last of them
+  uint32_t* base;      // [n_lanes] first of a listed lane's places in free_ids
+  uint32_t* had;       // [n_lanes] its tokens before the call
+  uint32_t* copy_lane;  // [n_lanes] list places whose last page is copied
+  uint32_t* copy_from;  // [n_lanes] ... and that page
+  uint32_t* from;      // [n_pages] pages moved (compact)
+};
+
+uint64_t up16(uint64_t x) { return (x + 15) & ~15ull; }
+
+Work split_work(void* w, int n_pages, int n_lanes) {
+  uint8_t* p = static_cast<uint8_t*>(w);
+  const uint64_t pg = up16((uint64_t)n_pages * 4), ln = up16((uint64_t)n_lanes * 4);
+  Work r;
+  r.plan = reinterpret_cast<Plan*>(p), p += 64;
+  r.free_ids = reinterpret_cast<uint32_t*>(p), p += pg;
+  r.uses = reinterpret_cast<uint32_t*>(p), p += pg;
+  r.last = reinterpret_cast<uint32_t*>(p), p += pg;
+  r.from = r.uses;
+  r.base = reinterpret_cast<uint32_t*>(p), p += ln;
+  r.had = reinterpret_cast<uint32_t*>(p), p += ln;
+  r.copy_lane = reinterpret_cast<uint32_t*>(p), p += ln;
+  r.copy_from = reinterpret_cast<uint32_t*>(p);
+  return r;
+}
+
+uint64_t work_bytes(int n_pages, int n_lanes) {
+  return 64 + 3 * up16((uint64_t)n_pages * 4) + 4 * up16((uint64_t)n_lanes * 4);
+}
+
+__device__ inline int pages_of(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
+
+// Exclusive prefix sum of x over the workgroup; *total gets the sum.
+__device__ inline uint32_t block_scan(uint32_t x, uint32_t* total) {
+  __shared__ uint32_t part[kPlan / 64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  uint32_t s = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t y = __shfl_up(s, d);
+    if (lane >= d) s += y;
+  }
+  if (lane == 63) part[w] = s;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) {
+    if (i < w) before += part[i];
+    all += part[i];
+  }
+  __syncthreads();
+  *total = all;
+  return before + s - x;
+}
+
+// Names each lane of the list in an LDS bitmap (n_lanes bits); false where one
+// is out of range or named twice.  The caller clears the bitmap first.
+__device__ inline bool name_lane(uint32_t* bits, int lane, int n_lanes) {
+  if (lane < 0 || lane >= n_lanes) return false;
+  return !(atomicOr(&bits[lane >> 5], 1u << (lane & 31)) >> (lane & 31) & 1u);
+}
+
+// ---- reserve -------------------------------------------------------------------
+// One workgroup decides the whole call: which last pages are copied, how many
+// pages each listed lane takes, and which (the lowest free ids).
+__global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, const int32_t* __restrict__ lanes,
+                                                        const int32_t* __restrict__ tokens, int n) {
+  __shared__ uint32_t bits[kMaxLanes / 32];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < (v.n_lanes + 31) / 32; i += kPlan) bits[i] = 0;
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan) {
+    const int lane = lanes[i], t = tokens[i];
+    if (!name_lane(bits, lane, v.n_lanes) || t < 0) {
+      atomicMin(&bad, FERRY_EINVAL);
+    } else {
+      const int had = v.len[lane];
+      w.had[i] = had;
+      if (had < 0 || (int64_t)had + t > (int64_t)v.max_pages * kPageTokens) {
+        atomicMin(&bad, FERRY_ECAPACITY);
+      } else if (had % kPageTokens) {
+        const uint32_t page = v.table[(uint64_t)lane * v.max_pages + had / kPageTokens];
+        if (page >= (uint32_t)v.n_pages) {
+          atomicMin(&bad, FERRY_ESTATE);
+        } else {
+          atomicExch(&w.uses[page], 0u);
+          atomicExch(&w.last[page], 0u);
+        }
+      }
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  if (bad) {
+    if (tid == 0) w.plan->ok = 0, set_error(v.error, bad);
+    return;
+  }
+  for (int i = tid; i < n; i += kPlan) {
+    const int had = (int)w.had[i];
+    if (had % kPageTokens) {
+      const uint32_t page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
+      atomicAdd(&w.uses[page], 1u);
+      atomicMax(&w.last[page], (uint32_t)i);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  // what each lane takes, in the order of the list
+  uint64_t need = 0;
+  uint32_t copies = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + tid;
+    uint32_t mine = 0, copy = 0, page = kNone;
+    if (i < n) {
+      const int had = (int)w.had[i];
+      if (had % kPageTokens) {
+        page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
+        const bool keeps = aload(&w.uses[page]) >= v.refs[page] && aload(&w.last[page]) == (uint32_t)i;
+        copy = !keeps;
+      }
+      mine = copy + (uint32_t)(pages_of(had + tokens[i]) - pages_of(had));
+    }
+    uint32_t all, all_copies;
+    const uint32_t at = block_scan(mine, &all), cat = block_scan(copy, &all_copies);
+    if (i < n) {
+      w.base[i] = (uint32_t)(need + at);
+      if (copy) w.copy_lane[copies + cat] = i, w.copy_from[copies + cat] = page;
+    }
+    need += all;
+    copies += all_copies;
+  }
+  // the lowest free ids
+  uint32_t got = 0;
+  for (int64_t p0 = 0; p0 < v.n_pages && got < need && need <= (uint64_t)v.n_pages; p0 += kPlan) {
+    const int64_t p = p0 + tid;
+    const uint32_t free = p < v.n_pages && v.refs[p] == 0;
+    uint32_t all;
+    const uint32_t at = got + block_scan(free, &all);
+    if (free && at < need) w.free_ids[at] = (uint32_t)p;
+    got += all;
+  }
+  if (tid == 0) {
+    w.plan->ok = got >= need;
+    w.plan->need = (uint32_t)need;
+    w.plan->copies = copies;
+    if (got < need) set_error(v.error, FERRY_ECAPACITY);
+  }
+}
+
+// 16-byte words of one page of one layer, all kv heads, by one workgroup.
+__device__ inline void copy_page(const PageView& v, int layer, uint32_t from, uint32_t to) {
+  const uint64_t bytes = (uint64_t)v.H * v.bb;
+  const u32x4* s = reinterpret_cast<const u32x4*>(v.pool + ((uint64_t)layer * v.n_pages + from) * bytes);
+  u32x4* d = reinterpret_cast<u32x4*>(v.pool + ((uint64_t)layer * v.n_pages + to) * bytes);
+  for (uint64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x) d[i] = s[i];
+  if (v.scales) {
+    const float* a = v.scales + ((uint64_t)layer * v.n_pages + from) * v.H * 2;
+    float* b = v.scales + ((uint64_t)layer * v.n_pages + to) * v.H * 2;
+    for (int i = threadIdx.x; i < v.H * 2; i += blockDim.x) b[i] = a[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32_t* __restrict__ lanes,
+                                                 const int32_t* __restrict__ tokens, int n) {
+  if (!w.plan->ok) return;
+  const uint32_t need = w.plan->need, copies = w.plan->copies;
+  const uint32_t step = gridDim.x * blockDim.x, at = blockIdx.x * blockDim.x + threadIdx.x;
+  for (uint32_t i = at; i < (uint32_t)n; i += step)
+    v.len[lanes[i]] = (int)w.had[i] + tokens[i];
+  // taken page r belongs to the last list place whose base is at most r
+  for (uint32_t r = at; r < need; r += step) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (w.base[mid] <= r) lo = mid; else hi = mid - 1;
+    }
+    const int had = (int)w.had[lo];
+    const uint32_t taken = (lo + 1 < n ? w.base[lo + 1] : need) - w.base[lo];
+    const int fresh = pages_of(had + tokens[lo]) - pages_of(had);
+    const bool copy = taken > (uint32_t)fresh;
+    const int col = pages_of(had) - (copy ? 1 : 0) + (int)(r - w.base[lo]);
+    const uint32_t id = w.free_ids[r];
+    v.table[(uint64_t)lanes[lo] * v.max_pages + col] = id;
+    v.refs[id] = 1;
+  }
+  for (uint64_t c = blockIdx.x; c < (uint64_t)copies * v.L; c += gridDim.x) {
+    const uint32_t k = (uint32_t)(c / v.L), from = w.copy_from[k];
+    if (c % v.L == 0 && threadIdx.x == 0) atomicSub(&v.refs[from], 1u);
+    copy_page(v, (int)(c % v.L), from, w.free_ids[w.base[w.copy_lane[k]]]);
+  }
+}
+
+// ---- fork and trim ----------------------------------------------------------------
+// One workgroup checks the list.  Fork (src != NULL): w.had gets the tokens each
+// dst will hold; trim: those each lane keeps, w.base what it held.
+__global__ __launch_bounds__(kPlan) void k_lanes_plan(PageView v, Work w, const int32_t* __restrict__ src,
+                                                      const int32_t* __restrict__ lanes,
+                                                      const int32_t* __restrict__ keep, int n) {
+  __shared__ uint32_t bits[kMaxLanes / 32];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < (v.n_lanes + 31) / 32; i += kPlan) bits[i] = 0;
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan)
+    if (!name_lane(bits, lanes[i], v.n_lanes)) atomicMin(&bad, FERRY_EINVAL);
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan) {
+    const int lane = lanes[i], from = src ? src[i] : lane;
+    bool fine = lane >= 0 && lane < v.n_lanes && from >= 0 && from < v.n_lanes;
+    if (fine) {
+      const int held = v.len[from], kept = keep ? keep[i] : src ? held : 0;
+      if (src) fine = v.len[lane] == 0 && !(bits[from >> 5] >> (from & 31) & 1u);
+      fine = fine && kept >= 0 && kept <= held && held <= v.max_pages * kPageTokens;
+      w.had[i] = kept;
+      w.base[i] = held;
+    }
+    if (!fine) atomicMin(&bad, FERRY_EINVAL);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    w.plan->ok = bad == 0;
+    if (bad) set_error(v.error, bad);
+  }
+}
+
+__global__ __launch_bounds__(256) void k_fork(PageView v, Work w, const int32_t* __restrict__ src,
+                                              const int32_t* __restrict__ dst, int n) {
+  if (!w.plan->ok) return;
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int kept = (int)w.had[i], pages = pages_of(kept);
+    const uint32_t* from = v.table + (uint64_t)src[i] * v.max_pages;
+    uint32_t* to = v.table + (uint64_t)dst[i] * v.max_pages;
+    for (int e = threadIdx.x; e < pages; e += blockDim.x) {
+      const uint32_t id = from[e];
+      to[e] = id;
+      if (id < (uint32_t)v.n_pages) atomicAdd(&v.refs[id], 1u);
+      else set_error(v.error, FERRY_ESTATE);
+    }
+    if (threadIdx.x == 0) v.len[dst[i]] = kept;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_trim(PageView v, Work w, const int32_t* __restrict__ lanes, int n) {
+  if (!w.plan->ok) return;
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int kept = (int)w.had[i], held = (int)w.base[i];
+    uint32_t* row = v.table + (uint64_t)lanes[i] * v.max_pages;
+    for (int e = pages_of(kept) + threadIdx.x; e < pages_of(held); e += blockDim.x) {
+      const uint32_t id = row[e];
+      row[e] = kNone;
+      if (id >= (uint32_t)v.n_pages || atomicSub(&v.refs[id], 1u) == 0) set_error(v.error, FERRY_ESTATE);
+    }
+    if (threadIdx.x == 0) v.len[lanes[i]] = kept;
+  }
+}
+
+// ---- compact ----------------------------------------------------------------------
+// One workgroup pairs the pages in use at or behind `live` with the free ids
+// before it, both in ascending order: the two lists do not meet, so the moves
+// need no order among themselves.  free_ids becomes the new id of every page.
+__global__ __launch_bounds__(kPlan) void k_compact_plan(PageView v, Work w, int32_t* live_out) {
+  const int tid = threadIdx.x;
+  uint32_t live = 0;
+  for (int64_t p0 = 0; p0 < v.n_pages; p0 += kPlan) {
+    const int64_t p = p0 + tid;
+    uint32_t all;
+    (void)block_scan(p < v.n_pages && v.refs[p] != 0, &all);
+    live += all;
+  }
+  uint32_t gaps = 0, moves = 0;
+  for (int64_t p0 = 0; p0 < v.n_pages; p0 += kPlan) {
+    const int64_t p = p0 + tid;
+    const bool used = p < v.n_pages && v.refs[p] != 0;
+    const uint32_t gap = p < live && !used, move = used && p >= live;
+    uint32_t all_gaps, all_moves;
+    const uint32_t g = gaps + block_scan(gap, &all_gaps), m = moves + block_scan(move, &all_moves);
+    if (gap) w.last[g] = (uint32_t)p;
+    if (move) w.from[m] = (uint32_t)p;
+    if (p < v.n_pages) w.free_ids[p] = (uint32_t)p;
+    gaps += all_gaps;
+    moves += all_moves;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (uint32_t m = tid; m < moves; m += kPlan) {
+    const uint32_t from = w.from[m], to = w.last[m];
+    w.free_ids[from] = to;
+    v.refs[to] = v.refs[from];
+    v.refs[from] = 0;
+  }
+  if (tid == 0) {
+    w.plan->copies = moves;
+    if (live_out) *live_out = (int32_t)live;
+  }
+}
+
+__global__ __launch_bounds__(256) void k_compact(PageView v, Work w) {
+  const uint32_t moves = w.plan->copies;
+  if (!moves) return;
+  for (uint64_t c = blockIdx.x; c < (uint64_t)moves * v.L; c += gridDim.x) {
+    const uint32_t m = (uint32_t)(c / v.L);
+    copy_page(v, (int)(c % v.L), w.from[m], w.last[m]);
+  }
+  for (int i = blockIdx.x; i < v.n_lanes; i += gridDim.x) {
+    uint32_t* row = v.table + (uint64_t)i * v.max_pages;
+    const int held = v.len[i];
+    const int pages = held <= 0 ? 0 : min(pages_of(held), v.max_pages);
+    for (int e = threadIdx.x; e < pages; e += blockDim.x) {
+      const uint32_t id = row[e];
+      if (id < (uint32_t)v.n_pages) row[e] = w.free_ids[id];
+      else set_error(v.error, FERRY_ESTATE);
+    }
+  }
+}
+
+// ---- append -------------------------------------------------------------------------
+struct AppendArgs {
+  int n, Hq, rot, pairs;
+  float factor;
+  const int32_t* lane;
+  const int32_t* pos;
+  const double* inv_freq;
+  const float* kv_scale;
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t qs[2], ks[2], vs[2], os[2];
+};
+
+template <int DT>
+__device__ inline float load_elem(const void* p, int64_t i) {
+  if constexpr (DT == FERRY_F32) return static_cast<const float*>(p)[i];
+  else if constexpr (DT == FERRY_F16) return (float)static_cast<const _Float16*>(p)[i];
+  else return bits_f32((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+}
+template <int DT>
+__device__ inline void store_elem(void* p, int64_t i, float x) {
+  if constexpr (DT == FERRY_F32) static_cast<float*>(p)[i] = x;
+  else if constexpr (DT == FERRY_F16) static_cast<_Float16*>(p)[i] = (_Float16)x;
+  else if constexpr (DT == FERRY_BF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(x);
+  else static_cast<uint8_t*>(p)[i] = f32_to_e4m3(x);
+}
+
+// A workgroup per token: the angles once for all heads, then an element per
+// thread at a time.
+template <int XT, int OT, int PT>
+__global__ __launch_bounds__(256) void k_append(PageView v, int layer, AppendArgs a) {
+  __shared__ float cs[64], sn[64];
+  const int t = blockIdx.x, tid = threadIdx.x;
+  const int lane = a.lane ? a.lane[t] : 0;
+  if (a.lane && lane < 0) return;
+  const int pos = a.pos[t];
+  uint32_t page = 0;
+  if (a.k) {
+    int bad = 0;
+    if (lane >= v.n_lanes || pos < 0 || pos >= v.len[lane] || pos / kPageTokens >= v.max_pages) {
+      bad = FERRY_ERANGE;
+    } else {
+      page = v.table[(uint64_t)lane * v.max_pages + pos / kPageTokens];
+      if (page >= (uint32_t)v.n_pages) bad = FERRY_ERANGE;
+      else if (v.refs && v.refs[page] > 1) bad = FERRY_ESTATE;
+    }
+    if (bad) {
+      if (tid == 0) set_error(v.error, bad);
+      return;
+    }
+  } 
+  if (tid < a.rot / 2) {
+    const double turns = (double)pos * a.inv_freq[tid];
+    cs[tid] = (float)cos(turns) * a.factor;
+    sn[tid] = (float)sin(turns) * a.factor;
+  }
+  __syncthreads();
+  auto turned = [&](auto tag, const void* x, int64_t base, int d) -> float {
+    constexpr int DT = decltype(tag)::value;
+    const float self = load_elem<DT>(x, base + d);
+    if (d >= a.rot) return self;
+    const int half = a.rot / 2;
+    const int i = a.pairs ? d / 2 : d % half;
+    const bool second = a.pairs ? d & 1 : d >= half;
+    const int mate = a.pairs ? d ^ 1 : second ? d - half : d + half;
+    const float other = load_elem<DT>(x, base + mate);
+    return second ? self * cs[i] + other * sn[i] : self * cs[i] - other * sn[i];
+  };
+  std::integral_constant<int, XT> xt;
+  if (a.q)
+    for (int e0 = 0; e0 < a.Hq * kPageDim; e0 += 256) {
+      const int e = e0 + tid, h = e / kPageDim, d = e % kPageDim;
+      float y = 0.0f;
+      if (e < a.Hq * kPageDim) y = turned(xt, a.q, t * a.qs[0] + h * a.qs[1], d);
+      __syncthreads();  // q_out may be q: a pair is read before it is written
+      if (e < a.Hq * kPageDim) store_elem<OT>(a.q_out, t * a.os[0] + h * a.os[1] + d, y);
+    }
+  if (!a.k) return;
+  for (int e = tid; e < v.H * kPageDim; e += 256) {
+    const int h = e / kPageDim, d = e % kPageDim;
+    const uint64_t rec = v.record(layer, page, h);
+    float k = turned(xt, a.k, t * a.ks[0] + h * a.ks[1], d);
+    float x = load_elem<XT>(a.v, t * a.vs[0] + h * a.vs[1] + d);
+    if constexpr (PT == FERRY_FP8_E4M3) {
+      const float sk = a.kv_scale[2 * h], sv = a.kv_scale[2 * h + 1];
+      k /= sk, x /= sv;
+      if (d == 0) v.scales[2 * rec] = sk, v.scales[2 * rec + 1] = sv;
+    }
+    uint8_t* to = v.pool + rec * v.bb;
+    store_elem<PT>(to, (pos % kPageTokens) * kPageDim + d, k);
+    store_elem<PT>(to, kPageTokens * kPageDim + (pos % kPageTokens) * kPageDim + d, x);
+  }
+}
+
+template <int XT, int OT>
+void launch_append(const PageView& v, int layer, const AppendArgs& a, int pt, hipStream_t s) {
+  switch (pt) {
+    case FERRY_F32: k_append<XT, OT, FERRY_F32><<<a.n, 256, 0, s>>>(v, layer, a); break;
+    case FERRY_F16: k_append<XT, OT, FERRY_F16><<<a.n, 256, 0, s>>>(v, layer, a); break;
+    case FERRY_BF16: k_append<XT, OT, FERRY_BF16><<<a.n, 256, 0, s>>>(v, layer, a); break;
+    default: k_append<XT, OT, FERRY_FP8_E4M3><<<a.n, 256, 0, s>>>(v, layer, a); break;
+  }
+}
+template <int XT>
+void launch_append(const PageView& v, int layer, const AppendArgs& a, int ot, int pt, hipStream_t s) {
+  if (ot == FERRY_F32) launch_append<XT, FERRY_F32>(v, layer, a, pt, s);
+  else if (ot == FERRY_F16) launch_append<XT, FERRY_F16>(v, layer, a, pt, s);
+  else launch_append<XT, FERRY_BF16>(v, layer, a, pt, s);
+}
+
+// The common start of the managing calls.
+int manage(const ferry_pages* p, int n, PageView* v, Work* w) {
+  if (int rc = page_geometry(p, v)) return rc;
+  if (n < 0 || n > p->n_lanes) return report(FERRY_EINVAL, "n must be in [0, n_lanes]");
+  if (int rc = page_buffers(p, true)) return rc;
+  *w = split_work(p->work, p->n_pages, p->n_lanes);
+  return FERRY_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ferry_pages_work_bytes(const ferry_pages* p, uint64_t* bytes) {
+  return entry([&]() -> int {
+    PageView v;
+    if (int rc = page_geometry(p, &v)) return rc;
+    if (!bytes) return report(FERRY_EINVAL, "null bytes");
+    *bytes = work_bytes(p->n_pages, p->n_lanes);
+    return FERRY_OK;
+  });
+}
+
+int ferry_pages_reserve(const ferry_pages* p, const int32_t* lanes, const int32_t* tokens, int32_t n,
+                        void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    Work w;
+    if (int rc = manage(p, n, &v, &w)) return rc;
+    if (n == 0) return FERRY_OK;
+    if (int rc = check_all({{lanes, "lanes"}, {tokens, "tokens"}}, p->device)) return rc;
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    k_reserve_plan<<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
+    const int64_t most = std::min<int64_t>((int64_t)n * v.L + 64, 8l * gpu_cus(p->device));
+    k_reserve<<<(unsigned)most, 256, 0, s>>>(v, w, lanes, tokens, n);
+    return launched("ferry_pages_reserve");
+  });
+}
+
+int ferry_pages_fork(const ferry_pages* p, const int32_t* src, const int32_t* dst, const int32_t* keep,
+                     int32_t n, void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    Work w;
+    if (int rc = manage(p, n, &v, &w)) return rc;
+    if (n == 0) return FERRY_OK;
+    if (int rc = check_all({{src, "src"}, {dst, "dst"}}, p->device)) return rc;
+    if (keep)
+      if (int rc = check_on(keep, "keep", p->device)) return rc;
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    k_lanes_plan<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
+    k_fork<<<n, 256, 0, s>>>(v, w, src, dst, n);
+    return launched("ferry_pages_fork");
+  });
+}
+
+int ferry_pages_trim(const ferry_pages* p, const int32_t* lanes, const int32_t* keep, int32_t n, void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    Work w;
+    if (int rc = manage(p, n, &v, &w)) return rc;
+    if (n == 0) return FERRY_OK;
+    if (int rc = check_on(lanes, "lanes", p->device)) return rc;
+    if (keep)
+      if (int rc = check_on(keep, "keep", p->device)) return rc;
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    k_lanes_plan<<<1, kPlan, 0, s>>>(v, w, nullptr, lanes, keep, n);
+    k_trim<<<n, 256, 0, s>>>(v, w, lanes, n);
+    return launched("ferry_pages_trim");
+  });
+}
+
+int ferry_pages_compact(const ferry_pages* p, int32_t* live, void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    Work w;
+    if (int rc = manage(p, 0, &v, &w)) return rc;
+    if (live)
+      if (int rc = check_on(live, "live", p->device)) return rc;
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    k_compact_plan<<<1, kPlan, 0, s>>>(v, w, live);
+    k_compact<<<(unsigned)std::min<int64_t>((int64_t)v.n_pages * v.L, 8l * gpu_cus(p->device)), 256, 0, s>>>(v, w);
+    return launched("ferry_pages_compact");
+  });
+}
+
+int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* a, void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    if (int rc = page_geometry(p, &v)) return rc;
+    if (!a) return report(FERRY_EINVAL, "null args");
+    if (layer < 0 || layer >= p->n_layers) return report(FERRY_EINVAL, "layer out of range");
+    if (a->n_tokens < 0) return report(FERRY_EINVAL, "n_tokens must not be negative");
+    if (a->x_dtype < FERRY_F32 || a->x_dtype > FERRY_BF16)
+      return report(FERRY_EINVAL, "x_dtype must be F32, F16 or BF16");
+    if (a->rot_dim < 2 || a->rot_dim > kPageDim || a->rot_dim % 2)
+      return report(FERRY_EINVAL, "rot_dim must be even, 2..128");
+    if (a->n_tokens == 0) return FERRY_OK;
+    if (!a->q && !a->k) return report(FERRY_EINVAL, "neither q nor k");
+    if (!a->k != !a->v) return report(FERRY_EINVAL, "k and v go together");
+    if (a->q && (a->q_out_dtype < FERRY_F32 || a->q_out_dtype > FERRY_BF16))
+      return report(FERRY_EINVAL, "q_out_dtype must be F32, F16 or BF16");
+    if (a->q && (a->q_heads < 1 || a->q_heads > 65536)) return report(FERRY_EINVAL, "q_heads out of range");
+    if (int rc = page_buffers(p, false)) return rc;
+    if (int rc = check_all({{a->pos, "pos"}, {a->inv_freq, "inv_freq"}}, p->device)) return rc;
+    if (a->k || a->lane)
+      if (int rc = check_on(a->lane, "lane", p->device)) return rc;
+    if (a->q)
+      if (int rc = check_all({{a->q, "q"}, {a->q_out, "q_out"}}, p->device)) return rc;
+    if (a->k)
+      if (int rc = check_all({{a->k, "k"}, {a->v, "v"}}, p->device)) return rc;
+    if (a->k && p->dtype == FERRY_FP8_E4M3)
+      if (int rc = check_on(a->kv_scale, "kv_scale", p->device)) return rc;
+    if (a->q && a->q_out == a->q &&
+        (a->q_out_dtype != a->x_dtype || a->q_stride[0] != a->q_out_stride[0] || a->q_stride[1] != a->q_out_stride[1]))
+      return report(FERRY_EINVAL, "q_out is q with another type or other strides");
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    AppendArgs d{a->n_tokens, a->q ? a->q_heads : 0, a->rot_dim, a->pairs != 0, a->factor, a->lane, a->pos,
+                 a->inv_freq, a->kv_scale, a->q, a->k, a->v, a->q_out,
+                 {a->q_stride[0], a->q_stride[1]}, {a->k_stride[0], a->k_stride[1]},
+                 {a->v_stride[0], a->v_stride[1]}, {a->q_out_stride[0], a->q_out_stride[1]}};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int ot = a->q ? a->q_out_dtype : a->x_dtype;
+    if (a->x_dtype == FERRY_F32) launch_append<FERRY_F32>(v, layer, d, ot, p->dtype, s);
+    else if (a->x_dtype == FERRY_F16) launch_append<FERRY_F16>(v, layer, d, ot, p->dtype, s);
+    else launch_append<FERRY_BF16>(v, layer, d, ot, p->dtype, s);
+    return launched("ferry_pages_append");
+  });
+}
+
+int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, double trained_ctx, double slow,
+                     double fast, double* out) {
+  return entry([&]() -> int {
+    if (!out) return report(FERRY_EINVAL, "null out");
+    if (rot_dim < 2 || rot_dim > kPageDim || rot_dim % 2) return report(FERRY_EINVAL, "rot_dim must be even, 2..128");
+    if (kind < FERRY_ROPE_PLAIN || kind > FERRY_ROPE_PARTS) return report(FERRY_EINVAL, "unknown kind");
+    if (!(base > 0.0) || !(stretch > 0.0) || !std::isfinite(base) || !std::isfinite(stretch))
+      return report(FERRY_EINVAL, "base and stretch must be positive");
+    if (kind == FERRY_ROPE_BASE && rot_dim < 4) return report(FERRY_EINVAL, "FERRY_ROPE_BASE needs rot_dim of 4 or more");
+    if (kind == FERRY_ROPE_PARTS && !(trained_ctx > 0.0 && fast > slow))
+      return report(FERRY_EINVAL, "FERRY_ROPE_PARTS needs trained_ctx > 0 and fast > slow");
+    if (kind == FERRY_ROPE_BASE) base *= std::pow(stretch, (double)rot_dim / (rot_dim - 2));
+    for (int i = 0; i < rot_dim / 2; ++i) {
+      const double f = std::pow(base, -2.0 * i / rot_dim);
+      double x = f;
+      if (kind == FERRY_ROPE_LINEAR) x = f / stretch;
+      if (kind == FERRY_ROPE_PARTS) {
+        const double turns = trained_ctx * f / (2.0 * M_PI);
+        const double keep = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
+        x = f * keep + f / stretch * (1.0 - keep);
+      }
+      out[i] = x;
+    }
+    return FERRY_OK;
+  });
+}
+
+}  // extern "C"

@@ -463,6 +463,177 @@ int ferry_owner_export_member(ferry_ctx* ctx, uint32_t lane, void* image, uint64
 int ferry_owner_import_member(ferry_ctx* ctx, uint32_t lane, const void* image, uint64_t image_bytes,
                               void* stream);
 
+/* ---- paged KV cache ----
+ * A cache in HBM of whole contexts: lanes (requests) of tokens in pages of 16,
+ * next to the executor's cache of selected blocks.  One page holds, per layer
+ * and kv head, one block record as the host tier does (K then V, each
+ * [16][128]; fp8 adds two fp32 scales per record), so a finished page's records
+ * are blocks that a tier can hold and ferry_sparse_decode attends to.  A lane's
+ * row of `table` lists its pages in order; `len` its tokens; `refs` how many
+ * table entries name each page (0 = free).  A page in use more than once is
+ * shared: forked lanes share the pages of their common start.
+ *
+ * Every buffer is the caller's, on GPU `device`:
+ *   pool   [n_layers][n_pages][kv_heads] records of block_bytes
+ *   scales [n_layers][n_pages][kv_heads][2] (K, V), fp8 only (else NULL)
+ *   table  [n_lanes][max_pages] page ids; unused entries are FERRY_EMPTY
+ *   len    [n_lanes]
+ *   refs   [n_pages]; NULL where the caller hands out the pages itself (the
+ *          calls below that need it then return FERRY_EINVAL)
+ *   error  [1] first device-side error (FERRY_E*), 0 if none; the calls never
+ *          clear it
+ *   work   ferry_pages_work_bytes() of scratch for the calls that manage pages,
+ *          NULL where none of them is used
+ * An empty cache is a table of FERRY_EMPTY, zero len and refs.  The calls make
+ * that device current and restore the caller's, launch on `stream` (a stream of
+ * `device`) and do not synchronise, allocate or copy to the host, so they can
+ * be captured.  Calls on one cache are ordered by the caller, as on its tensors:
+ * those that change a table, pages or refs run alone.  head_dim is 128,
+ * block_tokens 16, n_lanes at most 65536, max_pages at most 2^20.
+ * The reference has no dense cache; its members' shared and own hot sets
+ * (src/runtime/wla_multigpu.cuh:1871-2016) are the nearest thing. */
+typedef struct ferry_pages {
+  int32_t n_layers, kv_heads, head_dim, block_tokens, dtype;
+  int32_t n_pages, n_lanes, max_pages;
+  int32_t device;
+  int32_t pad;
+  void* pool;
+  float* scales;
+  uint32_t* table;
+  int32_t* len;
+  uint32_t* refs;
+  int32_t* error;
+  void* work;
+  uint64_t work_bytes;
+} ferry_pages;
+int ferry_pages_work_bytes(const ferry_pages* pages, uint64_t* bytes);
+
+/* Managing pages.  lanes, src, dst, tokens and keep are device arrays of n
+ * int32 (n >= 0).  A call is made whole or not at all: a lane that is out of
+ * range or named twice, or counts that do not fit, latch their error
+ * (FERRY_EINVAL, FERRY_ECAPACITY) and change nothing.
+ *
+ * ferry_pages_reserve grows lanes[i] by tokens[i] >= 0 tokens: len grows, pages
+ * are taken for them, and a last page that is begun and shared is copied first
+ * (K, V and scales, all layers), so that what is appended next is the lane's
+ * own.  Pages go out as the lowest free ids, in the order of the list, a lane's
+ * copy before its new pages; of several listed lanes that share a last page
+ * with no others the last one keeps it.  Not enough free pages, or more
+ * than max_pages in a lane: FERRY_ECAPACITY.
+ * ferry_pages_fork makes the empty lanes dst[i] share the first keep[i] tokens
+ * (keep NULL: all) of lanes src[i].  A src may be listed several times; a dst
+ * that holds tokens, or is also a src, is FERRY_EINVAL.
+ * ferry_pages_trim keeps the first keep[i] <= len tokens of lanes[i] (keep
+ * NULL: none, the lane ends) and gives back the pages behind them.
+ * ferry_pages_compact moves the pages in use into ids [0, live), those at and
+ * behind `live` into the free ids before it, both in ascending order, and
+ * renames them in every lane's table; live (device int32, may be NULL) gets
+ * their number. */
+int ferry_pages_reserve(const ferry_pages* pages, const int32_t* lanes, const int32_t* tokens,
+                        int32_t n, void* stream);
+int ferry_pages_fork(const ferry_pages* pages, const int32_t* src, const int32_t* dst,
+                     const int32_t* keep, int32_t n, void* stream);
+int ferry_pages_trim(const ferry_pages* pages, const int32_t* lanes, const int32_t* keep,
+                     int32_t n, void* stream);
+int ferry_pages_compact(const ferry_pages* pages, int32_t* live, void* stream);
+
+/* Rotary positions and the write into the pages, for n_tokens new tokens of any
+ * lanes (one layer): token t is at place pos[t] of lane[t].  The first rot_dim
+ * dims (even, 2..128) of q and k heads turn by pos[t] * inv_freq[i] in pairs
+ * (i, i + rot_dim / 2), or (2i, 2i + 1) with `pairs` != 0, times `factor`:
+ *   x_a' = factor (x_a cos - x_b sin),  x_b' = factor (x_b cos + x_a sin)
+ * (angles in 64 bits, products in 32, one rounding).  Then k and v go to the
+ * lane's page in its element type; fp8 pages hold the E4M3 code of x / scale
+ * with kv_scale [kv_heads][2] (K, V), which is also written beside the record:
+ * all tokens of a page have to come with the same.  q goes to q_out.
+ *   q, k, v [n_tokens][heads][128] of x_dtype (F32, F16 or BF16), q_out of
+ *   q_out_dtype; strides in elements between tokens and between heads
+ *   (the 128 values of a head are contiguous)
+ * q may be NULL (no queries) or k and v may be (then `lane` may be NULL too, and
+ * the cache is not touched); q_out may be q where type and strides are the same.  A
+ * token of lane < 0 is padding: nothing of it is read or written.  A place that
+ * the lane has not reserved (pos >= len, no page) latches FERRY_ERANGE, a page
+ * in use more than once FERRY_ESTATE; such a token is left out whole.  One call
+ * names a (lane, pos) at most once, else any of its tokens' values remain. */
+typedef struct ferry_append {
+  int32_t n_tokens, q_heads, x_dtype, q_out_dtype;
+  int32_t rot_dim, pairs;
+  float factor;
+  int32_t pad;
+  const int32_t* lane;
+  const int32_t* pos;
+  const double* inv_freq; /* [rot_dim / 2], radians per token (device) */
+  const float* kv_scale;
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2]; /* token, head */
+} ferry_append;
+int ferry_pages_append(const ferry_pages* pages, int32_t layer, const ferry_append* args,
+                       void* stream);
+
+/* Frequencies of rotary pairs for inv_freq, w_i = base^(-2i / rot_dim) and
+ * its forms for contexts `stretch` times the trained one (host; out
+ * [rot_dim / 2]):
+ *   FERRY_ROPE_PLAIN   w_i
+ *   FERRY_ROPE_LINEAR  w_i / stretch
+ *   FERRY_ROPE_BASE    base * stretch^(rot_dim / (rot_dim - 2)) for base
+ *   FERRY_ROPE_PARTS   w_i where a pair makes at least `fast` turns over
+ *                      trained_ctx tokens, w_i / stretch where at most `slow`, linear
+ *                      in the turns between them (goes with a `factor` of
+ *                      0.1 ln(stretch) + 1 where the model was trained so) */
+#define FERRY_ROPE_PLAIN 0
+#define FERRY_ROPE_LINEAR 1
+#define FERRY_ROPE_BASE 2
+#define FERRY_ROPE_PARTS 3
+int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, double trained_ctx,
+                     double slow, double fast, double* out);
+
+/* Attention of new query tokens over their lanes' pages (one layer).  Request
+ * r is lane lanes[r] with query rows [q_start[r], q_start[r + 1]) of q (q_start
+ * NULL: one row each), which are the last tokens of the lane: with n of them
+ * row j attends to the lane's first len - n + j + 1 tokens,
+ *   out = softmax(scale q K^T) V,  lse = ln sum exp(scale q K^T).
+ * A row that sees no token gives 0 and -inf; rows behind the last request are
+ * left as they were.  A token that a row does not see has no part in it,
+ * whatever its K and V hold.
+ * Groups: requests [group_start[g], group_start[g + 1]) have the same first
+ * shared[g] pages in their tables (as forked lanes do); those are read through
+ * the first one's table, once for the whole group instead of once per request.
+ * Requests outside every group, and n_groups 0, are attended alone.
+ *   lanes [n_req], q_start [n_req + 1], group_start [n_groups + 1] (ascending),
+ *   shared [n_groups]: int32 on the device.  A lane out of range, or -1, is an
+ *   empty request; one that is not -1, a page id outside the pool (read as page
+ *   0), a len past max_pages * 16 and offsets that do not ascend latch
+ *   FERRY_ERANGE.
+ *   q, out [n_tokens][q_heads][128]: fp32, fp16 and bf16 pages take theirs, fp8 pages
+ *   bf16; strides in elements between tokens and between heads
+ *   lse [n_tokens][q_heads] fp32 or NULL
+ *   work  ferry_pages_attend_work_bytes() of scratch (256-byte aligned), which
+ *   only this call uses until it has run
+ * Scores, softmax and sums are fp32; weights are rounded to the 16-bit type
+ * before they meet V.  Sums run in an order that follows from the batch's
+ * lengths and the GPU's CUs, the same in every call on the same inputs.  scale 0
+ * is 1 / sqrt(128). */
+typedef struct ferry_attend {
+  int32_t n_req, n_tokens, n_groups, q_heads;
+  float scale;
+  int32_t pad;
+  const int32_t* lanes;
+  const int32_t* q_start;
+  const int32_t* group_start;
+  const int32_t* shared;
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_stride[2], out_stride[2]; /* token, head */
+  void* work;
+  uint64_t work_bytes;
+} ferry_attend;
+int ferry_pages_attend_work_bytes(const ferry_pages* pages, const ferry_attend* args,
+                                  uint64_t* bytes);
+int ferry_pages_attend(const ferry_pages* pages, int32_t layer, const ferry_attend* args,
+                       void* stream);
+
 /* ---- bandwidth ceilings ----
  * Plain reads of the bytes the executor's kernels move, timed with HIP events
  * on `stream` over `iters` launches after one warm-up (synchronises):

@@ -1,0 +1,369 @@
+"""Attention over the pages of a paged KV cache on the GPU against softmax
+attention in float64.
+
+Tolerance, for a row with weights p and values v, A = sum p |v|, S = the largest
+sum over dims of |scale q k| of a token: the output's own rounding (half a step
+u of its type); each weight rounded to the 16-bit type (u A); a score's fp32 sum
+of 128 products, moving its weight and the weights' sum (2 x 130 x 2^-24 S A); the
+fp32 exponentials, sums over n tokens and the joins of parts
+((n / 8 + 64) x 2^-24 A)."""
+import numpy as np
+import pytest
+import torch
+
+import ferry_amd as F
+
+pytestmark = pytest.mark.gpu
+
+T, D = 16, 128
+TORCH = {F.F32: torch.float32, F.F16: torch.float16, F.BF16: torch.bfloat16, F.FP8: torch.float8_e4m3fn}
+U = {F.F32: 2.0 ** -24, F.F16: 2.0 ** -11, F.BF16: 2.0 ** -8, F.FP8: 2.0 ** -8}
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+class Case:
+    """A batch: lens[r] tokens in request r's lane, the last new[r] of them its
+    query rows; groups of (members, shared pages) take the requests in order."""
+
+    def __init__(self, dt, Hq, H, lens, new=None, groups=(), layers=1, layer=0, seed=0, q_std=2.0, spare=3):
+        self.dt, self.Hq, self.H, self.layer = dt, Hq, H, layer
+        n = len(lens)
+        self.lens = list(lens)
+        self.new = [1] * n if new is None else list(new)
+        g = self.g = torch.Generator(device="cuda").manual_seed(seed)
+        pages = [-(-x // T) for x in lens]
+        rng = np.random.default_rng(seed)
+        total = sum(pages) + sum(s for _, s in groups) + spare
+        ids = rng.permutation(total).tolist()
+        lanes = rng.permutation(n + 2)[:n]
+        wide = max(pages + [1]) + 2 + max([s for _, s in groups], default=0)
+        table = np.full((n + 2, wide), -1, np.int32)
+        at = 0
+        for m, s in groups:  # a group's table starts with its shared pages
+            common = [ids.pop() for _ in range(s)]
+            for r in range(at, at + m):
+                table[lanes[r], :s] = common
+            at += m
+        for r, x in enumerate(pages):
+            have = int((table[lanes[r]] >= 0).sum())
+            for i in range(have, x):
+                table[lanes[r], i] = ids.pop()
+        length = np.zeros(n + 2, np.int32)
+        length[lanes] = lens
+        shape = (layers, total, H, 2, T, D)
+        x = torch.randn(shape, device="cuda", generator=g)
+        scales = None
+        if dt == F.FP8:
+            x = (x * 96.0).clamp_(-448.0, 448.0)
+            scales = 0.5 / 96.0 * (0.5 + torch.rand(shape[:3] + (2,), device="cuda", generator=g))
+            scales[..., 1] *= 10.0 ** (2.0 * torch.rand(shape[:3], device="cuda", generator=g) - 1.0)
+        else:
+            x *= 0.5
+        self.p = F.Pages(x.to(TORCH[dt]), ints(table), ints(length), scales=scales)
+        self.qt = self.p.q_dtype
+        self.rows = sum(self.new)
+        self.q = (q_std * torch.randn((self.rows, Hq, D), device="cuda", generator=g)).to(self.qt)
+        self.lanes = lanes
+        self.groups = list(groups)
+        self.start = np.concatenate([[0], np.cumsum(self.new)]).astype(np.int32)
+
+    def args(self, decode=None):
+        decode = all(x == 1 for x in self.new) if decode is None else decode
+        a = dict(lanes=ints(self.lanes))
+        if not decode:
+            a["q_start"] = ints(self.start)
+        if self.groups:
+            a["group_start"] = ints(np.concatenate([[0], np.cumsum([m for m, _ in self.groups])]))
+            a["shared"] = ints([s for _, s in self.groups])
+        return a
+
+    def run(self, stream=None, **kw):
+        a = {**self.args(), **kw}
+        out = torch.full_like(self.q, 9.0)
+        lse = torch.full((self.rows, self.Hq), 9.0, device="cuda")
+        self.p.attend(self.layer, self.q, out, lse=lse, stream=stream, **a)
+        torch.cuda.synchronize()
+        self.p.check()
+        return out, lse
+
+    def tokens(self, r, head):
+        """K and V of request r's tokens as float64 [len, 128]."""
+        n = self.lens[r]
+        ids = self.p.table[int(self.lanes[r]), :-(-n // T)].long()
+        raw = self.p.pool.view(torch.uint8)[self.layer][ids, head]
+        x = raw.view(TORCH[self.dt]).double()
+        if self.dt == F.FP8:
+            x = x * self.p.scales[self.layer][ids, head].double().view(-1, 2, 1, 1)
+        return x[:, 0].reshape(-1, D)[:n], x[:, 1].reshape(-1, D)[:n]
+
+    def check(self, out, lse, scale=D ** -0.5):
+        G, u = self.Hq // self.H, U[self.dt]
+        worst = 0.0
+        for r, n in enumerate(self.lens):
+            a, b = self.start[r], self.start[r + 1]
+            for h in range(self.H):
+                k, v = self.tokens(r, h)
+                for row in range(a, b):
+                    see = n - (b - a) + (row - a) + 1
+                    o = out[row, h * G:(h + 1) * G].double()
+                    e = lse[row, h * G:(h + 1) * G].double()
+                    if see <= 0:
+                        assert not torch.any(o) and torch.all(e == -np.inf)
+                        continue
+                    q = self.q[row, h * G:(h + 1) * G].double()
+                    s = scale * (q @ k[:see].t())
+                    want_e = torch.logsumexp(s, 1)
+                    p = torch.exp(s - want_e.unsqueeze(1))
+                    want, A = p @ v[:see], p @ v[:see].abs()
+                    S = (abs(scale) * (q.abs() @ k[:see].abs().t())).max(1, keepdim=True).values
+                    soft = (2 * 130 * S + see / 8 + 64) * 2.0 ** -24
+                    bound = u * want.abs() + A * (u + soft) * (1 + u) + 2.0 ** -25
+                    assert torch.all(torch.isfinite(o))
+                    worst = max(worst, float(((o - want).abs() / bound).max()))
+                    assert torch.all((e - want_e).abs() <= 2 * soft.squeeze(1) + 2.0 ** -23 * want_e.abs())
+        assert worst <= 1.0, worst
+
+
+DTYPES = [F.BF16, F.F16, F.FP8, F.F32]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("Hq,H", [(8, 2), (1, 1), (4, 4), (64, 8), (12, 3), (5, 1), (32, 1), (160, 2)])
+def test_single_tokens(dt, Hq, H):
+    c = Case(dt, Hq, H, [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 129, 400], seed=Hq)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("groups,lens", [
+    ([(5, 3)], [48, 49, 70, 200, 64]),
+    ([(3, 1), (2, 9), (1, 4)], [17, 30, 90, 150, 290, 65]),
+    ([(2, 4)], [70, 65, 9, 100]),            # the others outside every group
+    ([(4, 0), (2, 2)], [7, 20, 33, 64, 32, 40]),  # nothing shared
+    ([(3, 20)], [330, 10, 300]),             # a member that ends inside the shared pages
+    ([(40, 7)], [112 + i for i in range(40)]),
+])
+def test_groups(dt, groups, lens):
+    c = Case(dt, 8, 2, lens, groups=groups, seed=len(lens))
+    out, lse = c.run()
+    c.check(out, lse)
+    if dt == F.F32:
+        return
+    # the same without the groups, within both sides' tolerance
+    alone = c.args()
+    alone.pop("group_start"), alone.pop("shared")
+    a, b = torch.empty_like(c.q), torch.empty_like(lse)
+    c.p.attend(c.layer, c.q, a, lse=b, **alone)
+    c.check(a, b)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("Hq,H", [(8, 2), (3, 3), (16, 1)])
+@pytest.mark.parametrize("new,lens,groups", [
+    ([1, 2, 3, 5], [1, 40, 64, 130], []),
+    ([33, 1, 70], [33, 90, 100], []),
+    ([130], [300], []),
+    ([7, 0, 4, 0], [7, 20, 64, 0], []),          # requests with no new tokens
+    ([2, 5, 1, 30], [130, 131, 129, 170], [(4, 8)]),
+    ([40, 20], [50, 100], [(2, 2)]),             # new tokens inside the shared pages
+    ([64, 64, 9], [128, 192, 80], [(2, 4)]),
+])
+def test_several_tokens(dt, Hq, H, new, lens, groups):
+    c = Case(dt, Hq, H, lens, new=new, groups=groups, seed=sum(new))
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,len_,groups", [(1, 5000, []), (2, 3001, []), (9, 2100, [(9, 128)]), (33, 1500, [(30, 90)])])
+def test_long_contexts(dt, n, len_, groups):
+    c = Case(dt, 8, 2, [len_ + 7 * i for i in range(n)], groups=groups, seed=n)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+def test_many_requests(dt):
+    rng = np.random.default_rng(1)
+    lens = rng.integers(1, 60, 1500)
+    c = Case(dt, 2, 1, lens, groups=[(int(m), 0) for m in [3] * 100] + [(1, 0)] * 7, seed=9)
+    c.check(*c.run())
+
+
+def test_layers_scale_and_strides():
+    c = Case(F.BF16, 6, 3, [20, 77], new=[3, 5], layers=3, layer=2, seed=4)
+    big = torch.zeros((c.rows, 11, D), dtype=c.qt, device="cuda")
+    big[:, 2:8] = c.q
+    out = torch.zeros((6, c.rows + 1, D + 8), dtype=c.qt, device="cuda")[:, 1:, :D].transpose(0, 1)
+    lse = torch.zeros((c.rows, 6), device="cuda")
+    c.p.attend(2, big[:, 2:8], out, scale=0.2, lse=lse, **c.args())
+    torch.cuda.synchronize()
+    c.check(out, lse, scale=0.2)
+    odd = torch.zeros(c.rows * 6 * D + 1, dtype=c.qt, device="cuda")[1:].view(c.rows, 6, D)
+    odd.copy_(c.q)  # not 16-byte aligned
+    odd_out = torch.zeros(c.rows * 6 * D + 1, dtype=c.qt, device="cuda")[1:].view(c.rows, 6, D)
+    c.p.attend(2, odd, odd_out, scale=0.2, lse=lse, **c.args())
+    torch.cuda.synchronize()
+    c.check(odd_out, lse, scale=0.2)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_negative_and_large_scores(dt):
+    c = Case(dt, 4, 2, [40, 100, 1], seed=3, q_std=30.0)
+    c.check(*c.run())
+    c = Case(dt, 4, 2, [40, 100, 1], seed=3, q_std=1.0)
+    c.q = -c.q.abs()
+    c.check(*c.run(scale=-1.0), scale=-1.0)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_no_row_sees(dt, bad):
+    """Behind a lane's end, and in pages no lane has, anything may stand."""
+    c = Case(dt, 8, 2, [1, 17, 30, 47, 64, 130], new=[1, 2, 9, 1, 1, 40], groups=[(2, 0), (2, 1)], seed=2)
+    want = c.run()
+    pool = c.p.pool
+    held = torch.zeros(pool.shape[1], T, dtype=torch.bool, device="cuda")
+    for r, n in enumerate(c.lens):
+        at = torch.arange(n, device="cuda")
+        held[c.p.table[int(c.lanes[r])][at // T].long(), at % T] = True
+    x = torch.full((1,), bad if dt != F.FP8 else float("nan"), device="cuda").to(TORCH[dt])
+    raw, code = pool.view(torch.uint8), x.view(torch.uint8)
+    es = code.numel()
+    raw = raw.view(*pool.shape[:-1], D, es)
+    mask = (~held)[None, :, None, None, :, None, None].expand(raw.shape)
+    raw.copy_(torch.where(mask, code.view(1, 1, 1, 1, 1, 1, es), raw))
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    c.check(*got)
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.F32])
+@pytest.mark.parametrize("new,G", [(4, 1), (9, 4), (70, 4)])
+def test_values_that_later_rows_see(dt, new, G):
+    """A new token's NaN and infinity reach the rows from it on, not those before."""
+    n = 100
+    c = Case(dt, 2 * G, 2, [n, 40], new=[new, 1], seed=new)
+    plain = c.run()[0]
+    at = n - 3  # a token that the last rows see
+    page = int(c.p.table[int(c.lanes[0]), at // T])
+    c.p.pool[0, page, 0, 1, at % T, 5] = float("nan")
+    c.p.pool[0, page, 0, 1, at % T, 77] = float("inf")
+    c.p.pool[0, page, 1, 0, at % T, 3] = float("nan")
+    out = c.run()[0]
+    first = new - 3  # rows from here on see it
+    assert torch.equal(out[:first], plain[:first]) and torch.equal(out[new:], plain[new:])
+    tail = out[first:new]
+    assert torch.all(torch.isnan(tail[:, :G, 5])) and torch.all(tail[:, :G, 77] == float("inf"))
+    assert torch.all(torch.isnan(tail[:, G:]))
+    rest = [d for d in range(D) if d not in (5, 77)]
+    assert torch.equal(tail[:, :G][..., rest], plain[first:new, :G][..., rest])
+
+
+def test_requests_without_a_lane_and_rows_behind_the_last():
+    c = Case(F.BF16, 8, 2, [20, 30, 40, 50], new=[2, 3, 1, 2], seed=8)
+    out, lse = c.run()
+    c.check(out, lse)
+    lanes = np.array(c.lanes).copy()
+    lanes[1] = -1
+    q = torch.cat([c.q, c.q])  # a padded batch
+    got = torch.full_like(q, 3.0)
+    c.p.attend(0, q, got, **{**c.args(), "lanes": ints(lanes)})
+    torch.cuda.synchronize()
+    c.p.check()
+    assert torch.equal(got[:2], out[:2]) and not torch.any(got[2:5]) and torch.equal(got[5:8], out[5:8])
+    assert torch.all(got[8:] == 3.0)
+
+
+def test_what_is_out_of_range_is_reported():
+    c = Case(F.F16, 4, 2, [20, 30], seed=8)
+    for what in ("lane", "page", "length", "offsets"):
+        a, keep = c.args(), None
+        table, length = c.p.table.clone(), c.p.length.clone()
+        if what == "lane":
+            a["lanes"] = ints([int(c.lanes[0]), 99])
+        elif what == "page":
+            c.p.table[int(c.lanes[1]), 0] = 1 << 30
+        elif what == "length":
+            c.p.length[int(c.lanes[1])] = 16 * c.p.table.shape[1] + 5
+            c.p.table[int(c.lanes[1])] = 0
+        else:
+            a["q_start"] = ints([0, 5, 1])
+        out = torch.zeros_like(c.q)
+        c.p.attend(0, c.q, out, **a)
+        with pytest.raises(F.FerryError) as e:
+            c.p.check()
+        assert e.value.code == -3
+        assert torch.all(torch.isfinite(out))
+        c.p.table.copy_(table), c.p.length.copy_(length)
+    c.check(*c.run())
+
+
+def test_a_pool_past_four_gibibytes():
+    H, P = 8, 70000
+    c = Case(F.BF16, 16, H, [70, 33], seed=1)
+    p = F.Pages.empty(1, H, P, 4, 8, F.BF16)
+    n = c.p.pool.shape[1]
+    p.pool[:, P - n:] = c.p.pool
+    p.table[:, :c.p.table.shape[1]] = torch.where(c.p.table >= 0, c.p.table + (P - n), c.p.table)
+    p.length.copy_(c.p.length)
+    want = c.run()
+    c.p = p
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+def test_the_same_bits_in_every_call(dt):
+    """On another stream, captured, and beside another graph of the same cache."""
+    c = Case(dt, 8, 2, [900, 1000, 70, 2000], groups=[(2, 50)], seed=12)
+    want, want_lse = c.run()
+    c.check(want, want_lse)
+    s = torch.cuda.Stream()
+    got, lse = c.run(stream=s)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    d = Case(dt, 8, 2, [100, 33], new=[30, 4], seed=13)
+    other = d.run()[0]
+    a, b = c.args(), d.args()
+    outs = [torch.empty_like(c.q), torch.empty_like(d.q)]
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for g, k, kw, o in zip(graphs, (c, d), (a, b), outs):
+        with torch.cuda.graph(g, stream=s):
+            k.p.attend(0, k.q, o, **kw)
+    t = torch.cuda.Stream()
+    for i in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(t):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], other)
+        c.run()
+
+
+def test_no_rows():
+    c = Case(F.BF16, 8, 2, [20], seed=1)
+    e = c.q[:0]
+    c.p.attend(0, e, e.clone(), ints([]))
+    c.p.attend(0, e, e.clone(), ints(c.lanes), q_start=ints([0, 0]))
+    c.p.check()
+
+
+def test_refusals_on_the_host():
+    c = Case(F.FP8, 8, 2, [20], seed=1)
+    out = torch.empty_like(c.q)
+    with pytest.raises(ValueError, match="dtype"):
+        c.p.attend(0, c.q.float(), out, ints(c.lanes))
+    with pytest.raises(ValueError, match="shape"):
+        c.p.attend(0, c.q, out[:, :4], ints(c.lanes))
+    with pytest.raises(F.FerryError, match="multiple"):
+        c.p.attend(0, c.q[:, :7], out[:, :7], ints(c.lanes))
+    with pytest.raises(F.FerryError, match="one token"):
+        c.p.attend(0, torch.cat([c.q, c.q]), torch.cat([out, out]), ints(c.lanes))
+    with pytest.raises(F.FerryError, match="layer"):
+        c.p.attend(1, c.q, out, ints(c.lanes))
+    with pytest.raises(ValueError, match="shared"):
+        c.p.attend(0, c.q, out, ints(c.lanes), group_start=ints([0, 1]))
