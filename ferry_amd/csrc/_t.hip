@@ -1,0 +1,1210 @@
+// pages_attn.hip -- attention of new query tokens over the pages of their lanes
+// (ferry_pages_attend), with pages that a group of requests shares read once.
+//
+// Rows and segments.  A row is one query token and one query head; the G =
+// q_heads / kv_heads heads of a kv head attend to the same K and V, so the rows of
+// consecutive tokens, [token][G], are consecutive columns of the same products.
+// A segment is a run of rows and the pages they all attend to: the shared pages of
+// a group with the rows of all its members, or the remaining pages of one request
+// with its own rows.  A row's output joins its (at most two) segments.
+//
+// Schedule.  A segment's rows are cut into tiles (16 to 128 rows), its pages into
+// steps of four; a unit of work is one step of one tile of one kv head.  All units
+// of the call, in the order (segment, kv head, tile, step), are cut into equal runs,
+// one per workgroup of a grid that fills the GPU once: ragged lengths balance, and
+// a long axis is split where there are few rows.  Every workgroup finds its run from
+// the lengths by itself (a prefix sum over the segments), so nothing is planned on
+// the host and a captured call follows the lengths of its replay.  A tile that one
+// workgroup finishes alone, of a row with one segment, is written out; otherwise its
+// (max, sum, output) in fp32 go to scratch, and k_attend_join adds them up in order.
+// The result depends on the lengths and on the number of CUs, not on timing.
+//
+// Softmax.  One pass with the running maximum m and sum of each row, in base 2.  m is
+// raised only when a score exceeds it by kRaise, so weights may grow to 2^kRaise
+// (fp16 and bf16 hold them as exactly as those below 1) and the accumulator is rarely
+// rescaled.  Scores, maxima, sums and the accumulator are fp32; weights are rounded
+// to the operand type for the second product (half a step relative, as large as
+// the rounding of the output).
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "attn_common.hpp"
+#include "pages.hpp"
+
+using namespace ferry_amd;
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kStep = 4;           // pages per step
+constexpr int kWide = 128;         // rows of the widest tile
+constexpr float kRaise = 8.0f;     // log2 of the largest weight between raises of the max
+constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
+constexpr int kPad = 132;          // floats per row of the merge buffer
+
+struct AttendArgs {
+  int n_req, n_tokens, n_groups, Hq, G;
+  float scale;
+  const int32_t* lanes;
+  const int32_t* q_start;
+  const int32_t* group_start;
+  const int32_t* shared;
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t qs[2], os[2];
+  int aligned;  // q and out rows are 16-byte aligned
+};
+
+// Where a row's parts of one segment are (per kv head).
+struct Where {
+  int first;  // first workgroup of its tile
+  int count;  // workgroups that share the tile; 1: the row's own place; 0: written out
+  int row;    // row within the tile
+  int has;    // own pages only: bit 0: the row has shared pages too, bit 1: it sees a token
+};
+
+// Scratch.  rows = n_tokens * G.
+struct Scratch {
+  Where* where;    // [2 (shared, own)][H][rows]
+  float* part_ml;  // [2 * grid][tile rows][2]: the first and the last tile of each workgroup
+  float* part_o;   // [2 * grid][tile rows][128]
+  float* row_ml;   // [2][H][rows][2]: whole tiles of rows with two segments
+  float* row_o;    // [2][H][rows][128]
+  int tile_rows;   // rows per part
+};
+
+// ---- element types -------------------------------------------------------------
+template <int DT>
+struct Kv {
+  static constexpr bool F8 = DT == FERRY_FP8_E4M3, F32 = DT == FERRY_F32;
+  static constexpr bool BF = DT == FERRY_BF16 || F8;  // operand type of the products
+  static constexpr int ES = F32 ? 4 : F8 ? 1 : 2;
+  static constexpr int ROW = kPageDim * ES;          // bytes of a token's K or V
+  static constexpr int HALF = kPageTokens * ROW;     // bytes of a record's K
+  static constexpr int NK = ROW / 64;                // 16-byte K words per lane and page
+  static constexpr int VW = 2 * ES;                  // dwords of V per token and lane
+};
+
+template <bool BF>
+__device__ inline uint32_t pack2(float a, float b) {
+  const f32x2 x = {a, b};
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+}
+
+// 4 E4M3 codes -> 4 exact bf16 values
+__device__ inline u32x2 e4m3x4_to_bf16(uint32_t w) {
+  const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+  const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+  return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+template <bool BF>
+__device__ inline f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {  // 16 x 16 x 32
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ inline f32x4 mma16h(u32x2 a, u32x2 b, f32x4 c) {  // 16 x 16 x 16
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a),
+                                                     __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
+                                                 __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ inline f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {  // 32 x 32 x 16
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// The value weights are taken against: m, or 0 while no score was finite.
+__device__ inline float against(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// One V element of a record as fp32 (fp8: the code's value).
+template <int DT>
+__device__ inline float v_elem(const uint8_t* rec, int tok, int d) {
+  const uint8_t* p = rec + Kv<DT>::HALF;
+  const int i = tok * kPageDim + d;
+  if constexpr (DT == FERRY_F32) return reinterpret_cast<const float*>(p)[i];
+  else if constexpr (DT == FERRY_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+  else if constexpr (DT == FERRY_BF16) return bits_f32((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
+  else return bits_f32(e4m3x4_to_bf16(p[i])[0] << 16);
+}
+__device__ inline bool finite(float x) { return (f32_bits(x) & 0x7F800000u) != 0x7F800000u; }
+
+// A dword of two 16-bit operand values (or one fp32) with what is not finite set
+// to zero; *found is set where there was such a value.
+template <int DT>
+__device__ inline uint32_t only_finite(uint32_t w, bool* found) {
+  if constexpr (Kv<DT>::F32) {
+    const bool bad = (w & 0x7F800000u) == 0x7F800000u;
+    *found |= bad;
+    return bad ? 0u : w;
+  } else {
+    constexpr uint32_t e = Kv<DT>::BF ? 0x7F80u : 0x7C00u;
+    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
+    *found |= lo || hi;
+    return w & (lo ? 0xFFFF0000u : ~0u) & (hi ? 0x0000FFFFu : ~0u);
+  }
+}
+
+// ---- segments -------------------------------------------------------------------
+struct Seg {
+  int own;        // 1: one request's own pages, 0: a group's shared pages
+  int row0, rows;  // its rows
+  int tile, tiles;  // rows per tile, tiles
+  int p0, p1;     // pages [p0, p1) of the lane's table
+  int base, len;  // own: the first row's token sees `base` tokens; tokens of the lane
+  int lane;       // whose table is read; -1: no pages
+  int req;        // request, or group
+};
+
+// Rows per tile: what one wavefront's 16- or 32-column products hold where there are
+// few rows (the tile is then bound by its pages' bytes and the wavefronts share out
+// the pages), else the 128 rows of four wavefronts that share pages in LDS.  fp32
+// pages have the 16-row form only.
+template <int DT>
+__device__ inline int tile_rows(int rows) {
+  if (Kv<DT>::F32 || rows <= 16) return 16;
+  return rows <= 32 ? 32 : rows <= 64 ? 64 : kWide;
+}
+
+__device__ inline int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+__device__ inline int pages_of(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
+
+// First row's token of request r (r = n_req: the end), made to stay in the batch.
+__device__ inline int token_of(const AttendArgs& a, int r) {
+  return a.q_start ? clampi(a.q_start[r], 0, a.n_tokens) : r;
+}
+__device__ inline int lane_of(const PageView& v, const AttendArgs& a, int r) {
+  const int lane = a.lanes[r];
+  return lane >= 0 && lane < v.n_lanes ? lane : -1;
+}
+__device__ inline int len_of(const PageView& v, int lane) {
+  return lane < 0 ? 0 : clampi(v.len[lane], 0, v.max_pages * kPageTokens);
+}
+
+// Shared pages of request r: those of the last group that starts at or before it,
+// if that has not ended.
+__device__ inline int shared_of(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int r) {
+  if (a.n_groups == 0 || gs[0] > r) return 0;
+  int lo = 0, hi = a.n_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (gs[mid] <= r) lo = mid; else hi = mid - 1;
+  }
+  return r < gs[lo + 1] ? clampi(gp[lo], 0, v.max_pages) : 0;
+}
+
+// Segment s: groups first, then requests.  gs, gp: the groups' offsets and pages.
+template <int DT>
+__device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int s) {
+  Seg g;
+  if (s < a.n_groups) {
+    const int b = clampi(gs[s], 0, a.n_req), e = clampi(gs[s + 1], b, a.n_req);
+    g.own = 0, g.req = s, g.p0 = 0, g.p1 = clampi(gp[s], 0, v.max_pages);
+    g.lane = -1, g.base = g.len = 0;
+    for (int r = b; r < e && g.lane < 0; ++r) g.lane = lane_of(v, a, r);
+    const int t0 = token_of(a, b), t1 = max(t0, token_of(a, e));
+    g.row0 = t0 * a.G;
+    g.rows = g.p1 > 0 && g.lane >= 0 ? (t1 - t0) * a.G : 0;
+  } else {
+    const int r = s - a.n_groups, t0 = token_of(a, r), t1 = max(t0, token_of(a, r + 1));
+    g.own = 1, g.req = r, g.lane = lane_of(v, a, r), g.len = len_of(v, g.lane);
+    g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G;
+    g.base = g.len - (t1 - t0) + 1;
+    g.p0 = g.lane < 0 ? 0 : shared_of(v, a, gs, gp, r);
+    g.p1 = max(g.p0, pages_of(g.len));
+  }
+  g.tile = tile_rows<DT>(g.rows);
+  g.tiles = (g.rows + g.tile - 1) / g.tile;
+  return g;
+}
+
+// Steps of tile j: up to the last token its last row sees, and at least one, so
+// that every tile has a workgroup that writes its rows.
+__device__ inline int tile_steps(const Seg& g, int j, int G) {
+  int p1 = g.p1;
+  if (g.own) {
+    const int last = clampi(g.base + (min((j + 1) * g.tile, g.rows) - 1) / G, 0, g.len);
+    p1 = min(p1, pages_of(last));
+  }
+  return max(1, (p1 - g.p0 + kStep - 1) / kStep);
+}
+__device__ inline uint64_t seg_steps(const Seg& g, int G) {
+  if (!g.own) return (uint64_t)g.tiles * tile_steps(g, 0, G);
+  uint64_t n = 0;
+  for (int j = 0; j < g.tiles; ++j) n += tile_steps(g, j, G);
+  return n;
+}
+
+// ---- one tile --------------------------------------------------------------------
+// What a tile's products need, the same for all threads.
+struct Tile {
+  const uint32_t* table;  // the lane's pages
+  int row0, rows;  // first row, rows (<= the tile's width)
+  int h;           // kv head
+  int p0, p1;      // pages of this workgroup's steps of it
+  int lim_lo, lim_hi;  // tokens that its least and its most seeing row see
+};
+
+struct Shared {
+  union {
+    float merge[4 * 32 * kPad];  // [wavefront][row][dim]: accumulators of wavefronts that share rows
+    struct {
+      uint8_t k[2][kStep * 4096], v[2][kStep * 4096];  // two steps' tokens, chunks swizzled
+    } kv;
+  };
+  float ml[4][32][2];
+  int lim[kWide];  // tokens that each row sees
+  int lim_lo, lim_hi;
+  int odd[2];      // a step's V holds what is not finite
+  float ks[2][kStep], vs[2][kStep];
+  int gs[kGroupsInLds + 1], gp[kGroupsInLds];
+  uint64_t sums[kThreads / 64];
+  int seg;
+  uint64_t seg_at;
+};
+
+// 8 query values of a row as two 16-bit values per dword.
+__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned) {
+  if (aligned) return *reinterpret_cast<const u32x4*>(p);
+  u32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  return x;
+}
+
+// Element offset of row `row`'s query (or output) in a tensor of strides s.
+__device__ inline int64_t row_at(const AttendArgs& a, const int64_t (&s)[2], int row, int h) {
+  const int t = row / a.G;
+  return t * s[0] + (int64_t)(h * a.G + (row - t * a.G)) * s[1];
+}
+
+__device__ inline uint32_t checked_page(const PageView& v, uint32_t id) {
+  if (id < (uint32_t)v.n_pages) return id;
+  set_error(v.error, FERRY_ERANGE);
+  return 0;
+}
+
+// Adds what V holds that is not finite (left out of the product) to the rows that
+// see it.  w: the 16 tokens' weights [token][32 columns] in LDS; outputs(part) adds
+// part(dim) to each of the lane's outputs.
+template <int DT, class Outputs>
+__device__ inline void add_not_finite(const uint8_t* rec, const float* w, int col, int t0, int lim,
+                                      Outputs&& outputs) {
+  for (int t = 0; t < kPageTokens && t0 + t < lim; ++t) {
+    const float p = w[t * 32 + col];
+    outputs([&](int d) {
+      asm volatile("" ::: "memory");  // one value at a time: this is rare, its registers are not
+      const float x = v_elem<DT>(rec, t, d);
+      return finite(x) ? 0.0f : p * x;
+    });
+  }
+}
+
+// The K and V words of one page that a lane holds for the 16-column products.
+template <int DT>
+struct PageRegs {
+  u32x4 k[Kv<DT>::NK];
+  uint32_t v[4][Kv<DT>::VW];
+  float ks, vs;
+};
+
+template <int DT>
+__device__ inline void load_page(const PageView& v, uint64_t rec, PageRegs<DT>& r) {
+  using K = Kv<DT>;
+  const int l = threadIdx.x & 63, n = l & 15, grp = l >> 4;
+  const uint8_t* kp = v.pool + rec * (2u * K::HALF);
+  const u32x4* k = reinterpret_cast<const u32x4*>(kp + n * K::ROW + grp * 16);
+#pragma unroll
+  for (int w = 0; w < K::NK; ++w) r.k[w] = load_kv<true>(k + 4 * w);
+  const uint8_t* vp = kp + K::HALF + (4 * grp) * K::ROW + n * (8 * K::ES);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (K::F8) {
+      const u32x2 x = load_kv<true>(reinterpret_cast<const u32x2*>(vp + t * K::ROW));
+      r.v[t][0] = x[0], r.v[t][1] = x[1];
+    } else {
+#pragma unroll
+      for (int w = 0; w < K::VW / 4; ++w) {
+        const u32x4 x = load_kv<true>(reinterpret_cast<const u32x4*>(vp + t * K::ROW) + w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.v[t][4 * w + i] = x[i];
+      }
+    }
+  }
+  if constexpr (K::F8) {
+    const float2 s = load_scales(v.scales + 2 * rec);
+    r.ks = s.x, r.vs = s.y;
+  } else {
+    r.ks = r.vs = 1.0f;
+  }
+}
+
+// A tile of few rows.  Columns of 16 x 16 products are rows: a wavefront holds NT
+// tiles of 16, RG wavefronts hold the tile's rows, and the 4 / RG such teams share
+// out the pages, straight from memory into registers, two pages ahead.  Lane l of a
+// wavefront: column n = l % 16, quarter grp = l / 16.
+//   S^T[16 tokens][16 rows] = K Q^T: lane holds tokens 4 grp + i of row n,
+//   O^T[128 dims][16 rows] += V^T P^T: that is just the P^T operand of the next
+//   product, and V^T's is V[4 grp + i][8 n .. 8 n + 7] as loaded, so that the
+//   accumulator holds dims 32 grp + 8 i + nb of row n (o[nb][i]).
+// Bound by the pages' bytes: 64 rows take 384 matrix cycles a page and wavefront,
+// 8 KiB a page, which 256 CUs could read at 50 TB/s.
+template <int DT, int NT, int RG>
+struct Narrow {
+  using K = Kv<DT>;
+  u32x4 q[NT][K::F32 ? 8 : 4];
+  f32x4 o[NT][8];
+  float m[NT], sum[NT];
+  int lim[NT];
+
+  // One page.  MASKED: some row does not see all of its tokens.
+  template <bool MASKED>
+  __device__ __forceinline__ void consume(const PageView& v, const PageRegs<DT>& r, uint64_t rec, int t0,
+                                          int lim_hi, float scale, float* weights) {
+    const int l = threadIdx.x & 63, n = l & 15, grp = l >> 4;
+    bool odd = false;
+    u32x4 k16[4];
+    if constexpr (K::F8) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const u32x2 a = e4m3x4_to_bf16(r.k[w][0]), b = e4m3x4_to_bf16(r.k[w][1]);
+        const u32x2 c = e4m3x4_to_bf16(r.k[w][2]), d = e4m3x4_to_bf16(r.k[w][3]);
+        k16[2 * w] = u32x4{a[0], a[1], b[0], b[1]};
+        k16[2 * w + 1] = u32x4{c[0], c[1], d[0], d[1]};
+      }
+    } else if constexpr (!K::F32) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) k16[w] = r.k[w];
+    }
+    // V rows as operand values: 8 dims of 4 tokens
+    constexpr int VD = K::F32 ? 8 : 4;
+    uint32_t vv[4][VD];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if constexpr (K::F8) {
+        const u32x2 a = e4m3x4_to_bf16(r.v[t][0]), b = e4m3x4_to_bf16(r.v[t][1]);
+        vv[t][0] = a[0], vv[t][1] = a[1], vv[t][2] = b[0], vv[t][3] = b[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < VD; ++i) vv[t][i] = r.v[t][i];
+      }
+    }
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool seen = t0 + 4 * grp + t < lim_hi;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < VD; ++i) vv[t][i] = seen ? only_finite<DT>(vv[t][i], &bad) : 0u;
+        odd |= bad && seen;
+      }
+      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    }
+    u32x2 vop[8];
+    if constexpr (!K::F32) {
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) {
+        const uint32_t sel = (nb & 1) ? 0x07060302u : 0x05040100u;
+        vop[nb] = u32x2{__builtin_amdgcn_perm(vv[1][nb >> 1], vv[0][nb >> 1], sel),
+                        __builtin_amdgcn_perm(vv[3][nb >> 1], vv[2][nb >> 1], sel)};
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (K::F32) {
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f32(r.k[w][e]), bits_f32(q[nt][w][e]), s, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) s = mma16<K::BF>(k16[w], q[nt][w], s);
+      }
+      const float c = K::F8 ? scale * r.ks : scale;
+      float x[4], top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        x[t] = s[t] * c;
+        if (MASKED && t0 + 4 * grp + t >= lim[nt]) x[t] = -INFINITY;
+        top = fmaxf(top, x[t]);
+      }
+      top = max_over_groups(top);
+      const bool raise = top > m[nt] + kRaise;
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+        const float f = raise ? exp2_fast(m[nt] - top) : 1.0f;
+        m[nt] = raise ? top : m[nt];
+        sum[nt] *= f;
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) o[nt][nb] *= f;
+      }
+      const float ref = against(m[nt]);
+      float p[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) p[t] = exp2_fast(x[t] - ref);
+      sum[nt] += (p[0] + p[1]) + (p[2] + p[3]);
+      if constexpr (K::F8) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) p[t] *= r.vs;
+      }
+      if (MASKED && odd)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) weights[(4 * grp + t) * 32 + 16 * nt + n] = p[t];
+      if constexpr (K::F32) {
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[nt][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f32(vv[t][nb]), p[t], o[nt][nb], 0, 0, 0);
+      } else {
+        const u32x2 pop = {pack2<K::BF>(p[0], p[1]), pack2<K::BF>(p[2], p[3])};
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) o[nt][nb] = mma16h<K::BF>(vop[nb], pop, o[nt][nb]);
+      }
+    }
+    if (MASKED && odd) {
+      wave_fence();
+      const uint8_t* at = v.pool + rec * (2u * K::HALF);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        add_not_finite<DT>(at, weights, 16 * nt + n, t0, lim[nt], [&](auto&& part) {
+#pragma unroll
+          for (int nb = 0; nb < 8; ++nb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[nt][nb][i] += part(32 * grp + 8 * i + nb);
+        });
+      wave_fence();
+    }
+  }
+
+  // The tile's steps; then sh.merge and sh.ml hold each wavefront's rows.
+  __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = l & 15, grp = l >> 4, rg = wave % RG, team = wave / RG;
+    const float scale = a.scale * 1.4426950408889634f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = (rg * NT + nt) * 16 + n;
+      lim[nt] = row < t.rows ? sh.lim[row] : 0;
+      m[nt] = -INFINITY, sum[nt] = 0.0f;
+#pragma unroll
+      for (int nb = 0; nb < 8; ++nb) o[nt][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
+#pragma unroll
+      for (int w = 0; w < (K::F32 ? 8 : 4); ++w) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (row < t.rows) {
+          if constexpr (K::F32) {
+            const float* p = static_cast<const float*>(a.q) + at + 4 * (4 * w + grp);
+            if (a.aligned) x = *reinterpret_cast<const u32x4*>(p);
+            else x = u32x4{f32_bits(p[0]), f32_bits(p[1]), f32_bits(p[2]), f32_bits(p[3])};
+          } else {
+            const int d = K::F8 ? 16 * (4 * (w >> 1) + grp) + 8 * (w & 1) : 8 * (4 * w + grp);
+            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned);
+          }
+        }
+        q[nt][w] = x;
+      }
+    }
+    float* weights = sh.merge + wave * 32 * kPad;
+    // page i of this team: [p0, p1) in steps of kStep, RG of them a step
+    const int count = (t.p1 - t.p0 + kStep - 1) / kStep * RG;
+    auto page_no = [&](int i) { return t.p0 + kStep * (i / RG) + team * RG + i % RG; };
+    uint32_t ids = 0;  // lane j: the table's entry for page 64 k + j
+    auto fill_ids = [&](int i0) {
+      const int p = page_no(i0 + l);
+      ids = p < t.p1 && i0 + l < count ? checked_page(v, t.table[p]) : 0u;
+    };
+    auto rec_of = [&](int i) {
+      return v.record(layer, (uint32_t)__builtin_amdgcn_readlane((int)ids, i & 63), t.h);
+    };
+    if (t.p0 < t.p1) {
+      fill_ids(0);
+      PageRegs<DT> r[2];
+      uint64_t rec[2];
+      auto fetch = [&](int i, int b) {  // past the last page its entry is 0: a page that is not used
+        if ((i & 63) == 0 && i) fill_ids(i);
+        rec[b] = rec_of(i);
+        load_page<DT>(v, rec[b], r[b]);
+      };
+      auto use = [&](int i, int b) {
+        const int p = page_no(i), t0 = p * kPageTokens;
+        if (p >= t.p1) return;
+        if (t0 + kPageTokens > t.lim_lo) consume<true>(v, r[b], rec[b], t0, t.lim_hi, scale, weights);
+        else consume<false>(v, r[b], rec[b], t0, t.lim_hi, scale, weights);
+      };
+      fetch(0, 0);
+      for (int i = 0; i < count; i += 2) {
+        fetch(i + 1, 1);
+        use(i, 0);
+        fetch(i + 2, 0);
+        use(i + 1, 1);
+      }
+    }
+    // hand over: [wavefront][row][dim]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sum[nt] = sum_over_groups(sum[nt]);
+      float* to = sh.merge + (wave * 32 + nt * 16 + n) * kPad + 32 * grp;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int nb = 0; nb < 8; nb += 4)
+          *reinterpret_cast<f32x4*>(to + 8 * i + nb) =
+              f32x4{o[nt][nb][i], o[nt][nb + 1][i], o[nt][nb + 2][i], o[nt][nb + 3][i]};
+      if (grp == 0) sh.ml[wave][nt * 16 + n][0] = m[nt], sh.ml[wave][nt * 16 + n][1] = sum[nt];
+    }
+  }
+};
+
+// Writes a row's 8 output dims from d on (x: the sum of weighted values, inv: 1 / sum).
+template <int DT>
+__device__ inline void write_out(const AttendArgs& a, int64_t at, int d, const float (&x)[8], float inv) {
+  if constexpr (DT == FERRY_F32) {
+    float* p = static_cast<float*>(a.out) + at + d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = x[i] * inv;
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2<Kv<DT>::BF>(x[2 * i] * inv, x[2 * i + 1] * inv);
+    uint16_t* p = static_cast<uint16_t*>(a.out) + at + d;
+    if (a.aligned) {
+      *reinterpret_cast<u32x4*>(p) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// Joins the teams of a Narrow tile and writes its rows: to the output where they are
+// finished (`to_o` null), else as a part.
+template <int DT, int NT, int RG>
+__device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Shared& sh, float* to_ml, float* to_o) {
+  constexpr int TEAMS = 4 / RG, ROWS = 16 * NT * RG;
+#pragma unroll
+  for (int r0 = 0; r0 < ROWS; r0 += 16) {
+    const int row = r0 + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    if (row >= t.rows) continue;
+    const int rg = row / (16 * NT), at = row % (16 * NT);
+    float m = -INFINITY, sum = 0.0f, x[8] = {};
+#pragma unroll
+    for (int k = 0; k < TEAMS; ++k) m = fmaxf(m, sh.ml[k * RG + rg][at][0]);
+    const float ref = against(m);
+#pragma unroll
+    for (int k = 0; k < TEAMS; ++k) {
+      const int w = k * RG + rg;
+      const float f = exp2_fast(sh.ml[w][at][0] - ref);
+      sum += f * sh.ml[w][at][1];
+      const float* o = sh.merge + (w * 32 + at) * kPad + d;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += f * o[i];
+    }
+    if (!to_o) {
+      const bool none = sh.lim[row] <= 0;
+      write_out<DT>(a, row_at(a, a.os, t.row0 + row, t.h), d, x, none ? 0.0f : 1.0f / sum);
+      if (a.lse && d == 0) {
+        const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
+        a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        *reinterpret_cast<f32x4*>(to_o + (int64_t)row * kPageDim + d + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+      if (d == 0) to_ml[2 * row] = m, to_ml[2 * row + 1] = sum;
+    }
+  }
+}
+
+// A tile of up to 128 rows: four wavefronts of 32, which share each step's 64 tokens
+// in LDS (16-bit values, two steps: one is used while the next one's loads, begun a
+// step earlier, are on their way through registers).  Columns of 32 x 32 x 16
+// products are rows; lane l: column l % 32, half h = l / 32.
+//   S^T[64 tokens][32 rows]: register i of token tile tt is token 32 tt + 8 (i / 4) +
+//   4 h + i % 4, so registers 8 j .. 8 j + 7 are the P^T operand of the product over
+//   tokens 16 j .. 16 j + 15 in the order (4 h + 0..3, 8 + 4 h + 0..3), and the V^T
+//   operand in that order is two transposing LDS reads.
+// A token's sixteen 16-byte chunks are stored at chunk ^ swizzle(token): the reads of
+// K (one chunk of 32 tokens) and of V (four chunks of 8 tokens) then spread over all
+// banks.
+__device__ inline int swizzle(int tok) { return (tok & 3) << 2 | (tok >> 2 & 3); }
+
+template <int DT>
+struct Wide {
+  using K = Kv<DT>;
+  typedef std::conditional_t<K::F8, u32x2, u32x4> Word;  // 8 values
+  u32x4 q[8];
+  f32x16 o[4];
+  float m, sum;
+  int lim;
+
+  __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = l & 31, h = l >> 5, row = wave * 32 + col;
+    const float scale = a.scale * 1.4426950408889634f;
+    const bool busy = wave * 32 < t.rows;  // the others only help to load
+    lim = row < t.rows ? sh.lim[row] : 0;
+    m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned)
+                          : u32x4{0u, 0u, 0u, 0u};
+    const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
+    uint32_t ids = 0;
+    auto fill_ids = [&](int s) {  // lane j: page 4 s + j
+      const int p = t.p0 + kStep * s + l;
+      ids = p < t.p1 ? checked_page(v, t.table[p]) : 0u;
+    };
+    Word kr[kStep], vr[kStep];
+    float sc[kStep] = {};
+    // thread: token tid / 16 of each page, chunk tid % 16
+    const int tok = tid >> 4, chunk = tid & 15;
+    auto fetch = [&](int s) {
+      if (s && (s & 15) == 0) fill_ids(s);
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        if (t.p0 + kStep * s + i < t.p1) {
+          const uint64_t rec =
+              v.record(layer, (uint32_t)__builtin_amdgcn_readlane((int)ids, (kStep * s + i) & 63), t.h);
+          const Word* p = reinterpret_cast<const Word*>(v.pool + rec * (2u * K::HALF)) + tid;
+          kr[i] = p[0];
+          vr[i] = p[K::HALF / sizeof(Word)];
+          if constexpr (K::F8)
+            if (tid < 2) sc[i] = v.scales[2 * rec + tid];
+        }
+      }
+    };
+    auto widen = [&](const Word& w) -> u32x4 {
+      if constexpr (K::F8) {
+        const u32x2 x = e4m3x4_to_bf16(w[0]), y = e4m3x4_to_bf16(w[1]);
+        return u32x4{x[0], x[1], y[0], y[1]};
+      } else {
+        return w;
+      }
+    };
+    auto store = [&](int s, int b) {
+      const int t0 = (t.p0 + kStep * s) * kPageTokens;
+      const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const int at_ = ((kPageTokens * i + tok) << 8) + ((chunk ^ swizzle(tok)) << 4);
+        u32x4 x = widen(vr[i]);
+        if (masked) {
+          const bool seen = t0 + kPageTokens * i + tok < t.lim_hi && t.p0 + kStep * s + i < t.p1;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            bool f = false;
+            x[w] = seen ? only_finite<DT>(x[w], &f) : 0u;
+            bad |= f && seen;
+          }
+        }
+        *reinterpret_cast<u32x4*>(sh.kv.k[b] + at_) = widen(kr[i]);
+        *reinterpret_cast<u32x4*>(sh.kv.v[b] + at_) = x;
+        if constexpr (K::F8) {
+          if (tid == 0) sh.ks[b][i] = sc[i];
+          if (tid == 1) sh.vs[b][i] = sc[i];
+        }
+      }
+      if (bad) sh.odd[b] = 1;
+    };
+    if (tid < 2) sh.odd[tid] = 0;
+    fill_ids(0);
+    fetch(0);
+    __syncthreads();
+    store(0, 0);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+      const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
+      if (s + 1 < steps) fetch(s + 1);
+      const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
+      const bool odd = masked && sh.odd[b];
+      uint32_t pop[16];
+      if (busy) {
+        f32x16 x[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[tt][i] = 0.0f;
+          const uint8_t* kp = sh.kv.k[b] + ((32 * tt + col) << 8);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            x[tt] = mma32<K::BF>(*reinterpret_cast<const u32x4*>(kp + (((2 * c + h) ^ swizzle(col)) << 4)), q[c], x[tt]);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float c = K::F8 ? scale * sh.ks[b][2 * tt + (i >> 3)] : scale;
+            x[tt][i] *= c;
+            if (masked && t0 + 32 * tt + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) x[tt][i] = -INFINITY;
+            top = fmaxf(top, x[tt][i]);
+          }
+        {
+          const mx_u32x2 two = pair_values<32>(top);
+          top = fmaxf(bits_f32(two[0]), bits_f32(two[1]));
+        }
+        const bool raise = top > m + kRaise;
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+          const float f = raise ? exp2_fast(m - top) : 1.0f;
+          m = raise ? top : m;
+          sum *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] *= f;
+        }
+        const float ref = against(m);
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float p0 = exp2_fast(x[tt][i] - ref), p1 = exp2_fast(x[tt][i + 1] - ref);
+            sum += p0 + p1;
+            if constexpr (K::F8) {
+              const float f = sh.vs[b][2 * tt + (i >> 3)];
+              p0 *= f, p1 *= f;
+            }
+            pop[8 * tt + i / 2] = pack2<K::BF>(p0, p1);
+          }
+        // lane's addresses for the transposing reads: token row (l % 16) / 4, dims 4 (l % 4)
+        const int rt = 4 * h + (l >> 2 & 3), rd = 16 * (l >> 4 & 1) + 4 * (l & 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 pj = {pop[4 * j], pop[4 * j + 1], pop[4 * j + 2], pop[4 * j + 3]};
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            auto part = [&](int tok_) {
+              const int d = 32 * dt + rd;
+              uint8_t* p = sh.kv.v[b] + (tok_ << 8) + (((d >> 3) ^ swizzle(tok_)) << 4) + (d & 4) * 2;
+              return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) i16x4*)p));
+            };
+            const u32x2 lo = part(16 * j + rt), hi = part(16 * j + 8 + rt);
+            o[dt] = mma32<K::BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pj, o[dt]);
+          }
+        }
+      }
+      if (odd) {  // the same for all wavefronts
+        __syncthreads();  // every wavefront is done with this step's K: its room holds the weights
+        float* w = reinterpret_cast<float*>(sh.kv.k[b]) + wave * 1024;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // 32 tokens of 32 rows at a time
+          if (busy)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t two = pop[8 * half + i / 2];
+              float x;
+              if constexpr (K::BF) x = bits_f32(i & 1 ? two & 0xFFFF0000u : two << 16);
+              else x = (float)__builtin_bit_cast(f16x2, two)[i & 1];
+              w[(8 * (i >> 2) + 4 * h + (i & 3)) * 32 + col] = x;
+            }
+          wave_fence();
+          if (busy)
+            for (int i = 0; i < 2; ++i) {
+              const int p = t.p0 + kStep * s + 2 * half + i;
+              if (p >= t.p1) break;
+              const uint64_t rec = v.record(layer, checked_page(v, t.table[p]), t.h);
+              add_not_finite<DT>(v.pool + rec * (2u * K::HALF), w + 512 * i, col, p * kPageTokens, lim,
+                                 [&](auto&& part) {
+#pragma unroll
+                                   for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                                     for (int e = 0; e < 16; ++e)
+                                       o[dt][e] += part(32 * dt + 8 * (e >> 2) + 4 * h + (e & 3));
+                                 });
+            }
+          wave_fence();
+        }
+        __syncthreads();
+        if (tid == 0) sh.odd[b] = 0;
+      }
+      if (s + 1 < steps) store(s + 1, b ^ 1);
+      __syncthreads();
+    }
+    {
+      const mx_u32x2 two = pair_values<32>(sum);
+      sum = bits_f32(two[0]) + bits_f32(two[1]);
+    }
+  }
+
+  __device__ inline void write(const AttendArgs& a, const Tile& t, float* to_ml, float* to_o) {
+    const int l = threadIdx.x & 63, h = l >> 5, row = (threadIdx.x >> 6) * 32 + (l & 31);
+    if (row >= t.rows) return;
+    if (to_o) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f32x4*>(to_o + (int64_t)row * kPageDim + 32 * dt + 2 * e + 4 * h) =
+              f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
+      if (h == 0) to_ml[2 * row] = m, to_ml[2 * row + 1] = sum;
+      return;
+    }
+    const float inv = lim <= 0 ? 0.0f : 1.0f / sum;
+    uint16_t* p = static_cast<uint16_t*>(a.out) + row_at(a, a.os, t.row0 + row, t.h) + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const u32x2 w = {pack2<K::BF>(o[dt][e] * inv, o[dt][e + 1] * inv),
+                         pack2<K::BF>(o[dt][e + 2] * inv, o[dt][e + 3] * inv)};
+        uint16_t* to = p + 32 * dt + 2 * e;
+        if (a.aligned) {
+          *reinterpret_cast<u32x2*>(to) = w;
+        } else {
+          to[0] = (uint16_t)w[0], to[1] = (uint16_t)(w[0] >> 16), to[2] = (uint16_t)w[1], to[3] = (uint16_t)(w[1] >> 16);
+        }
+      }
+    if (a.lse && h == 0) {
+      const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
+      a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+    }
+  }
+};
+
+// ---- the call -------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, grid = gridDim.x;
+  // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
+  // that tiles of the same pages meet in its L2
+  const int wg = grid % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (grid / 8) + (int)blockIdx.x / 8;
+  const int nseg = a.n_groups + a.n_req;
+  const int *gs = a.group_start, *gp = a.shared;
+  if (a.n_groups && a.n_groups <= kGroupsInLds) {
+    for (int i = tid; i <= a.n_groups; i += kThreads) {
+      sh.gs[i] = a.group_start[i];
+      if (i < a.n_groups) sh.gp[i] = a.shared[i];
+    }
+    gs = sh.gs, gp = sh.gp;
+    __syncthreads();
+  }
+  // units of this thread's segments, and their sum over all threads before it
+  const int per_thread = (nseg + kThreads - 1) / kThreads, s0 = min(tid * per_thread, nseg),
+            s1 = min(s0 + per_thread, nseg);
+  uint64_t mine = 0;
+  for (int s = s0; s < s1; ++s) {
+    const Seg g = segment<DT>(v, a, gs, gp, s);
+    mine += seg_steps(g, a.G) * v.H;
+    if (wg == 0) {  // what is out of range, once
+      bool bad = false;
+      if (g.own) {
+        const int lane = a.lanes[g.req];
+        bad = lane < -1 || lane >= v.n_lanes || (g.lane >= 0 && v.len[g.lane] != g.len);
+        if (a.q_start)
+          bad |= a.q_start[g.req] < 0 || a.q_start[g.req] > a.q_start[g.req + 1] || a.q_start[g.req + 1] > a.n_tokens;
+      } else {
+        bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
+      }
+      if (bad) set_error(v.error, FERRY_ERANGE);
+    }
+  }
+  uint64_t before = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t y = __shfl_up(before, d);
+    if ((tid & 63) >= d) before += y;
+  }
+  if ((tid & 63) == 63) sh.sums[tid >> 6] = before;
+  __syncthreads();
+  uint64_t total = 0;
+  for (int i = 0; i < kThreads / 64; ++i) {
+    if (i < tid >> 6) before += sh.sums[i];
+    total += sh.sums[i];
+  }
+  before -= mine;
+  const uint64_t per = (total + grid - 1) / grid;
+  const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
+  if (u0 >= u1) return;
+  if (u0 >= before && u0 < before + mine) {  // one thread
+    uint64_t at = before;
+    int s = s0;
+    for (;; ++s) {
+      const uint64_t n = seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+      if (u0 < at + n) break;
+      at += n;
+    }
+    sh.seg = s, sh.seg_at = at;
+  }
+  __syncthreads();
+
+  int s = sh.seg;
+  uint64_t u = u0, at = sh.seg_at;
+  while (u < u1) {
+    Seg g = segment<DT>(v, a, gs, gp, s);
+    uint64_t steps = seg_steps(g, a.G);
+    while (u >= at + steps * v.H) {  // the next segment with rows
+      at += steps * v.H;
+      g = segment<DT>(v, a, gs, gp, ++s);
+      steps = seg_steps(g, a.G);
+    }
+    int h = (int)((u - at) / steps);
+    uint64_t tile_at = at + h * steps;  // unit of the tile's first step
+    int j = 0, len = 0;
+    for (;; ++j) {
+      len = tile_steps(g, j, a.G);
+      if (u < tile_at + len) break;
+      tile_at += len;
+    }
+    const int k0 = (int)(u - tile_at), k1 = (int)min((uint64_t)len, (uint64_t)k0 + (u1 - u));
+    Tile t;
+    t.row0 = g.row0 + j * g.tile, t.rows = min(g.tile, g.rows - j * g.tile), t.h = h;
+    t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
+    if (t.p1 < t.p0) t.p1 = t.p0;
+    t.table = v.table + (uint64_t)(g.lane < 0 ? 0 : g.lane) * v.max_pages;
+    __syncthreads();  // the last tile's rows are written
+    if (tid == 0) sh.lim_lo = 0x7FFFFFFF, sh.lim_hi = 0;
+    __syncthreads();
+    const int first = (int)(tile_at / per);
+    const int count = (int)((tile_at + len - 1) / per) - first + 1;
+    const bool two = g.own ? a.n_groups && g.p0 > 0 : true;
+    if (tid < t.rows) {
+      const int row = t.row0 + tid, tok = row / a.G;
+      int lim;
+      if (g.own) {
+        lim = clampi(g.base + (tok - g.row0 / a.G), 0, g.len);
+      } else {
+        int lo = tok, len_;
+        if (a.q_start) {  // the request of this token
+          lo = clampi(gs[g.req], 0, a.n_req);
+          int hi = clampi(gs[g.req + 1], lo, a.n_req) - 1;
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (token_of(a, mid) <= tok) lo = mid; else hi = mid - 1;
+          }
+        }
+        len_ = len_of(v, lane_of(v, a, lo));
+        lim = min(clampi(len_ - token_of(a, lo + 1) + tok + 1, 0, len_), g.p1 * kPageTokens);
+      }
+      sh.lim[tid] = lim;
+      atomicMin(&sh.lim_lo, lim);
+      atomicMax(&sh.lim_hi, lim);
+      if (k0 == 0)
+        ws.where[((uint64_t)g.own * v.H + h) * a.n_tokens * a.G + row] =
+            Where{first, !two && count == 1 ? 0 : count, tid, (two ? 1 : 0) | (lim > 0 ? 2 : 0)};
+    }
+    __syncthreads();
+    t.lim_lo = sh.lim_lo, t.lim_hi = sh.lim_hi;
+    float *to_ml = nullptr, *to_o = nullptr;
+    if (count > 1) {
+      const uint64_t part = 2 * (uint64_t)wg + (wg == first ? 1 : 0);
+      to_ml = ws.part_ml + part * ws.tile_rows * 2;
+      to_o = ws.part_o + part * ws.tile_rows * kPageDim;
+    } else if (two) {
+      const uint64_t r = ((uint64_t)g.own * v.H + h) * a.n_tokens * a.G + t.row0;
+      to_ml = ws.row_ml + r * 2;
+      to_o = ws.row_o + r * kPageDim;
+    }
+    auto narrow = [&](auto nt, auto rg) {
+      Narrow<DT, decltype(nt)::value, decltype(rg)::value> x;
+      x.run(v, layer, a, t, sh);
+      __syncthreads();
+      narrow_write<DT, decltype(nt)::value, decltype(rg)::value>(a, t, sh, to_ml, to_o);
+    };
+    std::integral_constant<int, 1> one;
+    if constexpr (Kv<DT>::F32) {
+      narrow(one, one);
+    } else {
+      std::integral_constant<int, 2> two_;
+      Wide<DT> x; x.run(v, layer, a, t, sh); x.write(a, t, to_ml, to_o);
+}
+    u += k1 - k0;
+  }
+}
+
+// Rows with parts: a wavefront each, two dims a lane.  Parts in the order of their
+// pages, the shared ones first.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid) {
+  const int l = threadIdx.x & 63;
+  const uint64_t rows = (uint64_t)a.n_tokens * a.G, all = rows * v.H;
+  const uint64_t r = (uint64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (r >= all) return;
+  const int h = (int)(r / rows), row = (int)(r % rows), tok = row / a.G;
+  if (tok < token_of(a, 0) || tok >= token_of(a, a.n_req)) return;
+  const Where own = ws.where[((uint64_t)v.H + h) * rows + row];
+  if (own.count == 0) return;
+  Where part[2];
+  part[1] = own;
+  part[0] = own.has & 1 ? ws.where[(uint64_t)h * rows + row] : Where{0, 0, 0, 0};
+  int n[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {  // stay in the scratch, whatever the offsets were
+    part[k].first = clampi(part[k].first, 0, grid - 1);
+    part[k].row = clampi(part[k].row, 0, ws.tile_rows - 1);
+    n[k] = clampi(part[k].count, 0, grid - part[k].first);
+  }
+  auto place = [&](int i, const float** o) -> const float* {
+    const int k = i >= n[0], at = i - (k ? n[0] : 0);
+    if (n[k] == 1 && own.has & 1) {
+      const uint64_t p = ((uint64_t)k * v.H + h) * rows + row;
+      *o = ws.row_o + p * kPageDim;
+      return ws.row_ml + p * 2;
+    }
+    const uint64_t p = (2 * (uint64_t)(part[k].first + at) + (at == 0 ? 1 : 0)) * ws.tile_rows + part[k].row;
+    *o = ws.part_o + p * kPageDim;
+    return ws.part_ml + p * 2;
+  };
+  const int parts = n[0] + n[1];
+  float m = -INFINITY;
+  const float* o;
+  for (int i = l; i < parts; i += 64) m = fmaxf(m, place(i, &o)[0]);
+#pragma unroll
+  for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = against(m);
+  float sum = 0.0f, x = 0.0f, y = 0.0f;
+  for (int i = 0; i < parts; ++i) {
+    const float* ml = place(i, &o);
+    const float f = exp2_fast(ml[0] - ref);
+    const float2 w = *reinterpret_cast<const float2*>(o + 2 * l);
+    sum += f * ml[1];
+    x += f * w.x;
+    y += f * w.y;
+  }
+  const bool none = !(own.has & 2);
+  const float inv = none ? 0.0f : 1.0f / sum;
+  const int64_t at = row_at(a, a.os, row, h) + 2 * l;
+  if constexpr (Kv<DT>::F32) {
+    float* p = static_cast<float*>(a.out) + at;
+    p[0] = x * inv, p[1] = y * inv;
+  } else {
+    const uint32_t w = pack2<Kv<DT>::BF>(x * inv, y * inv);
+    uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+    p[0] = (uint16_t)w, p[1] = (uint16_t)(w >> 16);
+  }
+  if (a.lse && l == 0)
+    a.lse[(int64_t)tok * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// ---- host ------------------------------------------------------------------------
+int check_attend(const ferry_pages* p, const ferry_attend* a, PageView* v) {
+  if (int rc = page_geometry(p, v)) return rc;
+  if (!a) return report(FERRY_EINVAL, "null args");
+  if (a->n_req < 0 || a->n_tokens < 0 || a->n_groups < 0 || a->n_groups > a->n_req)
+    return report(FERRY_EINVAL, "n_req, n_tokens and n_groups must not be negative, n_groups at most n_req");
+  if (a->q_heads < 1 || a->q_heads > 65535 || a->q_heads % p->kv_heads)
+    return report(FERRY_EINVAL, "q_heads must be a multiple of kv_heads");
+  if ((int64_t)a->n_tokens * (a->q_heads / p->kv_heads) > 0x3FFFFFFF)
+    return report(FERRY_EINVAL, "too many query rows");
+  if (!a->q_start && a->n_tokens != a->n_req)
+    return report(FERRY_EINVAL, "without q_start a request has one token");
+  return FERRY_OK;
+}
+
+uint64_t up256(uint64_t x) { return (x + 255) & ~255ull; }
+
+// Workgroups of a call, and its scratch at `base` (null: sizes only).
+int plan_attend(const ferry_pages* p, const ferry_attend* a, uint8_t* base, Scratch* ws, uint64_t* bytes) {
+  const int grid = 2 * gpu_cus(p->device);
+  const uint64_t rows = (uint64_t)a->n_tokens * (a->q_heads / p->kv_heads), H = p->kv_heads;
+  const uint64_t tile = p->dtype == FERRY_F32 ? 16 : std::min<uint64_t>(kWide, rows);
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    uint8_t* r = base + at;
+    at += up256(n);
+    return r;
+  };
+  ws->tile_rows = (int)tile;
+  ws->where = reinterpret_cast<Where*>(take(2 * H * rows * sizeof(Where)));
+  ws->part_ml = reinterpret_cast<float*>(take(2ull * grid * tile * 8));
+  ws->part_o = reinterpret_cast<float*>(take(2ull * grid * tile * kPageDim * 4));
+  const uint64_t twice = a->n_groups ? 2 * H * rows : 0;
+  ws->row_ml = reinterpret_cast<float*>(take(twice * 8));
+  ws->row_o = reinterpret_cast<float*>(take(twice * kPageDim * 4));
+  *bytes = at;
+  return grid;
+}
+
+template <int DT>
+void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int grid, hipStream_t s) {
+  k_attend<DT><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+  const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
+  k_attend_join<DT><<<(unsigned)((all + 3) / 4), kThreads, 0, s>>>(v, a, ws, grid);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ferry_pages_attend_work_bytes(const ferry_pages* p, const ferry_attend* a, uint64_t* bytes) {
+  return entry([&]() -> int {
+    PageView v;
+    if (int rc = check_attend(p, a, &v)) return rc;
+    if (!bytes) return report(FERRY_EINVAL, "null bytes");
+    Scratch ws;
+    plan_attend(p, a, nullptr, &ws, bytes);
+    return FERRY_OK;
+  });
+}
+
+int ferry_pages_attend(const ferry_pages* p, int32_t layer, const ferry_attend* a, void* stream) {
+  return entry([&]() -> int {
+    PageView v;
+    if (int rc = check_attend(p, a, &v)) return rc;
+    if (layer < 0 || layer >= p->n_layers) return report(FERRY_EINVAL, "layer out of range");
+    if (a->n_req == 0 || a->n_tokens == 0) return FERRY_OK;
+    if (int rc = page_buffers(p, false)) return rc;
+    if (int rc = check_all({{a->lanes, "lanes"}, {a->q, "q"}, {a->out, "out"}, {a->work, "work"}}, p->device)) return rc;
+    if (a->q_start)
+      if (int rc = check_on(a->q_start, "q_start", p->device)) return rc;
+    if (a->n_groups)
+      if (int rc = check_all({{a->group_start, "group_start"}, {a->shared, "shared"}}, p->device)) return rc;
+    if (a->lse)
+      if (int rc = check_on(a->lse, "lse", p->device)) return rc;
+    Scratch ws;
+    uint64_t need = 0;
+    const int grid = plan_attend(p, a, static_cast<uint8_t*>(a->work), &ws, &need);
+    if (a->work_bytes < need) return report(FERRY_EINVAL, "work is smaller than ferry_pages_attend_work_bytes");
+    if (reinterpret_cast<uintptr_t>(a->work) % 256) return report(FERRY_EINVAL, "work must be 256-byte aligned");
+    OnDevice on(p->device);
+    if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
+    const int es = p->dtype == FERRY_F32 ? 4 : 2;
+    uint64_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out);
+    for (int i = 0; i < 2; ++i) low |= (uint64_t)(a->q_stride[i] * es) | (uint64_t)(a->out_stride[i] * es);
+    AttendArgs d{a->n_req, a->n_tokens, a->n_groups, a->q_heads, a->q_heads / p->kv_heads,
+                 a->scale != 0.0f ? a->scale : 0.08838834764831845f, a->lanes, a->q_start, a->group_start,
+                 a->shared, a->q, a->out, a->lse, {a->q_stride[0], a->q_stride[1]},
+                 {a->out_stride[0], a->out_stride[1]}, low % 16 == 0};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+     launch_attend<FERRY_F16>(v, layer, d, ws, grid, s);
+    return launched("ferry_pages_attend");
+  });
+}
+
+}  // extern "C"

@@ -291,12 +291,18 @@ struct Shared {
   uint64_t seg_at;
 };
 
-// 8 query values of a row as two 16-bit values per dword.
-__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned) {
-  if (aligned) return *reinterpret_cast<const u32x4*>(p);
+// 8 query values of a row as two 16-bit values per dword, times the sign of the
+// scale (scores are then compared before they are scaled).
+__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned, uint32_t sign) {
   u32x4 x;
+  if (aligned) {
+    x = *reinterpret_cast<const u32x4*>(p);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= sign;
   return x;
 }
 
@@ -529,7 +535,7 @@ struct Narrow {
             else x = u32x4{f32_bits(p[0]), f32_bits(p[1]), f32_bits(p[2]), f32_bits(p[3])};
           } else {
             const int d = K::F8 ? 16 * (4 * (w >> 1) + grp) + 8 * (w & 1) : 8 * (4 * w + grp);
-            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned);
+            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned, 0u);
           }
         }
         q[nt][w] = x;
@@ -657,6 +663,20 @@ __device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Shared& 
 // A token's sixteen 16-byte chunks are stored at chunk ^ swizzle(token): the reads of
 // K (one chunk of 32 tokens) and of V (four chunks of 8 tokens) then spread over all
 // banks.
+// An LDS address as a number, and what is there: 16 bytes, or 4 values of a column
+// (the 16 lanes of a group name 4 tokens of 16 dims, 4 dims each).
+__device__ inline uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+template <class T>
+__device__ inline T lds(uint32_t at) {
+  return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
+}
+__device__ inline u32x2 lds_turned(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
+}
+
 __device__ inline int swizzle(int tok) { return (tok & 3) << 2 | (tok >> 2 & 3); }
 
 template <int DT>
@@ -671,7 +691,8 @@ struct Wide {
   __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
     const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = l & 31, h = l >> 5, row = wave * 32 + col;
-    const float scale = a.scale * 1.4426950408889634f;
+    const float scale = fabsf(a.scale) * 1.4426950408889634f;
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const bool busy = wave * 32 < t.rows;  // the others only help to load
     lim = row < t.rows ? sh.lim[row] : 0;
     m = -INFINITY, sum = 0.0f;
@@ -682,7 +703,7 @@ struct Wide {
     const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
 #pragma unroll
     for (int s = 0; s < 8; ++s)
-      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned)
+      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned, sign)
                           : u32x4{0u, 0u, 0u, 0u};
     const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
     uint32_t ids = 0;
@@ -743,43 +764,52 @@ struct Wide {
       }
       if (bad) sh.odd[b] = 1;
     };
+    // K: token col, chunk h; V: token 4 h + (l % 16) / 4, dims 16 (l / 16 % 2) + 4 (l % 4)
+    const uint32_t k_lane = lds_at(sh.kv.k[0]) + (col << 8) + ((h ^ swizzle(col)) << 4);
+    const int vt = 4 * h + (l >> 2 & 3), vd = 16 * (l >> 4 & 1) + 4 * (l & 3);
+    const uint32_t v_lane = lds_at(sh.kv.v[0]) + (vt << 8) + (((vd >> 3) ^ swizzle(vt)) << 4) + (vd & 4) * 2;
     if (tid < 2) sh.odd[tid] = 0;
     fill_ids(0);
     fetch(0);
     __syncthreads();
     store(0, 0);
     __syncthreads();
-    for (int s = 0; s < steps; ++s) {
+    // One step; MASKED: some row does not see all of its tokens.
+    auto step = [&](auto masked_, int s) {
+      constexpr bool MASKED = decltype(masked_)::value;
       const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
       if (s + 1 < steps) fetch(s + 1);
-      const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
-      const bool odd = masked && sh.odd[b];
+      const bool odd = MASKED && sh.odd[b];
       uint32_t pop[16];
+      // The lane's places in this step's K and V; the others follow by flipping address
+      // bits.  Opaque, so that they are not all kept in registers over the loop.
+      uint32_t k_at = k_lane + (b << 14), v_at = v_lane + (b << 14);
+      asm volatile("" : "+v"(k_at), "+v"(v_at));
       if (busy) {
         f32x16 x[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[tt][i] = 0.0f;
-          const uint8_t* kp = sh.kv.k[b] + ((32 * tt + col) << 8);
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            x[tt] = mma32<K::BF>(*reinterpret_cast<const u32x4*>(kp + (((2 * c + h) ^ swizzle(col)) << 4)), q[c], x[tt]);
+          for (int c = 0; c < 8; ++c)  // chunk 2 c + h of token 32 tt + col
+            x[tt] = mma32<K::BF>(lds<u32x4>((k_at ^ c << 5) + 8192 * tt), q[c], x[tt]);
         }
-        float top = -INFINITY;
+        float c[kStep], top = -INFINITY;  // c: factor on a page's scores
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * sh.ks[b][i] : scale;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float c = K::F8 ? scale * sh.ks[b][2 * tt + (i >> 3)] : scale;
-            x[tt][i] *= c;
-            if (masked && t0 + 32 * tt + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) x[tt][i] = -INFINITY;
-            top = fmaxf(top, x[tt][i]);
-          }
+        for (int i = 0; i < 32; ++i) {
+          float& y = reinterpret_cast<float*>(&x[i >> 4])[i & 15];
+          if (K::F8) y *= c[i >> 3];
+          if (MASKED && t0 + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) y = -INFINITY;
+          top = fmaxf(top, y);
+        }
         {
           const mx_u32x2 two = pair_values<32>(top);
           top = fmaxf(bits_f32(two[0]), bits_f32(two[1]));
         }
+        if (!K::F8) top *= scale;
         const bool raise = top > m + kRaise;
         if (__builtin_amdgcn_ballot_w64(raise)) {
           const float f = raise ? exp2_fast(m - top) : 1.0f;
@@ -790,31 +820,25 @@ struct Wide {
         }
         const float ref = against(m);
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float p0 = exp2_fast(x[tt][i] - ref), p1 = exp2_fast(x[tt][i + 1] - ref);
-            sum += p0 + p1;
-            if constexpr (K::F8) {
-              const float f = sh.vs[b][2 * tt + (i >> 3)];
-              p0 *= f, p1 *= f;
-            }
-            pop[8 * tt + i / 2] = pack2<K::BF>(p0, p1);
+        for (int i = 0; i < 32; i += 2) {
+          const float y0 = x[i >> 4][i & 15], y1 = x[i >> 4][(i & 15) + 1];
+          float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
+          float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
+          sum += p0 + p1;
+          if constexpr (K::F8) {
+            const float f = sh.vs[b][i >> 3];
+            p0 *= f, p1 *= f;
           }
-        // lane's addresses for the transposing reads: token row (l % 16) / 4, dims 4 (l % 4)
-        const int rt = 4 * h + (l >> 2 & 3), rd = 16 * (l >> 4 & 1) + 4 * (l & 3);
+          pop[i / 2] = pack2<K::BF>(p0, p1);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const u32x4 pj = {pop[4 * j], pop[4 * j + 1], pop[4 * j + 2], pop[4 * j + 3]};
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
-            auto part = [&](int tok_) {
-              const int d = 32 * dt + rd;
-              uint8_t* p = sh.kv.v[b] + (tok_ << 8) + (((d >> 3) ^ swizzle(tok_)) << 4) + (d & 4) * 2;
-              return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) i16x4*)p));
-            };
-            const u32x2 lo = part(16 * j + rt), hi = part(16 * j + 8 + rt);
+            // tokens 16 j + 4 h .. + 3 and those 8 behind, whose swizzle flips chunk bit 1
+            const u32x2 lo = lds_turned((v_at ^ dt << 6) + 4096 * j);
+            const u32x2 hi = lds_turned((v_at ^ dt << 6 ^ 32) + 4096 * j + 2048);
             o[dt] = mma32<K::BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pj, o[dt]);
           }
         }
@@ -855,7 +879,11 @@ struct Wide {
       }
       if (s + 1 < steps) store(s + 1, b ^ 1);
       __syncthreads();
-    }
+    };
+    // the steps that every row sees whole, then the others
+    const int whole = clampi((t.lim_lo - t.p0 * kPageTokens) / (kStep * kPageTokens), 0, steps);
+    for (int s = 0; s < whole; ++s) step(std::false_type{}, s);
+    for (int s = whole; s < steps; ++s) step(std::true_type{}, s);
     {
       const mx_u32x2 two = pair_values<32>(sum);
       sum = bits_f32(two[0]) + bits_f32(two[1]);
@@ -900,7 +928,7 @@ struct Wide {
 // ---- the call -------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
-  __shared__ Shared sh;
+  __shared__ __attribute__((aligned(1024))) Shared sh;
   const int tid = threadIdx.x, grid = gridDim.x;
   // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
   // that tiles of the same pages meet in its L2
