@@ -273,6 +273,13 @@ struct Tile {
   int lim_lo, lim_hi;  // tokens that its least and its most seeing row see
 };
 
+// A segment in the order of all units.
+struct SegAt {
+  Seg g;
+  uint64_t at, steps;  // its first unit; steps of all its tiles (per kv head)
+};
+constexpr int kListed = 32;
+
 struct Shared {
   union {
     float merge[4 * 32 * kPad];  // [wavefront][row][dim]: accumulators of wavefronts that share rows
@@ -287,16 +294,23 @@ struct Shared {
   float ks[2][kStep], vs[2][kStep];
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
   uint64_t sums[kThreads / 64];
-  int seg;
-  uint64_t seg_at;
+  int seg;          // first segment of this workgroup's run
+  int group_lim;    // least number of tokens that a row of the current group sees
+  SegAt list[kListed];  // consecutive segments of the run
 };
 
-// 8 query values of a row as two 16-bit values per dword.
-__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned) {
-  if (aligned) return *reinterpret_cast<const u32x4*>(p);
+// 8 query values of a row as two 16-bit values per dword, times the sign of the
+// scale (scores are then compared before they are scaled).
+__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned, uint32_t sign) {
   u32x4 x;
+  if (aligned) {
+    x = *reinterpret_cast<const u32x4*>(p);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= sign;
   return x;
 }
 
@@ -529,7 +543,7 @@ struct Narrow {
             else x = u32x4{f32_bits(p[0]), f32_bits(p[1]), f32_bits(p[2]), f32_bits(p[3])};
           } else {
             const int d = K::F8 ? 16 * (4 * (w >> 1) + grp) + 8 * (w & 1) : 8 * (4 * w + grp);
-            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned);
+            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned, 0u);
           }
         }
         q[nt][w] = x;
@@ -657,6 +671,20 @@ __device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Shared& 
 // A token's sixteen 16-byte chunks are stored at chunk ^ swizzle(token): the reads of
 // K (one chunk of 32 tokens) and of V (four chunks of 8 tokens) then spread over all
 // banks.
+// An LDS address as a number, and what is there: 16 bytes, or 4 values of a column
+// (the 16 lanes of a group name 4 tokens of 16 dims, 4 dims each).
+__device__ inline uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+template <class T>
+__device__ inline T lds(uint32_t at) {
+  return *(__attribute__((address_space(3))) const T*)(uintptr_t)at;
+}
+__device__ inline u32x2 lds_turned(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
+}
+
 __device__ inline int swizzle(int tok) { return (tok & 3) << 2 | (tok >> 2 & 3); }
 
 template <int DT>
@@ -671,7 +699,8 @@ struct Wide {
   __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
     const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = l & 31, h = l >> 5, row = wave * 32 + col;
-    const float scale = a.scale * 1.4426950408889634f;
+    const float scale = fabsf(a.scale) * 1.4426950408889634f;
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
     const bool busy = wave * 32 < t.rows;  // the others only help to load
     lim = row < t.rows ? sh.lim[row] : 0;
     m = -INFINITY, sum = 0.0f;
@@ -682,7 +711,7 @@ struct Wide {
     const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
 #pragma unroll
     for (int s = 0; s < 8; ++s)
-      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned)
+      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned, sign)
                           : u32x4{0u, 0u, 0u, 0u};
     const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
     uint32_t ids = 0;
@@ -743,43 +772,52 @@ struct Wide {
       }
       if (bad) sh.odd[b] = 1;
     };
+    // K: token col, chunk h; V: token 4 h + (l % 16) / 4, dims 16 (l / 16 % 2) + 4 (l % 4)
+    const uint32_t k_lane = lds_at(sh.kv.k[0]) + (col << 8) + ((h ^ swizzle(col)) << 4);
+    const int vt = 4 * h + (l >> 2 & 3), vd = 16 * (l >> 4 & 1) + 4 * (l & 3);
+    const uint32_t v_lane = lds_at(sh.kv.v[0]) + (vt << 8) + (((vd >> 3) ^ swizzle(vt)) << 4) + (vd & 4) * 2;
     if (tid < 2) sh.odd[tid] = 0;
     fill_ids(0);
     fetch(0);
     __syncthreads();
     store(0, 0);
     __syncthreads();
-    for (int s = 0; s < steps; ++s) {
+    // One step; MASKED: some row does not see all of its tokens.
+    auto step = [&](auto masked_, int s) {
+      constexpr bool MASKED = decltype(masked_)::value;
       const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
       if (s + 1 < steps) fetch(s + 1);
-      const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
-      const bool odd = masked && sh.odd[b];
+      const bool odd = MASKED && sh.odd[b];
       uint32_t pop[16];
+      // The lane's places in this step's K and V; the others follow by flipping address
+      // bits.  Opaque, so that they are not all kept in registers over the loop.
+      uint32_t k_at = k_lane + (b << 14), v_at = v_lane + (b << 14);
+      asm volatile("" : "+v"(k_at), "+v"(v_at));
       if (busy) {
         f32x16 x[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[tt][i] = 0.0f;
-          const uint8_t* kp = sh.kv.k[b] + ((32 * tt + col) << 8);
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            x[tt] = mma32<K::BF>(*reinterpret_cast<const u32x4*>(kp + (((2 * c + h) ^ swizzle(col)) << 4)), q[c], x[tt]);
+          for (int c = 0; c < 8; ++c)  // chunk 2 c + h of token 32 tt + col
+            x[tt] = mma32<K::BF>(lds<u32x4>((k_at ^ c << 5) + 8192 * tt), q[c], x[tt]);
         }
-        float top = -INFINITY;
+        float c[kStep], top = -INFINITY;  // c: factor on a page's scores
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+        for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * sh.ks[b][i] : scale;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float c = K::F8 ? scale * sh.ks[b][2 * tt + (i >> 3)] : scale;
-            x[tt][i] *= c;
-            if (masked && t0 + 32 * tt + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) x[tt][i] = -INFINITY;
-            top = fmaxf(top, x[tt][i]);
-          }
+        for (int i = 0; i < 32; ++i) {
+          float& y = reinterpret_cast<float*>(&x[i >> 4])[i & 15];
+          if (K::F8) y *= c[i >> 3];
+          if (MASKED && t0 + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) y = -INFINITY;
+          top = fmaxf(top, y);
+        }
         {
           const mx_u32x2 two = pair_values<32>(top);
           top = fmaxf(bits_f32(two[0]), bits_f32(two[1]));
         }
+        if (!K::F8) top *= scale;
         const bool raise = top > m + kRaise;
         if (__builtin_amdgcn_ballot_w64(raise)) {
           const float f = raise ? exp2_fast(m - top) : 1.0f;
@@ -790,31 +828,25 @@ struct Wide {
         }
         const float ref = against(m);
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float p0 = exp2_fast(x[tt][i] - ref), p1 = exp2_fast(x[tt][i + 1] - ref);
-            sum += p0 + p1;
-            if constexpr (K::F8) {
-              const float f = sh.vs[b][2 * tt + (i >> 3)];
-              p0 *= f, p1 *= f;
-            }
-            pop[8 * tt + i / 2] = pack2<K::BF>(p0, p1);
+        for (int i = 0; i < 32; i += 2) {
+          const float y0 = x[i >> 4][i & 15], y1 = x[i >> 4][(i & 15) + 1];
+          float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
+          float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
+          sum += p0 + p1;
+          if constexpr (K::F8) {
+            const float f = sh.vs[b][i >> 3];
+            p0 *= f, p1 *= f;
           }
-        // lane's addresses for the transposing reads: token row (l % 16) / 4, dims 4 (l % 4)
-        const int rt = 4 * h + (l >> 2 & 3), rd = 16 * (l >> 4 & 1) + 4 * (l & 3);
+          pop[i / 2] = pack2<K::BF>(p0, p1);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const u32x4 pj = {pop[4 * j], pop[4 * j + 1], pop[4 * j + 2], pop[4 * j + 3]};
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
-            auto part = [&](int tok_) {
-              const int d = 32 * dt + rd;
-              uint8_t* p = sh.kv.v[b] + (tok_ << 8) + (((d >> 3) ^ swizzle(tok_)) << 4) + (d & 4) * 2;
-              return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) i16x4*)p));
-            };
-            const u32x2 lo = part(16 * j + rt), hi = part(16 * j + 8 + rt);
+            // tokens 16 j + 4 h .. + 3 and those 8 behind, whose swizzle flips chunk bit 1
+            const u32x2 lo = lds_turned((v_at ^ dt << 6) + 4096 * j);
+            const u32x2 hi = lds_turned((v_at ^ dt << 6 ^ 32) + 4096 * j + 2048);
             o[dt] = mma32<K::BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pj, o[dt]);
           }
         }
@@ -855,7 +887,11 @@ struct Wide {
       }
       if (s + 1 < steps) store(s + 1, b ^ 1);
       __syncthreads();
-    }
+    };
+    // the steps that every row sees whole, then the others
+    const int whole = clampi((t.lim_lo - t.p0 * kPageTokens) / (kStep * kPageTokens), 0, steps);
+    for (int s = 0; s < whole; ++s) step(std::false_type{}, s);
+    for (int s = whole; s < steps; ++s) step(std::true_type{}, s);
     {
       const mx_u32x2 two = pair_values<32>(sum);
       sum = bits_f32(two[0]) + bits_f32(two[1]);
@@ -900,7 +936,7 @@ struct Wide {
 // ---- the call -------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
-  __shared__ Shared sh;
+  __shared__ __attribute__((aligned(1024))) Shared sh;
   const int tid = threadIdx.x, grid = gridDim.x;
   // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
   // that tiles of the same pages meet in its L2
@@ -919,16 +955,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
   const int per_thread = (nseg + kThreads - 1) / kThreads, s0 = min(tid * per_thread, nseg),
             s1 = min(s0 + per_thread, nseg);
   uint64_t mine = 0;
+  Seg kept;  // the thread's only segment, where it has one
+  uint64_t kept_steps = 0;
   for (int s = s0; s < s1; ++s) {
-    const Seg g = segment<DT>(v, a, gs, gp, s);
-    mine += seg_steps(g, a.G) * v.H;
+    kept = segment<DT>(v, a, gs, gp, s);
+    kept_steps = seg_steps(kept, a.G);
+    mine += kept_steps * v.H;
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
-      if (g.own) {
-        const int lane = a.lanes[g.req];
-        bad = lane < -1 || lane >= v.n_lanes || (g.lane >= 0 && v.len[g.lane] != g.len);
+      if (kept.own) {
+        const int lane = a.lanes[kept.req];
+        bad = lane < -1 || lane >= v.n_lanes || (kept.lane >= 0 && v.len[kept.lane] != kept.len);
         if (a.q_start)
-          bad |= a.q_start[g.req] < 0 || a.q_start[g.req] > a.q_start[g.req + 1] || a.q_start[g.req + 1] > a.n_tokens;
+          bad |= a.q_start[kept.req] < 0 || a.q_start[kept.req] > a.q_start[kept.req + 1] ||
+                 a.q_start[kept.req + 1] > a.n_tokens;
       } else {
         bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
       }
@@ -949,38 +989,72 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
     total += sh.sums[i];
   }
   before -= mine;
-  const uint64_t per = (total + grid - 1) / grid;
+  total = first_lane_u64(total);
+  const uint64_t per = first_lane_u64((total + grid - 1) / grid);
   const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
   if (u0 >= u1) return;
-  if (u0 >= before && u0 < before + mine) {  // one thread
+  const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
+  // Each thread lists those of its segments that are among the next kListed from s on.
+  auto list = [&](int from) {
+    uint64_t at = before;
+    for (int s = s0; s < s1; ++s) {
+      SegAt x;
+      x.g = per_thread == 1 ? kept : segment<DT>(v, a, gs, gp, s);
+      x.steps = per_thread == 1 ? kept_steps : seg_steps(x.g, a.G);
+      x.at = at;
+      if (s >= from && s < from + kListed) sh.list[s - from] = x;
+      at += x.steps * v.H;
+    }
+    __syncthreads();
+  };
+  if (u0 >= before && u0 < before + mine) {  // one thread: it has the run's first segment
     uint64_t at = before;
     int s = s0;
-    for (;; ++s) {
-      const uint64_t n = seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
-      if (u0 < at + n) break;
-      at += n;
-    }
-    sh.seg = s, sh.seg_at = at;
+    if (per_thread > 1)
+      for (;; ++s) {
+        at += seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+        if (u0 < at) break;
+      }
+    sh.seg = s;
   }
   __syncthreads();
 
-  int s = sh.seg;
-  uint64_t u = u0, at = sh.seg_at;
+  int s = first_lane_i(sh.seg), from = s;
+  list(from);
+  uint64_t u = u0, tile_at = 0;
+  int h = -1, j = 0, group = -1;
+  SegAt x;
+  auto listed = [&](int i) {  // the same for all lanes, and known to be
+    const SegAt& y = sh.list[i];
+    const int* w = reinterpret_cast<const int*>(&y.g);
+    int* to = reinterpret_cast<int*>(&x.g);
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(Seg) / 4); ++k) to[k] = first_lane_i(w[k]);
+    x.at = first_lane_u64(y.at), x.steps = first_lane_u64(y.steps);
+  };
+  listed(0);
   while (u < u1) {
-    Seg g = segment<DT>(v, a, gs, gp, s);
-    uint64_t steps = seg_steps(g, a.G);
-    while (u >= at + steps * v.H) {  // the next segment with rows
-      at += steps * v.H;
-      g = segment<DT>(v, a, gs, gp, ++s);
-      steps = seg_steps(g, a.G);
+    if (u >= x.at + x.steps * v.H) {  // the next segment
+      if (++s == from + kListed) {
+        __syncthreads();
+        from = s;
+        list(from);
+      }
+      listed(s - from);
+      h = -1;
+      continue;
     }
-    int h = (int)((u - at) / steps);
-    uint64_t tile_at = at + h * steps;  // unit of the tile's first step
-    int j = 0, len = 0;
-    for (;; ++j) {
-      len = tile_steps(g, j, a.G);
-      if (u < tile_at + len) break;
+    const Seg& g = x.g;
+    if (h < 0) {
+      h = u == x.at ? 0 : (int)((u - x.at) / x.steps);
+      tile_at = x.at + h * x.steps;  // unit of the tile's first step
+      j = 0;
+    }
+    int len = tile_steps(g, j, a.G);
+    while (u >= tile_at + len) {
       tile_at += len;
+      if (++j == g.tiles) j = 0, ++h;
+      len = tile_steps(g, j, a.G);
     }
     const int k0 = (int)(u - tile_at), k1 = (int)min((uint64_t)len, (uint64_t)k0 + (u1 - u));
     Tile t;
@@ -988,19 +1062,42 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
     t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
     if (t.p1 < t.p0) t.p1 = t.p0;
     t.table = v.table + (uint64_t)(g.lane < 0 ? 0 : g.lane) * v.max_pages;
-    __syncthreads();  // the last tile's rows are written
-    if (tid == 0) sh.lim_lo = 0x7FFFFFFF, sh.lim_hi = 0;
-    __syncthreads();
-    const int first = (int)(tile_at / per);
-    const int count = (int)((tile_at + len - 1) / per) - first + 1;
+    // the workgroups that share the tile
+    const int first = tile_at >= u0 ? wg : wg - (int)(((uint32_t)(u0 - tile_at) + per32 - 1) / per32);
+    const int last = tile_at + len <= u1 ? wg : wg + (int)((uint32_t)(tile_at + len - 1 - u0) / per32);
+    const int count = last - first + 1;
     const bool two = g.own ? a.n_groups && g.p0 > 0 : true;
+    __syncthreads();  // the last tile's rows are written
+    if (!g.own && group != g.req) {  // a new group: what its rows see at least
+      group = g.req;
+      if (tid == 0) sh.group_lim = 0x7FFFFFFF;
+      __syncthreads();
+      const int b = clampi(gs[g.req], 0, a.n_req), e = clampi(gs[g.req + 1], b, a.n_req);
+      for (int r = b + tid; r < e; r += kThreads) {
+        const int n = token_of(a, r + 1) - token_of(a, r);
+        if (n > 0) atomicMin(&sh.group_lim, max(0, len_of(v, lane_of(v, a, r)) - n + 1));
+      }
+      __syncthreads();
+    }
+    const bool all_seen = !g.own && first_lane_i(sh.group_lim) >= g.p1 * kPageTokens;
+    const int tok0 = t.row0 / a.G, tok1 = (t.row0 + t.rows - 1) / a.G;
+    if (g.own) {
+      t.lim_lo = clampi(g.base + tok0 - g.row0 / a.G, 0, g.len);
+      t.lim_hi = clampi(g.base + tok1 - g.row0 / a.G, 0, g.len);
+    } else {
+      t.lim_lo = t.lim_hi = g.p1 * kPageTokens;
+      if (!all_seen) {
+        if (tid == 0) sh.lim_lo = 0x7FFFFFFF, sh.lim_hi = 0;
+        __syncthreads();
+      }
+    }
     if (tid < t.rows) {
       const int row = t.row0 + tid, tok = row / a.G;
-      int lim;
+      int lim = t.lim_lo;
       if (g.own) {
         lim = clampi(g.base + (tok - g.row0 / a.G), 0, g.len);
-      } else {
-        int lo = tok, len_;
+      } else if (!all_seen) {
+        int lo = tok;
         if (a.q_start) {  // the request of this token
           lo = clampi(gs[g.req], 0, a.n_req);
           int hi = clampi(gs[g.req + 1], lo, a.n_req) - 1;
@@ -1009,18 +1106,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
             if (token_of(a, mid) <= tok) lo = mid; else hi = mid - 1;
           }
         }
-        len_ = len_of(v, lane_of(v, a, lo));
-        lim = min(clampi(len_ - token_of(a, lo + 1) + tok + 1, 0, len_), g.p1 * kPageTokens);
+        const int n = len_of(v, lane_of(v, a, lo));
+        lim = min(clampi(n - token_of(a, lo + 1) + tok + 1, 0, n), g.p1 * kPageTokens);
+        atomicMin(&sh.lim_lo, lim);
+        atomicMax(&sh.lim_hi, lim);
       }
       sh.lim[tid] = lim;
-      atomicMin(&sh.lim_lo, lim);
-      atomicMax(&sh.lim_hi, lim);
       if (k0 == 0)
         ws.where[((uint64_t)g.own * v.H + h) * a.n_tokens * a.G + row] =
             Where{first, !two && count == 1 ? 0 : count, tid, (two ? 1 : 0) | (lim > 0 ? 2 : 0)};
     }
     __syncthreads();
-    t.lim_lo = sh.lim_lo, t.lim_hi = sh.lim_hi;
+    if (!g.own && !all_seen) t.lim_lo = first_lane_i(sh.lim_lo), t.lim_hi = first_lane_i(sh.lim_hi);
     float *to_ml = nullptr, *to_o = nullptr;
     if (count > 1) {
       const uint64_t part = 2 * (uint64_t)wg + (wg == first ? 1 : 0);
@@ -1202,7 +1299,10 @@ int ferry_pages_attend(const ferry_pages* p, int32_t layer, const ferry_attend* 
                  a->shared, a->q, a->out, a->lse, {a->q_stride[0], a->q_stride[1]},
                  {a->out_stride[0], a->out_stride[1]}, low % 16 == 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-     launch_attend<FERRY_F16>(v, layer, d, ws, grid, s);
+    if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, grid, s);
+    else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, grid, s);
+    else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, grid, s);
+    else launch_attend<FERRY_FP8_E4M3>(v, layer, d, ws, grid, s);
     return launched("ferry_pages_attend");
   });
 }

@@ -273,6 +273,13 @@ struct Tile {
   int lim_lo, lim_hi;  // tokens that its least and its most seeing row see
 };
 
+// A segment in the order of all units.
+struct SegAt {
+  Seg g;
+  uint64_t at, steps;  // its first unit; steps of all its tiles (per kv head)
+};
+constexpr int kListed = 32;
+
 struct Shared {
   union {
     float merge[4 * 32 * kPad];  // [wavefront][row][dim]: accumulators of wavefronts that share rows
@@ -287,8 +294,9 @@ struct Shared {
   float ks[2][kStep], vs[2][kStep];
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
   uint64_t sums[kThreads / 64];
-  int seg;
-  uint64_t seg_at;
+  int seg;          // first segment of this workgroup's run
+  int group_lim;    // least number of tokens that a row of the current group sees
+  SegAt list[kListed];  // consecutive segments of the run
 };
 
 // 8 query values of a row as two 16-bit values per dword, times the sign of the
@@ -947,16 +955,20 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
   const int per_thread = (nseg + kThreads - 1) / kThreads, s0 = min(tid * per_thread, nseg),
             s1 = min(s0 + per_thread, nseg);
   uint64_t mine = 0;
+  Seg kept;  // the thread's only segment, where it has one
+  uint64_t kept_steps = 0;
   for (int s = s0; s < s1; ++s) {
-    const Seg g = segment<DT>(v, a, gs, gp, s);
-    mine += seg_steps(g, a.G) * v.H;
+    kept = segment<DT>(v, a, gs, gp, s);
+    kept_steps = seg_steps(kept, a.G);
+    mine += kept_steps * v.H;
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
-      if (g.own) {
-        const int lane = a.lanes[g.req];
-        bad = lane < -1 || lane >= v.n_lanes || (g.lane >= 0 && v.len[g.lane] != g.len);
+      if (kept.own) {
+        const int lane = a.lanes[kept.req];
+        bad = lane < -1 || lane >= v.n_lanes || (kept.lane >= 0 && v.len[kept.lane] != kept.len);
         if (a.q_start)
-          bad |= a.q_start[g.req] < 0 || a.q_start[g.req] > a.q_start[g.req + 1] || a.q_start[g.req + 1] > a.n_tokens;
+          bad |= a.q_start[kept.req] < 0 || a.q_start[kept.req] > a.q_start[kept.req + 1] ||
+                 a.q_start[kept.req + 1] > a.n_tokens;
       } else {
         bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
       }
@@ -977,38 +989,74 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
     total += sh.sums[i];
   }
   before -= mine;
-  const uint64_t per = (total + grid - 1) / grid;
+  total = first_lane_u64(total);
+  const uint64_t per = first_lane_u64((total + grid - 1) / grid);
   const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
   if (u0 >= u1) return;
-  if (u0 >= before && u0 < before + mine) {  // one thread
+  const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
+  // Each thread lists those of its segments that are among the kListed from `from` on.
+  auto list = [&](int from, auto first) {
+    const int s0 = min((int)threadIdx.x * per_thread, nseg), s1 = min(s0 + per_thread, nseg);
+    uint64_t at = before;
+    for (int s = s0; s < s1; ++s) {
+      SegAt x;
+      const bool have = decltype(first)::value && per_thread == 1;
+      x.g = have ? kept : segment<DT>(v, a, gs, gp, s);
+      x.steps = have ? kept_steps : seg_steps(x.g, a.G);
+      x.at = at;
+      if (s >= from && s < from + kListed) sh.list[s - from] = x;
+      at += x.steps * v.H;
+    }
+    __syncthreads();
+  };
+  if (u0 >= before && u0 < before + mine) {  // one thread: it has the run's first segment
     uint64_t at = before;
     int s = s0;
-    for (;; ++s) {
-      const uint64_t n = seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
-      if (u0 < at + n) break;
-      at += n;
-    }
-    sh.seg = s, sh.seg_at = at;
+    if (per_thread > 1)
+      for (;; ++s) {
+        at += seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+        if (u0 < at) break;
+      }
+    sh.seg = s;
   }
   __syncthreads();
 
-  int s = sh.seg;
-  uint64_t u = u0, at = sh.seg_at;
+  int s = first_lane_i(sh.seg), from = s;
+  list(from, std::true_type{});
+  uint64_t u = u0, tile_at = 0;
+  int h = -1, j = 0, group = -1;
+  SegAt x;
+  auto listed = [&](int i) {  // the same for all lanes, and known to be
+    const SegAt& y = sh.list[i];
+    const int* w = reinterpret_cast<const int*>(&y.g);
+    int* to = reinterpret_cast<int*>(&x.g);
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(Seg) / 4); ++k) to[k] = first_lane_i(w[k]);
+    x.at = first_lane_u64(y.at), x.steps = first_lane_u64(y.steps);
+  };
+  listed(0);
   while (u < u1) {
-    Seg g = segment<DT>(v, a, gs, gp, s);
-    uint64_t steps = seg_steps(g, a.G);
-    while (u >= at + steps * v.H) {  // the next segment with rows
-      at += steps * v.H;
-      g = segment<DT>(v, a, gs, gp, ++s);
-      steps = seg_steps(g, a.G);
+    if (u >= x.at + x.steps * v.H) {  // the next segment
+      if (++s == from + kListed) {
+        __syncthreads();
+        from = s;
+        list(from, std::false_type{});
+      }
+      listed(s - from);
+      h = -1;
+      continue;
     }
-    int h = (int)((u - at) / steps);
-    uint64_t tile_at = at + h * steps;  // unit of the tile's first step
-    int j = 0, len = 0;
-    for (;; ++j) {
-      len = tile_steps(g, j, a.G);
-      if (u < tile_at + len) break;
+    const Seg& g = x.g;
+    if (h < 0) {
+      h = u == x.at ? 0 : (int)((u - x.at) / x.steps);
+      tile_at = x.at + h * x.steps;  // unit of the tile's first step
+      j = 0;
+    }
+    int len = tile_steps(g, j, a.G);
+    while (u >= tile_at + len) {
       tile_at += len;
+      if (++j == g.tiles) j = 0, ++h;
+      len = tile_steps(g, j, a.G);
     }
     const int k0 = (int)(u - tile_at), k1 = (int)min((uint64_t)len, (uint64_t)k0 + (u1 - u));
     Tile t;
@@ -1016,19 +1064,42 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
     t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
     if (t.p1 < t.p0) t.p1 = t.p0;
     t.table = v.table + (uint64_t)(g.lane < 0 ? 0 : g.lane) * v.max_pages;
-    __syncthreads();  // the last tile's rows are written
-    if (tid == 0) sh.lim_lo = 0x7FFFFFFF, sh.lim_hi = 0;
-    __syncthreads();
-    const int first = (int)(tile_at / per);
-    const int count = (int)((tile_at + len - 1) / per) - first + 1;
+    // the workgroups that share the tile
+    const int first = tile_at >= u0 ? wg : wg - (int)(((uint32_t)(u0 - tile_at) + per32 - 1) / per32);
+    const int last = tile_at + len <= u1 ? wg : wg + (int)((uint32_t)(tile_at + len - 1 - u0) / per32);
+    const int count = last - first + 1;
     const bool two = g.own ? a.n_groups && g.p0 > 0 : true;
+    __syncthreads();  // the last tile's rows are written
+    if (!g.own && group != g.req) {  // a new group: what its rows see at least
+      group = g.req;
+      if (tid == 0) sh.group_lim = 0x7FFFFFFF;
+      __syncthreads();
+      const int b = clampi(gs[g.req], 0, a.n_req), e = clampi(gs[g.req + 1], b, a.n_req);
+      for (int r = b + tid; r < e; r += kThreads) {
+        const int n = token_of(a, r + 1) - token_of(a, r);
+        if (n > 0) atomicMin(&sh.group_lim, max(0, len_of(v, lane_of(v, a, r)) - n + 1));
+      }
+      __syncthreads();
+    }
+    const bool all_seen = !g.own && first_lane_i(sh.group_lim) >= g.p1 * kPageTokens;
+    const int tok0 = t.row0 / a.G, tok1 = (t.row0 + t.rows - 1) / a.G;
+    if (g.own) {
+      t.lim_lo = clampi(g.base + tok0 - g.row0 / a.G, 0, g.len);
+      t.lim_hi = clampi(g.base + tok1 - g.row0 / a.G, 0, g.len);
+    } else {
+      t.lim_lo = t.lim_hi = g.p1 * kPageTokens;
+      if (!all_seen) {
+        if (tid == 0) sh.lim_lo = 0x7FFFFFFF, sh.lim_hi = 0;
+        __syncthreads();
+      }
+    }
     if (tid < t.rows) {
       const int row = t.row0 + tid, tok = row / a.G;
-      int lim;
+      int lim = t.lim_lo;
       if (g.own) {
         lim = clampi(g.base + (tok - g.row0 / a.G), 0, g.len);
-      } else {
-        int lo = tok, len_;
+      } else if (!all_seen) {
+        int lo = tok;
         if (a.q_start) {  // the request of this token
           lo = clampi(gs[g.req], 0, a.n_req);
           int hi = clampi(gs[g.req + 1], lo, a.n_req) - 1;
@@ -1037,18 +1108,18 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
             if (token_of(a, mid) <= tok) lo = mid; else hi = mid - 1;
           }
         }
-        len_ = len_of(v, lane_of(v, a, lo));
-        lim = min(clampi(len_ - token_of(a, lo + 1) + tok + 1, 0, len_), g.p1 * kPageTokens);
+        const int n = len_of(v, lane_of(v, a, lo));
+        lim = min(clampi(n - token_of(a, lo + 1) + tok + 1, 0, n), g.p1 * kPageTokens);
+        atomicMin(&sh.lim_lo, lim);
+        atomicMax(&sh.lim_hi, lim);
       }
       sh.lim[tid] = lim;
-      atomicMin(&sh.lim_lo, lim);
-      atomicMax(&sh.lim_hi, lim);
       if (k0 == 0)
         ws.where[((uint64_t)g.own * v.H + h) * a.n_tokens * a.G + row] =
             Where{first, !two && count == 1 ? 0 : count, tid, (two ? 1 : 0) | (lim > 0 ? 2 : 0)};
     }
     __syncthreads();
-    t.lim_lo = sh.lim_lo, t.lim_hi = sh.lim_hi;
+    if (!g.own && !all_seen) t.lim_lo = first_lane_i(sh.lim_lo), t.lim_hi = first_lane_i(sh.lim_hi);
     float *to_ml = nullptr, *to_o = nullptr;
     if (count > 1) {
       const uint64_t part = 2 * (uint64_t)wg + (wg == first ? 1 : 0);
