@@ -54,6 +54,8 @@ constexpr int kWide = 128;         // rows of the widest tile
 constexpr float kRaise = 8.0f;     // log2 of the largest weight between raises of the max
 constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
 constexpr int kPad = 132;          // floats per row of the merge buffer
+constexpr int kNarrowPerCu = 2;    // workgroups per CU where all tiles have 16 rows (else 2)
+constexpr int kTileCost = 2;       // what a tile costs beside its steps, in steps
 
 struct AttendArgs {
   int n_req, n_tokens, n_groups, Hq, G;
@@ -145,32 +147,33 @@ __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // The value weights are taken against: m, or 0 while no score was finite.
 __device__ inline float against(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// One V element of a record as fp32 (fp8: the code's value).
+// One K or V element of a record as fp32 (fp8: the code's value), one of q.
 template <int DT>
-__device__ inline float v_elem(const uint8_t* rec, int tok, int d) {
-  const uint8_t* p = rec + Kv<DT>::HALF;
+__device__ inline float k_elem(const uint8_t* p, int tok, int d) {
   const int i = tok * kPageDim + d;
   if constexpr (DT == FERRY_F32) return reinterpret_cast<const float*>(p)[i];
   else if constexpr (DT == FERRY_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
   else if constexpr (DT == FERRY_BF16) return bits_f32((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
   else return bits_f32(e4m3x4_to_bf16(p[i])[0] << 16);
 }
+template <int DT>
+__device__ inline float v_elem(const uint8_t* rec, int tok, int d) {
+  return k_elem<DT>(rec + Kv<DT>::HALF, tok, d);
+}
+template <int DT>
+__device__ inline float q_elem(const void* q, int64_t i) {
+  if constexpr (DT == FERRY_F32) return static_cast<const float*>(q)[i];
+  else if constexpr (DT == FERRY_F16) return (float)static_cast<const _Float16*>(q)[i];
+  else return bits_f32((uint32_t)static_cast<const uint16_t*>(q)[i] << 16);
+}
 __device__ inline bool finite(float x) { return (f32_bits(x) & 0x7F800000u) != 0x7F800000u; }
 
-// A dword of two 16-bit operand values (or one fp32) with what is not finite set
-// to zero; *found is set where there was such a value.
+// Whether a dword of two 16-bit operand values (or one fp32) holds what is not finite.
 template <int DT>
-__device__ inline uint32_t only_finite(uint32_t w, bool* found) {
-  if constexpr (Kv<DT>::F32) {
-    const bool bad = (w & 0x7F800000u) == 0x7F800000u;
-    *found |= bad;
-    return bad ? 0u : w;
-  } else {
-    constexpr uint32_t e = Kv<DT>::BF ? 0x7F80u : 0x7C00u;
-    const bool lo = (w & e) == e, hi = (w >> 16 & e) == e;
-    *found |= lo || hi;
-    return w & (lo ? 0xFFFF0000u : ~0u) & (hi ? 0x0000FFFFu : ~0u);
-  }
+__device__ inline bool not_finite(uint32_t w) {
+  if constexpr (Kv<DT>::F32) return (w & 0x7F800000u) == 0x7F800000u;
+  constexpr uint32_t e = Kv<DT>::BF ? 0x7F80u : 0x7C00u;
+  return (w & e) == e || (w >> 16 & e) == e;
 }
 
 // ---- segments -------------------------------------------------------------------
@@ -247,7 +250,8 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
 }
 
 // Steps of tile j: up to the last token its last row sees, and at least one, so
-// that every tile has a workgroup that writes its rows.
+// that every tile has a workgroup that writes its rows.  In the order of all units
+// kTileCost more stand for its beginning and end.
 __device__ inline int tile_steps(const Seg& g, int j, int G) {
   int p1 = g.p1;
   if (g.own) {
@@ -257,21 +261,58 @@ __device__ inline int tile_steps(const Seg& g, int j, int G) {
   return max(1, (p1 - g.p0 + kStep - 1) / kStep);
 }
 __device__ inline uint64_t seg_steps(const Seg& g, int G) {
-  if (!g.own) return (uint64_t)g.tiles * tile_steps(g, 0, G);
+  if (!g.own) return (uint64_t)g.tiles * (tile_steps(g, 0, G) + kTileCost);
   uint64_t n = 0;
-  for (int j = 0; j < g.tiles; ++j) n += tile_steps(g, j, G);
+  for (int j = 0; j < g.tiles; ++j) n += tile_steps(g, j, G) + kTileCost;
   return n;
+}
+
+// The thread's number, anew: what a tile's code derives from it is then computed for
+// each tile.  Otherwise the compiler computes all lane addresses of all tile forms
+// once, before the loop over the tiles, and keeps them in spilled registers.
+__device__ inline int this_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// What is `at` bytes behind a scalar address in global memory.
+template <class T>
+__device__ inline T global_at(const void* base, uint32_t at) {
+  typedef __attribute__((address_space(1))) const uint8_t* Bytes;
+  return *(__attribute__((address_space(1))) const T*)((Bytes)base + at);
+}
+template <class T>
+__device__ inline T stream_at(const void* base, uint32_t at) {  // not kept in the caches
+  typedef __attribute__((address_space(1))) const uint8_t* Bytes;
+  return __builtin_nontemporal_load((__attribute__((address_space(1))) const T*)((Bytes)base + at));
 }
 
 // ---- one tile --------------------------------------------------------------------
 // What a tile's products need, the same for all threads.
 struct Tile {
   const uint32_t* table;  // the lane's pages
+  const uint8_t* base;    // page 0's record of this layer and kv head
+  const float* scales;    // ... and its scales (fp8)
+  uint32_t page_bytes;    // from one page's record to the next one's
   int row0, rows;  // first row, rows (<= the tile's width)
   int h;           // kv head
   int p0, p1;      // pages of this workgroup's steps of it
   int lim_lo, lim_hi;  // tokens that its least and its most seeing row see
 };
+
+// A record that is the same for all lanes, in scalar registers.
+template <class T>
+__device__ inline T uniform(const T& x) {
+  static_assert(sizeof(T) % 4 == 0, "whole words");
+  int w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w[i] = first_lane_i(w[i]);
+  T y;
+  __builtin_memcpy(&y, w, sizeof(T));
+  return y;
+}
 
 // A segment in the order of all units.
 struct SegAt {
@@ -280,17 +321,22 @@ struct SegAt {
 };
 constexpr int kListed = 32;
 
+// FORMS: 1: 16-row tiles only, 2: up to 64 rows, 3: 128-row tiles too.
+template <int FORMS>
 struct Shared {
+  struct Kv {
+    uint8_t k[2][kStep * 4096], v[2][kStep * 4096];
+  };
+  struct None {};
   union {
-    float merge[4 * 32 * kPad];  // [wavefront][row][dim]: accumulators of wavefronts that share rows
-    struct {
-      uint8_t k[2][kStep * 4096], v[2][kStep * 4096];  // two steps' tokens, chunks swizzled
-    } kv;
+    float merge[4 * (FORMS == 1 ? 16 : 32) * kPad];  // [wavefront][row][dim]: accumulators to be joined
+    std::conditional_t<FORMS == 3, Kv, None> kv;     // two steps' tokens, chunks swizzled
   };
   float ml[4][32][2];
   int lim[kWide];  // tokens that each row sees
   int lim_lo, lim_hi;
   int odd[2];      // a step's V holds what is not finite
+  int left_out;    // the tile has pages that were left out for that
   float ks[2][kStep], vs[2][kStep];
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
   uint64_t sums[kThreads / 64];
@@ -326,22 +372,6 @@ __device__ inline uint32_t checked_page(const PageView& v, uint32_t id) {
   return 0;
 }
 
-// Adds what V holds that is not finite (left out of the product) to the rows that
-// see it.  w: the 16 tokens' weights [token][32 columns] in LDS; outputs(part) adds
-// part(dim) to each of the lane's outputs.
-template <int DT, class Outputs>
-__device__ inline void add_not_finite(const uint8_t* rec, const float* w, int col, int t0, int lim,
-                                      Outputs&& outputs) {
-  for (int t = 0; t < kPageTokens && t0 + t < lim; ++t) {
-    const float p = w[t * 32 + col];
-    outputs([&](int d) {
-      asm volatile("" ::: "memory");  // one value at a time: this is rare, its registers are not
-      const float x = v_elem<DT>(rec, t, d);
-      return finite(x) ? 0.0f : p * x;
-    });
-  }
-}
-
 // The K and V words of one page that a lane holds for the 16-column products.
 template <int DT>
 struct PageRegs {
@@ -350,32 +380,35 @@ struct PageRegs {
   float ks, vs;
 };
 
+// The address is a scalar and a lane's 32-bit offset.
 template <int DT>
-__device__ inline void load_page(const PageView& v, uint64_t rec, PageRegs<DT>& r) {
+__device__ inline void load_page(const Tile& t, int kv_heads, uint32_t page, int l, PageRegs<DT>& r) {
   using K = Kv<DT>;
-  const int l = threadIdx.x & 63, n = l & 15, grp = l >> 4;
-  const uint8_t* kp = v.pool + rec * (2u * K::HALF);
-  const u32x4* k = reinterpret_cast<const u32x4*>(kp + n * K::ROW + grp * 16);
+  const uint32_t n = l & 15, grp = l >> 4;
+  const uint8_t* kp = t.base + (uint64_t)page * t.page_bytes;
+  const uint8_t* vp = kp + K::HALF;
+  const uint32_t k_at = n * K::ROW + grp * 16, v_at = 4 * grp * K::ROW + n * (8 * K::ES);
 #pragma unroll
-  for (int w = 0; w < K::NK; ++w) r.k[w] = load_kv<true>(k + 4 * w);
-  const uint8_t* vp = kp + K::HALF + (4 * grp) * K::ROW + n * (8 * K::ES);
+  for (int w = 0; w < K::NK; ++w) r.k[w] = stream_at<u32x4>(kp, k_at + 64 * w);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int i = 0; i < 4; ++i) {
     if constexpr (K::F8) {
-      const u32x2 x = load_kv<true>(reinterpret_cast<const u32x2*>(vp + t * K::ROW));
-      r.v[t][0] = x[0], r.v[t][1] = x[1];
+      const u32x2 x = stream_at<u32x2>(vp, v_at + i * K::ROW);
+      r.v[i][0] = x[0], r.v[i][1] = x[1];
     } else {
 #pragma unroll
       for (int w = 0; w < K::VW / 4; ++w) {
-        const u32x4 x = load_kv<true>(reinterpret_cast<const u32x4*>(vp + t * K::ROW) + w);
+        const u32x4 x = stream_at<u32x4>(vp, v_at + i * K::ROW + 16 * w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.v[t][4 * w + i] = x[i];
+        for (int j = 0; j < 4; ++j) r.v[i][4 * w + j] = x[j];
       }
     }
   }
   if constexpr (K::F8) {
-    const float2 s = load_scales(v.scales + 2 * rec);
-    r.ks = s.x, r.vs = s.y;
+    int z;  // a vector load: it is counted in order with the others
+    asm("v_mov_b32 %0, 0" : "=v"(z));
+    const f32x2 s = global_at<f32x2>(t.scales + (uint64_t)page * (2u * kv_heads), z);
+    r.ks = s[0], r.vs = s[1];
   } else {
     r.ks = r.vs = 1.0f;
   }
@@ -399,25 +432,11 @@ struct Narrow {
   float m[NT], sum[NT];
   int lim[NT];
 
-  // One page.  MASKED: some row does not see all of its tokens.
+  // One page.  MASKED: some row does not see all of its tokens; false: left out,
+  // as V holds what is not finite among those that one sees.
   template <bool MASKED>
-  __device__ __forceinline__ void consume(const PageView& v, const PageRegs<DT>& r, uint64_t rec, int t0,
-                                          int lim_hi, float scale, float* weights) {
-    const int l = threadIdx.x & 63, n = l & 15, grp = l >> 4;
-    bool odd = false;
-    u32x4 k16[4];
-    if constexpr (K::F8) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const u32x2 a = e4m3x4_to_bf16(r.k[w][0]), b = e4m3x4_to_bf16(r.k[w][1]);
-        const u32x2 c = e4m3x4_to_bf16(r.k[w][2]), d = e4m3x4_to_bf16(r.k[w][3]);
-        k16[2 * w] = u32x4{a[0], a[1], b[0], b[1]};
-        k16[2 * w + 1] = u32x4{c[0], c[1], d[0], d[1]};
-      }
-    } else if constexpr (!K::F32) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) k16[w] = r.k[w];
-    }
+  __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, int lim_hi, float scale) {
+    const int grp = l >> 4;
     // V rows as operand values: 8 dims of 4 tokens
     constexpr int VD = K::F32 ? 8 : 4;
     uint32_t vv[4][VD];
@@ -432,15 +451,30 @@ struct Narrow {
       }
     }
     if constexpr (MASKED) {
+      bool odd = false;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const bool seen = t0 + 4 * grp + t < lim_hi;
-        bool bad = false;
+        const bool seen = t < lim_hi - t0 - 4 * grp;
 #pragma unroll
-        for (int i = 0; i < VD; ++i) vv[t][i] = seen ? only_finite<DT>(vv[t][i], &bad) : 0u;
-        odd |= bad && seen;
+        for (int i = 0; i < VD; ++i) {
+          odd |= seen && not_finite<DT>(vv[t][i]);
+          vv[t][i] = seen ? vv[t][i] : 0u;
+        }
       }
-      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+      if (__builtin_amdgcn_ballot_w64(odd)) return false;
+    }
+    u32x4 k16[4];
+    if constexpr (K::F8) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const u32x2 a = e4m3x4_to_bf16(r.k[w][0]), b = e4m3x4_to_bf16(r.k[w][1]);
+        const u32x2 c = e4m3x4_to_bf16(r.k[w][2]), d = e4m3x4_to_bf16(r.k[w][3]);
+        k16[2 * w] = u32x4{a[0], a[1], b[0], b[1]};
+        k16[2 * w + 1] = u32x4{c[0], c[1], d[0], d[1]};
+      }
+    } else if constexpr (!K::F32) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) k16[w] = r.k[w];
     }
     u32x2 vop[8];
     if constexpr (!K::F32) {
@@ -469,7 +503,7 @@ struct Narrow {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         x[t] = s[t] * c;
-        if (MASKED && t0 + 4 * grp + t >= lim[nt]) x[t] = -INFINITY;
+        if (MASKED && t >= lim[nt] - t0 - 4 * grp) x[t] = -INFINITY;
         top = fmaxf(top, x[t]);
       }
       top = max_over_groups(top);
@@ -490,9 +524,6 @@ struct Narrow {
 #pragma unroll
         for (int t = 0; t < 4; ++t) p[t] *= r.vs;
       }
-      if (MASKED && odd)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) weights[(4 * grp + t) * 32 + 16 * nt + n] = p[t];
       if constexpr (K::F32) {
 #pragma unroll
         for (int nb = 0; nb < 8; ++nb)
@@ -505,24 +536,13 @@ struct Narrow {
         for (int nb = 0; nb < 8; ++nb) o[nt][nb] = mma16h<K::BF>(vop[nb], pop, o[nt][nb]);
       }
     }
-    if (MASKED && odd) {
-      wave_fence();
-      const uint8_t* at = v.pool + rec * (2u * K::HALF);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        add_not_finite<DT>(at, weights, 16 * nt + n, t0, lim[nt], [&](auto&& part) {
-#pragma unroll
-          for (int nb = 0; nb < 8; ++nb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][nb][i] += part(32 * grp + 8 * i + nb);
-        });
-      wave_fence();
-    }
+    return true;
   }
 
   // The tile's steps; then sh.merge and sh.ml hold each wavefront's rows.
-  __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
-    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  template <class Sh>
+  __device__ inline void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
+    const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = l & 15, grp = l >> 4, rg = wave % RG, team = wave / RG;
     const float scale = a.scale * 1.4426950408889634f;
 #pragma unroll
@@ -549,46 +569,43 @@ struct Narrow {
         q[nt][w] = x;
       }
     }
-    float* weights = sh.merge + wave * 32 * kPad;
     // page i of this team: [p0, p1) in steps of kStep, RG of them a step
     const int count = (t.p1 - t.p0 + kStep - 1) / kStep * RG;
     auto page_no = [&](int i) { return t.p0 + kStep * (i / RG) + team * RG + i % RG; };
     uint32_t ids = 0;  // lane j: the table's entry for page 64 k + j
     auto fill_ids = [&](int i0) {
       const int p = page_no(i0 + l);
-      ids = p < t.p1 && i0 + l < count ? checked_page(v, t.table[p]) : 0u;
+      ids = p < t.p1 && i0 + l < count ? checked_page(v, global_at<uint32_t>(t.table, 4 * p)) : 0u;
     };
-    auto rec_of = [&](int i) {
-      return v.record(layer, (uint32_t)__builtin_amdgcn_readlane((int)ids, i & 63), t.h);
-    };
+    auto id_of = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)ids, i & 63); };
     if (t.p0 < t.p1) {
       fill_ids(0);
       PageRegs<DT> r[2];
-      uint64_t rec[2];
       auto fetch = [&](int i, int b) {  // past the last page its entry is 0: a page that is not used
         if ((i & 63) == 0 && i) fill_ids(i);
-        rec[b] = rec_of(i);
-        load_page<DT>(v, rec[b], r[b]);
+        load_page<DT>(t, v.H, id_of(i), l, r[b]);
       };
-      auto use = [&](int i, int b) {
-        const int p = page_no(i), t0 = p * kPageTokens;
-        if (p >= t.p1) return;
-        if (t0 + kPageTokens > t.lim_lo) consume<true>(v, r[b], rec[b], t0, t.lim_hi, scale, weights);
-        else consume<false>(v, r[b], rec[b], t0, t.lim_hi, scale, weights);
-      };
+      // pages that every row sees whole, two at a time, then the others
+      const int seen = t.lim_lo / kPageTokens - t.p0;  // such pages of all teams
+      const int mine = clampi(seen / kStep * RG + clampi(seen % kStep - team * RG, 0, RG), 0, count);
       fetch(0, 0);
-      for (int i = 0; i < count; i += 2) {
+      int i = 0;
+      for (; i + 1 < mine; i += 2) {
         fetch(i + 1, 1);
-        use(i, 0);
+        consume<false>(r[0], l, 0, 0, scale);
         fetch(i + 2, 0);
-        use(i + 1, 1);
+        consume<false>(r[1], l, 0, 0, scale);
+      }
+      for (; page_no(i) < t.p1; ++i) {
+        if (!consume<true>(r[0], l, page_no(i) * kPageTokens, t.lim_hi, scale)) sh.left_out = 1;
+        fetch(i + 1, 0);
       }
     }
     // hand over: [wavefront][row][dim]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       sum[nt] = sum_over_groups(sum[nt]);
-      float* to = sh.merge + (wave * 32 + nt * 16 + n) * kPad + 32 * grp;
+      float* to = sh.merge + (wave * 16 * NT + nt * 16 + n) * kPad + 32 * grp;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -623,12 +640,13 @@ __device__ inline void write_out(const AttendArgs& a, int64_t at, int d, const f
 
 // Joins the teams of a Narrow tile and writes its rows: to the output where they are
 // finished (`to_o` null), else as a part.
-template <int DT, int NT, int RG>
-__device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Shared& sh, float* to_ml, float* to_o) {
+template <int DT, int NT, int RG, class Sh>
+__device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Sh& sh, float* to_ml, float* to_o) {
   constexpr int TEAMS = 4 / RG, ROWS = 16 * NT * RG;
+  const int tid = this_thread();
 #pragma unroll
   for (int r0 = 0; r0 < ROWS; r0 += 16) {
-    const int row = r0 + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    const int row = r0 + tid / 16, d = tid % 16 * 8;
     if (row >= t.rows) continue;
     const int rg = row / (16 * NT), at = row % (16 * NT);
     float m = -INFINITY, sum = 0.0f, x[8] = {};
@@ -640,7 +658,7 @@ __device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Shared& 
       const int w = k * RG + rg;
       const float f = exp2_fast(sh.ml[w][at][0] - ref);
       sum += f * sh.ml[w][at][1];
-      const float* o = sh.merge + (w * 32 + at) * kPad + d;
+      const float* o = sh.merge + (w * 16 * NT + at) * kPad + d;
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] += f * o[i];
     }
@@ -696,8 +714,9 @@ struct Wide {
   float m, sum;
   int lim;
 
-  __device__ inline void run(const PageView& v, int layer, const AttendArgs& a, const Tile& t, Shared& sh) {
-    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  template <class Sh>
+  __device__ inline void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
+    const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = l & 31, h = l >> 5, row = wave * 32 + col;
     const float scale = fabsf(a.scale) * 1.4426950408889634f;
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -717,24 +736,24 @@ struct Wide {
     uint32_t ids = 0;
     auto fill_ids = [&](int s) {  // lane j: page 4 s + j
       const int p = t.p0 + kStep * s + l;
-      ids = p < t.p1 ? checked_page(v, t.table[p]) : 0u;
+      ids = p < t.p1 ? checked_page(v, global_at<uint32_t>(t.table, 4 * p)) : 0u;
     };
     Word kr[kStep], vr[kStep];
     float sc[kStep] = {};
     // thread: token tid / 16 of each page, chunk tid % 16
     const int tok = tid >> 4, chunk = tid & 15;
+    const uint32_t at_word = tid * (uint32_t)sizeof(Word);
     auto fetch = [&](int s) {
       if (s && (s & 15) == 0) fill_ids(s);
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
         if (t.p0 + kStep * s + i < t.p1) {
-          const uint64_t rec =
-              v.record(layer, (uint32_t)__builtin_amdgcn_readlane((int)ids, (kStep * s + i) & 63), t.h);
-          const Word* p = reinterpret_cast<const Word*>(v.pool + rec * (2u * K::HALF)) + tid;
-          kr[i] = p[0];
-          vr[i] = p[K::HALF / sizeof(Word)];
+          const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)ids, (kStep * s + i) & 63);
+          const uint8_t* p = t.base + (uint64_t)page * t.page_bytes;
+          kr[i] = global_at<Word>(p, at_word);
+          vr[i] = global_at<Word>(p + K::HALF, at_word);
           if constexpr (K::F8)
-            if (tid < 2) sc[i] = v.scales[2 * rec + tid];
+            if (tid < 2) sc[i] = global_at<float>(t.scales + (uint64_t)page * (2u * v.H), 4 * tid);
         }
       }
     };
@@ -758,9 +777,8 @@ struct Wide {
           const bool seen = t0 + kPageTokens * i + tok < t.lim_hi && t.p0 + kStep * s + i < t.p1;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            bool f = false;
-            x[w] = seen ? only_finite<DT>(x[w], &f) : 0u;
-            bad |= f && seen;
+            bad |= seen && not_finite<DT>(x[w]);
+            x[w] = seen ? x[w] : 0u;
           }
         }
         *reinterpret_cast<u32x4*>(sh.kv.k[b] + at_) = widen(kr[i]);
@@ -787,13 +805,13 @@ struct Wide {
       constexpr bool MASKED = decltype(masked_)::value;
       const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
       if (s + 1 < steps) fetch(s + 1);
-      const bool odd = MASKED && sh.odd[b];
+      const bool odd = MASKED && sh.odd[b];  // left out, as V holds what is not finite
       uint32_t pop[16];
       // The lane's places in this step's K and V; the others follow by flipping address
       // bits.  Opaque, so that they are not all kept in registers over the loop.
       uint32_t k_at = k_lane + (b << 14), v_at = v_lane + (b << 14);
       asm volatile("" : "+v"(k_at), "+v"(v_at));
-      if (busy) {
+      if (busy && !odd) {
         f32x16 x[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -803,6 +821,7 @@ struct Wide {
           for (int c = 0; c < 8; ++c)  // chunk 2 c + h of token 32 tt + col
             x[tt] = mma32<K::BF>(lds<u32x4>((k_at ^ c << 5) + 8192 * tt), q[c], x[tt]);
         }
+        const int mine = lim - t0 - 4 * h;  // of the lane's tokens, in steps of 4 and gaps of 4
         float c[kStep], top = -INFINITY;  // c: factor on a page's scores
 #pragma unroll
         for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * sh.ks[b][i] : scale;
@@ -810,7 +829,7 @@ struct Wide {
         for (int i = 0; i < 32; ++i) {
           float& y = reinterpret_cast<float*>(&x[i >> 4])[i & 15];
           if (K::F8) y *= c[i >> 3];
-          if (MASKED && t0 + 8 * (i >> 2) + 4 * h + (i & 3) >= lim) y = -INFINITY;
+          if (MASKED && 8 * (i >> 2) + (i & 3) >= mine) y = -INFINITY;
           top = fmaxf(top, y);
         }
         {
@@ -851,39 +870,9 @@ struct Wide {
           }
         }
       }
-      if (odd) {  // the same for all wavefronts
-        __syncthreads();  // every wavefront is done with this step's K: its room holds the weights
-        float* w = reinterpret_cast<float*>(sh.kv.k[b]) + wave * 1024;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // 32 tokens of 32 rows at a time
-          if (busy)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const uint32_t two = pop[8 * half + i / 2];
-              float x;
-              if constexpr (K::BF) x = bits_f32(i & 1 ? two & 0xFFFF0000u : two << 16);
-              else x = (float)__builtin_bit_cast(f16x2, two)[i & 1];
-              w[(8 * (i >> 2) + 4 * h + (i & 3)) * 32 + col] = x;
-            }
-          wave_fence();
-          if (busy)
-            for (int i = 0; i < 2; ++i) {
-              const int p = t.p0 + kStep * s + 2 * half + i;
-              if (p >= t.p1) break;
-              const uint64_t rec = v.record(layer, checked_page(v, t.table[p]), t.h);
-              add_not_finite<DT>(v.pool + rec * (2u * K::HALF), w + 512 * i, col, p * kPageTokens, lim,
-                                 [&](auto&& part) {
-#pragma unroll
-                                   for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                                     for (int e = 0; e < 16; ++e)
-                                       o[dt][e] += part(32 * dt + 8 * (e >> 2) + 4 * h + (e & 3));
-                                 });
-            }
-          wave_fence();
-        }
+      if (MASKED) {
         __syncthreads();
-        if (tid == 0) sh.odd[b] = 0;
+        if (odd && tid == 0) sh.odd[b] = 0, sh.left_out = 1;
       }
       if (s + 1 < steps) store(s + 1, b ^ 1);
       __syncthreads();
@@ -899,7 +888,7 @@ struct Wide {
   }
 
   __device__ inline void write(const AttendArgs& a, const Tile& t, float* to_ml, float* to_o) {
-    const int l = threadIdx.x & 63, h = l >> 5, row = (threadIdx.x >> 6) * 32 + (l & 31);
+    const int tid = this_thread(), l = tid & 63, h = l >> 5, row = (tid >> 6) * 32 + (l & 31);
     if (row >= t.rows) return;
     if (to_o) {
 #pragma unroll
@@ -933,10 +922,76 @@ struct Wide {
   }
 };
 
-// ---- the call -------------------------------------------------------------------
+// The last value of a row: two dims a lane (x, y: the sums of weighted values).
 template <int DT>
-__global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
-  __shared__ __attribute__((aligned(1024))) Shared sh;
+__device__ inline void finish_row(const AttendArgs& a, int row, int h, float m, float sum, float x, float y,
+                                  bool none) {
+  const int l = threadIdx.x & 63;
+  const float inv = none ? 0.0f : 1.0f / sum;
+  const int64_t at = row_at(a, a.os, row, h) + 2 * l;
+  if constexpr (Kv<DT>::F32) {
+    float* p = static_cast<float*>(a.out) + at;
+    p[0] = x * inv, p[1] = y * inv;
+  } else {
+    const uint32_t w = pack2<Kv<DT>::BF>(x * inv, y * inv);
+    uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+    p[0] = (uint16_t)w, p[1] = (uint16_t)(w >> 16);
+  }
+  if (a.lse && l == 0)
+    a.lse[(int64_t)(row / a.G) * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// The pages that a tile's products left out: a value that is not finite must not
+// meet the zero weight of a row that does not see it, so here each row takes only
+// the tokens it sees, one at a time, two dims a lane.  ml, o: the tile's rows as a
+// part, which this adds to.  unit: pages that are left out together.
+template <int DT>
+__device__ inline void add_left_out(const PageView& v, const AttendArgs& a, const Tile& t, int unit,
+                                                             const int* lims, float* ml, float* o) {
+  using K = Kv<DT>;
+  const int tid = this_thread(), l = tid & 63, wave = tid >> 6;
+  const float scale = a.scale * 1.4426950408889634f;
+  const int whole = max(0, t.lim_lo / kPageTokens - t.p0) / unit * unit;
+  for (int p = t.p0 + whole; p < t.p1; p += unit) {
+    bool odd = false;
+    for (int i = 0; i < unit && p + i < t.p1; ++i) {
+      const uint8_t* rec = t.base + (uint64_t)checked_page(v, t.table[p + i]) * t.page_bytes;
+      for (int e = l; e < kPageTokens * kPageDim; e += 64)
+        odd |= (p + i) * kPageTokens + e / kPageDim < t.lim_hi && !finite(v_elem<DT>(rec, e / kPageDim, e % kPageDim));
+    }
+    if (!__builtin_amdgcn_ballot_w64(odd)) continue;
+    for (int row = wave; row < t.rows; row += kThreads / 64) {
+      const int lim = lims[row];
+      const int64_t at = row_at(a, a.qs, t.row0 + row, t.h) + 2 * l;
+      const float q0 = q_elem<DT>(a.q, at), q1 = q_elem<DT>(a.q, at + 1);
+      float m = ml[2 * row], sum = ml[2 * row + 1];
+      float x = o[(int64_t)row * kPageDim + 2 * l], y = o[(int64_t)row * kPageDim + 2 * l + 1];
+      for (int tok = p * kPageTokens; tok < min(lim, min(p + unit, t.p1) * kPageTokens); ++tok) {
+        const uint64_t page = checked_page(v, t.table[tok / kPageTokens]);
+        const uint8_t* rec = t.base + page * t.page_bytes;
+        const float* sc = t.scales + page * (2u * v.H);
+        const int i = tok % kPageTokens;
+        float s = q0 * k_elem<DT>(rec, i, 2 * l) + q1 * k_elem<DT>(rec, i, 2 * l + 1);
+        for (int d = 32; d; d /= 2) s += __shfl_xor(s, d);
+        s *= K::F8 ? scale * sc[0] : scale;
+        const float top = fmaxf(m, s), f = exp2_fast(m - against(top)), w = exp2_fast(s - against(top));
+        const float wv = K::F8 ? w * sc[1] : w;
+        m = top;
+        sum = sum * f + w;
+        x = x * f + wv * v_elem<DT>(rec, i, 2 * l);
+        y = y * f + wv * v_elem<DT>(rec, i, 2 * l + 1);
+      }
+      o[(int64_t)row * kPageDim + 2 * l] = x, o[(int64_t)row * kPageDim + 2 * l + 1] = y;
+      if (l == 0) ml[2 * row] = m, ml[2 * row + 1] = sum;
+    }
+  }
+}
+
+// ---- the call -------------------------------------------------------------------
+template <int DT, int FORMS>
+__global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_attend(PageView v, int layer,
+                                                                                   AttendArgs a, Scratch ws) {
+  __shared__ __attribute__((aligned(1024))) Shared<FORMS> sh;
   const int tid = threadIdx.x, grid = gridDim.x;
   // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
   // that tiles of the same pages meet in its L2
@@ -996,7 +1051,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
   const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
   // Each thread lists those of its segments that are among the kListed from `from` on.
   auto list = [&](int from, auto first) {
-    const int s0 = min((int)threadIdx.x * per_thread, nseg), s1 = min(s0 + per_thread, nseg);
+    const int s0 = min(this_thread() * per_thread, nseg), s1 = min(s0 + per_thread, nseg);
     uint64_t at = before;
     for (int s = s0; s < s1; ++s) {
       SegAt x;
@@ -1026,16 +1081,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
   uint64_t u = u0, tile_at = 0;
   int h = -1, j = 0, group = -1;
   SegAt x;
-  auto listed = [&](int i) {  // the same for all lanes, and known to be
-    const SegAt& y = sh.list[i];
-    const int* w = reinterpret_cast<const int*>(&y.g);
-    int* to = reinterpret_cast<int*>(&x.g);
-#pragma unroll
-    for (int k = 0; k < (int)(sizeof(Seg) / 4); ++k) to[k] = first_lane_i(w[k]);
-    x.at = first_lane_u64(y.at), x.steps = first_lane_u64(y.steps);
-  };
+  auto listed = [&](int i) { x = uniform(sh.list[i]); };
   listed(0);
   while (u < u1) {
+    const int tid = this_thread();
     if (u >= x.at + x.steps * v.H) {  // the next segment
       if (++s == from + kListed) {
         __syncthreads();
@@ -1053,17 +1102,25 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
       j = 0;
     }
     int len = tile_steps(g, j, a.G);
-    while (u >= tile_at + len) {
-      tile_at += len;
+    while (u >= tile_at + len + kTileCost) {
+      tile_at += len + kTileCost;
       if (++j == g.tiles) j = 0, ++h;
       len = tile_steps(g, j, a.G);
     }
-    const int k0 = (int)(u - tile_at), k1 = (int)min((uint64_t)len, (uint64_t)k0 + (u1 - u));
+    const int k0 = first_lane_i((int)(u - tile_at));
+    if (k0 >= len) {  // the end of a tile that the workgroup before has done
+      u = tile_at + len + kTileCost;
+      continue;
+    }
+    const int k1 = first_lane_i((int)min((uint64_t)len, (uint64_t)k0 + (u1 - u)));
     Tile t;
     t.row0 = g.row0 + j * g.tile, t.rows = min(g.tile, g.rows - j * g.tile), t.h = h;
     t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
     if (t.p1 < t.p0) t.p1 = t.p0;
     t.table = v.table + (uint64_t)(g.lane < 0 ? 0 : g.lane) * v.max_pages;
+    t.page_bytes = (uint32_t)v.H * (2u * Kv<DT>::HALF);
+    t.base = v.pool + (uint64_t)layer * v.n_pages * t.page_bytes + (uint32_t)h * (2u * Kv<DT>::HALF);
+    t.scales = v.scales + ((uint64_t)layer * v.n_pages * v.H + h) * 2;
     // the workgroups that share the tile
     const int first = tile_at >= u0 ? wg : wg - (int)(((uint32_t)(u0 - tile_at) + per32 - 1) / per32);
     const int last = tile_at + len <= u1 ? wg : wg + (int)((uint32_t)(tile_at + len - 1 - u0) / per32);
@@ -1093,6 +1150,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
         __syncthreads();
       }
     }
+    if (tid == 0) sh.left_out = 0;
     if (tid < t.rows) {
       const int row = t.row0 + tid, tok = row / a.G;
       int lim = t.lim_lo;
@@ -1120,6 +1178,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
     }
     __syncthreads();
     if (!g.own && !all_seen) t.lim_lo = first_lane_i(sh.lim_lo), t.lim_hi = first_lane_i(sh.lim_hi);
+    t = uniform(t);
     float *to_ml = nullptr, *to_o = nullptr;
     if (count > 1) {
       const uint64_t part = 2 * (uint64_t)wg + (wg == first ? 1 : 0);
@@ -1130,27 +1189,49 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend(PageView v, int layer, A
       to_ml = ws.row_ml + r * 2;
       to_o = ws.row_o + r * kPageDim;
     }
-    auto narrow = [&](auto nt, auto rg) {
-      Narrow<DT, decltype(nt)::value, decltype(rg)::value> x;
-      x.run(v, layer, a, t, sh);
+    // Writes the rows by `write`; with pages left out, as a part first, in any case.
+    auto finish = [&](int unit, auto&& write) {
       __syncthreads();
-      narrow_write<DT, decltype(nt)::value, decltype(rg)::value>(a, t, sh, to_ml, to_o);
+      if (!sh.left_out) {
+        write(to_ml, to_o);
+        return;
+      }
+      // a tile that is written out ends here: the last part's place is free
+      float* ml = to_o ? to_ml : ws.part_ml + (2 * (uint64_t)wg + 1) * ws.tile_rows * 2;
+      float* o = to_o ? to_o : ws.part_o + (2 * (uint64_t)wg + 1) * ws.tile_rows * kPageDim;
+      write(ml, o);
+      __threadfence_block();
+      __syncthreads();
+      add_left_out<DT>(v, a, t, unit, sh.lim, ml, o);
+      if (to_o) return;
+      __threadfence_block();
+      __syncthreads();
+      for (int row = tid >> 6; row < t.rows; row += kThreads / 64) {
+        const float* r = o + (int64_t)row * kPageDim + 2 * (tid & 63);
+        finish_row<DT>(a, t.row0 + row, t.h, ml[2 * row], ml[2 * row + 1], r[0], r[1], sh.lim[row] <= 0);
+      }
+    };
+    auto narrow = [&](auto nt, auto rg) {
+      constexpr int NT = decltype(nt)::value, RG = decltype(rg)::value;
+      Narrow<DT, NT, RG> x;
+      x.run(v, a, t, sh);
+      finish(1, [&](float* ml, float* o) { narrow_write<DT, NT, RG>(a, t, sh, ml, o); });
     };
     std::integral_constant<int, 1> one;
-    if constexpr (Kv<DT>::F32) {
+    std::integral_constant<int, 2> pair;
+    if constexpr (FORMS == 1) {
       narrow(one, one);
     } else {
-      std::integral_constant<int, 2> two_;
       if (g.tile == 16) narrow(one, one);
-      else if (g.tile == 32) narrow(two_, one);
-      else if (g.tile == 64) narrow(two_, two_);
-      else {
+      else if (g.tile == 32) narrow(pair, one);
+      else if (FORMS == 2 || g.tile == 64) narrow(pair, pair);
+      else if constexpr (FORMS == 3) {
         Wide<DT> x;
-        x.run(v, layer, a, t, sh);
-        x.write(a, t, to_ml, to_o);
+        x.run(v, a, t, sh);
+        finish(kStep, [&](float* ml, float* o) { x.write(a, t, ml, o); });
       }
     }
-    u += k1 - k0;
+    u = k1 == len ? tile_at + len + kTileCost : u1;
   }
 }
 
@@ -1203,19 +1284,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs
     x += f * w.x;
     y += f * w.y;
   }
-  const bool none = !(own.has & 2);
-  const float inv = none ? 0.0f : 1.0f / sum;
-  const int64_t at = row_at(a, a.os, row, h) + 2 * l;
-  if constexpr (Kv<DT>::F32) {
-    float* p = static_cast<float*>(a.out) + at;
-    p[0] = x * inv, p[1] = y * inv;
-  } else {
-    const uint32_t w = pack2<Kv<DT>::BF>(x * inv, y * inv);
-    uint16_t* p = static_cast<uint16_t*>(a.out) + at;
-    p[0] = (uint16_t)w, p[1] = (uint16_t)(w >> 16);
-  }
-  if (a.lse && l == 0)
-    a.lse[(int64_t)tok * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+  finish_row<DT>(a, row, h, m, sum, x, y, !(own.has & 2));
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1235,9 +1304,16 @@ int check_attend(const ferry_pages* p, const ferry_attend* a, PageView* v) {
 
 uint64_t up256(uint64_t x) { return (x + 255) & ~255ull; }
 
+// The tile forms a call may need: a segment has at most the rows of the whole batch,
+// without groups and with one token per request those of one token.
+int attend_forms(const ferry_pages* p, const ferry_attend* a) {
+  const int64_t G = a->q_heads / p->kv_heads, rows = a->n_groups || a->q_start ? a->n_tokens * G : G;
+  return p->dtype == FERRY_F32 || rows <= 16 ? 1 : rows <= 64 ? 2 : 3;
+}
+
 // Workgroups of a call, and its scratch at `base` (null: sizes only).
 int plan_attend(const ferry_pages* p, const ferry_attend* a, uint8_t* base, Scratch* ws, uint64_t* bytes) {
-  const int grid = 2 * gpu_cus(p->device);
+  const int grid = (attend_forms(p, a) == 1 ? kNarrowPerCu : 2) * gpu_cus(p->device);
   const uint64_t rows = (uint64_t)a->n_tokens * (a->q_heads / p->kv_heads), H = p->kv_heads;
   const uint64_t tile = p->dtype == FERRY_F32 ? 16 : std::min<uint64_t>(kWide, rows);
   uint64_t at = 0;
@@ -1258,8 +1334,13 @@ int plan_attend(const ferry_pages* p, const ferry_attend* a, uint8_t* base, Scra
 }
 
 template <int DT>
-void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int grid, hipStream_t s) {
-  k_attend<DT><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int forms, int grid,
+                   hipStream_t s) {
+  if (forms == 1) k_attend<DT, 1><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+  if constexpr (DT != FERRY_F32) {
+    if (forms == 2) k_attend<DT, 2><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+    if (forms == 3) k_attend<DT, 3><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+  }
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
   k_attend_join<DT><<<(unsigned)((all + 3) / 4), kThreads, 0, s>>>(v, a, ws, grid);
 }
@@ -1308,10 +1389,11 @@ int ferry_pages_attend(const ferry_pages* p, int32_t layer, const ferry_attend* 
                  a->shared, a->q, a->out, a->lse, {a->q_stride[0], a->q_stride[1]},
                  {a->out_stride[0], a->out_stride[1]}, low % 16 == 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, grid, s);
-    else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, grid, s);
-    else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, grid, s);
-    else launch_attend<FERRY_FP8_E4M3>(v, layer, d, ws, grid, s);
+    const int forms = attend_forms(p, a);
+    if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, forms, grid, s);
+    else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, forms, grid, s);
+    else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, forms, grid, s);
+    else launch_attend<FERRY_FP8_E4M3>(v, layer, d, ws, forms, grid, s);
     return launched("ferry_pages_attend");
   });
 }

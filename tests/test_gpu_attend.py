@@ -253,12 +253,17 @@ def test_values_that_later_rows_see(dt, new, G):
     c.p.pool[0, page, 1, 0, at % T, 3] = float("nan")
     out = c.run()[0]
     first = new - 3  # rows from here on see it
-    assert torch.equal(out[:first], plain[:first]) and torch.equal(out[new:], plain[new:])
+    assert torch.all(torch.isfinite(out[:first])) and torch.equal(out[new:], plain[new:])
     tail = out[first:new]
     assert torch.all(torch.isnan(tail[:, :G, 5])) and torch.all(tail[:, :G, 77] == float("inf"))
     assert torch.all(torch.isnan(tail[:, G:]))
-    rest = [d for d in range(D) if d not in (5, 77)]
-    assert torch.equal(tail[:, :G][..., rest], plain[first:new, :G][..., rest])
+    # Everything else is what a finite value there gives, within the tolerance above
+    # (both are that near to the formula): the token's page may be summed in another
+    # order, for the rows before it too.
+    c.p.pool[0, page, 0, 1, at % T, 5] = c.p.pool[0, page, 0, 1, at % T, 77] = 0.0
+    c.p.pool[0, page, 1, 0, at % T, 3] = 0.0
+    fine, lse = c.run()
+    c.check(torch.where(torch.isfinite(out), out, fine), lse)
 
 
 def test_requests_without_a_lane_and_rows_behind_the_last():
