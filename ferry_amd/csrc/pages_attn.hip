@@ -55,7 +55,6 @@ constexpr float kRaise = 8.0f;     // log2 of the largest weight between raises 
 constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
 constexpr int kPad = 132;          // floats per row of the merge buffer
 constexpr int kNarrowPerCu = 2;    // workgroups per CU where all tiles have 16 rows (else 2)
-constexpr int kTileCost = 2;       // what a tile costs beside its steps, in steps
 
 struct AttendArgs {
   int n_req, n_tokens, n_groups, Hq, G;
@@ -212,8 +211,19 @@ __device__ inline int len_of(const PageView& v, int lane) {
   return lane < 0 ? 0 : clampi(v.len[lane], 0, v.max_pages * kPageTokens);
 }
 
+// Pages that the requests [b, e) of a group attend to together: none where they have
+// a widest tile's rows each, and would read the pages once per tile in any case.  Alone,
+// their rows have one segment and need no join.
+template <int DT>
+__device__ inline int group_pages(const PageView& v, const AttendArgs& a, int b, int e, int shared) {
+  constexpr int kRows = Kv<DT>::F32 ? 16 : kWide;
+  const int64_t rows = (int64_t)(token_of(a, e) - token_of(a, b)) * a.G;
+  return rows >= (int64_t)kRows * (e - b) ? 0 : clampi(shared, 0, v.max_pages);
+}
+
 // Shared pages of request r: those of the last group that starts at or before it,
 // if that has not ended.
+template <int DT>
 __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int r) {
   if (a.n_groups == 0 || gs[0] > r) return 0;
   int lo = 0, hi = a.n_groups - 1;
@@ -221,7 +231,8 @@ __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const in
     const int mid = (lo + hi + 1) >> 1;
     if (gs[mid] <= r) lo = mid; else hi = mid - 1;
   }
-  return r < gs[lo + 1] ? clampi(gp[lo], 0, v.max_pages) : 0;
+  const int b = clampi(gs[lo], 0, a.n_req), e = clampi(gs[lo + 1], b, a.n_req);
+  return r < e ? group_pages<DT>(v, a, b, e, gp[lo]) : 0;
 }
 
 // Segment s: groups first, then requests.  gs, gp: the groups' offsets and pages.
@@ -230,7 +241,7 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
   Seg g;
   if (s < a.n_groups) {
     const int b = clampi(gs[s], 0, a.n_req), e = clampi(gs[s + 1], b, a.n_req);
-    g.own = 0, g.req = s, g.p0 = 0, g.p1 = clampi(gp[s], 0, v.max_pages);
+    g.own = 0, g.req = s, g.p0 = 0, g.p1 = group_pages<DT>(v, a, b, e, gp[s]);
     g.lane = -1, g.base = g.len = 0;
     for (int r = b; r < e && g.lane < 0; ++r) g.lane = lane_of(v, a, r);
     const int t0 = token_of(a, b), t1 = max(t0, token_of(a, e));
@@ -241,7 +252,7 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
     g.own = 1, g.req = r, g.lane = lane_of(v, a, r), g.len = len_of(v, g.lane);
     g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G;
     g.base = g.len - (t1 - t0) + 1;
-    g.p0 = g.lane < 0 ? 0 : shared_of(v, a, gs, gp, r);
+    g.p0 = g.lane < 0 ? 0 : shared_of<DT>(v, a, gs, gp, r);
     g.p1 = max(g.p0, pages_of(g.len));
   }
   g.tile = tile_rows<DT>(g.rows);
@@ -250,8 +261,7 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
 }
 
 // Steps of tile j: up to the last token its last row sees, and at least one, so
-// that every tile has a workgroup that writes its rows.  In the order of all units
-// kTileCost more stand for its beginning and end.
+// that every tile has a workgroup that writes its rows.
 __device__ inline int tile_steps(const Seg& g, int j, int G) {
   int p1 = g.p1;
   if (g.own) {
@@ -260,10 +270,19 @@ __device__ inline int tile_steps(const Seg& g, int j, int G) {
   }
   return max(1, (p1 - g.p0 + kStep - 1) / kStep);
 }
-__device__ inline uint64_t seg_steps(const Seg& g, int G) {
-  if (!g.own) return (uint64_t)g.tiles * (tile_steps(g, 0, G) + kTileCost);
+// Units of work: step_units() for a step, tile_units() for a tile's beginning and end.
+// Step i of a tile belongs to the workgroup whose run holds the first of its units.
+__device__ inline int step_units(const Seg& g) { return g.tile == kWide ? 3 : 2; }
+__device__ inline int tile_units(const Seg& g) { return g.tile == kWide ? 9 : 4; }
+constexpr int kMostStepUnits = 3;
+__device__ inline int tile_work(const Seg& g, int j, int G) {
+  return tile_steps(g, j, G) * step_units(g) + tile_units(g);
+}
+// ... of all tiles of a segment, per kv head
+__device__ inline uint64_t seg_work(const Seg& g, int G) {
+  if (!g.own) return (uint64_t)g.tiles * tile_work(g, 0, G);
   uint64_t n = 0;
-  for (int j = 0; j < g.tiles; ++j) n += tile_steps(g, j, G) + kTileCost;
+  for (int j = 0; j < g.tiles; ++j) n += tile_work(g, j, G);
   return n;
 }
 
@@ -317,7 +336,7 @@ __device__ inline T uniform(const T& x) {
 // A segment in the order of all units.
 struct SegAt {
   Seg g;
-  uint64_t at, steps;  // its first unit; steps of all its tiles (per kv head)
+  uint64_t at, work;  // its first unit; units of all its tiles (per kv head)
 };
 constexpr int kListed = 32;
 
@@ -541,7 +560,7 @@ struct Narrow {
 
   // The tile's steps; then sh.merge and sh.ml hold each wavefront's rows.
   template <class Sh>
-  __device__ inline void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
+  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
     const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = l & 15, grp = l >> 4, rg = wave % RG, team = wave / RG;
     const float scale = a.scale * 1.4426950408889634f;
@@ -581,7 +600,7 @@ struct Narrow {
     if (t.p0 < t.p1) {
       fill_ids(0);
       PageRegs<DT> r[2];
-      auto fetch = [&](int i, int b) {  // past the last page its entry is 0: a page that is not used
+      auto fetch = [&](int i, int b) __attribute__((always_inline)) {  // past the last page its entry is 0: a page that is not used
         if ((i & 63) == 0 && i) fill_ids(i);
         load_page<DT>(t, v.H, id_of(i), l, r[b]);
       };
@@ -641,7 +660,7 @@ __device__ inline void write_out(const AttendArgs& a, int64_t at, int d, const f
 // Joins the teams of a Narrow tile and writes its rows: to the output where they are
 // finished (`to_o` null), else as a part.
 template <int DT, int NT, int RG, class Sh>
-__device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Sh& sh, float* to_ml, float* to_o) {
+__device__ __forceinline__ void narrow_write(const AttendArgs& a, const Tile& t, Sh& sh, float* to_ml, float* to_o) {
   constexpr int TEAMS = 4 / RG, ROWS = 16 * NT * RG;
   const int tid = this_thread();
 #pragma unroll
@@ -667,7 +686,7 @@ __device__ inline void narrow_write(const AttendArgs& a, const Tile& t, Sh& sh, 
       write_out<DT>(a, row_at(a, a.os, t.row0 + row, t.h), d, x, none ? 0.0f : 1.0f / sum);
       if (a.lse && d == 0) {
         const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
-        a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+        a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
       }
     } else {
 #pragma unroll
@@ -715,7 +734,7 @@ struct Wide {
   int lim;
 
   template <class Sh>
-  __device__ inline void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
+  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
     const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = l & 31, h = l >> 5, row = wave * 32 + col;
     const float scale = fabsf(a.scale) * 1.4426950408889634f;
@@ -743,7 +762,7 @@ struct Wide {
     // thread: token tid / 16 of each page, chunk tid % 16
     const int tok = tid >> 4, chunk = tid & 15;
     const uint32_t at_word = tid * (uint32_t)sizeof(Word);
-    auto fetch = [&](int s) {
+    auto fetch = [&](int s) __attribute__((always_inline)) {
       if (s && (s & 15) == 0) fill_ids(s);
 #pragma unroll
       for (int i = 0; i < kStep; ++i) {
@@ -765,7 +784,7 @@ struct Wide {
         return w;
       }
     };
-    auto store = [&](int s, int b) {
+    auto store = [&](int s, int b) __attribute__((always_inline)) {
       const int t0 = (t.p0 + kStep * s) * kPageTokens;
       const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
       bool bad = false;
@@ -801,7 +820,7 @@ struct Wide {
     store(0, 0);
     __syncthreads();
     // One step; MASKED: some row does not see all of its tokens.
-    auto step = [&](auto masked_, int s) {
+    auto step = [&](auto masked_, int s) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked_)::value;
       const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
       if (s + 1 < steps) fetch(s + 1);
@@ -827,9 +846,10 @@ struct Wide {
         for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * sh.ks[b][i] : scale;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          float& y = reinterpret_cast<float*>(&x[i >> 4])[i & 15];
+          float y = x[i >> 4][i & 15];
           if (K::F8) y *= c[i >> 3];
           if (MASKED && 8 * (i >> 2) + (i & 3) >= mine) y = -INFINITY;
+          x[i >> 4][i & 15] = y;
           top = fmaxf(top, y);
         }
         {
@@ -887,7 +907,7 @@ struct Wide {
     }
   }
 
-  __device__ inline void write(const AttendArgs& a, const Tile& t, float* to_ml, float* to_o) {
+  __device__ __forceinline__ void write(const AttendArgs& a, const Tile& t, float* to_ml, float* to_o) {
     const int tid = this_thread(), l = tid & 63, h = l >> 5, row = (tid >> 6) * 32 + (l & 31);
     if (row >= t.rows) return;
     if (to_o) {
@@ -917,14 +937,14 @@ struct Wide {
       }
     if (a.lse && h == 0) {
       const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
-      a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+      a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
     }
   }
 };
 
 // The last value of a row: two dims a lane (x, y: the sums of weighted values).
 template <int DT>
-__device__ inline void finish_row(const AttendArgs& a, int row, int h, float m, float sum, float x, float y,
+__device__ __forceinline__ void finish_row(const AttendArgs& a, int row, int h, float m, float sum, float x, float y,
                                   bool none) {
   const int l = threadIdx.x & 63;
   const float inv = none ? 0.0f : 1.0f / sum;
@@ -938,7 +958,7 @@ __device__ inline void finish_row(const AttendArgs& a, int row, int h, float m, 
     p[0] = (uint16_t)w, p[1] = (uint16_t)(w >> 16);
   }
   if (a.lse && l == 0)
-    a.lse[(int64_t)(row / a.G) * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+    a.lse[(int64_t)(row / a.G) * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 // The pages that a tile's products left out: a value that is not finite must not
@@ -946,7 +966,7 @@ __device__ inline void finish_row(const AttendArgs& a, int row, int h, float m, 
 // the tokens it sees, one at a time, two dims a lane.  ml, o: the tile's rows as a
 // part, which this adds to.  unit: pages that are left out together.
 template <int DT>
-__device__ inline void add_left_out(const PageView& v, const AttendArgs& a, const Tile& t, int unit,
+__device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs& a, const Tile& t, int unit,
                                                              const int* lims, float* ml, float* o) {
   using K = Kv<DT>;
   const int tid = this_thread(), l = tid & 63, wave = tid >> 6;
@@ -1011,11 +1031,11 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
             s1 = min(s0 + per_thread, nseg);
   uint64_t mine = 0;
   Seg kept;  // the thread's only segment, where it has one
-  uint64_t kept_steps = 0;
+  uint64_t kept_work = 0;
   for (int s = s0; s < s1; ++s) {
     kept = segment<DT>(v, a, gs, gp, s);
-    kept_steps = seg_steps(kept, a.G);
-    mine += kept_steps * v.H;
+    kept_work = seg_work(kept, a.G);
+    mine += kept_work * v.H;
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
       if (kept.own) {
@@ -1045,22 +1065,23 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
   }
   before -= mine;
   total = first_lane_u64(total);
-  const uint64_t per = first_lane_u64((total + grid - 1) / grid);
+  // no run is shorter than a step, so that each one within a tile begins one
+  const uint64_t per = max((uint64_t)kMostStepUnits, first_lane_u64((total + grid - 1) / grid));
   const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
   if (u0 >= u1) return;
   const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
   // Each thread lists those of its segments that are among the kListed from `from` on.
-  auto list = [&](int from, auto first) {
+  auto list = [&](int from, auto first) __attribute__((always_inline)) {
     const int s0 = min(this_thread() * per_thread, nseg), s1 = min(s0 + per_thread, nseg);
     uint64_t at = before;
     for (int s = s0; s < s1; ++s) {
       SegAt x;
       const bool have = decltype(first)::value && per_thread == 1;
       x.g = have ? kept : segment<DT>(v, a, gs, gp, s);
-      x.steps = have ? kept_steps : seg_steps(x.g, a.G);
+      x.work = have ? kept_work : seg_work(x.g, a.G);
       x.at = at;
       if (s >= from && s < from + kListed) sh.list[s - from] = x;
-      at += x.steps * v.H;
+      at += x.work * v.H;
     }
     __syncthreads();
   };
@@ -1069,7 +1090,7 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
     int s = s0;
     if (per_thread > 1)
       for (;; ++s) {
-        at += seg_steps(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+        at += seg_work(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
         if (u0 < at) break;
       }
     sh.seg = s;
@@ -1085,7 +1106,7 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
   listed(0);
   while (u < u1) {
     const int tid = this_thread();
-    if (u >= x.at + x.steps * v.H) {  // the next segment
+    if (u >= x.at + x.work * v.H) {  // the next segment
       if (++s == from + kListed) {
         __syncthreads();
         from = s;
@@ -1097,22 +1118,22 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
     }
     const Seg& g = x.g;
     if (h < 0) {
-      h = u == x.at ? 0 : (int)((u - x.at) / x.steps);
-      tile_at = x.at + h * x.steps;  // unit of the tile's first step
+      h = u == x.at ? 0 : (int)((u - x.at) / x.work);
+      tile_at = x.at + h * x.work;  // unit of the tile's first step
       j = 0;
     }
-    int len = tile_steps(g, j, a.G);
-    while (u >= tile_at + len + kTileCost) {
-      tile_at += len + kTileCost;
+    int work = tile_work(g, j, a.G);
+    while (u >= tile_at + work) {
+      tile_at += work;
       if (++j == g.tiles) j = 0, ++h;
-      len = tile_steps(g, j, a.G);
+      work = tile_work(g, j, a.G);
     }
-    const int k0 = first_lane_i((int)(u - tile_at));
-    if (k0 >= len) {  // the end of a tile that the workgroup before has done
-      u = tile_at + len + kTileCost;
-      continue;
-    }
-    const int k1 = first_lane_i((int)min((uint64_t)len, (uint64_t)k0 + (u1 - u)));
+    // this workgroup's steps [k0, k1) of the tile's `len`
+    const int per_step = step_units(g), len = first_lane_i(tile_steps(g, j, a.G));
+    const int k0 = first_lane_i(((int)(u - tile_at) + per_step - 1) / per_step);
+    const int k1 = first_lane_i((int)min((uint64_t)len, (u1 - tile_at + per_step - 1) / per_step));
+    u = tile_at + work;
+    if (k0 >= k1) continue;  // the workgroup before has done them all
     Tile t;
     t.row0 = g.row0 + j * g.tile, t.rows = min(g.tile, g.rows - j * g.tile), t.h = h;
     t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
@@ -1123,7 +1144,8 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
     t.scales = v.scales + ((uint64_t)layer * v.n_pages * v.H + h) * 2;
     // the workgroups that share the tile
     const int first = tile_at >= u0 ? wg : wg - (int)(((uint32_t)(u0 - tile_at) + per32 - 1) / per32);
-    const int last = tile_at + len <= u1 ? wg : wg + (int)((uint32_t)(tile_at + len - 1 - u0) / per32);
+    const uint64_t end = tile_at + (uint32_t)(len - 1) * per_step;  // the last step's unit
+    const int last = end < u1 ? wg : wg + (int)((uint32_t)(end - u0) / per32);
     const int count = last - first + 1;
     const bool two = g.own ? a.n_groups && g.p0 > 0 : true;
     __syncthreads();  // the last tile's rows are written
@@ -1190,7 +1212,7 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
       to_o = ws.row_o + r * kPageDim;
     }
     // Writes the rows by `write`; with pages left out, as a part first, in any case.
-    auto finish = [&](int unit, auto&& write) {
+    auto finish = [&](int unit, auto&& write) __attribute__((always_inline)) {
       __syncthreads();
       if (!sh.left_out) {
         write(to_ml, to_o);
@@ -1211,11 +1233,11 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
         finish_row<DT>(a, t.row0 + row, t.h, ml[2 * row], ml[2 * row + 1], r[0], r[1], sh.lim[row] <= 0);
       }
     };
-    auto narrow = [&](auto nt, auto rg) {
+    auto narrow = [&](auto nt, auto rg) __attribute__((always_inline)) {
       constexpr int NT = decltype(nt)::value, RG = decltype(rg)::value;
       Narrow<DT, NT, RG> x;
       x.run(v, a, t, sh);
-      finish(1, [&](float* ml, float* o) { narrow_write<DT, NT, RG>(a, t, sh, ml, o); });
+      finish(1, [&](float* ml, float* o) __attribute__((always_inline)) { narrow_write<DT, NT, RG>(a, t, sh, ml, o); });
     };
     std::integral_constant<int, 1> one;
     std::integral_constant<int, 2> pair;
@@ -1228,63 +1250,85 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
       else if constexpr (FORMS == 3) {
         Wide<DT> x;
         x.run(v, a, t, sh);
-        finish(kStep, [&](float* ml, float* o) { x.write(a, t, ml, o); });
+        finish(kStep, [&](float* ml, float* o) __attribute__((always_inline)) { x.write(a, t, ml, o); });
       }
     }
-    u = k1 == len ? tile_at + len + kTileCost : u1;
   }
 }
 
-// Rows with parts: a wavefront each, two dims a lane.  Parts in the order of their
-// pages, the shared ones first.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid) {
-  const int l = threadIdx.x & 63;
-  const uint64_t rows = (uint64_t)a.n_tokens * a.G, all = rows * v.H;
-  const uint64_t r = (uint64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (r >= all) return;
-  const int h = (int)(r / rows), row = (int)(r % rows), tok = row / a.G;
-  if (tok < token_of(a, 0) || tok >= token_of(a, a.n_req)) return;
-  const Where own = ws.where[((uint64_t)v.H + h) * rows + row];
-  if (own.count == 0) return;
-  Where part[2];
-  part[1] = own;
-  part[0] = own.has & 1 ? ws.where[(uint64_t)h * rows + row] : Where{0, 0, 0, 0};
-  int n[2];
+// Joins the parts of the rows that have some, in the order of their pages, the shared
+// ones first; two dims a lane.  A row's parts are shared out to WAVES wavefronts
+// (4 where the rows are few and their parts may be many, else 1).  Bound by the
+// latency of three dependent reads (where, part, write); eight parts' reads are on
+// their way at once.
+template <int DT, int WAVES>
+__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid, int each) {
+  constexpr int kAhead = 8;
+  __shared__ float got[WAVES > 1 ? 4 : 1][kPageDim + 2];
+  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t rows = (uint32_t)a.n_tokens * a.G;
+  const uint64_t all = (uint64_t)rows * v.H;
+  const uint64_t r0 = WAVES > 1 ? blockIdx.x : ((uint64_t)blockIdx.x * (kThreads / 64) + wave) * each;
+  const uint64_t r1 = WAVES > 1 ? r0 + 1 : min(all, r0 + each);
+  const int tok0 = token_of(a, 0), tok1 = token_of(a, a.n_req);
+  for (uint64_t r = r0; r < r1; ++r) {
+    const uint32_t h = (uint32_t)(r / rows), row = (uint32_t)(r % rows);
+    const int tok = row / a.G;
+    if (tok < tok0 || tok >= tok1) continue;
+    const Where own = uniform(ws.where[((uint64_t)v.H + h) * rows + row]);
+    if (own.count == 0) continue;
+    Where part[2] = {Where{0, 0, 0, 0}, own};
+    if (own.has & 1) part[0] = uniform(ws.where[(uint64_t)h * rows + row]);
+    int n[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {  // stay in the scratch, whatever the offsets were
-    part[k].first = clampi(part[k].first, 0, grid - 1);
-    part[k].row = clampi(part[k].row, 0, ws.tile_rows - 1);
-    n[k] = clampi(part[k].count, 0, grid - part[k].first);
-  }
-  auto place = [&](int i, const float** o) -> const float* {
-    const int k = i >= n[0], at = i - (k ? n[0] : 0);
-    if (n[k] == 1 && own.has & 1) {
-      const uint64_t p = ((uint64_t)k * v.H + h) * rows + row;
-      *o = ws.row_o + p * kPageDim;
-      return ws.row_ml + p * 2;
+    for (int k = 0; k < 2; ++k) {  // stay in the scratch, whatever the offsets were
+      part[k].first = clampi(part[k].first, 0, grid - 1);
+      part[k].row = clampi(part[k].row, 0, ws.tile_rows - 1);
+      n[k] = clampi(part[k].count, 0, grid - part[k].first);
     }
-    const uint64_t p = (2 * (uint64_t)(part[k].first + at) + (at == 0 ? 1 : 0)) * ws.tile_rows + part[k].row;
-    *o = ws.part_o + p * kPageDim;
-    return ws.part_ml + p * 2;
-  };
-  const int parts = n[0] + n[1];
-  float m = -INFINITY;
-  const float* o;
-  for (int i = l; i < parts; i += 64) m = fmaxf(m, place(i, &o)[0]);
+    const int parts = n[0] + n[1];
+    float m = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+    for (int i0 = WAVES > 1 ? wave : 0; i0 < parts; i0 += kAhead * WAVES) {
+      float2 ml[kAhead], o[kAhead];
 #pragma unroll
-  for (int d = 32; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-  const float ref = against(m);
-  float sum = 0.0f, x = 0.0f, y = 0.0f;
-  for (int i = 0; i < parts; ++i) {
-    const float* ml = place(i, &o);
-    const float f = exp2_fast(ml[0] - ref);
-    const float2 w = *reinterpret_cast<const float2*>(o + 2 * l);
-    sum += f * ml[1];
-    x += f * w.x;
-    y += f * w.y;
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = min(i0 + j * WAVES, parts - 1), k = i >= n[0], at = i - (k ? n[0] : 0);
+        const bool whole = n[k] == 1 && (own.has & 1);  // in the row's own place
+        const uint64_t p = whole ? ((uint64_t)k * v.H + h) * rows + row
+                                 : (2 * (uint64_t)(part[k].first + at) + (at == 0 ? 1 : 0)) * ws.tile_rows + part[k].row;
+        ml[j] = reinterpret_cast<const float2*>(whole ? ws.row_ml : ws.part_ml)[p];
+        o[j] = reinterpret_cast<const float2*>((whole ? ws.row_o : ws.part_o) + p * kPageDim)[l];
+      }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * WAVES < parts) top = fmaxf(top, ml[j].x);
+      const float ref = against(top), f = exp2_fast(m - ref);
+      m = top, sum *= f, x *= f, y *= f;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float w = i0 + j * WAVES < parts ? exp2_fast(ml[j].x - ref) : 0.0f;
+        if (i0 + j * WAVES < parts) sum += w * ml[j].y, x += w * o[j].x, y += w * o[j].y;
+      }
+    }
+    if constexpr (WAVES > 1) {
+      got[wave][2 * l] = x, got[wave][2 * l + 1] = y;
+      if (l == 0) got[wave][kPageDim] = m, got[wave][kPageDim + 1] = sum;
+      __syncthreads();
+      if (wave) return;
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) top = fmaxf(top, got[k][kPageDim]);
+      const float ref = against(top);
+      sum = x = y = 0.0f, m = top;
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) {
+        const float w = exp2_fast(got[k][kPageDim] - ref);
+        sum += w * got[k][kPageDim + 1], x += w * got[k][2 * l], y += w * got[k][2 * l + 1];
+      }
+    }
+    finish_row<DT>(a, row, h, m, sum, x, y, !(own.has & 2));
   }
-  finish_row<DT>(a, row, h, m, sum, x, y, !(own.has & 2));
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1341,8 +1385,16 @@ void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scra
     if (forms == 2) k_attend<DT, 2><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
     if (forms == 3) k_attend<DT, 3><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
   }
+  // Four wavefronts per row where the rows do not fill the GPU with one; with many
+  // rows (prompts, most of them finished by one workgroup) a wavefront looks at several.
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
-  k_attend_join<DT><<<(unsigned)((all + 3) / 4), kThreads, 0, s>>>(v, a, ws, grid);
+  if (all <= (uint64_t)grid) {
+    k_attend_join<DT, 4><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid, 1);
+  } else {
+    const int each = (int)std::min<uint64_t>(64, (all + 16ull * grid - 1) / (16ull * grid));
+    const uint64_t waves = (all + each - 1) / each;
+    k_attend_join<DT, 1><<<(unsigned)((waves + 3) / 4), kThreads, 0, s>>>(v, a, ws, grid, each);
+  }
 }
 
 }  // namespace
