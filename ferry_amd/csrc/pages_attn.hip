@@ -1257,78 +1257,92 @@ __global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_att
 }
 
 // Joins the parts of the rows that have some, in the order of their pages, the shared
-// ones first; two dims a lane.  A row's parts are shared out to WAVES wavefronts
-// (4 where the rows are few and their parts may be many, else 1).  Bound by the
-// latency of three dependent reads (where, part, write); eight parts' reads are on
-// their way at once.
-template <int DT, int WAVES>
-__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid, int each) {
-  constexpr int kAhead = 8;
-  __shared__ float got[WAVES > 1 ? 4 : 1][kPageDim + 2];
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// ones first.  16 lanes take a row, 8 dims each; SPLIT such teams share out a row's
+// parts (16, a workgroup, where the rows are few and their parts may be many, else 1).
+// Bound by the latency of three dependent reads (where, part, write), so many rows are
+// in flight and four parts of each.
+template <int DT, int SPLIT>
+__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid) {
+  constexpr int kTeams = kThreads / 16, kAhead = 4;
+  __shared__ float got[SPLIT > 1 ? kTeams : 1][kPad];
+  const int team = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
   const uint32_t rows = (uint32_t)a.n_tokens * a.G;
   const uint64_t all = (uint64_t)rows * v.H;
-  const uint64_t r0 = WAVES > 1 ? blockIdx.x : ((uint64_t)blockIdx.x * (kThreads / 64) + wave) * each;
-  const uint64_t r1 = WAVES > 1 ? r0 + 1 : min(all, r0 + each);
-  const int tok0 = token_of(a, 0), tok1 = token_of(a, a.n_req);
-  for (uint64_t r = r0; r < r1; ++r) {
-    const uint32_t h = (uint32_t)(r / rows), row = (uint32_t)(r % rows);
-    const int tok = row / a.G;
-    if (tok < tok0 || tok >= tok1) continue;
-    const Where own = uniform(ws.where[((uint64_t)v.H + h) * rows + row]);
-    if (own.count == 0) continue;
-    Where part[2] = {Where{0, 0, 0, 0}, own};
-    if (own.has & 1) part[0] = uniform(ws.where[(uint64_t)h * rows + row]);
-    int n[2];
+  const uint64_t r = SPLIT > 1 ? blockIdx.x : (uint64_t)blockIdx.x * kTeams + team;
+  if (r >= all) return;
+  const uint32_t h = (uint32_t)(r / rows), row = (uint32_t)(r % rows);
+  const int tok = row / a.G;
+  if (tok < token_of(a, 0) || tok >= token_of(a, a.n_req)) return;
+  const Where own = ws.where[all + r];
+  if (own.count == 0) return;
+  Where part[2] = {Where{0, 0, 0, 0}, own};
+  if (own.has & 1) part[0] = ws.where[r];
+  int n[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {  // stay in the scratch, whatever the offsets were
-      part[k].first = clampi(part[k].first, 0, grid - 1);
-      part[k].row = clampi(part[k].row, 0, ws.tile_rows - 1);
-      n[k] = clampi(part[k].count, 0, grid - part[k].first);
-    }
-    const int parts = n[0] + n[1];
-    float m = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
-    for (int i0 = WAVES > 1 ? wave : 0; i0 < parts; i0 += kAhead * WAVES) {
-      float2 ml[kAhead], o[kAhead];
+  for (int k = 0; k < 2; ++k) {  // stay in the scratch, whatever the offsets were
+    part[k].first = clampi(part[k].first, 0, grid - 1);
+    part[k].row = clampi(part[k].row, 0, ws.tile_rows - 1);
+    n[k] = clampi(part[k].count, 0, grid - part[k].first);
+  }
+  const int parts = n[0] + n[1];
+  float m = -INFINITY, sum = 0.0f, x[8] = {};
+  for (int i0 = SPLIT > 1 ? team : 0; i0 < parts; i0 += kAhead * SPLIT) {
+    float2 ml[kAhead];
+    f32x4 lo[kAhead], hi[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int i = min(i0 + j * WAVES, parts - 1), k = i >= n[0], at = i - (k ? n[0] : 0);
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * SPLIT, k = i >= n[0], at = i - (k ? n[0] : 0);
+      if (i < parts) {
         const bool whole = n[k] == 1 && (own.has & 1);  // in the row's own place
-        const uint64_t p = whole ? ((uint64_t)k * v.H + h) * rows + row
+        const uint64_t p = whole ? k * all + r
                                  : (2 * (uint64_t)(part[k].first + at) + (at == 0 ? 1 : 0)) * ws.tile_rows + part[k].row;
         ml[j] = reinterpret_cast<const float2*>(whole ? ws.row_ml : ws.part_ml)[p];
-        o[j] = reinterpret_cast<const float2*>((whole ? ws.row_o : ws.part_o) + p * kPageDim)[l];
-      }
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (i0 + j * WAVES < parts) top = fmaxf(top, ml[j].x);
-      const float ref = against(top), f = exp2_fast(m - ref);
-      m = top, sum *= f, x *= f, y *= f;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float w = i0 + j * WAVES < parts ? exp2_fast(ml[j].x - ref) : 0.0f;
-        if (i0 + j * WAVES < parts) sum += w * ml[j].y, x += w * o[j].x, y += w * o[j].y;
+        const f32x4* o = reinterpret_cast<const f32x4*>((whole ? ws.row_o : ws.part_o) + p * kPageDim + d);
+        lo[j] = o[0], hi[j] = o[1];
+      } else {
+        ml[j] = float2{-INFINITY, 0.0f};
+        lo[j] = hi[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
     }
-    if constexpr (WAVES > 1) {
-      got[wave][2 * l] = x, got[wave][2 * l + 1] = y;
-      if (l == 0) got[wave][kPageDim] = m, got[wave][kPageDim + 1] = sum;
-      __syncthreads();
-      if (wave) return;
-      float top = -INFINITY;
+    float top = m;
 #pragma unroll
-      for (int k = 0; k < WAVES; ++k) top = fmaxf(top, got[k][kPageDim]);
-      const float ref = against(top);
-      sum = x = y = 0.0f, m = top;
+    for (int j = 0; j < kAhead; ++j) top = fmaxf(top, ml[j].x);
+    const float ref = against(top), f = exp2_fast(m - ref);
+    m = top, sum *= f;
 #pragma unroll
-      for (int k = 0; k < WAVES; ++k) {
-        const float w = exp2_fast(got[k][kPageDim] - ref);
-        sum += w * got[k][kPageDim + 1], x += w * got[k][2 * l], y += w * got[k][2 * l + 1];
-      }
+    for (int e = 0; e < 8; ++e) x[e] *= f;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float w = exp2_fast(ml[j].x - ref);
+      sum += w * ml[j].y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += w * lo[j][e], x[4 + e] += w * hi[j][e];
     }
-    finish_row<DT>(a, row, h, m, sum, x, y, !(own.has & 2));
   }
+  if constexpr (SPLIT > 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) got[team][d + e] = x[e];
+    if (d == 0) got[team][kPageDim] = m, got[team][kPageDim + 1] = sum;
+    __syncthreads();
+    if (team) return;
+    float top = -INFINITY;
+    for (int k = 0; k < kTeams; ++k) top = fmaxf(top, got[k][kPageDim]);
+    const float ref = against(top);
+    m = top, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+    for (int k = 0; k < kTeams; ++k) {
+      const float w = exp2_fast(got[k][kPageDim] - ref);
+      sum += w * got[k][kPageDim + 1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] += w * got[k][d + e];
+    }
+  }
+  const bool none = !(own.has & 2);
+  write_out<DT>(a, row_at(a, a.os, row, h), d, x, none ? 0.0f : 1.0f / sum);
+  if (a.lse && d == 0)
+    a.lse[(int64_t)tok * a.Hq + h * a.G + row % a.G] =
+        none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 // ---- host ------------------------------------------------------------------------
@@ -1385,16 +1399,10 @@ void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scra
     if (forms == 2) k_attend<DT, 2><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
     if (forms == 3) k_attend<DT, 3><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
   }
-  // Four wavefronts per row where the rows do not fill the GPU with one; with many
-  // rows (prompts, most of them finished by one workgroup) a wavefront looks at several.
+  // a workgroup per row where that does not fill the GPU twice
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
-  if (all <= (uint64_t)grid) {
-    k_attend_join<DT, 4><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid, 1);
-  } else {
-    const int each = (int)std::min<uint64_t>(64, (all + 16ull * grid - 1) / (16ull * grid));
-    const uint64_t waves = (all + each - 1) / each;
-    k_attend_join<DT, 1><<<(unsigned)((waves + 3) / 4), kThreads, 0, s>>>(v, a, ws, grid, each);
-  }
+  if (all <= 2ull * grid) k_attend_join<DT, 16><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid);
+  else k_attend_join<DT, 1><<<(unsigned)((all + 15) / 16), kThreads, 0, s>>>(v, a, ws, grid);
 }
 
 }  // namespace
