@@ -20,6 +20,7 @@ Reference interfaces mirrored (clearleo126/ferry, paths relative to its tree):
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 import torch  # noqa: F401  (HIP runtime + device memory; load before the library)
@@ -214,10 +215,10 @@ _PROTOS = {
     "ferry_pages_fork": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _vp, _i32, _vp]),
     "ferry_pages_trim": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _i32, _vp]),
     "ferry_pages_compact": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp]),
-    "ferry_pages_append": (C.c_int, [C.POINTER(PagesDesc), _i32, C.POINTER(AppendArgs), _vp]),
-    "ferry_pages_attend_work_bytes": (C.c_int, [C.POINTER(PagesDesc), C.POINTER(AttendArgs),
-                                                C.POINTER(C.c_uint64)]),
-    "ferry_pages_attend": (C.c_int, [C.POINTER(PagesDesc), _i32, C.POINTER(AttendArgs), _vp]),
+    # (args: AppendArgs / AttendArgs by reference, or packed as below)
+    "ferry_pages_append": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp]),
+    "ferry_pages_attend_work_bytes": (C.c_int, [C.POINTER(PagesDesc), _vp, C.POINTER(C.c_uint64)]),
+    "ferry_pages_attend": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp]),
     "ferry_rope_freqs": (C.c_int, [C.c_int, _i32, C.c_double, C.c_double, C.c_double, C.c_double,
                                    C.c_double, _vp]),
     "ferry_refgen_selections": (C.c_int, [_i32, _i32, _i32, _i32, C.c_uint64, _vp]),
@@ -617,6 +618,9 @@ def rope_freqs(kind, rot_dim, base=10000.0, stretch=1.0, trained_ctx=0.0, slow=1
 
 
 _X_DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_APPEND = struct.Struct("@6ifi8P8q")  # AppendArgs, AttendArgs: packing them takes a tenth of
+_ATTEND = struct.Struct("@4ifi7P4qPQ")  # the time of filling a ctypes structure
+assert _APPEND.size == C.sizeof(AppendArgs) and _ATTEND.size == C.sizeof(AttendArgs)
 _PAGE_TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16,
                FP8: torch.float8_e4m3fn}
 
@@ -676,7 +680,7 @@ class Pages:
         self.pool, self.table, self.length, self.refs = pool, table, length, refs
         self.scales, self.error, self.dtype, self._work = scales, error, dtype, work
         self.q_dtype = torch.bfloat16 if dtype == FP8 else _PAGE_TORCH[dtype]
-        self._d, self._r = d, C.byref(d)
+        self._d, self._r, self._attend_bytes = d, C.byref(d), {}
 
     @classmethod
     def empty(cls, n_layers, kv_heads, n_pages, n_lanes, max_pages, dtype=BF16, device=0):
@@ -693,11 +697,16 @@ class Pages:
 
     def _s(self, stream):
         if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
+            return torch._C._cuda_getCurrentRawStream(self.device)
         return getattr(stream, "cuda_stream", stream)
 
     def _list(self, t, name, n):
-        return None if t is None else _dev(t, name, n, _I32, self.device)
+        if t is None:
+            return None
+        if t.dtype is torch.int32 and t.get_device() == self.device and t.is_contiguous() \
+                and t.numel() >= n:
+            return t.data_ptr()
+        return _dev(t, name, n, _I32, self.device)  # says what is wrong
 
     def check(self):
         """Raise the first error the device found since the last check
@@ -736,17 +745,17 @@ class Pages:
 
     # ---- tokens -----------------------------------------------------------------
     def _rows(self, t, name, rows, heads, dtypes):
-        """Pointer and (token, head) strides of a [rows, heads, 128] tensor."""
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != self.device:
+        """Pointer and strides between tokens and heads of a [rows, heads, 128] tensor."""
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.device:
             raise ValueError(f"{name}: expected a CUDA tensor on cuda:{self.device}")
         if t.dtype not in dtypes:
             raise ValueError(f"{name}: dtype {t.dtype}, expected {' or '.join(map(str, dtypes))}")
-        if t.dim() != 3 or t.shape[0] != rows or (heads and t.shape[1] != heads) or t.shape[2] != 128:
+        if t.dim() != 3 or t.shape != (rows, heads or t.shape[1], 128):
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{rows}, {heads or 'heads'}, 128]")
-        s = t.stride()
-        if s[2] != 1:
+        a, b, c = t.stride()
+        if c != 1:
             raise ValueError(f"{name}: a head's 128 values must be contiguous")
-        return t.data_ptr(), _i64x2(s[0], s[1])
+        return t.data_ptr(), a, b
 
     def append(self, layer, lane, pos, k=None, v=None, q=None, q_out=None, inv_freq=None, factor=1.0,
                pairs=False, kv_scale=None, stream=None):
@@ -757,26 +766,26 @@ class Pages:
         x = q if q is not None else k
         if x is None:
             raise ValueError("neither q nor k")
-        a = AppendArgs(n_tokens=n, x_dtype=_X_DTYPE.get(x.dtype, -1), rot_dim=2 * inv_freq.numel(),
-                       pairs=int(pairs), factor=factor)
-        a.pos = self._list(pos, "pos", n)
-        a.lane = self._list(lane, "lane", n)
-        a.inv_freq = _dev(inv_freq, "inv_freq", 1, (torch.float64,), self.device)
+        heads, out_type = 0, 0
+        qp = op = kp = vp = sp = (0, 0, 0)
         if q is not None:
-            a.q, a.q_stride = self._rows(q, "q", n, 0, _X_DTYPE)
-            a.q_heads = q.shape[1]
-            a.q_out, a.q_out_stride = self._rows(q_out, "q_out", n, a.q_heads, _X_DTYPE)
-            a.q_out_dtype = _X_DTYPE[q_out.dtype]
+            heads = q.shape[1]
+            qp = self._rows(q, "q", n, 0, _X_DTYPE)
+            op = self._rows(q_out, "q_out", n, heads, _X_DTYPE)
+            out_type = _X_DTYPE[q_out.dtype]
         if k is not None or v is not None:
             H = self._d.kv_heads
-            a.k, a.k_stride = self._rows(k, "k", n, H, (x.dtype,))
-            a.v, a.v_stride = self._rows(v, "v", n, H, (x.dtype,))
+            kp = self._rows(k, "k", n, H, (x.dtype,))
+            vp = self._rows(v, "v", n, H, (x.dtype,))
             if self.dtype == FP8:
-                a.kv_scale = _dev(kv_scale, "kv_scale", 2 * H, _F32, self.device)
+                sp = (_dev(kv_scale, "kv_scale", 2 * H, _F32, self.device),)
+        a = _APPEND.pack(n, heads, _X_DTYPE.get(x.dtype, -1), out_type, 2 * inv_freq.numel(), bool(pairs),
+                         factor, 0, self._list(lane, "lane", n) or 0, self._list(pos, "pos", n),
+                         _dev(inv_freq, "inv_freq", 1, (torch.float64,), self.device), sp[0],
+                         qp[0], kp[0], vp[0], op[0], qp[1], qp[2], kp[1], kp[2], vp[1], vp[2], op[1], op[2])
         if n == 0 and 0 <= layer < self._d.n_layers:
             return  # empty tensors have no address
-        _check(lib.ferry_pages_append(self._r, layer, C.byref(a), self._s(stream)),
-               "ferry_pages_append")
+        _check(lib.ferry_pages_append(self._r, layer, a, self._s(stream)), "ferry_pages_append")
 
     def attend(self, layer, q, out, lanes, q_start=None, group_start=None, shared=None, scale=0.0,
                lse=None, stream=None):
@@ -784,29 +793,34 @@ class Pages:
         of request r are [q_start[r], q_start[r+1]); None: one row each), into
         out; requests [group_start[g], group_start[g+1]) share their first
         shared[g] pages."""
-        n = lanes.numel()
-        a = AttendArgs(n_req=n, n_tokens=q.shape[0], scale=scale)
+        n, rows, heads, groups, sp = lanes.numel(), q.shape[0], q.shape[1], 0, None
         dt = (self.q_dtype,)
-        a.q, a.q_stride = self._rows(q, "q", a.n_tokens, 0, dt)
-        a.q_heads = q.shape[1]
-        a.out, a.out_stride = self._rows(out, "out", a.n_tokens, a.q_heads, dt)
-        a.lanes = self._list(lanes, "lanes", n)
-        a.q_start = self._list(q_start, "q_start", n + 1)
+        qp, qa, qb = self._rows(q, "q", rows, 0, dt)
+        op, oa, ob = self._rows(out, "out", rows, heads, dt)
         if group_start is not None:
-            a.n_groups = group_start.numel() - 1
-            a.group_start = self._list(group_start, "group_start", 1)
-            a.shared = _dev(shared, "shared", a.n_groups, _I32, self.device)
-        if lse is not None:
-            a.lse = _dev(lse, "lse", a.n_tokens * a.q_heads, _F32, self.device)
-        b = C.c_uint64()
-        _check(lib.ferry_pages_attend_work_bytes(self._r, C.byref(a), C.byref(b)),
-               "ferry_pages_attend_work_bytes")
-        work = torch.empty(b.value, dtype=torch.uint8, device=self.pool.device)
-        a.work, a.work_bytes = work.data_ptr(), b.value
+            groups = group_start.numel() - 1
+            sp = _dev(shared, "shared", groups, _I32, self.device)
+        ep = None if lse is None else _dev(lse, "lse", rows * heads, _F32, self.device)
+        # the scratch's size follows from these, the same in every call on this cache
+        shape = (n, rows, groups, heads, q_start is None)
+        need = self._attend_bytes.get(shape)
+        if need is None:
+            b = C.c_uint64()
+            a = AttendArgs(n, rows, groups, heads, scale, q_start=None if q_start is None else 1)
+            _check(lib.ferry_pages_attend_work_bytes(self._r, C.byref(a), C.byref(b)),
+                   "ferry_pages_attend_work_bytes")
+            if len(self._attend_bytes) >= 4096:
+                self._attend_bytes.clear()
+            need = self._attend_bytes[shape] = b.value
+        work = torch.empty(need, dtype=torch.uint8, device=self.pool.device)
+        a = _ATTEND.pack(n, rows, groups, heads, scale, 0, self._list(lanes, "lanes", n),
+                         self._list(q_start, "q_start", n + 1) or 0,
+                         self._list(group_start, "group_start", 1) or 0, sp or 0, qp, op, ep or 0,
+                         qa, qb, oa, ob, work.data_ptr(), need)
         s = self._s(stream)
-        if stream is not None and s != torch.cuda.current_stream(self.device).cuda_stream:
+        if stream is not None and s != self._s(None):
             work.record_stream(torch.cuda.ExternalStream(s, device=self.device))
-        _check(lib.ferry_pages_attend(self._r, layer, C.byref(a), s), "ferry_pages_attend")
+        _check(lib.ferry_pages_attend(self._r, layer, a, s), "ferry_pages_attend")
 
 
 _hip = None
