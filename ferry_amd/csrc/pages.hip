@@ -4,7 +4,9 @@
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
+#include "attn_common.hpp"
 #include "pages.hpp"
 
 using namespace ferry_amd;
@@ -121,20 +123,21 @@ uint64_t work_bytes(int n_pages, int n_lanes) {
 
 __device__ inline int pages_of(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
 
-// Exclusive prefix sum of x over the workgroup; *total gets the sum.
-__device__ inline uint32_t block_scan(uint32_t x, uint32_t* total) {
-  __shared__ uint32_t part[kPlan / 64];
+// Exclusive prefix sum of x over the workgroup of kPlan threads; *total gets the sum.
+__device__ inline uint64_t block_scan(uint64_t x, uint64_t* total) {
+  __shared__ uint64_t part[kPlan / 64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  uint32_t s = x;
+  uint64_t s = x;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const uint32_t y = __shfl_up(s, d);
+    const uint64_t y = __shfl_up(s, d);
     if (lane >= d) s += y;
   }
   if (lane == 63) part[w] = s;
   __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (int i = 0; i < (int)blockDim.x / 64; ++i) {
+  uint64_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kPlan / 64; ++i) {
     if (i < w) before += part[i];
     all += part[i];
   }
@@ -151,16 +154,64 @@ __device__ inline bool name_lane(uint32_t* bits, int lane, int n_lanes) {
 }
 
 // ---- reserve -------------------------------------------------------------------
+constexpr int kIdsInLds = 4096;  // pages that the plan hands out by itself
+constexpr int kOwnPages = 64;    // ... of one lane
+
+// The lowest `need` free ids (refs 0) into w.free_ids and the first of them into ids;
+// returns how many there are.  first: refs of pages 4 tid .. 4 tid + 3.
+__device__ inline uint64_t find_free(const PageView& v, const Work& w, uint64_t need, uint32_t* ids,
+                                     const uint32_t (&first)[4]) {
+  uint64_t got = 0;
+  auto take = [&](int64_t p0, auto count, auto&& refs) {
+    constexpr int N = decltype(count)::value;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += refs(i) == 0;
+    uint64_t all, at = got + block_scan(n, &all);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (refs(i) == 0) {
+        if (at < need) {
+          w.free_ids[at] = (uint32_t)(p0 + i);
+          if (at < kIdsInLds) ids[at] = (uint32_t)(p0 + i);
+        }
+        ++at;
+      }
+    got += all;
+  };
+  take(4ll * threadIdx.x, std::integral_constant<int, 4>{}, [&](int i) { return first[i]; });
+  // the rest 16 to a thread, all of them on their way at once
+  for (int64_t c = 4 * kPlan; c < v.n_pages && got < need; c += 16 * kPlan) {
+    const int64_t p0 = c + 16ll * threadIdx.x;
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = p0 + i < v.n_pages ? v.refs[p0 + i] : 1u;
+    take(p0, std::integral_constant<int, 16>{}, [&](int i) { return r[i]; });
+  }
+  return got;
+}
+
 // One workgroup decides the whole call: which last pages are copied, how many
-// pages each listed lane takes, and which (the lowest free ids).
+// pages each listed lane takes, and which (the lowest free ids).  It is a chain of
+// dependent reads: a lane's length, its last page, that page's refs, while the first
+// refs are on their way.  SMALL: a thread per listed lane; the lanes of a shared
+// page are then counted in LDS, else by atomics in the scratch.
+template <bool SMALL>
 __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, const int32_t* __restrict__ lanes,
                                                         const int32_t* __restrict__ tokens, int n) {
   __shared__ uint32_t bits[kMaxLanes / 32];
-  __shared__ int bad;
+  __shared__ uint32_t ids[kIdsInLds];
+  __shared__ uint32_t last_page[SMALL ? kPlan : 1];
+  __shared__ int bad, sharing, longest;
   const int tid = threadIdx.x;
+  uint32_t first[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) first[i] = 4 * tid + i < v.n_pages ? v.refs[4 * tid + i] : 1u;
   for (int i = tid; i < (v.n_lanes + 31) / 32; i += kPlan) bits[i] = 0;
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = sharing = longest = 0;
   __syncthreads();
+  int my_lane = 0, my_had = 0, my_tokens = 0;  // SMALL: the thread's lane
+  uint32_t my_page = kNone, my_refs = 0;
   for (int i = tid; i < n; i += kPlan) {
     const int lane = lanes[i], t = tokens[i];
     if (!name_lane(bits, lane, v.n_lanes) || t < 0) {
@@ -168,12 +219,16 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
     } else {
       const int had = v.len[lane];
       w.had[i] = had;
+      my_lane = lane, my_had = had, my_tokens = t;
       if (had < 0 || (int64_t)had + t > (int64_t)v.max_pages * kPageTokens) {
         atomicMin(&bad, FERRY_ECAPACITY);
       } else if (had % kPageTokens) {
         const uint32_t page = v.table[(uint64_t)lane * v.max_pages + had / kPageTokens];
         if (page >= (uint32_t)v.n_pages) {
           atomicMin(&bad, FERRY_ESTATE);
+        } else if constexpr (SMALL) {
+          my_page = page, my_refs = v.refs[page];
+          if (my_refs > 1) sharing = 1;
         } else {
           atomicExch(&w.uses[page], 0u);
           atomicExch(&w.last[page], 0u);
@@ -181,70 +236,103 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
       }
     }
   }
-  __threadfence();
+  if constexpr (SMALL) last_page[tid] = my_page;
   __syncthreads();
   if (bad) {
     if (tid == 0) w.plan->ok = 0, set_error(v.error, bad);
     return;
   }
-  for (int i = tid; i < n; i += kPlan) {
-    const int had = (int)w.had[i];
-    if (had % kPageTokens) {
-      const uint32_t page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
-      atomicAdd(&w.uses[page], 1u);
-      atomicMax(&w.last[page], (uint32_t)i);
-    }
-  }
-  __threadfence();
-  __syncthreads();
-  // what each lane takes, in the order of the list
-  uint64_t need = 0;
-  uint32_t copies = 0;
-  for (int i0 = 0; i0 < n; i0 += kPlan) {
-    const int i = i0 + tid;
-    uint32_t mine = 0, copy = 0, page = kNone;
-    if (i < n) {
+  if constexpr (!SMALL) {
+    for (int i = tid; i < n; i += kPlan) {
       const int had = (int)w.had[i];
       if (had % kPageTokens) {
-        page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
-        const bool keeps = aload(&w.uses[page]) >= v.refs[page] && aload(&w.last[page]) == (uint32_t)i;
-        copy = !keeps;
+        const uint32_t page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
+        atomicAdd(&w.uses[page], 1u);
+        atomicMax(&w.last[page], (uint32_t)i);
       }
-      mine = copy + (uint32_t)(pages_of(had + tokens[i]) - pages_of(had));
     }
-    uint32_t all, all_copies;
-    const uint32_t at = block_scan(mine, &all), cat = block_scan(copy, &all_copies);
-    if (i < n) {
-      w.base[i] = (uint32_t)(need + at);
-      if (copy) w.copy_lane[copies + cat] = i, w.copy_from[copies + cat] = page;
-    }
-    need += all;
-    copies += all_copies;
+    __syncthreads();
   }
-  // the lowest free ids
-  uint32_t got = 0;
-  for (int64_t p0 = 0; p0 < v.n_pages && got < need && need <= (uint64_t)v.n_pages; p0 += kPlan) {
-    const int64_t p = p0 + tid;
-    const uint32_t free = p < v.n_pages && v.refs[p] == 0;
-    uint32_t all;
-    const uint32_t at = got + block_scan(free, &all);
-    if (free && at < need) w.free_ids[at] = (uint32_t)p;
-    got += all;
+  // what each lane takes, in the order of the list (copies in the high half of a sum)
+  uint64_t need = 0;
+  uint32_t copies = 0, my_base = 0, my_fresh = 0;
+  bool my_copy = false;
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + tid;
+    uint32_t fresh = 0, page = my_page;
+    bool copy = false;
+    if (i < n) {
+      const int had = SMALL ? my_had : (int)w.had[i], t = SMALL ? my_tokens : tokens[i];
+      if (had % kPageTokens) {
+        // of the listed lanes that share the page, with no others, the last one keeps it
+        if constexpr (SMALL) {
+          if (my_refs > 1) {
+            uint32_t uses = 0;
+            int last = 0;
+            for (int j = 0; j < n; ++j)
+              if (last_page[j] == my_page) ++uses, last = j;
+            copy = uses < my_refs || last != i;
+          }
+        } else {
+          page = v.table[(uint64_t)lanes[i] * v.max_pages + had / kPageTokens];
+          copy = aload(&w.uses[page]) < v.refs[page] || aload(&w.last[page]) != (uint32_t)i;
+        }
+      }
+      fresh = (uint32_t)(pages_of(had + t) - pages_of(had));
+    }
+    uint64_t all;
+    const uint64_t at = block_scan((uint64_t)copy << 40 | (copy + fresh), &all), mask = (1ull << 40) - 1;
+    if (i < n) {
+      w.base[i] = my_base = (uint32_t)(need + (at & mask));
+      my_copy = copy, my_fresh = fresh;
+      const uint32_t c = copies + (uint32_t)(at >> 40);
+      if (copy) w.copy_lane[c] = i, w.copy_from[c] = page;
+      if (SMALL && copy + fresh > kOwnPages) longest = 1;
+    }
+    need += all & mask;
+    copies += (uint32_t)(all >> 40);
+  }
+  const uint64_t got = need <= (uint64_t)v.n_pages ? find_free(v, w, need, ids, first) : 0;
+  __syncthreads();
+  // the plan hands out few pages by itself
+  const bool own = SMALL && need <= kIdsInLds && !longest, ok = need <= got;
+  if (own && ok && tid < n) {
+    v.len[my_lane] = my_had + my_tokens;
+    uint32_t* row = v.table + (uint64_t)my_lane * v.max_pages + pages_of(my_had) - (my_copy ? 1 : 0);
+    for (uint32_t e = 0; e < my_copy + my_fresh; ++e) {
+      const uint32_t id = ids[my_base + e];
+      row[e] = id;
+      v.refs[id] = 1;
+    }
   }
   if (tid == 0) {
-    w.plan->ok = got >= need;
-    w.plan->need = (uint32_t)need;
+    w.plan->ok = ok;
+    w.plan->need = own ? 0 : (uint32_t)need;
     w.plan->copies = copies;
-    if (got < need) set_error(v.error, FERRY_ECAPACITY);
+    if (!ok) set_error(v.error, FERRY_ECAPACITY);
   }
 }
 
-// 16-byte words of one page of one layer, all kv heads, by one workgroup.
+// One page of one layer, all kv heads, by one workgroup.  KEEP: the copy is soon read
+// (a lane's last page); else it streams past the caches: 5.9 against 4.7 TB/s.
+template <bool KEEP>
 __device__ inline void copy_page(const PageView& v, int layer, uint32_t from, uint32_t to) {
-  const uint64_t bytes = (uint64_t)v.H * v.bb;
-  const u32x4* s = reinterpret_cast<const u32x4*>(v.pool + ((uint64_t)layer * v.n_pages + from) * bytes);
-  u32x4* d = reinterpret_cast<u32x4*>(v.pool + ((uint64_t)layer * v.n_pages + to) * bytes);
-  for (uint64_t i = threadIdx.x; i < bytes / 16; i += blockDim.x) d[i] = s[i];
+  constexpr int kEach = 4;  // words of a thread on their way at once
+  const uint32_t words = (uint32_t)v.H * (v.bb / 16);
+  const u32x4* s = reinterpret_cast<const u32x4*>(v.pool) + ((uint64_t)layer * v.n_pages + from) * words;
+  u32x4* d = reinterpret_cast<u32x4*>(v.pool) + ((uint64_t)layer * v.n_pages + to) * words;
+  for (uint32_t i0 = threadIdx.x; i0 < words; i0 += kEach * blockDim.x) {
+    u32x4 x[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (i0 + j * blockDim.x < words) x[j] = load_kv<!KEEP>(s + i0 + j * blockDim.x);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (i0 + j * blockDim.x < words) {
+        if constexpr (KEEP) d[i0 + j * blockDim.x] = x[j];
+        else __builtin_nontemporal_store(x[j], d + i0 + j * blockDim.x);
+      }
+  }
   if (v.scales) {
     const float* a = v.scales + ((uint64_t)layer * v.n_pages + from) * v.H * 2;
     float* b = v.scales + ((uint64_t)layer * v.n_pages + to) * v.H * 2;
@@ -257,8 +345,8 @@ __global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32
   if (!w.plan->ok) return;
   const uint32_t need = w.plan->need, copies = w.plan->copies;
   const uint32_t step = gridDim.x * blockDim.x, at = blockIdx.x * blockDim.x + threadIdx.x;
-  for (uint32_t i = at; i < (uint32_t)n; i += step)
-    v.len[lanes[i]] = (int)w.had[i] + tokens[i];
+  if (need)
+    for (uint32_t i = at; i < (uint32_t)n; i += step) v.len[lanes[i]] = (int)w.had[i] + tokens[i];
   // taken page r belongs to the last list place whose base is at most r
   for (uint32_t r = at; r < need; r += step) {
     int lo = 0, hi = n - 1;
@@ -278,72 +366,115 @@ __global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32
   for (uint64_t c = blockIdx.x; c < (uint64_t)copies * v.L; c += gridDim.x) {
     const uint32_t k = (uint32_t)(c / v.L), from = w.copy_from[k];
     if (c % v.L == 0 && threadIdx.x == 0) atomicSub(&v.refs[from], 1u);
-    copy_page(v, (int)(c % v.L), from, w.free_ids[w.base[w.copy_lane[k]]]);
+    copy_page<true>(v, (int)(c % v.L), from, w.free_ids[w.base[w.copy_lane[k]]]);
   }
 }
 
 // ---- fork and trim ----------------------------------------------------------------
-// One workgroup checks the list.  Fork (src != NULL): w.had gets the tokens each
-// dst will hold; trim: those each lane keeps, w.base what it held.
-__global__ __launch_bounds__(kPlan) void k_lanes_plan(PageView v, Work w, const int32_t* __restrict__ src,
-                                                      const int32_t* __restrict__ lanes,
-                                                      const int32_t* __restrict__ keep, int n) {
+// Checks a list of lanes (fork: src and dst); every thread of the workgroup gets the
+// error, 0 if it is fine.  fine(i): whether entry i's counts are, once its lanes are.
+template <class Fine>
+__device__ inline int check_lanes(const PageView& v, const int32_t* __restrict__ src,
+                                  const int32_t* __restrict__ lanes, int n, Fine&& fine) {
   __shared__ uint32_t bits[kMaxLanes / 32];
   __shared__ int bad;
-  const int tid = threadIdx.x;
-  for (int i = tid; i < (v.n_lanes + 31) / 32; i += kPlan) bits[i] = 0;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  for (int i = tid; i < (v.n_lanes + 31) / 32; i += threads) bits[i] = 0;
   if (tid == 0) bad = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += kPlan)
-    if (!name_lane(bits, lanes[i], v.n_lanes)) atomicMin(&bad, FERRY_EINVAL);
+  for (int i = tid; i < n; i += threads)
+    if (!name_lane(bits, lanes[i], v.n_lanes)) bad = FERRY_EINVAL;
   __syncthreads();
-  for (int i = tid; i < n; i += kPlan) {
+  for (int i = tid; i < n; i += threads) {
     const int lane = lanes[i], from = src ? src[i] : lane;
-    bool fine = lane >= 0 && lane < v.n_lanes && from >= 0 && from < v.n_lanes;
-    if (fine) {
-      const int held = v.len[from], kept = keep ? keep[i] : src ? held : 0;
-      if (src) fine = v.len[lane] == 0 && !(bits[from >> 5] >> (from & 31) & 1u);
-      fine = fine && kept >= 0 && kept <= held && held <= v.max_pages * kPageTokens;
-      w.had[i] = kept;
-      w.base[i] = held;
-    }
-    if (!fine) atomicMin(&bad, FERRY_EINVAL);
+    bool ok = lane >= 0 && lane < v.n_lanes && from >= 0 && from < v.n_lanes;
+    if (ok && src) ok = !(bits[from >> 5] >> (from & 31) & 1u);
+    if (!ok || !fine(i, from, lane)) bad = FERRY_EINVAL;
   }
   __syncthreads();
-  if (tid == 0) {
-    w.plan->ok = bad == 0;
-    if (bad) set_error(v.error, bad);
+  return bad;
+}
+
+// Tokens that entry i of a fork or trim keeps of what lane `from` holds; false: not so many.
+__device__ inline bool kept_tokens(const PageView& v, const int32_t* keep, int i, int from, int otherwise,
+                                   int* kept) {
+  const int held = v.len[from];
+  *kept = keep ? keep[i] : otherwise < 0 ? held : otherwise;
+  return *kept >= 0 && *kept <= held && held <= v.max_pages * kPageTokens;
+}
+
+// One workgroup checks a fork's list; w.had gets the tokens each dst will hold.
+__device__ inline bool fork_plan(const PageView& v, const Work& w, const int32_t* src, const int32_t* dst,
+                                 const int32_t* keep, int n) {
+  const int bad = check_lanes(v, src, dst, n, [&](int i, int from, int lane) {
+    int kept;
+    const bool ok = kept_tokens(v, keep, i, from, -1, &kept) && v.len[lane] == 0;
+    w.had[i] = kept;
+    return ok;
+  });
+  if (bad && threadIdx.x == 0) set_error(v.error, bad);
+  return bad == 0;
+}
+// Entry e of a forked row.
+__device__ inline void fork_entry(const PageView& v, int src, int dst, int e) {
+  const uint32_t id = v.table[(uint64_t)src * v.max_pages + e];
+  v.table[(uint64_t)dst * v.max_pages + e] = id;
+  if (id < (uint32_t)v.n_pages) atomicAdd(&v.refs[id], 1u);
+  else set_error(v.error, FERRY_ESTATE);
+}
+
+// A short list of short tables: the one workgroup that checks it copies the rows too,
+// a wavefront each.
+__global__ __launch_bounds__(kPlan) void k_fork_small(PageView v, Work w, const int32_t* __restrict__ src,
+                                                      const int32_t* __restrict__ dst,
+                                                      const int32_t* __restrict__ keep, int n) {
+  if (!fork_plan(v, w, src, dst, keep, n)) return;
+  for (int i = threadIdx.x >> 6; i < n; i += kPlan / 64) {
+    const int kept = (int)w.had[i], from = src[i], to = dst[i];
+    for (int e = threadIdx.x & 63; e < pages_of(kept); e += 64) fork_entry(v, from, to, e);
+    if ((threadIdx.x & 63) == 0) v.len[to] = kept;
   }
 }
 
+__global__ __launch_bounds__(kPlan) void k_fork_plan(PageView v, Work w, const int32_t* __restrict__ src,
+                                                     const int32_t* __restrict__ dst,
+                                                     const int32_t* __restrict__ keep, int n) {
+  const bool ok = fork_plan(v, w, src, dst, keep, n);
+  if (threadIdx.x == 0) w.plan->ok = ok;
+}
 __global__ __launch_bounds__(256) void k_fork(PageView v, Work w, const int32_t* __restrict__ src,
                                               const int32_t* __restrict__ dst, int n) {
   if (!w.plan->ok) return;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int kept = (int)w.had[i], pages = pages_of(kept);
-    const uint32_t* from = v.table + (uint64_t)src[i] * v.max_pages;
-    uint32_t* to = v.table + (uint64_t)dst[i] * v.max_pages;
-    for (int e = threadIdx.x; e < pages; e += blockDim.x) {
-      const uint32_t id = from[e];
-      to[e] = id;
-      if (id < (uint32_t)v.n_pages) atomicAdd(&v.refs[id], 1u);
-      else set_error(v.error, FERRY_ESTATE);
-    }
-    if (threadIdx.x == 0) v.len[dst[i]] = kept;
+    const int kept = (int)w.had[i], from = src[i], to = dst[i];
+    for (int e = threadIdx.x; e < pages_of(kept); e += blockDim.x) fork_entry(v, from, to, e);
+    if (threadIdx.x == 0) v.len[to] = kept;
   }
 }
 
-__global__ __launch_bounds__(256) void k_trim(PageView v, Work w, const int32_t* __restrict__ lanes, int n) {
-  if (!w.plan->ok) return;
+// Every workgroup checks the list for itself and trims its own lanes of it.  What
+// another one has done by then does not change the answer: a lane's length only
+// becomes what it keeps, and a list that is not fine is left alone by all.
+__global__ __launch_bounds__(256) void k_trim(PageView v, const int32_t* __restrict__ lanes,
+                                              const int32_t* __restrict__ keep, int n) {
+  const int bad = check_lanes(v, nullptr, lanes, n, [&](int i, int from, int) {
+    int kept;
+    return kept_tokens(v, keep, i, from, 0, &kept);
+  });
+  if (bad) {
+    if (threadIdx.x == 0 && blockIdx.x == 0) set_error(v.error, bad);
+    return;
+  }
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
-    const int kept = (int)w.had[i], held = (int)w.base[i];
-    uint32_t* row = v.table + (uint64_t)lanes[i] * v.max_pages;
+    const int lane = lanes[i], kept = keep ? keep[i] : 0, held = v.len[lane];
+    uint32_t* row = v.table + (uint64_t)lane * v.max_pages;
     for (int e = pages_of(kept) + threadIdx.x; e < pages_of(held); e += blockDim.x) {
       const uint32_t id = row[e];
       row[e] = kNone;
       if (id >= (uint32_t)v.n_pages || atomicSub(&v.refs[id], 1u) == 0) set_error(v.error, FERRY_ESTATE);
     }
-    if (threadIdx.x == 0) v.len[lanes[i]] = kept;
+    __syncthreads();  // all have read the length
+    if (threadIdx.x == 0) v.len[lane] = kept;
   }
 }
 
@@ -351,29 +482,49 @@ __global__ __launch_bounds__(256) void k_trim(PageView v, Work w, const int32_t*
 // One workgroup pairs the pages in use at or behind `live` with the free ids
 // before it, both in ascending order: the two lists do not meet, so the moves
 // need no order among themselves.  free_ids becomes the new id of every page.
+// EACH pages of a thread are on their way at once; where that covers the pool (ONE)
+// they are read once.
+template <int EACH, bool ONE>
 __global__ __launch_bounds__(kPlan) void k_compact_plan(PageView v, Work w, int32_t* live_out) {
   const int tid = threadIdx.x;
-  uint32_t live = 0;
-  for (int64_t p0 = 0; p0 < v.n_pages; p0 += kPlan) {
-    const int64_t p = p0 + tid;
-    uint32_t all;
-    (void)block_scan(p < v.n_pages && v.refs[p] != 0, &all);
-    live += all;
+  auto read = [&](int64_t p0, uint32_t (&r)[EACH]) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) r[i] = p0 + i < v.n_pages ? v.refs[p0 + i] : 0u;
+  };
+  uint32_t mine = 0, r[EACH];
+  for (int64_t c = 0; c < v.n_pages; c += EACH * kPlan) {
+    read(c + (int64_t)EACH * tid, r);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += r[i] != 0;
   }
+  uint64_t all;
+  (void)block_scan(mine, &all);
+  const int64_t live = (int64_t)all;
   uint32_t gaps = 0, moves = 0;
-  for (int64_t p0 = 0; p0 < v.n_pages; p0 += kPlan) {
-    const int64_t p = p0 + tid;
-    const bool used = p < v.n_pages && v.refs[p] != 0;
-    const uint32_t gap = p < live && !used, move = used && p >= live;
-    uint32_t all_gaps, all_moves;
-    const uint32_t g = gaps + block_scan(gap, &all_gaps), m = moves + block_scan(move, &all_moves);
-    if (gap) w.last[g] = (uint32_t)p;
-    if (move) w.from[m] = (uint32_t)p;
-    if (p < v.n_pages) w.free_ids[p] = (uint32_t)p;
-    gaps += all_gaps;
-    moves += all_moves;
+  for (int64_t c = 0; c < v.n_pages; c += EACH * kPlan) {
+    const int64_t p0 = c + (int64_t)EACH * tid;
+    if (!ONE) read(p0, r);
+    uint64_t n = 0;  // gaps below, moves in the high half
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (p0 + i < live) n += r[i] == 0;
+      else n += (uint64_t)(r[i] != 0) << 32;
+    }
+    const uint64_t at = block_scan(n, &all);
+    uint32_t g = gaps + (uint32_t)at, m = moves + (uint32_t)(at >> 32);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (p0 + i >= v.n_pages) break;
+      w.free_ids[p0 + i] = (uint32_t)(p0 + i);
+      if (p0 + i < live) {
+        if (r[i] == 0) w.last[g++] = (uint32_t)(p0 + i);
+      } else if (r[i] != 0) {
+        w.from[m++] = (uint32_t)(p0 + i);
+      }
+    }
+    gaps += (uint32_t)all;
+    moves += (uint32_t)(all >> 32);
   }
-  __threadfence_block();
   __syncthreads();
   for (uint32_t m = tid; m < moves; m += kPlan) {
     const uint32_t from = w.from[m], to = w.last[m];
@@ -392,7 +543,7 @@ __global__ __launch_bounds__(256) void k_compact(PageView v, Work w) {
   if (!moves) return;
   for (uint64_t c = blockIdx.x; c < (uint64_t)moves * v.L; c += gridDim.x) {
     const uint32_t m = (uint32_t)(c / v.L);
-    copy_page(v, (int)(c % v.L), w.from[m], w.last[m]);
+    copy_page<false>(v, (int)(c % v.L), w.from[m], w.last[m]);
   }
   for (int i = blockIdx.x; i < v.n_lanes; i += gridDim.x) {
     uint32_t* row = v.table + (uint64_t)i * v.max_pages;
@@ -721,7 +872,8 @@ int ferry_pages_reserve(const ferry_pages* p, const int32_t* lanes, const int32_
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    k_reserve_plan<<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
+    if (n <= kPlan) k_reserve_plan<true><<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
+    else k_reserve_plan<false><<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
     const int64_t most = std::min<int64_t>((int64_t)n * v.L + 64, 8l * gpu_cus(p->device));
     k_reserve<<<(unsigned)most, 256, 0, s>>>(v, w, lanes, tokens, n);
     return launched("ferry_pages_reserve");
@@ -741,8 +893,14 @@ int ferry_pages_fork(const ferry_pages* p, const int32_t* src, const int32_t* ds
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    k_lanes_plan<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
-    k_fork<<<n, 256, 0, s>>>(v, w, src, dst, n);
+    // One launch where a wavefront has at most eight 64-entry rows' worth (24 lanes of 58
+    // pages: 4 us, 6.5 in two launches), which bounds what the workgroup does alone.
+    if ((int64_t)n * p->max_pages <= 8192) {
+      k_fork_small<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
+    } else {
+      k_fork_plan<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
+      k_fork<<<n, 256, 0, s>>>(v, w, src, dst, n);
+    }
     return launched("ferry_pages_fork");
   });
 }
@@ -759,8 +917,8 @@ int ferry_pages_trim(const ferry_pages* p, const int32_t* lanes, const int32_t* 
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    k_lanes_plan<<<1, kPlan, 0, s>>>(v, w, nullptr, lanes, keep, n);
-    k_trim<<<n, 256, 0, s>>>(v, w, lanes, n);
+    // each workgroup reads the whole list: a long one goes to fewer of them
+    k_trim<<<n <= 1024 ? n : 256, 256, 0, s>>>(v, lanes, keep, n);
     return launched("ferry_pages_trim");
   });
 }
@@ -775,7 +933,8 @@ int ferry_pages_compact(const ferry_pages* p, int32_t* live, void* stream) {
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    k_compact_plan<<<1, kPlan, 0, s>>>(v, w, live);
+    if (v.n_pages <= 4 * kPlan) k_compact_plan<4, true><<<1, kPlan, 0, s>>>(v, w, live);
+    else k_compact_plan<16, false><<<1, kPlan, 0, s>>>(v, w, live);
     k_compact<<<(unsigned)std::min<int64_t>((int64_t)v.n_pages * v.L, 8l * gpu_cus(p->device)), 256, 0, s>>>(v, w);
     return launched("ferry_pages_compact");
   });
