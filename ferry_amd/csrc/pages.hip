@@ -85,7 +85,7 @@ struct Plan {
   int ok;         // the call is made
   uint32_t need;  // pages taken (reserve)
   uint32_t copies;  // pages copied (reserve) or moved (compact)
-  uint32_t pad;
+  int handed;     // tables, lengths and refs hold the pages taken (reserve)
 };
 struct Work {
   Plan* plan;
@@ -307,14 +307,15 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
   }
   if (tid == 0) {
     w.plan->ok = ok;
-    w.plan->need = own ? 0 : (uint32_t)need;
+    w.plan->need = (uint32_t)need;
+    w.plan->handed = own;
     w.plan->copies = copies;
     if (!ok) set_error(v.error, FERRY_ECAPACITY);
   }
 }
 
 // One page of one layer, all kv heads, by one workgroup.  KEEP: the copy is soon read
-// (a lane's last page); else it streams past the caches: 5.9 against 4.7 TB/s.
+// (a lane's last page); else it streams past the caches: 5.0 against 4.7 TB/s (1.66 GB moved).
 template <bool KEEP>
 __device__ inline void copy_page(const PageView& v, int layer, uint32_t from, uint32_t to) {
   constexpr int kEach = 4;  // words of a thread on their way at once
@@ -343,9 +344,9 @@ __device__ inline void copy_page(const PageView& v, int layer, uint32_t from, ui
 __global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32_t* __restrict__ lanes,
                                                  const int32_t* __restrict__ tokens, int n) {
   if (!w.plan->ok) return;
-  const uint32_t need = w.plan->need, copies = w.plan->copies;
+  const uint32_t need = w.plan->handed ? 0 : w.plan->need, copies = w.plan->copies;
   const uint32_t step = gridDim.x * blockDim.x, at = blockIdx.x * blockDim.x + threadIdx.x;
-  if (need)
+  if (!w.plan->handed)
     for (uint32_t i = at; i < (uint32_t)n; i += step) v.len[lanes[i]] = (int)w.had[i] + tokens[i];
   // taken page r belongs to the last list place whose base is at most r
   for (uint32_t r = at; r < need; r += step) {
@@ -894,7 +895,7 @@ int ferry_pages_fork(const ferry_pages* p, const int32_t* src, const int32_t* ds
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
     // One launch where a wavefront has at most eight 64-entry rows' worth (24 lanes of 58
-    // pages: 4 us, 6.5 in two launches), which bounds what the workgroup does alone.
+    // pages: 3.9 us, 6.4 in two launches), which bounds what the workgroup does alone.
     if ((int64_t)n * p->max_pages <= 8192) {
       k_fork_small<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
     } else {

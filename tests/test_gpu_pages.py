@@ -223,6 +223,25 @@ def test_lists_longer_than_a_workgroup_and_many_pages():
     assert b.call("reserve", [n], [640]) == 0
 
 
+@pytest.mark.parametrize("n", [1, 1024, 1025, 2500])
+def test_growing_within_begun_pages(n):
+    # no page is taken, with and without lanes that take one
+    b = Both(n + 2, n + 1, 2, F.F16, 1, 1)
+    order = list(range(n))[::-1]
+    assert b.call("reserve", order, [1] * n) == 0
+    assert b.call("reserve", order, [15 - i % 3 for i in range(n)]) == 0
+    assert b.call("reserve", order, [0] * n) == 0
+    assert b.call("reserve", [n] + order[1:], [3] + [0] * (n - 1)) == 0
+
+
+def test_many_copies_by_a_long_list():
+    n = 1500
+    b = Both(2 * n, n, 3, F.FP8, 2, 1)
+    assert b.call("reserve", [7], [20]) == 0
+    assert b.call("fork", [7] * (n - 1), [i for i in range(n) if i != 7]) == 0
+    assert b.call("reserve", list(range(n)), [1 + 20 * (i % 2) for i in range(n)]) == 0
+
+
 def test_a_page_past_four_gibibytes_is_copied():
     # records past 2^32 bytes: forked there, copied on growth, moved back by compact
     H, P = 8, 70000  # 64 KiB a page, 4.6 GB
