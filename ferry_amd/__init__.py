@@ -812,14 +812,17 @@ class Pages:
             if len(self._attend_bytes) >= 4096:
                 self._attend_bytes.clear()
             need = self._attend_bytes[shape] = b.value
-        work = torch.empty(need, dtype=torch.uint8, device=self.pool.device)
+        s = self._s(stream)
+        if stream is None or s == self._s(None):
+            work = torch.empty(need, dtype=torch.uint8, device=self.pool.device)
+        else:  # of the stream that uses it: what the current one frees it may still use
+            with torch.cuda.stream(torch.cuda.ExternalStream(s, self.device) if s
+                                   else torch.cuda.default_stream(self.device)):
+                work = torch.empty(need, dtype=torch.uint8, device=self.pool.device)
         a = _ATTEND.pack(n, rows, groups, heads, scale, 0, self._list(lanes, "lanes", n),
                          self._list(q_start, "q_start", n + 1) or 0,
                          self._list(group_start, "group_start", 1) or 0, sp or 0, qp, op, ep or 0,
                          qa, qb, oa, ob, work.data_ptr(), need)
-        s = self._s(stream)
-        if stream is not None and s != self._s(None):
-            work.record_stream(torch.cuda.ExternalStream(s, device=self.device))
         _check(lib.ferry_pages_attend(self._r, layer, a, s), "ferry_pages_attend")
 
 

@@ -54,7 +54,7 @@ constexpr int kWide = 128;         // rows of the widest tile
 constexpr float kRaise = 8.0f;     // log2 of the largest weight between raises of the max
 constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
 constexpr int kPad = 132;          // floats per row of the merge buffer
-constexpr int kNarrowPerCu = 2;    // workgroups per CU where all tiles have 16 rows (else 2)
+constexpr int kPerCu = 2;          // workgroups per CU
 
 struct AttendArgs {
   int n_req, n_tokens, n_groups, Hq, G;
@@ -435,7 +435,7 @@ __device__ inline void load_page(const Tile& t, int kv_heads, uint32_t page, int
 
 // A tile of few rows.  Columns of 16 x 16 products are rows: a wavefront holds NT
 // tiles of 16, RG wavefronts hold the tile's rows, and the 4 / RG such teams share
-// out the pages, straight from memory into registers, two pages ahead.  Lane l of a
+// out the pages, straight from memory into registers, a page ahead.  Lane l of a
 // wavefront: column n = l % 16, quarter grp = l / 16.
 //   S^T[16 tokens][16 rows] = K Q^T: lane holds tokens 4 grp + i of row n,
 //   O^T[128 dims][16 rows] += V^T P^T: that is just the P^T operand of the next
@@ -1009,8 +1009,7 @@ __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs
 
 // ---- the call -------------------------------------------------------------------
 template <int DT, int FORMS>
-__global__ __launch_bounds__(kThreads, FORMS == 1 ? kNarrowPerCu : 2) void k_attend(PageView v, int layer,
-                                                                                   AttendArgs a, Scratch ws) {
+__global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
   __shared__ __attribute__((aligned(1024))) Shared<FORMS> sh;
   const int tid = threadIdx.x, grid = gridDim.x;
   // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
@@ -1371,7 +1370,7 @@ int attend_forms(const ferry_pages* p, const ferry_attend* a) {
 
 // Workgroups of a call, and its scratch at `base` (null: sizes only).
 int plan_attend(const ferry_pages* p, const ferry_attend* a, uint8_t* base, Scratch* ws, uint64_t* bytes) {
-  const int grid = (attend_forms(p, a) == 1 ? kNarrowPerCu : 2) * gpu_cus(p->device);
+  const int grid = kPerCu * gpu_cus(p->device);
   const uint64_t rows = (uint64_t)a->n_tokens * (a->q_heads / p->kv_heads), H = p->kv_heads;
   const uint64_t tile = p->dtype == FERRY_F32 ? 16 : std::min<uint64_t>(kWide, rows);
   uint64_t at = 0;
