@@ -8,7 +8,7 @@
 // a group with the rows of all its members, or the remaining pages of one request
 // with its own rows.  A row's output joins its (at most two) segments.
 //
-// Schedule.  A segment's rows are cut into tiles (16 to 128 rows), its pages into
+// Schedule.  A segment's rows are cut into tiles (16, 32 or 128 rows), its pages into
 // steps of four; a unit of work is one step of one tile of one kv head.  All units
 // of the call, in the order (segment, kv head, tile, step), are cut into equal runs,
 // one per workgroup of a grid that fills the GPU once: ragged lengths balance, and
@@ -186,14 +186,15 @@ struct Seg {
   int req;        // request, or group
 };
 
-// Rows per tile: what one wavefront's 16- or 32-column products hold where there are
-// few rows (the tile is then bound by its pages' bytes and the wavefronts share out
-// the pages), else the 128 rows of four wavefronts that share pages in LDS.  fp32
-// pages have the 16-row form only.
+// Rows per tile: what each wavefront can hold where there are few rows (the tile is then
+// bound by its pages' bytes and the wavefronts share out the pages), else the 128 rows
+// of four wavefronts that share pages in LDS.  16 agents of 4 rows on 517 shared pages:
+// 134 us in the 128-row form, 189 in a 64-row form of the first kind; 8 agents: 181 us
+// with 32 rows, 227 in the 128-row form.  fp32 pages have the 16-row form only.
 template <int DT>
 __device__ inline int tile_rows(int rows) {
   if (Kv<DT>::F32 || rows <= 16) return 16;
-  return rows <= 32 ? 32 : rows <= 64 ? 64 : kWide;
+  return rows <= 32 ? 32 : kWide;
 }
 
 __device__ inline int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -272,17 +273,25 @@ __device__ inline int tile_steps(const Seg& g, int j, int G) {
 }
 // Units of work: step_units() for a step, tile_units() for a tile's beginning and end.
 // Step i of a tile belongs to the workgroup whose run holds the first of its units.
-__device__ inline int step_units(const Seg& g) { return g.tile == kWide ? 3 : 2; }
-__device__ inline int tile_units(const Seg& g) { return g.tile == kWide ? 9 : 4; }
-constexpr int kMostStepUnits = 3;
+// A unit is a fifth of a microsecond of a workgroup, measured in batches of all forms
+// (samples of one prompt, agents in groups, prompts in chunks) on a full GPU.
+template <int DT>
+__device__ constexpr int step_units(int tile) {
+  constexpr bool F8 = Kv<DT>::F8;
+  return Kv<DT>::F32 ? 16 : tile == 16 ? (F8 ? 4 : 8) : tile == 32 ? (F8 ? 7 : 11) : (F8 ? 11 : 9);
+}
+template <int DT>
+__device__ constexpr int tile_units(int tile) { return tile == 16 ? 26 : tile == 32 ? 35 : 65; }
+template <int DT>
 __device__ inline int tile_work(const Seg& g, int j, int G) {
-  return tile_steps(g, j, G) * step_units(g) + tile_units(g);
+  return tile_steps(g, j, G) * step_units<DT>(g.tile) + tile_units<DT>(g.tile);
 }
 // ... of all tiles of a segment, per kv head
+template <int DT>
 __device__ inline uint64_t seg_work(const Seg& g, int G) {
-  if (!g.own) return (uint64_t)g.tiles * tile_work(g, 0, G);
+  if (!g.own) return (uint64_t)g.tiles * tile_work<DT>(g, 0, G);
   uint64_t n = 0;
-  for (int j = 0; j < g.tiles; ++j) n += tile_work(g, j, G);
+  for (int j = 0; j < g.tiles; ++j) n += tile_work<DT>(g, j, G);
   return n;
 }
 
@@ -354,9 +363,8 @@ struct Shared {
   float ml[4][32][2];
   int lim[kWide];  // tokens that each row sees
   int lim_lo, lim_hi;
-  int odd[2];      // a step's V holds what is not finite
+  int odd[3];      // a step's V holds what is not finite (step s: place s % 3)
   int left_out;    // the tile has pages that were left out for that
-  float ks[2][kStep], vs[2][kStep];
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
   uint64_t sums[kThreads / 64];
   int seg;          // first segment of this workgroup's run
@@ -433,17 +441,18 @@ __device__ inline void load_page(const Tile& t, int kv_heads, uint32_t page, int
   }
 }
 
-// A tile of few rows.  Columns of 16 x 16 products are rows: a wavefront holds NT
-// tiles of 16, RG wavefronts hold the tile's rows, and the 4 / RG such teams share
-// out the pages, straight from memory into registers, a page ahead.  Lane l of a
-// wavefront: column n = l % 16, quarter grp = l / 16.
+// A tile of few rows.  Columns of 16 x 16 products are rows: each wavefront holds all
+// NT tiles of 16, and the four share out the pages, straight from memory into
+// registers, a page ahead.  Lane l of a wavefront: column n = l % 16, quarter
+// grp = l / 16.
 //   S^T[16 tokens][16 rows] = K Q^T: lane holds tokens 4 grp + i of row n,
 //   O^T[128 dims][16 rows] += V^T P^T: that is just the P^T operand of the next
 //   product, and V^T's is V[4 grp + i][8 n .. 8 n + 7] as loaded, so that the
 //   accumulator holds dims 32 grp + 8 i + nb of row n (o[nb][i]).
-// Bound by the pages' bytes: 64 rows take 384 matrix cycles a page and wavefront,
-// 8 KiB a page, which 256 CUs could read at 50 TB/s.
-template <int DT, int NT, int RG>
+// Bound by the pages' bytes: 32 rows take 192 matrix cycles a page and wavefront,
+// 8 KiB a page, which 256 CUs could read at 100 TB/s.  221,000 tokens of 8 kv heads
+// (906 MB), bf16: 149 us, 6.1 TB/s.
+template <int DT, int NT>
 struct Narrow {
   using K = Kv<DT>;
   u32x4 q[NT][K::F32 ? 8 : 4];
@@ -562,11 +571,11 @@ struct Narrow {
   template <class Sh>
   __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
     const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = l & 15, grp = l >> 4, rg = wave % RG, team = wave / RG;
+    const int n = l & 15, grp = l >> 4;
     const float scale = a.scale * 1.4426950408889634f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = (rg * NT + nt) * 16 + n;
+      const int row = nt * 16 + n;
       lim[nt] = row < t.rows ? sh.lim[row] : 0;
       m[nt] = -INFINITY, sum[nt] = 0.0f;
 #pragma unroll
@@ -588,9 +597,10 @@ struct Narrow {
         q[nt][w] = x;
       }
     }
-    // page i of this team: [p0, p1) in steps of kStep, RG of them a step
-    const int count = (t.p1 - t.p0 + kStep - 1) / kStep * RG;
-    auto page_no = [&](int i) { return t.p0 + kStep * (i / RG) + team * RG + i % RG; };
+    // page i of this wavefront: one of each of the steps of kStep pages in [p0, p1)
+    static_assert(kStep == kThreads / 64, "a page per wavefront and step");
+    const int count = (t.p1 - t.p0 + kStep - 1) / kStep;
+    auto page_no = [&](int i) { return t.p0 + kStep * i + wave; };
     uint32_t ids = 0;  // lane j: the table's entry for page 64 k + j
     auto fill_ids = [&](int i0) {
       const int p = page_no(i0 + l);
@@ -606,7 +616,7 @@ struct Narrow {
       };
       // pages that every row sees whole, two at a time, then the others
       const int seen = t.lim_lo / kPageTokens - t.p0;  // such pages of all teams
-      const int mine = clampi(seen / kStep * RG + clampi(seen % kStep - team * RG, 0, RG), 0, count);
+      const int mine = clampi(seen / kStep + (seen % kStep > wave ? 1 : 0), 0, count);
       fetch(0, 0);
       int i = 0;
       for (; i + 1 < mine; i += 2) {
@@ -659,25 +669,22 @@ __device__ inline void write_out(const AttendArgs& a, int64_t at, int d, const f
 
 // Joins the teams of a Narrow tile and writes its rows: to the output where they are
 // finished (`to_o` null), else as a part.
-template <int DT, int NT, int RG, class Sh>
+template <int DT, int NT, class Sh>
 __device__ __forceinline__ void narrow_write(const AttendArgs& a, const Tile& t, Sh& sh, float* to_ml, float* to_o) {
-  constexpr int TEAMS = 4 / RG, ROWS = 16 * NT * RG;
   const int tid = this_thread();
 #pragma unroll
-  for (int r0 = 0; r0 < ROWS; r0 += 16) {
+  for (int r0 = 0; r0 < 16 * NT; r0 += 16) {
     const int row = r0 + tid / 16, d = tid % 16 * 8;
     if (row >= t.rows) continue;
-    const int rg = row / (16 * NT), at = row % (16 * NT);
     float m = -INFINITY, sum = 0.0f, x[8] = {};
 #pragma unroll
-    for (int k = 0; k < TEAMS; ++k) m = fmaxf(m, sh.ml[k * RG + rg][at][0]);
+    for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, sh.ml[w][row][0]);
     const float ref = against(m);
 #pragma unroll
-    for (int k = 0; k < TEAMS; ++k) {
-      const int w = k * RG + rg;
-      const float f = exp2_fast(sh.ml[w][at][0] - ref);
-      sum += f * sh.ml[w][at][1];
-      const float* o = sh.merge + (w * 16 * NT + at) * kPad + d;
+    for (int w = 0; w < kThreads / 64; ++w) {
+      const float f = exp2_fast(sh.ml[w][row][0] - ref);
+      sum += f * sh.ml[w][row][1];
+      const float* o = sh.merge + (w * 16 * NT + row) * kPad + d;
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] += f * o[i];
     }
@@ -698,9 +705,8 @@ __device__ __forceinline__ void narrow_write(const AttendArgs& a, const Tile& t,
 }
 
 // A tile of up to 128 rows: four wavefronts of 32, which share each step's 64 tokens
-// in LDS (16-bit values, two steps: one is used while the next one's loads, begun a
-// step earlier, are on their way through registers).  Columns of 32 x 32 x 16
-// products are rows; lane l: column l % 32, half h = l / 32.
+// in LDS as 16-bit values.  Columns of 32 x 32 x 16 products are rows; lane l: column
+// l % 32, half h = l / 32.
 //   S^T[64 tokens][32 rows]: register i of token tile tt is token 32 tt + 8 (i / 4) +
 //   4 h + i % 4, so registers 8 j .. 8 j + 7 are the P^T operand of the product over
 //   tokens 16 j .. 16 j + 15 in the order (4 h + 0..3, 8 + 4 h + 0..3), and the V^T
@@ -708,6 +714,13 @@ __device__ __forceinline__ void narrow_write(const AttendArgs& a, const Tile& t,
 // A token's sixteen 16-byte chunks are stored at chunk ^ swizzle(token): the reads of
 // K (one chunk of 32 tokens) and of V (four chunks of 8 tokens) then spread over all
 // banks.
+// K is a step ahead of V: while one step's weights are computed the next one's scores
+// are, and the loads of V of the next and K of the one after it are on their way,
+// straight into LDS (fp8: through registers, widened on the way).  A step is 1,024
+// matrix cycles a wavefront, and as many of vector instructions next to them.  3,600
+// rows of 32 heads over 6,700 tokens (377 GFLOP), fp16: 477 us, 790 TFLOP/s; 564 us
+// with products, weights and loads one after the other.  The GPU's clock falls to 1.5
+// GHz meanwhile (a library product of 8192^3 reaches 1,137 TFLOP/s).
 // An LDS address as a number, and what is there: 16 bytes, or 4 values of a column
 // (the 16 lanes of a group name 4 tokens of 16 dims, 4 dims each).
 __device__ inline uint32_t lds_at(const void* p) {
@@ -722,6 +735,13 @@ __device__ inline u32x2 lds_turned(uint32_t at) {
                                        (__attribute__((address_space(3))) i16x4*)(uintptr_t)at));
 }
 
+// 16 bytes per lane from memory straight into LDS, lane after lane from `to` on.  The
+// wait is the caller's: the compiler does not know of them.
+__device__ inline void load_lds(uint32_t to, const void* base, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(first_lane_i((int)to)), "v"(at), "s"(uniform(base)) : "memory");
+}
+
 __device__ inline int swizzle(int tok) { return (tok & 3) << 2 | (tok >> 2 & 3); }
 
 template <int DT>
@@ -732,6 +752,39 @@ struct Wide {
   f32x16 o[4];
   float m, sum;
   int lim;
+
+  // The largest of a lane's scores of step s.  fp8: they get their pages' scales; MASKED:
+  // what the row does not see becomes -inf.
+  template <bool MASKED>
+  struct Largest {
+    float c[kStep], scale;  // factor on a page's scores
+    int mine;               // of the lane's tokens, in steps of 4 and gaps of 4
+    __device__ __forceinline__ Largest(const Wide& w, const Tile& t, int s, int steps, int h, float scale, float scales)
+        : scale(scale), mine(s < steps ? w.lim - (t.p0 + kStep * s) * kPageTokens - 4 * h : 0) {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * scale_of(scales, s, i) : scale;
+    }
+    __device__ __forceinline__ void among(f32x16 (&x)[2], int from, int n, float& top) const {
+#pragma unroll
+      for (int i = from; i < from + n; ++i) {
+        float y = x[i >> 4][i & 15];
+        if (K::F8) y *= c[i >> 3];
+        if (MASKED && 8 * (i >> 2) + (i & 3) >= mine) y = -INFINITY;
+        x[i >> 4][i & 15] = y;
+        top = fmaxf(top, y);
+      }
+    }
+    __device__ __forceinline__ float of_row(float top) const {  // scaled
+      const mx_u32x2 two = pair_values<32>(top);
+      top = fmaxf(bits_f32(two[0]), bits_f32(two[1]));
+      return K::F8 ? top : top * scale;
+    }
+  };
+
+  // fp8: of the scales of a window's pages that of page i of step s
+  static __device__ __forceinline__ float scale_of(float scales, int s, int i) {
+    return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(scales), (kStep * s + i) & 63));
+  }
 
   template <class Sh>
   __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile& t, Sh& sh) {
@@ -752,29 +805,42 @@ struct Wide {
       q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned, sign)
                           : u32x4{0u, 0u, 0u, 0u};
     const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
-    uint32_t ids = 0;
-    auto fill_ids = [&](int s) {  // lane j: page 4 s + j
-      const int p = t.p0 + kStep * s + l;
-      ids = p < t.p1 ? checked_page(v, global_at<uint32_t>(t.table, 4 * p)) : 0u;
+    // Page ids: lane j holds page 64 w + j of window w; the next window is read ahead.
+    auto read_ids = [&](int w) __attribute__((always_inline)) {
+      const int p = t.p0 + 64 * w + l;
+      return p < t.p1 ? global_at<uint32_t>(t.table, 4 * p) : 0u;
     };
-    Word kr[kStep], vr[kStep];
-    float sc[kStep] = {};
-    // thread: token tid / 16 of each page, chunk tid % 16
-    const int tok = tid >> 4, chunk = tid & 15;
-    const uint32_t at_word = tid * (uint32_t)sizeof(Word);
-    auto fetch = [&](int s) __attribute__((always_inline)) {
-      if (s && (s & 15) == 0) fill_ids(s);
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        if (t.p0 + kStep * s + i < t.p1) {
-          const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)ids, (kStep * s + i) & 63);
-          const uint8_t* p = t.base + (uint64_t)page * t.page_bytes;
-          kr[i] = global_at<Word>(p, at_word);
-          vr[i] = global_at<Word>(p + K::HALF, at_word);
-          if constexpr (K::F8)
-            if (tid < 2) sc[i] = global_at<float>(t.scales + (uint64_t)page * (2u * v.H), 4 * tid);
-        }
-      }
+    uint32_t ids = checked_page(v, read_ids(0)), ids_next = 0;
+    uint32_t pages[kStep];  // of the step whose K was loaded last
+    // The thread's 16 bytes of a page in LDS: token tid / 16, chunk tid % 16 ^ swizzle.
+    const int tok = tid >> 4;
+    const uint32_t at_word = tok * K::ROW + ((tid & 15) ^ swizzle(tok)) * (uint32_t)sizeof(Word);
+    const uint32_t k_base = lds_at(sh.kv.k[0]) + wave * 1024, v_base = lds_at(sh.kv.v[0]) + wave * 1024;
+    Word kr[K::F8 ? kStep : 1], vr[K::F8 ? kStep : 1];  // fp8: on their way
+    // fp8: the scales of the windows' pages, of K where step s + 1 is, of V where s is
+    f32x2 scales = {};
+    float k_scales = 0.0f, v_scales = 0.0f;
+    auto read_scales = [&]() __attribute__((always_inline)) {
+      if constexpr (K::F8) scales = *reinterpret_cast<const f32x2*>(t.scales + (uint64_t)ids * (2u * v.H));
+    };
+    // Page i of the step whose K or V is loaded next.  Pages from p1 on are page 0: they
+    // are loaded for nothing.
+    auto window = [&](int s) __attribute__((always_inline)) {  // before K of step s > 1
+      if ((s - 1 & 15) == 0) k_scales = scales[0];
+      if ((s - 2 & 15) == 0) v_scales = scales[1];
+      if ((s & 15) == 0) ids = checked_page(v, ids_next), read_scales();
+      if ((s & 15) == 8) ids_next = read_ids(s / 16 + 1);
+    };
+    auto begin_k = [&](int i, int s, Word& to) __attribute__((always_inline)) {
+      pages[i] = (uint32_t)__builtin_amdgcn_readlane((int)ids, (kStep * s + i) & 63);
+      const uint8_t* p = t.base + (uint64_t)pages[i] * t.page_bytes;
+      if constexpr (K::F8) to = global_at<Word>(uniform(p), at_word);
+      else load_lds(k_base + ((s & 1) << 14) + (i << 12), p, at_word);
+    };
+    auto begin_v = [&](int i, int s) __attribute__((always_inline)) {  // the step of the last begin_k
+      const uint8_t* p = t.base + (uint64_t)pages[i] * t.page_bytes + K::HALF;
+      if constexpr (K::F8) vr[i] = global_at<Word>(uniform(p), at_word);
+      else load_lds(v_base + ((s & 1) << 14) + (i << 12), p, at_word);
     };
     auto widen = [&](const Word& w) -> u32x4 {
       if constexpr (K::F8) {
@@ -784,123 +850,192 @@ struct Wide {
         return w;
       }
     };
-    auto store = [&](int s, int b) __attribute__((always_inline)) {
-      const int t0 = (t.p0 + kStep * s) * kPageTokens;
-      const bool masked = t0 + kStep * kPageTokens > t.lim_lo;
-      bool bad = false;
+    // fp8: stores what was loaded, with room in LDS for 16-bit values.
+    auto store_k = [&](const Word (&w)[K::F8 ? kStep : 1], int s) __attribute__((always_inline)) {
+      if constexpr (K::F8) {
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) {
-        const int at_ = ((kPageTokens * i + tok) << 8) + ((chunk ^ swizzle(tok)) << 4);
-        u32x4 x = widen(vr[i]);
-        if (masked) {
+        for (int i = 0; i < kStep; ++i) *reinterpret_cast<u32x4*>(sh.kv.k[s & 1] + 4096 * i + tid * 16) = widen(w[i]);
+      }
+    };
+    // Ends the loads of V of step s: what no row sees of it becomes zero.
+    auto land = [&](int s) __attribute__((always_inline)) {
+      const uint32_t to = tid * 16;
+      if constexpr (K::F8) {
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) *reinterpret_cast<u32x4*>(sh.kv.v[s & 1] + 4096 * i + to) = widen(vr[i]);
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const int t0 = (t.p0 + kStep * s) * kPageTokens;
+      if (s < steps && t0 + kStep * kPageTokens > t.lim_lo) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+          u32x4* at = reinterpret_cast<u32x4*>(sh.kv.v[s & 1] + 4096 * i + to);
+          u32x4 x = *at;
           const bool seen = t0 + kPageTokens * i + tok < t.lim_hi && t.p0 + kStep * s + i < t.p1;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             bad |= seen && not_finite<DT>(x[w]);
             x[w] = seen ? x[w] : 0u;
           }
+          *at = x;
         }
-        *reinterpret_cast<u32x4*>(sh.kv.k[b] + at_) = widen(kr[i]);
-        *reinterpret_cast<u32x4*>(sh.kv.v[b] + at_) = x;
-        if constexpr (K::F8) {
-          if (tid == 0) sh.ks[b][i] = sc[i];
-          if (tid == 1) sh.vs[b][i] = sc[i];
-        }
+        if (bad) sh.odd[s % 3] = 1;
       }
-      if (bad) sh.odd[b] = 1;
+      __syncthreads();
     };
     // K: token col, chunk h; V: token 4 h + (l % 16) / 4, dims 16 (l / 16 % 2) + 4 (l % 4)
     const uint32_t k_lane = lds_at(sh.kv.k[0]) + (col << 8) + ((h ^ swizzle(col)) << 4);
     const int vt = 4 * h + (l >> 2 & 3), vd = 16 * (l >> 4 & 1) + 4 * (l & 3);
     const uint32_t v_lane = lds_at(sh.kv.v[0]) + (vt << 8) + (((vd >> 3) ^ swizzle(vt)) << 4) + (vd & 4) * 2;
-    if (tid < 2) sh.odd[tid] = 0;
-    fill_ids(0);
-    fetch(0);
-    __syncthreads();
-    store(0, 0);
-    __syncthreads();
-    // One step; MASKED: some row does not see all of its tokens.
-    auto step = [&](auto masked_, int s) __attribute__((always_inline)) {
+    // S^T of step s
+    auto products = [&](f32x16 (&x)[2], int s) __attribute__((always_inline)) {
+      // The lane's place in this step's K; the others follow by flipping address bits.
+      // Opaque, so that they are not all kept in registers over the loop.
+      uint32_t at = k_lane + ((s & 1) << 14);
+      asm("" : "+v"(at));
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[tt][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)  // chunk 2 c + h of token 32 tt + col
+          x[tt] = mma32<K::BF>(lds<u32x4>((at ^ c << 5) + 8192 * tt), q[c], x[tt]);
+      }
+    };
+    auto raise_to = [&](float top, bool raise) __attribute__((always_inline)) {
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+        const float f = raise ? exp2_fast(m - top) : 1.0f;
+        m = raise ? top : m;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= f;
+      }
+    };
+    // weights of scores y0, y1, the lane's i-th and next of step s
+    auto weights2 = [&](float y0, float y1, float ref, int s, int i) __attribute__((always_inline)) {
+      float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
+      float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
+      sum += p0 + p1;
+      if constexpr (K::F8) {
+        const float f = scale_of(v_scales, s, i >> 3);
+        p0 *= f, p1 *= f;
+      }
+      return pack2<K::BF>(p0, p1);
+    };
+    auto begin_step = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        begin_v(i, s);
+        begin_k(i, s + 1, kr[K::F8 ? i : 0]);
+      }
+    };
+    // the steps that every row sees whole
+    const int whole = clampi((t.lim_lo - t.p0 * kPageTokens) / (kStep * kPageTokens), 0, steps);
+    f32x16 x[2], y[2];
+    {
+      Word k0[K::F8 ? kStep : 1];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) begin_k(i, 0, k0[K::F8 ? i : 0]);
+      read_scales();
+      begin_step(0);
+      k_scales = scales[0], v_scales = scales[1];
+      store_k(k0, 0);
+      store_k(kr, 1);
+      if (tid < 3) sh.odd[tid] = 0;
+      land(0);
+      if (busy) {
+        products(x, 0);
+        const Largest<true> see(*this, t, 0, steps, h, scale, k_scales);
+        float top = -INFINITY;
+        see.among(x, 0, 32, top);
+        top = see.of_row(top);
+        raise_to(top, top > m + kRaise);
+      }
+    }
+    // Step s, whose scores are in x, while those of step s + 1 come into y (MASKED: some row
+    // may not see them all): next to each product a part of the weights, then of the
+    // maximum, is computed and a load begun, and operands are read three products ahead.
+    auto step = [&](auto masked_, f32x16 (&x)[2], f32x16 (&y)[2], int s) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked_)::value;
-      const int b = s & 1, t0 = (t.p0 + kStep * s) * kPageTokens;
-      if (s + 1 < steps) fetch(s + 1);
-      const bool odd = MASKED && sh.odd[b];  // left out, as V holds what is not finite
-      uint32_t pop[16];
-      // The lane's places in this step's K and V; the others follow by flipping address
-      // bits.  Opaque, so that they are not all kept in registers over the loop.
-      uint32_t k_at = k_lane + (b << 14), v_at = v_lane + (b << 14);
-      asm volatile("" : "+v"(k_at), "+v"(v_at));
-      if (busy && !odd) {
-        f32x16 x[2];
+      window(s + 2);
+      if (MASKED) {
+        if (tid == 0) sh.odd[(s + 2) % 3] = 0;
+        if (first_lane_i(sh.odd[s % 3])) {  // left out, as V holds what is not finite
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
+          for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[tt][i] = 0.0f;
-#pragma unroll
-          for (int c = 0; c < 8; ++c)  // chunk 2 c + h of token 32 tt + col
-            x[tt] = mma32<K::BF>(lds<u32x4>((k_at ^ c << 5) + 8192 * tt), q[c], x[tt]);
+          for (int i = 0; i < kStep; ++i) *reinterpret_cast<u32x4*>(sh.kv.v[s & 1] + 4096 * i + tid * 16) = u32x4{0u, 0u, 0u, 0u};
+          if (tid == 0) sh.left_out = 1;
+          __syncthreads();
         }
-        const int mine = lim - t0 - 4 * h;  // of the lane's tokens, in steps of 4 and gaps of 4
-        float c[kStep], top = -INFINITY;  // c: factor on a page's scores
+      }
+      if (busy) {
+        uint32_t k_at = k_lane + ((s + 1 & 1) << 14), v_at = v_lane + ((s & 1) << 14), pop[16];
+        asm("" : "+v"(k_at), "+v"(v_at));
+        auto read_k = [&](int i) __attribute__((always_inline)) {
+          return lds<u32x4>((k_at ^ (i >> 1) << 5) + 8192 * (i & 1));
+        };
+        auto read_v = [&](int i) __attribute__((always_inline)) {
+          // tokens 16 j + 4 h .. + 3 and those 8 behind, whose swizzle flips chunk bit 1
+          const u32x2 lo = lds_turned((v_at ^ (i & 3) << 6) + 4096 * (i >> 2));
+          const u32x2 hi = lds_turned((v_at ^ (i & 3) << 6 ^ 32) + 4096 * (i >> 2) + 2048);
+          return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        auto begin = [&](int i) __attribute__((always_inline)) {
+          if (i >= 2 * kStep) return;
+          if (i & 1) begin_k(i >> 1, s + 2, kr[K::F8 ? i >> 1 : 0]);
+          else begin_v(i >> 1, s + 1);
+        };
+        u32x4 a[4];
 #pragma unroll
-        for (int i = 0; i < kStep; ++i) c[i] = K::F8 ? scale * sh.ks[b][i] : scale;
+        for (int i = 0; i < 3; ++i) a[i] = read_k(i);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float y = x[i >> 4][i & 15];
-          if (K::F8) y *= c[i >> 3];
-          if (MASKED && 8 * (i >> 2) + (i & 3) >= mine) y = -INFINITY;
-          x[i >> 4][i & 15] = y;
-          top = fmaxf(top, y);
-        }
-        {
-          const mx_u32x2 two = pair_values<32>(top);
-          top = fmaxf(bits_f32(two[0]), bits_f32(two[1]));
-        }
-        if (!K::F8) top *= scale;
-        const bool raise = top > m + kRaise;
-        if (__builtin_amdgcn_ballot_w64(raise)) {
-          const float f = raise ? exp2_fast(m - top) : 1.0f;
-          m = raise ? top : m;
-          sum *= f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] *= f;
-        }
+        for (int i = 0; i < 16; ++i) y[0][i] = y[1][i] = 0.0f;
         const float ref = against(m);
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float y0 = x[i >> 4][i & 15], y1 = x[i >> 4][(i & 15) + 1];
-          float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
-          float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
-          sum += p0 + p1;
-          if constexpr (K::F8) {
-            const float f = sh.vs[b][i >> 3];
-            p0 *= f, p1 *= f;
-          }
-          pop[i / 2] = pack2<K::BF>(p0, p1);
+        for (int i = 0; i < 16; ++i) {
+          a[i + 3 & 3] = i + 3 < 16 ? read_k(i + 3) : read_v(i - 13);
+          y[i & 1] = mma32<K::BF>(a[i & 3], q[i >> 1], y[i & 1]);
+          if (!K::F8) begin(i);
+          pop[i] = weights2(x[i >> 3][2 * i & 15], x[i >> 3][(2 * i & 15) + 1], ref, s, 2 * i);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        const Largest<MASKED> see(*this, t, s + 1, steps, h, scale, k_scales);
+        float top = -INFINITY;
+        bool raise = false;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4 pj = {pop[4 * j], pop[4 * j + 1], pop[4 * j + 2], pop[4 * j + 3]};
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt) {
-            // tokens 16 j + 4 h .. + 3 and those 8 behind, whose swizzle flips chunk bit 1
-            const u32x2 lo = lds_turned((v_at ^ dt << 6) + 4096 * j);
-            const u32x2 hi = lds_turned((v_at ^ dt << 6 ^ 32) + 4096 * j + 2048);
-            o[dt] = mma32<K::BF>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pj, o[dt]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          if (i + 3 < 16) a[i + 3 & 3] = read_v(i + 3);
+          o[i & 3] = mma32<K::BF>(a[i & 3], u32x4{pop[i & 12], pop[(i & 12) + 1], pop[(i & 12) + 2], pop[(i & 12) + 3]},
+                                  o[i & 3]);
+          if (K::F8) begin(i);  // into the registers that x has left
+          if (i >= 2 && i < 10) see.among(y, 4 * (i - 2), 4, top);
+          if (i == 11) top = see.of_row(top);
+          if (i == 12) raise = top > m + kRaise;
+          __builtin_amdgcn_sched_barrier(0);
         }
+        raise_to(top, raise);
+      } else {
+        begin_step(s + 1);
       }
-      if (MASKED) {
-        __syncthreads();
-        if (odd && tid == 0) sh.odd[b] = 0, sh.left_out = 1;
-      }
-      if (s + 1 < steps) store(s + 1, b ^ 1);
-      __syncthreads();
+      store_k(kr, s + 2);
+      land(s + 1);
     };
-    // the steps that every row sees whole, then the others
-    const int whole = clampi((t.lim_lo - t.p0 * kPageTokens) / (kStep * kPageTokens), 0, steps);
-    for (int s = 0; s < whole; ++s) step(std::false_type{}, s);
-    for (int s = whole; s < steps; ++s) step(std::true_type{}, s);
+    int s = 0;
+    if constexpr (K::F8) {
+      for (; s + 1 < whole; ++s) {
+        step(std::false_type{}, x, y, s);
+        x[0] = y[0], x[1] = y[1];
+      }
+    } else {  // two at a time need no copies, but registers that fp8 does not have
+      for (; s + 2 < whole; s += 2) step(std::false_type{}, x, y, s), step(std::false_type{}, y, x, s + 1);
+    }
+    for (; s < steps; ++s) {
+      step(std::true_type{}, x, y, s);
+      x[0] = y[0], x[1] = y[1];
+    }
     {
       const mx_u32x2 two = pair_values<32>(sum);
       sum = bits_f32(two[0]) + bits_f32(two[1]);
@@ -1033,7 +1168,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   uint64_t kept_work = 0;
   for (int s = s0; s < s1; ++s) {
     kept = segment<DT>(v, a, gs, gp, s);
-    kept_work = seg_work(kept, a.G);
+    kept_work = seg_work<DT>(kept, a.G);
     mine += kept_work * v.H;
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
@@ -1065,7 +1200,9 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   before -= mine;
   total = first_lane_u64(total);
   // no run is shorter than a step, so that each one within a tile begins one
-  const uint64_t per = max((uint64_t)kMostStepUnits, first_lane_u64((total + grid - 1) / grid));
+  constexpr int kMost = FORMS == 1 ? step_units<DT>(16) : 11;
+  static_assert(FORMS == 1 || (step_units<DT>(16) <= kMost && step_units<DT>(32) <= kMost && step_units<DT>(kWide) <= kMost));
+  const uint64_t per = max((uint64_t)kMost, first_lane_u64((total + grid - 1) / grid));
   const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
   if (u0 >= u1) return;
   const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
@@ -1077,7 +1214,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       SegAt x;
       const bool have = decltype(first)::value && per_thread == 1;
       x.g = have ? kept : segment<DT>(v, a, gs, gp, s);
-      x.work = have ? kept_work : seg_work(x.g, a.G);
+      x.work = have ? kept_work : seg_work<DT>(x.g, a.G);
       x.at = at;
       if (s >= from && s < from + kListed) sh.list[s - from] = x;
       at += x.work * v.H;
@@ -1089,7 +1226,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     int s = s0;
     if (per_thread > 1)
       for (;; ++s) {
-        at += seg_work(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+        at += seg_work<DT>(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
         if (u0 < at) break;
       }
     sh.seg = s;
@@ -1121,14 +1258,14 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       tile_at = x.at + h * x.work;  // unit of the tile's first step
       j = 0;
     }
-    int work = tile_work(g, j, a.G);
+    int work = tile_work<DT>(g, j, a.G);
     while (u >= tile_at + work) {
       tile_at += work;
       if (++j == g.tiles) j = 0, ++h;
-      work = tile_work(g, j, a.G);
+      work = tile_work<DT>(g, j, a.G);
     }
     // this workgroup's steps [k0, k1) of the tile's `len`
-    const int per_step = step_units(g), len = first_lane_i(tile_steps(g, j, a.G));
+    const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps(g, j, a.G));
     const int k0 = first_lane_i(((int)(u - tile_at) + per_step - 1) / per_step);
     const int k1 = first_lane_i((int)min((uint64_t)len, (u1 - tile_at + per_step - 1) / per_step));
     u = tile_at + work;
@@ -1232,20 +1369,19 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
         finish_row<DT>(a, t.row0 + row, t.h, ml[2 * row], ml[2 * row + 1], r[0], r[1], sh.lim[row] <= 0);
       }
     };
-    auto narrow = [&](auto nt, auto rg) __attribute__((always_inline)) {
-      constexpr int NT = decltype(nt)::value, RG = decltype(rg)::value;
-      Narrow<DT, NT, RG> x;
+    auto narrow = [&](auto nt) __attribute__((always_inline)) {
+      constexpr int NT = decltype(nt)::value;
+      Narrow<DT, NT> x;
       x.run(v, a, t, sh);
-      finish(1, [&](float* ml, float* o) __attribute__((always_inline)) { narrow_write<DT, NT, RG>(a, t, sh, ml, o); });
+      finish(1, [&](float* ml, float* o) __attribute__((always_inline)) { narrow_write<DT, NT>(a, t, sh, ml, o); });
     };
     std::integral_constant<int, 1> one;
     std::integral_constant<int, 2> pair;
     if constexpr (FORMS == 1) {
-      narrow(one, one);
+      narrow(one);
     } else {
-      if (g.tile == 16) narrow(one, one);
-      else if (g.tile == 32) narrow(pair, one);
-      else if (FORMS == 2 || g.tile == 64) narrow(pair, pair);
+      if (g.tile == 16) narrow(one);
+      else if (FORMS == 2 || g.tile == 32) narrow(pair);
       else if constexpr (FORMS == 3) {
         Wide<DT> x;
         x.run(v, a, t, sh);
@@ -1365,7 +1501,7 @@ uint64_t up256(uint64_t x) { return (x + 255) & ~255ull; }
 // without groups and with one token per request those of one token.
 int attend_forms(const ferry_pages* p, const ferry_attend* a) {
   const int64_t G = a->q_heads / p->kv_heads, rows = a->n_groups || a->q_start ? a->n_tokens * G : G;
-  return p->dtype == FERRY_F32 || rows <= 16 ? 1 : rows <= 64 ? 2 : 3;
+  return p->dtype == FERRY_F32 || rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
 }
 
 // Workgroups of a call, and its scratch at `base` (null: sizes only).
