@@ -68,6 +68,8 @@ struct AttendArgs {
   float* lse;
   int64_t qs[2], os[2];
   int aligned;  // q and out rows are 16-byte aligned
+  uint32_t g_mul;  // row / G = row * g_mul >> g_shift, for rows below 2^30
+  int g_shift;
 };
 
 // Where a row's parts of one segment are (per kv head).
@@ -175,6 +177,10 @@ __device__ inline bool not_finite(uint32_t w) {
   return (w & e) == e || (w >> 16 & e) == e;
 }
 
+__device__ inline int token_of_row(const AttendArgs& a, int row) {
+  return (int)((uint64_t)(uint32_t)row * a.g_mul >> a.g_shift);
+}
+
 // ---- segments -------------------------------------------------------------------
 struct Seg {
   int own;        // 1: one request's own pages, 0: a group's shared pages
@@ -184,6 +190,8 @@ struct Seg {
   int base, len;  // own: the first row's token sees `base` tokens; tokens of the lane
   int lane;       // whose table is read; -1: no pages
   int req;        // request, or group
+  int tok0;       // first row's token
+  int group;      // own: the group that the request belongs to, -1: none
 };
 
 // Rows per tile: what each wavefront can hold where there are few rows (the tile is then
@@ -225,7 +233,9 @@ __device__ inline int group_pages(const PageView& v, const AttendArgs& a, int b,
 // Shared pages of request r: those of the last group that starts at or before it,
 // if that has not ended.
 template <int DT>
-__device__ inline int shared_of(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int r) {
+__device__ inline int shared_of(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int r,
+                                int* group) {
+  *group = -1;
   if (a.n_groups == 0 || gs[0] > r) return 0;
   int lo = 0, hi = a.n_groups - 1;
   while (lo < hi) {
@@ -233,7 +243,9 @@ __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const in
     if (gs[mid] <= r) lo = mid; else hi = mid - 1;
   }
   const int b = clampi(gs[lo], 0, a.n_req), e = clampi(gs[lo + 1], b, a.n_req);
-  return r < e ? group_pages<DT>(v, a, b, e, gp[lo]) : 0;
+  if (r >= e) return 0;
+  *group = lo;
+  return group_pages<DT>(v, a, b, e, gp[lo]);
 }
 
 // Segment s: groups first, then requests.  gs, gp: the groups' offsets and pages.
@@ -246,14 +258,15 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
     g.lane = -1, g.base = g.len = 0;
     for (int r = b; r < e && g.lane < 0; ++r) g.lane = lane_of(v, a, r);
     const int t0 = token_of(a, b), t1 = max(t0, token_of(a, e));
-    g.row0 = t0 * a.G;
+    g.tok0 = t0, g.row0 = t0 * a.G, g.group = s;
     g.rows = g.p1 > 0 && g.lane >= 0 ? (t1 - t0) * a.G : 0;
   } else {
     const int r = s - a.n_groups, t0 = token_of(a, r), t1 = max(t0, token_of(a, r + 1));
     g.own = 1, g.req = r, g.lane = lane_of(v, a, r), g.len = len_of(v, g.lane);
-    g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G;
+    g.tok0 = t0, g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G;
     g.base = g.len - (t1 - t0) + 1;
-    g.p0 = g.lane < 0 ? 0 : shared_of<DT>(v, a, gs, gp, r);
+    const int shared = shared_of<DT>(v, a, gs, gp, r, &g.group);
+    g.p0 = g.lane < 0 ? 0 : shared;
     g.p1 = max(g.p0, pages_of(g.len));
   }
   g.tile = tile_rows<DT>(g.rows);
@@ -263,10 +276,10 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
 
 // Steps of tile j: up to the last token its last row sees, and at least one, so
 // that every tile has a workgroup that writes its rows.
-__device__ inline int tile_steps(const Seg& g, int j, int G) {
+__device__ inline int tile_steps(const AttendArgs& a, const Seg& g, int j) {
   int p1 = g.p1;
   if (g.own) {
-    const int last = clampi(g.base + (min((j + 1) * g.tile, g.rows) - 1) / G, 0, g.len);
+    const int last = clampi(g.base + token_of_row(a, min((j + 1) * g.tile, g.rows) - 1), 0, g.len);
     p1 = min(p1, pages_of(last));
   }
   return max(1, (p1 - g.p0 + kStep - 1) / kStep);
@@ -283,15 +296,15 @@ __device__ constexpr int step_units(int tile) {
 template <int DT>
 __device__ constexpr int tile_units(int tile) { return tile == 16 ? 26 : tile == 32 ? 35 : 65; }
 template <int DT>
-__device__ inline int tile_work(const Seg& g, int j, int G) {
-  return tile_steps(g, j, G) * step_units<DT>(g.tile) + tile_units<DT>(g.tile);
+__device__ inline int tile_work(const AttendArgs& a, const Seg& g, int j) {
+  return tile_steps(a, g, j) * step_units<DT>(g.tile) + tile_units<DT>(g.tile);
 }
 // ... of all tiles of a segment, per kv head
 template <int DT>
-__device__ inline uint64_t seg_work(const Seg& g, int G) {
-  if (!g.own) return (uint64_t)g.tiles * tile_work<DT>(g, 0, G);
+__device__ inline uint64_t seg_work(const AttendArgs& a, const Seg& g) {
+  if (!g.own) return (uint64_t)g.tiles * tile_work<DT>(a, g, 0);
   uint64_t n = 0;
-  for (int j = 0; j < g.tiles; ++j) n += tile_work<DT>(g, j, G);
+  for (int j = 0; j < g.tiles; ++j) n += tile_work<DT>(a, g, j);
   return n;
 }
 
@@ -368,7 +381,7 @@ struct Shared {
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
   uint64_t sums[kThreads / 64];
   int seg;          // first segment of this workgroup's run
-  int group_lim;    // least number of tokens that a row of the current group sees
+  int gl[kGroupsInLds];  // least number of tokens that a row of a group sees
   SegAt list[kListed];  // consecutive segments of the run
 };
 
@@ -389,7 +402,7 @@ __device__ inline u32x4 load_q8(const uint16_t* p, bool aligned, uint32_t sign) 
 
 // Element offset of row `row`'s query (or output) in a tensor of strides s.
 __device__ inline int64_t row_at(const AttendArgs& a, const int64_t (&s)[2], int row, int h) {
-  const int t = row / a.G;
+  const int t = token_of_row(a, row);
   return t * s[0] + (int64_t)(h * a.G + (row - t * a.G)) * s[1];
 }
 
@@ -692,7 +705,7 @@ __device__ __forceinline__ void narrow_write(const AttendArgs& a, const Tile& t,
       const bool none = sh.lim[row] <= 0;
       write_out<DT>(a, row_at(a, a.os, t.row0 + row, t.h), d, x, none ? 0.0f : 1.0f / sum);
       if (a.lse && d == 0) {
-        const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
+        const int tok = token_of_row(a, t.row0 + row), g = t.row0 + row - tok * a.G;
         a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
       }
     } else {
@@ -1071,7 +1084,7 @@ struct Wide {
         }
       }
     if (a.lse && h == 0) {
-      const int tok = (t.row0 + row) / a.G, g = (t.row0 + row) % a.G;
+      const int tok = token_of_row(a, t.row0 + row), g = t.row0 + row - tok * a.G;
       a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
     }
   }
@@ -1093,7 +1106,7 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int row, int h, 
     p[0] = (uint16_t)w, p[1] = (uint16_t)(w >> 16);
   }
   if (a.lse && l == 0)
-    a.lse[(int64_t)(row / a.G) * a.Hq + h * a.G + row % a.G] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    a.lse[(int64_t)token_of_row(a, row) * a.Hq + h * a.G + row - token_of_row(a, row) * a.G] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 // The pages that a tile's products left out: a value that is not finite must not
@@ -1155,7 +1168,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   if (a.n_groups && a.n_groups <= kGroupsInLds) {
     for (int i = tid; i <= a.n_groups; i += kThreads) {
       sh.gs[i] = a.group_start[i];
-      if (i < a.n_groups) sh.gp[i] = a.shared[i];
+      if (i < a.n_groups) sh.gp[i] = a.shared[i], sh.gl[i] = 0x7FFFFFFF;
     }
     gs = sh.gs, gp = sh.gp;
     __syncthreads();
@@ -1168,8 +1181,9 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   uint64_t kept_work = 0;
   for (int s = s0; s < s1; ++s) {
     kept = segment<DT>(v, a, gs, gp, s);
-    kept_work = seg_work<DT>(kept, a.G);
+    kept_work = seg_work<DT>(a, kept);
     mine += kept_work * v.H;
+    if (kept.own && kept.group >= 0 && kept.rows > 0 && gs == sh.gs) atomicMin(&sh.gl[kept.group], max(0, kept.base));
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
       if (kept.own) {
@@ -1214,7 +1228,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       SegAt x;
       const bool have = decltype(first)::value && per_thread == 1;
       x.g = have ? kept : segment<DT>(v, a, gs, gp, s);
-      x.work = have ? kept_work : seg_work<DT>(x.g, a.G);
+      x.work = have ? kept_work : seg_work<DT>(a, x.g);
       x.at = at;
       if (s >= from && s < from + kListed) sh.list[s - from] = x;
       at += x.work * v.H;
@@ -1226,7 +1240,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     int s = s0;
     if (per_thread > 1)
       for (;; ++s) {
-        at += seg_work<DT>(segment<DT>(v, a, gs, gp, s), a.G) * v.H;
+        at += seg_work<DT>(a, segment<DT>(v, a, gs, gp, s)) * v.H;
         if (u0 < at) break;
       }
     sh.seg = s;
@@ -1236,7 +1250,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   int s = first_lane_i(sh.seg), from = s;
   list(from, std::true_type{});
   uint64_t u = u0, tile_at = 0;
-  int h = -1, j = 0, group = -1;
+  int h = -1, j = 0;
   SegAt x;
   auto listed = [&](int i) { x = uniform(sh.list[i]); };
   listed(0);
@@ -1258,16 +1272,19 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       tile_at = x.at + h * x.work;  // unit of the tile's first step
       j = 0;
     }
-    int work = tile_work<DT>(g, j, a.G);
+    int work = tile_work<DT>(a, g, j);
     while (u >= tile_at + work) {
       tile_at += work;
       if (++j == g.tiles) j = 0, ++h;
-      work = tile_work<DT>(g, j, a.G);
+      work = tile_work<DT>(a, g, j);
     }
     // this workgroup's steps [k0, k1) of the tile's `len`
-    const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps(g, j, a.G));
-    const int k0 = first_lane_i(((int)(u - tile_at) + per_step - 1) / per_step);
-    const int k1 = first_lane_i((int)min((uint64_t)len, (u1 - tile_at + per_step - 1) / per_step));
+    const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps(a, g, j));
+    auto steps_in = [&](int units) {  // begun within so many units
+      const int n = units + per_step - 1;
+      return first_lane_i(g.tile == 16 ? n / step_units<DT>(16) : g.tile == 32 ? n / step_units<DT>(32) : n / step_units<DT>(kWide));
+    };
+    const int k0 = steps_in((int)(u - tile_at)), k1 = min(len, steps_in((int)min((uint64_t)work, u1 - tile_at)));
     u = tile_at + work;
     if (k0 >= k1) continue;  // the workgroup before has done them all
     Tile t;
@@ -1285,22 +1302,11 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     const int count = last - first + 1;
     const bool two = g.own ? a.n_groups && g.p0 > 0 : true;
     __syncthreads();  // the last tile's rows are written
-    if (!g.own && group != g.req) {  // a new group: what its rows see at least
-      group = g.req;
-      if (tid == 0) sh.group_lim = 0x7FFFFFFF;
-      __syncthreads();
-      const int b = clampi(gs[g.req], 0, a.n_req), e = clampi(gs[g.req + 1], b, a.n_req);
-      for (int r = b + tid; r < e; r += kThreads) {
-        const int n = token_of(a, r + 1) - token_of(a, r);
-        if (n > 0) atomicMin(&sh.group_lim, max(0, len_of(v, lane_of(v, a, r)) - n + 1));
-      }
-      __syncthreads();
-    }
-    const bool all_seen = !g.own && first_lane_i(sh.group_lim) >= g.p1 * kPageTokens;
-    const int tok0 = t.row0 / a.G, tok1 = (t.row0 + t.rows - 1) / a.G;
+    const bool all_seen = !g.own && gs == sh.gs && first_lane_i(sh.gl[g.req]) >= g.p1 * kPageTokens;
+    const int tok0 = token_of_row(a, t.row0), tok1 = token_of_row(a, t.row0 + t.rows - 1);
     if (g.own) {
-      t.lim_lo = clampi(g.base + tok0 - g.row0 / a.G, 0, g.len);
-      t.lim_hi = clampi(g.base + tok1 - g.row0 / a.G, 0, g.len);
+      t.lim_lo = clampi(g.base + tok0 - g.tok0, 0, g.len);
+      t.lim_hi = clampi(g.base + tok1 - g.tok0, 0, g.len);
     } else {
       t.lim_lo = t.lim_hi = g.p1 * kPageTokens;
       if (!all_seen) {
@@ -1310,10 +1316,10 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     }
     if (tid == 0) sh.left_out = 0;
     if (tid < t.rows) {
-      const int row = t.row0 + tid, tok = row / a.G;
+      const int row = t.row0 + tid, tok = token_of_row(a, row);
       int lim = t.lim_lo;
       if (g.own) {
-        lim = clampi(g.base + (tok - g.row0 / a.G), 0, g.len);
+        lim = clampi(g.base + (tok - g.tok0), 0, g.len);
       } else if (!all_seen) {
         int lo = tok;
         if (a.q_start) {  // the request of this token
@@ -1406,7 +1412,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs
   const uint64_t r = SPLIT > 1 ? blockIdx.x : (uint64_t)blockIdx.x * kTeams + team;
   if (r >= all) return;
   const uint32_t h = (uint32_t)(r / rows), row = (uint32_t)(r % rows);
-  const int tok = row / a.G;
+  const int tok = token_of_row(a, (int)row);
   if (tok < token_of(a, 0) || tok >= token_of(a, a.n_req)) return;
   const Where own = ws.where[all + r];
   if (own.count == 0) return;
@@ -1476,7 +1482,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs
   const bool none = !(own.has & 2);
   write_out<DT>(a, row_at(a, a.os, row, h), d, x, none ? 0.0f : 1.0f / sum);
   if (a.lse && d == 0)
-    a.lse[(int64_t)tok * a.Hq + h * a.G + row % a.G] =
+    a.lse[(int64_t)tok * a.Hq + h * a.G + row - tok * a.G] =
         none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
@@ -1582,7 +1588,9 @@ int ferry_pages_attend(const ferry_pages* p, int32_t layer, const ferry_attend* 
     AttendArgs d{a->n_req, a->n_tokens, a->n_groups, a->q_heads, a->q_heads / p->kv_heads,
                  a->scale != 0.0f ? a->scale : 0.08838834764831845f, a->lanes, a->q_start, a->group_start,
                  a->shared, a->q, a->out, a->lse, {a->q_stride[0], a->q_stride[1]},
-                 {a->out_stride[0], a->out_stride[1]}, low % 16 == 0};
+                 {a->out_stride[0], a->out_stride[1]}, low % 16 == 0, 0, 31};
+    while (1 << (d.g_shift - 31) < d.G) ++d.g_shift;
+    d.g_mul = (uint32_t)((1ull << d.g_shift) / d.G + 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int forms = attend_forms(p, a);
     if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, forms, grid, s);
