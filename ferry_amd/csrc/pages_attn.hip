@@ -956,7 +956,6 @@ struct Wide {
       k_scales = scales[0], v_scales = scales[1];
       store_k(k0, 0);
       store_k(kr, 1);
-      if (tid < 3) sh.odd[tid] = 0;
       land(0);
       if (busy) {
         products(x, 0);
@@ -1314,6 +1313,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
         __syncthreads();
       }
     }
+    if (tid < 3) sh.odd[tid] = 0;
     if (tid == 0) sh.left_out = 0;
     if (tid < t.rows) {
       const int row = t.row0 + tid, tok = token_of_row(a, row);
