@@ -645,9 +645,11 @@ __device__ inline void store8(void* p, int64_t at, const float (&x)[8]) {
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + at) = w;
   }
 }
-// x / s, correctly rounded, from inv = 1 / s
+// x / s, correctly rounded, from inv = 1 / s, where x * inv is finite; else by the
+// division itself (infinities, quotients that overflow, an s whose inverse does)
 __device__ inline float divide(float x, float s, float inv) {
   const float q = x * inv;
+  if (!(fabsf(q) < INFINITY)) return x / s;
   return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
 }
 

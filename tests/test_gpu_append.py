@@ -268,6 +268,32 @@ def test_values_out_of_the_8_bit_range_saturate():
     c.check(0, None, f, 1.0, False)
 
 
+@pytest.mark.parametrize("offset", [0, 1])  # 16-byte aligned, and not
+def test_quotients_at_the_ends_of_fp32(offset):
+    # infinities and quotients past fp32 saturate, NaN stays, zero stays zero, and scales
+    # whose inverse is no fp32 number divide all the same
+    x = [1e30, -1e30, np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-39, 3e-39, 7e-40, 1e38, 2.0 ** 127]
+    for s in (1e-10, 1e-40, 2.0 ** -149, 2.0 ** 127, 1e38, 1.0):
+        p = F.Pages.empty(1, 1, 1, 1, 1, F.FP8)
+        p.reserve(ints([0]), ints([16]))
+        buf = torch.zeros(2 * 128 + offset, device="cuda")
+        k, v = buf[offset:offset + 128].view(1, 1, 128), buf[offset + 128:].view(1, 1, 128)
+        v[0, 0, :len(x)] = torch.tensor(x)
+        p.append(0, ints([0]), ints([3]), k=k, v=v, inv_freq=torch.ones(64, dtype=torch.float64, device="cuda"),
+                 kv_scale=torch.tensor([[1.0, s]], device="cuda"))
+        torch.cuda.synchronize()
+        p.check()
+        f = np.float32(s).astype(np.float64)
+        with np.errstate(all="ignore"):
+            want = np.clip(np.float32(x).astype(np.float64) / f, -448.0, 448.0)
+        got = p.pool[0, 0, 0, 1, 3, :len(x)].double().cpu().numpy()
+        # half a step of E4M3 (2^-4 relative, 2^-10 below the normal range), and of fp32
+        bound = np.abs(want) * (2.0 ** -4 + 2.0 ** -23) + 2.0 ** -10
+        assert np.array_equal(np.isnan(got), np.isnan(want)), (s, got)
+        ok = ~np.isnan(want)
+        assert np.all(np.abs(got - want)[ok] <= bound[ok]), (s, got, want)
+
+
 def test_a_pool_past_four_gibibytes():
     H, P = 8, 70000
     p = F.Pages.empty(1, H, P, 1, 2, F.BF16)
