@@ -191,6 +191,59 @@ def test_many_requests(dt):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+def test_long_runs_of_wide_tiles(dt):
+    # so much work that a workgroup takes many steps of a 128-row tile: page ids and fp8
+    # scales come in windows of 16 steps.  A sample of requests and heads is checked.
+    rng = np.random.default_rng(2)
+    n, Hq, H = 64, 32, 8
+    lens = [int(x) for x in rng.integers(900, 2300, n)]
+    c = Case(dt, Hq, H, lens, new=[32 + int(x) for x in rng.integers(-20, 20, n)], seed=8)
+    out, lse = c.run()
+    for r in rng.permutation(n)[:10]:
+        for h in rng.permutation(H)[:2]:
+            near_rows(c, out, lse, int(r), int(h))
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+def test_wide_tiles_of_few_pages(dt):
+    # empty requests, rows that see nothing, tiles of 1 to 5 steps, a part of a tile's rows
+    lens = [0, 3, 16, 40, 64, 65, 127, 128, 129, 200, 256, 300]
+    new = [40, 40, 33, 40, 64, 20, 127, 100, 33, 33, 130, 70]
+    c = Case(dt, 4, 1, lens, new, seed=3)
+    lanes = c.lanes.copy()
+    c.check(*c.run())
+    c.lanes[4] = -1  # a request without a lane: its rows are empty
+    c.lens[4] = 0
+    out, lse = c.run()
+    c.lanes = lanes
+    c.check(out, lse)
+
+
+def near_rows(c, out, lse, r, h, scale=D ** -0.5):
+    """All rows of one request and kv head at once."""
+    G, u, n = c.Hq // c.H, U[c.dt], c.lens[r]
+    a, b = c.start[r], c.start[r + 1]
+    k, v = c.tokens(r, h)
+    q = c.q[a:b, h * G:(h + 1) * G].double()
+    s = scale * (q @ k.t())
+    S = abs(scale) * (q.abs() @ k.abs().t())
+    see = n - (b - a) + torch.arange(b - a, device="cuda") + 1
+    hidden = (torch.arange(n, device="cuda")[None] >= see[:, None])[:, None]
+    s = s.masked_fill(hidden, -np.inf)
+    S = S.masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+    want_e = torch.logsumexp(s, -1, keepdim=True)
+    p = torch.exp(s - want_e)
+    want, A = p @ v, p @ v.abs()
+    soft = (2 * 130 * S + see[:, None, None] / 8 + 64) * 2.0 ** -24
+    bound = u * want.abs() + A * (u + soft) * (1 + u) + 2.0 ** -25
+    o = out[a:b, h * G:(h + 1) * G].double()
+    worst = float(((o - want).abs() / bound).max())
+    assert worst <= 1.0, (r, h, worst)
+    e = lse[a:b, h * G:(h + 1) * G, None].double()
+    assert torch.all((e - want_e).abs() <= 2 * soft + 2.0 ** -23 * want_e.abs())
+
+
 def test_layers_scale_and_strides():
     c = Case(F.BF16, 6, 3, [20, 77], new=[3, 5], layers=3, layer=2, seed=4)
     big = torch.zeros((c.rows, 11, D), dtype=c.qt, device="cuda")
