@@ -766,6 +766,8 @@ class Pages:
         x = q if q is not None else k
         if x is None:
             raise ValueError("neither q nor k")
+        if inv_freq is None:
+            raise ValueError("inv_freq: expected a CUDA tensor")
         heads, out_type = 0, 0
         qp = op = kp = vp = sp = (0, 0, 0)
         if q is not None:

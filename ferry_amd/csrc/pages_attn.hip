@@ -1575,6 +1575,8 @@ int ferry_pages_attend(const ferry_pages* p, int32_t layer, const ferry_attend* 
       if (int rc = check_all({{a->group_start, "group_start"}, {a->shared, "shared"}}, p->device)) return rc;
     if (a->lse)
       if (int rc = check_on(a->lse, "lse", p->device)) return rc;
+    if (a->q == a->out && (a->q_stride[0] != a->out_stride[0] || a->q_stride[1] != a->out_stride[1]))
+      return report(FERRY_EINVAL, "out is q with other strides");
     Scratch ws;
     uint64_t need = 0;
     const int grid = plan_attend(p, a, static_cast<uint8_t*>(a->work), &ws, &need);

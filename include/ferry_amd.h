@@ -606,7 +606,8 @@ int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, dou
  *   0), a len past max_pages * 16 and offsets that do not ascend latch
  *   FERRY_ERANGE.
  *   q, out [n_tokens][q_heads][128]: fp32, fp16 and bf16 pages take theirs, fp8 pages
- *   bf16; strides in elements between tokens and between heads
+ *   bf16; strides in elements between tokens and between heads; out may be q where
+ *   the strides are the same
  *   lse [n_tokens][q_heads] fp32 or NULL
  *   work  ferry_pages_attend_work_bytes() of scratch (256-byte aligned), which
  *   only this call uses until it has run

@@ -353,3 +353,10 @@ def test_refusals_on_the_host():
         c.p.append(2, lane, pos, k=c.k, v=c.v, inv_freq=df, kv_scale=c.kv)
     with pytest.raises(F.FerryError, match="other"):
         c.p.append(0, None, pos, q=c.q, q_out=c.q.flatten().as_strided(c.q.shape, (128, 128, 1)), inv_freq=df)
+
+
+def test_no_frequencies():
+    p = F.Pages.empty(1, 1, 1, 1, 1, F.F16)
+    with pytest.raises(ValueError, match="inv_freq"):
+        p.append(0, ints([0]), ints([0]), q=torch.zeros((1, 1, 128), device="cuda"),
+                 q_out=torch.zeros((1, 1, 128), device="cuda"))

@@ -402,6 +402,37 @@ def test_the_same_bits_in_every_call(dt):
         c.run()
 
 
+@pytest.mark.parametrize("dt,new,groups", [(F.BF16, 1, ((6, 9),)), (F.FP8, 40, ()), (F.F16, 9, ((6, 9),)), (F.F32, 3, ())])
+def test_the_output_in_the_queries_place(dt, new, groups):
+    c = Case(dt, 8, 2, [300, 1500, 144, 200, 700, 160], [new] * 6, groups, seed=6)
+    out, lse = c.run()
+    q = c.q.clone()
+    c.p.attend(0, q, q, **c.args())
+    torch.cuda.synchronize()
+    assert torch.equal(q, out)
+
+
+def test_calls_on_two_streams_at_once():
+    # one cache, two batches, each call with its own scratch
+    a = Case(F.BF16, 16, 4, [900, 4000, 77, 2048], [50, 1, 77, 3], seed=9)
+    q = torch.randn((4, 16, 128), device="cuda", generator=a.g).to(a.qt)
+    lanes, first = ints(a.lanes), ints(a.start)
+    want = [torch.empty_like(a.q), torch.empty_like(q)]
+    a.p.attend(0, a.q, want[0], lanes, q_start=first)
+    a.p.attend(0, q, want[1], lanes)
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[torch.zeros_like(x) for x in want] for _ in range(6)]
+    torch.cuda.synchronize()
+    for x, y in got:
+        a.p.attend(0, a.q, x, lanes, q_start=first, stream=s[0])
+        a.p.attend(0, q, y, lanes, stream=s[1])
+    torch.cuda.synchronize()
+    a.p.check()
+    for x, y in got:
+        assert torch.equal(x, want[0]) and torch.equal(y, want[1])
+
+
 def test_no_rows():
     c = Case(F.BF16, 8, 2, [20], seed=1)
     e = c.q[:0]
@@ -425,3 +456,10 @@ def test_refusals_on_the_host():
         c.p.attend(1, c.q, out, ints(c.lanes))
     with pytest.raises(ValueError, match="shared"):
         c.p.attend(0, c.q, out, ints(c.lanes), group_start=ints([0, 1]))
+
+
+def test_the_queries_place_with_other_strides_is_refused():
+    c = Case(F.BF16, 8, 2, [20, 30], seed=1)
+    both = torch.zeros((2, 2, 8, 128), device="cuda", dtype=c.qt)
+    with pytest.raises(F.FerryError, match="other strides"):
+        c.p.attend(0, both[0], both[:, 0], ints(c.lanes))
