@@ -12,6 +12,8 @@ Reference interfaces mirrored (clearleo126/ferry, paths relative to its tree):
                            (src/workloads/kv_exec.cuh:188-292,
                            src/runtime/wla_multigpu.cuh:2527-2604)
   Executor.sparse_decode   attn_kernel / wla_attn_kernel (real attention here)
+  Pages, rope_freqs        (none: a paged cache of whole contexts; its pages are
+                           block records of the host tier)
   queue_selftest           bench_queue (src/benches/bench_queue.cu:62-123)
   SelGen / refgen_selections  replay_miss_stream (src/workloads/missstream.cuh:104)
   arrivals / Sched         request arrivals and the per-GPU tick loop
