@@ -62,9 +62,10 @@ _ERRORS = {-1: "EINVAL", -2: "EHIP", -3: "ERANGE", -4: "ECAPACITY", -5: "ENOMEM"
 
 
 class FerryError(RuntimeError):
-    def __init__(self, code, where):
+    def __init__(self, code, where, msg=None):
         self.code = code
-        msg = lib.ferry_last_error().decode()
+        if msg is None:  # the library's last refusal on the host
+            msg = lib.ferry_last_error().decode()
         super().__init__(f"{where}: {_ERRORS.get(code, code)} ({code}) {msg}")
 
 
@@ -716,7 +717,7 @@ class Pages:
         code = int(self.error.item())
         if code:
             self.error.zero_()
-            raise FerryError(code, "pages (found on the device)")
+            raise FerryError(code, "pages", "found on the device")
 
     # ---- managing pages ---------------------------------------------------------
     def reserve(self, lanes, tokens, stream=None):

@@ -463,3 +463,96 @@ def test_the_queries_place_with_other_strides_is_refused():
     both = torch.zeros((2, 2, 8, 128), device="cuda", dtype=c.qt)
     with pytest.raises(F.FerryError, match="other strides"):
         c.p.attend(0, both[0], both[:, 0], ints(c.lanes))
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+def test_wide_tiles_of_odd_strides_layers_and_scales(dt):
+    # query and output rows that are not 16-byte aligned, another layer, a negative scale
+    c = Case(dt, 10, 2, [200, 90, 1030], new=[60, 33, 41], layers=3, layer=2, seed=12, q_std=1.0)
+    n = 10 * 128 + 3
+    q = torch.zeros(c.rows * n + 1, device="cuda", dtype=c.qt)[1:].view(c.rows, n)[:, :1280].unflatten(1, (10, 128))
+    out = torch.full((c.rows * n + 5,), 3.0, device="cuda", dtype=c.qt)
+    rows = out[5:].view(c.rows, n)
+    q.copy_(c.q)
+    lse = torch.empty((c.rows, 10), device="cuda")
+    a = c.args()
+    c.p.attend(2, q, rows[:, :1280].unflatten(1, (10, 128)), lse=lse, scale=-0.11, **a)
+    torch.cuda.synchronize()
+    c.p.check()
+    c.check(rows[:, :1280].unflatten(1, (10, 128)), lse, scale=-float(np.float32(0.11)))
+    assert torch.all(rows[:, 1280:] == 3.0) and torch.all(out[:5] == 3.0)  # between the rows: left
+
+
+def test_wide_tiles_past_four_gibibytes():
+    H, P = 8, 70000
+    c = Case(F.F16, 16, H, [170, 133], new=[80, 40], seed=1)
+    p = F.Pages.empty(1, H, P, 4, 16, F.F16)
+    n = c.p.pool.shape[1]
+    p.pool[:, P - n:] = c.p.pool
+    p.table[:, :c.p.table.shape[1]] = torch.where(c.p.table >= 0, c.p.table + (P - n), c.p.table)
+    p.length.copy_(c.p.length)
+    want = c.run()
+    c.p = p
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+def test_wide_tiles_with_pages_out_of_range(dt):
+    # they are read as page 0 and reported
+    c = Case(dt, 4, 1, [300, 120], new=[50, 40], seed=5)
+    lane = int(c.lanes[0])
+    kept = c.p.table[lane].clone()
+    c.p.table[lane, 3] = c.p.pool.shape[1]
+    c.p.table[lane, 7] = -5
+    out, lse = torch.full_like(c.q, 9.0), torch.empty((c.rows, 4), device="cuda")
+    c.p.attend(0, c.q, out, lse=lse, **c.args())
+    with pytest.raises(F.FerryError, match="RANGE"):
+        c.p.check()
+    c.p.table[lane] = kept
+    c.p.table[lane, 3] = c.p.table[lane, 7] = 0
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+def test_several_values_that_later_rows_see(dt):
+    # NaN in steps next to each other and apart, in 128-row tiles that one workgroup takes whole
+    n, H, new = 64, 8, 500
+    lens = [int(x) for x in np.random.default_rng(1).integers(560, 700, n)]
+    c = Case(dt, H, H, lens, new=[new] * n, seed=4)
+    nan = torch.full((1,), float("nan"), device="cuda").to(TORCH[dt])
+    raw = c.p.pool.view(torch.uint8).view(*c.p.pool.shape[:-1], D, nan.element_size())
+    spots = []
+    for r, h, back, d in [(3, 0, 130, 5), (3, 0, 129, 9), (3, 0, 60, 5), (3, 0, 2, 64), (17, 5, 300, 127),
+                          (17, 5, 240, 0), (17, 5, 1, 1), (40, 7, 499, 33), (40, 7, 420, 33), (40, 7, 380, 2)]:
+        t = lens[r] - back
+        at = (0, int(c.p.table[int(c.lanes[r]), t // T]), h, 1, t % T, d)
+        spots.append((r, h, back, d, at, raw[at].clone()))
+        raw[at] = nan.view(torch.uint8)
+    out, lse = c.run()
+    for *_, at, was in spots:
+        raw[at] = was
+    fine = c.run()[0]
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    for r, h, back, d, *_ in spots:
+        bad[c.start[r] + new - back:c.start[r + 1], h, d] = True
+    assert torch.equal(torch.isnan(out), bad)
+    out = torch.where(bad, fine, out)
+    for r, h in [(3, 0), (17, 5), (40, 7), (3, 1), (41, 7), (63, 2)]:
+        near_rows(c, out, lse, r, h)
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+@pytest.mark.parametrize("new", [1, 2])
+def test_wide_groups_whose_members_end_within_the_shared_pages(dt, new):
+    lens = [700, 100, 481, 33, 480, 16, 1, 479, 512, 2, 640, 320, 0, 496, 15, 17] * 3
+    c = Case(dt, 8, 2, lens, new=[new] * len(lens), groups=[(16, 30), (31, 30), (1, 2)], seed=new)
+    c.check(*c.run())
+
+
+def test_more_groups_than_are_looked_up_in_lds():
+    n = 1300  # 650 groups of two, the last requests in none
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(1, 60, n + 7)]
+    c = Case(F.BF16, 2, 1, lens, groups=[(2, int(x)) for x in rng.integers(0, 3, n // 2)], seed=2)
+    c.check(*c.run())
