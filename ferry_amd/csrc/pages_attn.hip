@@ -965,6 +965,7 @@ struct Wide {
         top = see.of_row(top);
         raise_to(top, top > m + kRaise);
       }
+      __syncthreads();  // all have read K of step 0: the first step loads over it
     }
     // Step s, whose scores are in x, while those of step s + 1 come into y (MASKED: some row
     // may not see them all): next to each product a part of the weights, then of the

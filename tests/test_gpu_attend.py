@@ -556,3 +556,18 @@ def test_more_groups_than_are_looked_up_in_lds():
     lens = [int(x) for x in rng.integers(1, 60, n + 7)]
     c = Case(F.BF16, 2, 1, lens, groups=[(2, int(x)) for x in rng.integers(0, 3, n // 2)], seed=2)
     c.check(*c.run())
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+@pytest.mark.parametrize("rows", [33, 64, 96, 128])
+def test_the_first_steps_of_partly_filled_wide_tiles(dt, rows):
+    # Wavefronts without rows go ahead of those whose products read the first step's K, and
+    # load what comes after it.  1 to 5 steps a tile, whole ones and ends; the same bits in
+    # every call.
+    lens = [max(rows, n) for n in (1, 64, 65, 100, 128, 129, 192, 200, 256, 257, 320)]
+    c = Case(dt, 8, 8, lens, [rows] * len(lens), seed=rows)
+    want, lse = c.run()
+    c.check(want, lse)
+    for _ in range(20):
+        got = c.run()
+        assert torch.equal(got[0], want) and torch.equal(got[1], lse)
