@@ -473,10 +473,10 @@ struct Narrow {
   float m[NT], sum[NT];
   int lim[NT];
 
-  // One page.  MASKED: some row does not see all of its tokens; false: left out,
-  // as V holds what is not finite among those that one sees.
+  // One page.  MASKED: some row may not see all of its tokens; false: left out, as one
+  // does not and V holds what is not finite among those that one sees.
   template <bool MASKED>
-  __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, int lim_hi, float scale) {
+  __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, int lim_lo, int lim_hi, float scale) {
     const int grp = l >> 4;
     // V rows as operand values: 8 dims of 4 tokens
     constexpr int VD = K::F32 ? 8 : 4;
@@ -502,7 +502,7 @@ struct Narrow {
           vv[t][i] = seen ? vv[t][i] : 0u;
         }
       }
-      if (__builtin_amdgcn_ballot_w64(odd)) return false;
+      if (t0 + kPageTokens > lim_lo && __builtin_amdgcn_ballot_w64(odd)) return false;
     }
     u32x4 k16[4];
     if constexpr (K::F8) {
@@ -627,19 +627,20 @@ struct Narrow {
         if ((i & 63) == 0 && i) fill_ids(i);
         load_page<DT>(t, v.H, id_of(i), l, r[b]);
       };
-      // pages that every row sees whole, two at a time, then the others
+      // pages that every row sees whole, two at a time, then the others (the last of an odd
+      // number of whole ones among them, which is never left out)
       const int seen = t.lim_lo / kPageTokens - t.p0;  // such pages of all teams
       const int mine = clampi(seen / kStep + (seen % kStep > wave ? 1 : 0), 0, count);
       fetch(0, 0);
       int i = 0;
       for (; i + 1 < mine; i += 2) {
         fetch(i + 1, 1);
-        consume<false>(r[0], l, 0, 0, scale);
+        consume<false>(r[0], l, 0, 0, 0, scale);
         fetch(i + 2, 0);
-        consume<false>(r[1], l, 0, 0, scale);
+        consume<false>(r[1], l, 0, 0, 0, scale);
       }
       for (; page_no(i) < t.p1; ++i) {
-        if (!consume<true>(r[0], l, page_no(i) * kPageTokens, t.lim_hi, scale)) sh.left_out = 1;
+        if (!consume<true>(r[0], l, page_no(i) * kPageTokens, t.lim_lo, t.lim_hi, scale)) sh.left_out = 1;
         fetch(i + 1, 0);
       }
     }
@@ -1113,9 +1114,10 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int row, int h, 
     a.lse[(int64_t)token_of_row(a, row) * a.Hq + h * a.G + row - token_of_row(a, row) * a.G] = none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
-// The pages that a tile's products left out: a value that is not finite must not
-// meet the zero weight of a row that does not see it, so here each row takes only
-// the tokens it sees, one at a time, two dims a lane.  ml, o: the tile's rows as a
+// The pages that a tile's products left out, which are among those that not every row
+// sees whole: a value that is not finite must not meet the zero weight of a row that
+// does not see it, so here each row takes only the tokens it sees, one at a time, two
+// dims a lane.  ml, o: the tile's rows as a
 // part, which this adds to.  unit: pages that are left out together.
 template <int DT>
 __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs& a, const Tile& t, int unit,

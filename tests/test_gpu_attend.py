@@ -571,3 +571,76 @@ def test_the_first_steps_of_partly_filled_wide_tiles(dt, rows):
     for _ in range(20):
         got = c.run()
         assert torch.equal(got[0], want) and torch.equal(got[1], lse)
+
+
+def spoil(c, at):
+    """NaN and (not fp8) infinity in V of the tokens at[r] of requests r, kv head 0, dims 5
+    and 77; returns what undoes it."""
+    dims = [(5, float("nan"))] + ([] if c.dt == F.FP8 else [(77, float("inf"))])
+    es = c.p.pool.element_size()
+    raw = c.p.pool.view(torch.uint8).view(*c.p.pool.shape[:-1], D, es)
+    was = raw.clone()
+    for r, t in at.items():
+        page = int(c.p.table[int(c.lanes[r]), t // T])
+        for d, x in dims:
+            raw[c.layer, page, 0, 1, t % T, d] = \
+                torch.full((1,), x, device="cuda").to(TORCH[c.dt]).view(torch.uint8)
+    return lambda: raw.copy_(was)
+
+
+def check_spoiled(c, out, lse, at, fine):
+    """Rows that see token at[r] have its NaN and infinity, and nothing else of them: all
+    else is what a finite value there gives, which `fine` has in the spoiled places."""
+    G = c.Hq // c.H
+    nan, inf = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(out, dtype=torch.bool)
+    for r, t in at.items():
+        a, b = int(c.start[r]), int(c.start[r + 1])
+        first = max(a, b - (c.lens[r] - t))
+        nan[first:b, :G, 5] = True
+        inf[first:b, :G, 77] = c.dt != F.FP8
+    assert torch.equal(torch.isnan(out), nan)
+    assert torch.equal(out == float("inf"), inf)
+    c.check(torch.where(nan | inf, fine, out), lse)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new,G", [(1, 1), (8, 4), (5, 6)])
+def test_values_not_finite_in_every_page(dt, new, G):
+    # a request for each page of lanes of 16, 32, 100 and 700 tokens, all in one call
+    lens = [n for n in (16, 32, 100, 700) for _ in range(-(-n // T))]
+    where = [p for n in (16, 32, 100, 700) for p in range(-(-n // T))]
+    c = Case(dt, 2 * G, 2, lens, new=[new] * len(lens), seed=new)
+    fine = c.run()[0]
+    at = {r: min(n - 1, T * p + 9) for r, (n, p) in enumerate(zip(lens, where))}
+    undo = spoil(c, at)
+    out, lse = c.run()
+    # ... and a call for each, whose work is cut into runs of a step
+    one, one_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    for r in range(len(lens)):
+        a, b = int(c.start[r]), int(c.start[r + 1])
+        c.p.attend(0, c.q[a:b], one[a:b], ints(c.lanes[r:r + 1]), q_start=ints([0, new]), lse=one_lse[a:b])
+    torch.cuda.synchronize()
+    undo()
+    check_spoiled(c, out, lse, at, fine)
+    check_spoiled(c, one, one_lse, at, fine)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new,G", [(1, 4), (2, 5), (3, 16)])
+def test_values_not_finite_in_every_shared_page(dt, new, G):
+    # a group for each shared page, 3 members each; the last member of some ends within them
+    shared = [1, 2, 2] + [7] * 7 + [40] * 5
+    where = [0, 0, 1] + list(range(7)) + [0, 13, 26, 38, 39]
+    lens, at = [], {}
+    for s, p in zip(shared, where):
+        n = len(lens)
+        lens += [T * s + 30, T * s, max(new, T * s - 21)]
+        for r in range(n, n + 3):
+            if lens[r] > T * p + 9:
+                at[r] = T * p + 9
+    c = Case(dt, 2 * G, 2, lens, new=[new] * len(lens), groups=[(3, s) for s in shared], seed=new)
+    fine = c.run()[0]
+    undo = spoil(c, at)
+    out, lse = c.run()
+    undo()
+    check_spoiled(c, out, lse, at, fine)
