@@ -474,7 +474,7 @@ struct Narrow {
   int lim[NT];
 
   // One page.  MASKED: some row may not see all of its tokens; false: left out, as one
-  // does not and V holds what is not finite among those that one sees.
+  // does not and V or its scale holds what is not finite among those that one sees.
   template <bool MASKED>
   __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, int lim_lo, int lim_hi, float scale) {
     const int grp = l >> 4;
@@ -491,8 +491,10 @@ struct Narrow {
         for (int i = 0; i < VD; ++i) vv[t][i] = r.v[t][i];
       }
     }
+    float vs = r.vs;
     if constexpr (MASKED) {
-      bool odd = false;
+      if (t0 >= lim_hi) vs = 0.0f;  // no row sees the page
+      bool odd = K::F8 && !finite(vs);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const bool seen = t < lim_hi - t0 - 4 * grp;
@@ -563,7 +565,7 @@ struct Narrow {
       sum[nt] += (p[0] + p[1]) + (p[2] + p[3]);
       if constexpr (K::F8) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) p[t] *= r.vs;
+        for (int t = 0; t < 4; ++t) p[t] *= vs;
       }
       if constexpr (K::F32) {
 #pragma unroll
@@ -834,15 +836,21 @@ struct Wide {
     // fp8: the scales of the windows' pages, of K where step s + 1 is, of V where s is
     f32x2 scales = {};
     float k_scales = 0.0f, v_scales = 0.0f;
-    auto read_scales = [&]() __attribute__((always_inline)) {
-      if constexpr (K::F8) scales = *reinterpret_cast<const f32x2*>(t.scales + (uint64_t)ids * (2u * v.H));
+    // Pages that no row sees, those behind p1 among them, count as 0: their weights are 0
+    // and must not meet a scale that is not finite.
+    auto read_scales = [&](int w) __attribute__((always_inline)) {
+      if constexpr (K::F8) {
+        scales = *reinterpret_cast<const f32x2*>(t.scales + (uint64_t)ids * (2u * v.H));
+        const int p = t.p0 + 64 * w + l;
+        if (p >= t.p1 || p * kPageTokens >= t.lim_hi) scales[1] = 0.0f;
+      }
     };
     // Page i of the step whose K or V is loaded next.  Pages from p1 on are page 0: they
     // are loaded for nothing.
     auto window = [&](int s) __attribute__((always_inline)) {  // before K of step s > 1
       if ((s - 1 & 15) == 0) k_scales = scales[0];
       if ((s - 2 & 15) == 0) v_scales = scales[1];
-      if ((s & 15) == 0) ids = checked_page(v, ids_next), read_scales();
+      if ((s & 15) == 0) ids = checked_page(v, ids_next), read_scales(s / 16);
       if ((s & 15) == 8) ids_next = read_ids(s / 16 + 1);
     };
     auto begin_k = [&](int i, int s, Word& to) __attribute__((always_inline)) {
@@ -883,6 +891,9 @@ struct Wide {
       const int t0 = (t.p0 + kStep * s) * kPageTokens;
       if (s < steps && t0 + kStep * kPageTokens > t.lim_lo) {
         bool bad = false;
+        if constexpr (K::F8) {  // the lanes that hold the step's V scales
+          bad = l >> 2 == (s & 15) && !finite((s & 15) == 0 ? scales[1] : v_scales);
+        }
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
           u32x4* at = reinterpret_cast<u32x4*>(sh.kv.v[s & 1] + 4096 * i + to);
@@ -952,7 +963,7 @@ struct Wide {
       Word k0[K::F8 ? kStep : 1];
 #pragma unroll
       for (int i = 0; i < kStep; ++i) begin_k(i, 0, k0[K::F8 ? i : 0]);
-      read_scales();
+      read_scales(0);
       begin_step(0);
       k_scales = scales[0], v_scales = scales[1];
       store_k(k0, 0);
@@ -981,6 +992,7 @@ struct Wide {
           for (int i = 0; i < 32; ++i) x[i >> 4][i & 15] = -INFINITY;
 #pragma unroll
           for (int i = 0; i < kStep; ++i) *reinterpret_cast<u32x4*>(sh.kv.v[s & 1] + 4096 * i + tid * 16) = u32x4{0u, 0u, 0u, 0u};
+          if (K::F8 && l >> 2 == (s & 15)) v_scales = 0.0f;  // of its pages
           if (tid == 0) sh.left_out = 1;
           __syncthreads();
         }
@@ -1129,9 +1141,11 @@ __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs
   for (int p = t.p0 + whole; p < t.p1; p += unit) {
     bool odd = false;
     for (int i = 0; i < unit && p + i < t.p1; ++i) {
-      const uint8_t* rec = t.base + (uint64_t)checked_page(v, t.table[p + i]) * t.page_bytes;
+      const uint64_t page = checked_page(v, t.table[p + i]);
+      const uint8_t* rec = t.base + page * t.page_bytes;
       for (int e = l; e < kPageTokens * kPageDim; e += 64)
         odd |= (p + i) * kPageTokens + e / kPageDim < t.lim_hi && !finite(v_elem<DT>(rec, e / kPageDim, e % kPageDim));
+      if (K::F8) odd |= (p + i) * kPageTokens < t.lim_hi && !finite(t.scales[page * (2u * v.H) + 1]);
     }
     if (!__builtin_amdgcn_ballot_w64(odd)) continue;
     for (int row = wave; row < t.rows; row += kThreads / 64) {

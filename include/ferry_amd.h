@@ -595,7 +595,7 @@ int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, dou
  *   out = softmax(scale q K^T) V,  lse = ln sum exp(scale q K^T).
  * A row that sees no token gives 0 and -inf; rows behind the last request are
  * left as they were.  A token that a row does not see has no part in it,
- * whatever its K and V hold.
+ * whatever its K, V and their scales hold.
  * Groups: requests [group_start[g], group_start[g + 1]) have the same first
  * shared[g] pages in their tables (as forked lanes do); those are read through
  * the first one's table, once for the whole group instead of once per request.

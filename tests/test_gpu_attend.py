@@ -644,3 +644,73 @@ def test_values_not_finite_in_every_shared_page(dt, new, G):
     out, lse = c.run()
     undo()
     check_spoiled(c, out, lse, at, fine)
+
+
+def behind_a_free_page(c):
+    """The same case with a page in front that no lane holds."""
+    p = c.p
+    c.p = F.Pages(torch.cat([p.pool[:, :1].view(torch.uint8), p.pool.view(torch.uint8)], 1).view(p.pool.dtype),
+                  torch.where(p.table >= 0, p.table + 1, p.table), p.length,
+                  scales=torch.cat([p.scales[:, :1], p.scales], 1))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("new,groups", [([1, 2, 9, 1, 7, 8, 3], [(2, 0), (2, 1)]),
+                                        ([33, 40, 64, 128, 150, 35, 9], []),
+                                        ([9, 9, 12, 9, 9, 9, 9], [(5, 2), (2, 5)])])
+def test_scales_that_no_row_sees(new, groups, bad):
+    # of pages that no lane holds, page 0 among them, and of a lane's pages behind its end
+    c = Case(F.FP8, 8, 2, [33, 40, 64, 130, 150, 81, 95], new=new, groups=groups, seed=2, spare=40)
+    behind_a_free_page(c)
+    want = c.run()
+    held = torch.zeros(c.p.pool.shape[1], dtype=torch.bool, device="cuda")
+    for r, n in enumerate(c.lens):
+        row = c.p.table[int(c.lanes[r])]
+        held[row[:-(-n // T)].long()] = True
+        more = (~held).nonzero()[-1 - r]  # a page reserved behind them
+        row[-(-n // T)] = more[0]
+    c.p.scales[:, ~held] = bad
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    c.check(*got)
+
+
+@pytest.mark.parametrize("which,bad", [(0, float("nan")), (1, float("nan")), (1, float("inf"))])
+@pytest.mark.parametrize("new,G", [(4, 4), (8, 4), (30, 1), (70, 4), (300, 2)])
+def test_scales_that_later_rows_see(new, G, which, bad):
+    # of K (which 0) or V: nothing of them in the rows before their page's first token
+    n = 400
+    c = Case(F.FP8, 2 * G, 2, [n, 60, n], new=[new, 1, new], seed=new)
+    fine, lse = c.run()
+    c.check(fine, lse)
+    keep = c.p.scales.clone()
+    for r, back in ((0, 3), (2, new // 2), (2, new - 1)):
+        page = c.p.table[int(c.lanes[r]), (n - back) // T]
+        c.p.scales[0, page, 0, which] = bad
+    out, got_lse = c.run()
+    c.p.scales.copy_(keep)
+    sees = torch.zeros_like(out, dtype=torch.bool)
+    for r, back in ((0, 3), (2, new - 1)):
+        first = (n - back) // T * T  # the page's first token
+        a, b = int(c.start[r]), int(c.start[r + 1])
+        sees[max(a, b - (n - first)):b, :G] = True
+    assert torch.all(torch.isnan(out[sees]) if bad != bad else ~torch.isfinite(out[sees]))
+    assert torch.all(torch.isfinite(out[~sees]))
+    hit = sees[:, :, 0]
+    c.check(torch.where(sees, fine, out), torch.where(hit, lse, got_lse))
+
+
+@pytest.mark.parametrize("shared,new", [(7, 1), (7, 3), (30, 1), (30, 3)])
+def test_scales_in_shared_pages_that_some_members_see(shared, new):
+    lens = [16 * shared + 20, 16 * shared - 17, 16 * shared - 40, 16 * shared, new, 40]
+    c = Case(F.FP8, 16, 2, lens, new=[new] * 6, groups=[(5, shared)], seed=shared)
+    fine, lse = c.run()
+    page = shared - 2  # tokens that the members of 16 (shared - 2) or fewer do not see
+    c.p.scales[0, c.p.table[int(c.lanes[0]), page], 0, 1] = float("nan")
+    out, _ = c.run()
+    sees = torch.zeros_like(out, dtype=torch.bool)
+    for r, m in enumerate(lens[:5]):
+        a, b = int(c.start[r]), int(c.start[r + 1])
+        sees[max(a, b - max(0, m - 16 * page)):b, :8] = True
+    assert sees.any() and not sees.all() and torch.equal(torch.isnan(out), sees)
+    c.check(torch.where(sees, fine, out), lse)
