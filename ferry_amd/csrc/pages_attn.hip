@@ -19,12 +19,16 @@
 // (max, sum, output) in fp32 go to scratch, and k_attend_join adds them up in order.
 // The result depends on the lengths and on the number of CUs, not on timing.
 //
-// Softmax.  One pass with the running maximum m and sum of each row, in base 2.  m is
-// raised only when a score exceeds it by kRaise, so weights may grow to 2^kRaise
-// (fp16 and bf16 hold them as exactly as those below 1) and the accumulator is rarely
-// rescaled.  Scores, maxima, sums and the accumulator are fp32; weights are rounded
-// to the operand type for the second product (half a step relative, as large as
-// the rounding of the output).
+// Softmax.  One pass with a reference m and the sum of the weights 2^(score - m) of each
+// row, in base 2.  m is raised only when a score exceeds it by kMost, and then so that this
+// one's weight is 2^kTop: weights are at most 2^kMost and the accumulator is rarely
+// rescaled.  Scores, references, sums and the accumulator are fp32; weights are rounded to
+// the operand type for the second product.  That is half a step relative (2^-8 of a
+// weight in bf16, 2^-11 in fp16), as large as the rounding of the output, where the type
+// holds them as normal numbers: bf16 has fp32's range, but fp16 ends at 2^-14, so there
+// kTop is 7 and the row's largest weight is 2^7 .. 2^15.  A weight below 2^-21 of the largest
+// is then rounded to a multiple of 2^-31 of it, which for n tokens moves the output by
+// n 2^-32 of their values at most: as much as its own rounding from 2^21 tokens on.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -51,7 +55,6 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256;
 constexpr int kStep = 4;           // pages per step
 constexpr int kWide = 128;         // rows of the widest tile
-constexpr float kRaise = 8.0f;     // log2 of the largest weight between raises of the max
 constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
 constexpr int kPad = 132;          // floats per row of the merge buffer
 constexpr int kPerCu = 2;          // workgroups per CU
@@ -100,6 +103,8 @@ struct Kv {
   static constexpr int HALF = kPageTokens * ROW;     // bytes of a record's K
   static constexpr int NK = ROW / 64;                // 16-byte K words per lane and page
   static constexpr int VW = 2 * ES;                  // dwords of V per token and lane
+  // log2 of the largest weight, and of the largest when the reference is raised
+  static constexpr float kMost = DT == FERRY_F16 ? 15.0f : 8.0f, kTop = DT == FERRY_F16 ? 7.0f : 0.0f;
 };
 
 template <bool BF>
@@ -145,7 +150,7 @@ __device__ inline f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {  // 32 x 32 x 16
 }
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// The value weights are taken against: m, or 0 while no score was finite.
+// What weights are taken against: the reference m, or 0 while no score was finite.
 __device__ inline float against(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // One K or V element of a record as fp32 (fp8: the code's value), one of q.
@@ -550,10 +555,10 @@ struct Narrow {
         top = fmaxf(top, x[t]);
       }
       top = max_over_groups(top);
-      const bool raise = top > m[nt] + kRaise;
+      const bool raise = top > m[nt] + K::kMost;
       if (__builtin_amdgcn_ballot_w64(raise)) {
-        const float f = raise ? exp2_fast(m[nt] - top) : 1.0f;
-        m[nt] = raise ? top : m[nt];
+        const float to = raise ? top - K::kTop : m[nt], f = raise ? exp2_fast(m[nt] - to) : 1.0f;
+        m[nt] = to;
         sum[nt] *= f;
 #pragma unroll
         for (int nb = 0; nb < 8; ++nb) o[nt][nb] *= f;
@@ -931,8 +936,8 @@ struct Wide {
     };
     auto raise_to = [&](float top, bool raise) __attribute__((always_inline)) {
       if (__builtin_amdgcn_ballot_w64(raise)) {
-        const float f = raise ? exp2_fast(m - top) : 1.0f;
-        m = raise ? top : m;
+        const float to = raise ? top - K::kTop : m, f = raise ? exp2_fast(m - to) : 1.0f;
+        m = to;
         sum *= f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] *= f;
@@ -975,7 +980,7 @@ struct Wide {
         float top = -INFINITY;
         see.among(x, 0, 32, top);
         top = see.of_row(top);
-        raise_to(top, top > m + kRaise);
+        raise_to(top, top > m + K::kMost);
       }
       __syncthreads();  // all have read K of step 0: the first step loads over it
     }
@@ -1043,7 +1048,7 @@ struct Wide {
           if (K::F8) begin(i);  // into the registers that x has left
           if (i >= 2 && i < 10) see.among(y, 4 * (i - 2), 4, top);
           if (i == 11) top = see.of_row(top);
-          if (i == 12) raise = top > m + kRaise;
+          if (i == 12) raise = top > m + K::kMost;
           __builtin_amdgcn_sched_barrier(0);
         }
         raise_to(top, raise);

@@ -714,3 +714,38 @@ def test_scales_in_shared_pages_that_some_members_see(shared, new):
         sees[max(a, b - max(0, m - 16 * page)):b, :8] = True
     assert sees.any() and not sees.all() and torch.equal(torch.isnan(out), sees)
     c.check(torch.where(sees, fine, out), lse)
+
+
+@pytest.mark.parametrize("dt", [F.F16, F.BF16])
+@pytest.mark.parametrize("n,new", [(1 << 18, 1), (1 << 17, 128)])
+def test_a_long_tail_of_small_weights(dt, n, new):
+    # A token of weight 1 at the start of what each maximum is taken over (the pages of a
+    # wavefront, or all), all others 2^-25.5, which fp16 does not hold: together they are
+    # 2^-8.5 of it or more, and their values are of one sign and most of the output.  As many
+    # requests of the lane as there are workgroups, so that one takes the whole lane.
+    reqs, tops = 512, 4 if new == 1 else 1
+    g = torch.Generator(device="cuda").manual_seed(new)
+    pool = torch.zeros((1, n // T, 1, 2, T, D), dtype=TORCH[dt], device="cuda")
+    pool[0, :, 0, 1] = -(0.5 + torch.rand((n // T, T, D), device="cuda", generator=g)).to(TORCH[dt])
+    pool[0, :tops, 0, 0, 0, 0] = 12.5
+    pool[0, :tops, 0, 1, 0] = 2.0 ** -6
+    p = F.Pages(pool, torch.arange(n // T, dtype=torch.int32, device="cuda")[None], ints([n]))
+    q = torch.zeros((reqs * new, 1, D), dtype=TORCH[dt], device="cuda")
+    q[:, 0, 0] = 16.0
+    out, lse = torch.empty_like(q), torch.empty((reqs * new, 1), device="cuda")
+    p.attend(0, q, out, ints([0] * reqs), q_start=ints([new * i for i in range(reqs + 1)]), lse=lse)
+    torch.cuda.synchronize()
+    p.check()
+    k, v = pool[0, :, 0, 0].reshape(n, D).double(), pool[0, :, 0, 1].reshape(n, D).double()
+    s = D ** -0.5 * (k[:, 0] * 16.0)
+    u = U[dt]
+    for row in range(0, reqs * new, max(1, reqs * new // 50) + 1):
+        see = n - new + row % new + 1
+        want_e = torch.logsumexp(s[:see], 0)
+        w = torch.exp(s[:see] - want_e)
+        want, A = w @ v[:see], w @ v[:see].abs()
+        soft = (2 * 130 * float(s.max()) + see / 8 + 64) * 2.0 ** -24
+        # the bound above, and half of fp16's smallest step per weight: 2^-32 of the largest one
+        bound = u * want.abs() + A * (u + soft) * (1 + u) + 2.0 ** -25 + see * 2.0 ** -32 / tops * 1.5
+        assert torch.all((out[row, 0].double() - want).abs() <= bound)
+        assert abs(float(lse[row, 0]) - float(want_e)) <= 2 * soft + 2.0 ** -23 * abs(float(want_e))
