@@ -202,13 +202,13 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
   __shared__ uint32_t bits[kMaxLanes / 32];
   __shared__ uint32_t ids[kIdsInLds];
   __shared__ uint32_t last_page[SMALL ? kPlan : 1];
-  __shared__ int bad, sharing, longest;
+  __shared__ int bad, longest;
   const int tid = threadIdx.x;
   uint32_t first[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) first[i] = 4 * tid + i < v.n_pages ? v.refs[4 * tid + i] : 1u;
   for (int i = tid; i < (v.n_lanes + 31) / 32; i += kPlan) bits[i] = 0;
-  if (tid == 0) bad = sharing = longest = 0;
+  if (tid == 0) bad = longest = 0;
   __syncthreads();
   int my_lane = 0, my_had = 0, my_tokens = 0;  // SMALL: the thread's lane
   uint32_t my_page = kNone, my_refs = 0;
@@ -228,7 +228,6 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
           atomicMin(&bad, FERRY_ESTATE);
         } else if constexpr (SMALL) {
           my_page = page, my_refs = v.refs[page];
-          if (my_refs > 1) sharing = 1;
         } else {
           atomicExch(&w.uses[page], 0u);
           atomicExch(&w.last[page], 0u);
