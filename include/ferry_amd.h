@@ -611,8 +611,8 @@ int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, dou
  *   lse [n_tokens][q_heads] fp32 or NULL
  *   work  ferry_pages_attend_work_bytes() of scratch (256-byte aligned), which
  *   only this call uses until it has run
- * Scores, softmax and sums are fp32; weights are rounded to the 16-bit type
- * before they meet V.  Sums run in an order that follows from the batch's
+ * Scores, softmax and sums are fp32; weights are rounded to the queries' type
+ * before they meet V (an infinite V whose weight becomes 0 there gives NaN).  Sums run in an order that follows from the batch's
  * lengths and the GPU's CUs, the same in every call on the same inputs.  scale 0
  * is 1 / sqrt(128). */
 typedef struct ferry_attend {
