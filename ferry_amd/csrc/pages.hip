@@ -471,7 +471,12 @@ __global__ __launch_bounds__(256) void k_trim(PageView v, const int32_t* __restr
     for (int e = pages_of(kept) + threadIdx.x; e < pages_of(held); e += blockDim.x) {
       const uint32_t id = row[e];
       row[e] = kNone;
-      if (id >= (uint32_t)v.n_pages || atomicSub(&v.refs[id], 1u) == 0) set_error(v.error, FERRY_ESTATE);
+      if (id >= (uint32_t)v.n_pages) {
+        set_error(v.error, FERRY_ESTATE);
+      } else if ((int)atomicSub(&v.refs[id], 1u) <= 0) {  // counted as free: it stays so
+        atomicAdd(&v.refs[id], 1u);
+        set_error(v.error, FERRY_ESTATE);
+      }
     }
     __syncthreads();  // all have read the length
     if (threadIdx.x == 0) v.len[lane] = kept;

@@ -511,7 +511,10 @@ int ferry_pages_work_bytes(const ferry_pages* pages, uint64_t* bytes);
 /* Managing pages.  lanes, src, dst, tokens and keep are device arrays of n
  * int32 (n >= 0).  A call is made whole or not at all: a lane that is out of
  * range or named twice, or counts that do not fit, latch their error
- * (FERRY_EINVAL, FERRY_ECAPACITY) and change nothing.
+ * (FERRY_EINVAL, FERRY_ECAPACITY) and change nothing.  A cache that contradicts
+ * itself (a used table entry outside the pool, one of a page with a count of 0)
+ * latches FERRY_ESTATE where a call comes upon it; what is sound is done all the
+ * same, but by reserve, which then changes nothing.
  *
  * ferry_pages_reserve grows lanes[i] by tokens[i] >= 0 tokens: len grows, pages
  * are taken for them, and a last page that is begun and shared is copied first

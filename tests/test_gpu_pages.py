@@ -328,3 +328,37 @@ def test_refusals_on_the_host():
         bare.compact()
     p.reserve(ints([]), ints([]))  # nothing to do
     p.check()
+
+
+def test_tables_and_counts_that_contradict_each_other():
+    p = F.Pages.empty(1, 1, 12, 6, 4, F.BF16)
+    p.reserve(ints([0, 1]), ints([40, 33]))  # pages 0 1 2 and 3 4 5
+    p.fork(ints([0, 0]), ints([2, 3]))
+    p.check()
+    p.refs[1] = 0  # in three tables
+    p.trim(ints([0, 2, 3]))
+    with pytest.raises(F.FerryError) as e:
+        p.check()
+    assert e.value.code == ESTATE
+    # the pages' counts are those of free ones, not of 2^32 - 1 uses
+    assert p.refs.tolist() == [0, 0, 0, 1, 1, 1] + [0] * 6
+    p.table[1, 1] = 77  # no page of the pool
+    for call in (lambda: p.fork(ints([1]), ints([2])), lambda: p.trim(ints([2])), lambda: p.trim(ints([1]))):
+        call()
+        with pytest.raises(F.FerryError) as e:
+            p.check()
+        assert e.value.code == ESTATE
+    assert p.refs.tolist() == [0, 0, 0, 0, 1, 0] + [0] * 6  # page 4 is in no table any more
+    assert not p.length.any() and torch.all(p.table == -1)
+    p.refs[4] = 0
+    p.reserve(ints([5]), ints([64]))
+    p.check()
+    assert p.table[5].tolist() == [0, 1, 2, 3]
+    # reserve: nothing of the call is done
+    p.trim(ints([5]), ints([50]))
+    p.table[5, 3] = -1
+    p.reserve(ints([4, 5]), ints([20, 1]))
+    with pytest.raises(F.FerryError) as e:
+        p.check()
+    assert e.value.code == ESTATE
+    assert p.length.tolist() == [0, 0, 0, 0, 0, 50] and torch.all(p.table[4] == -1)
