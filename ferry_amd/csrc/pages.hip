@@ -94,6 +94,7 @@ struct Work {
   uint32_t* last;      // [n_pages] the last of them
   uint32_t* base;      // [n_lanes] first of a listed lane's places in free_ids
   uint32_t* had;       // [n_lanes] its tokens before the call
+  uint32_t* grown;     // [n_lanes] and after it
   uint32_t* copy_lane;  // [n_lanes] list places whose last page is copied
   uint32_t* copy_from;  // [n_lanes] ... and that page
   uint32_t* from;      // [n_pages] pages moved (compact)
@@ -112,13 +113,14 @@ Work split_work(void* w, int n_pages, int n_lanes) {
   r.from = r.uses;
   r.base = reinterpret_cast<uint32_t*>(p), p += ln;
   r.had = reinterpret_cast<uint32_t*>(p), p += ln;
+  r.grown = reinterpret_cast<uint32_t*>(p), p += ln;
   r.copy_lane = reinterpret_cast<uint32_t*>(p), p += ln;
   r.copy_from = reinterpret_cast<uint32_t*>(p);
   return r;
 }
 
 uint64_t work_bytes(int n_pages, int n_lanes) {
-  return 64 + 3 * up16((uint64_t)n_pages * 4) + 4 * up16((uint64_t)n_lanes * 4);
+  return 64 + 3 * up16((uint64_t)n_pages * 4) + 5 * up16((uint64_t)n_lanes * 4);
 }
 
 __device__ inline int pages_of(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
@@ -198,7 +200,7 @@ __device__ inline uint64_t find_free(const PageView& v, const Work& w, uint64_t 
 // page are then counted in LDS, else by atomics in the scratch.
 template <bool SMALL>
 __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, const int32_t* __restrict__ lanes,
-                                                        const int32_t* __restrict__ tokens, int n) {
+                                                        const int32_t* tokens, int n) {
   __shared__ uint32_t bits[kMaxLanes / 32];
   __shared__ uint32_t ids[kIdsInLds];
   __shared__ uint32_t last_page[SMALL ? kPlan : 1];
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
       atomicMin(&bad, FERRY_EINVAL);
     } else {
       const int had = v.len[lane];
-      w.had[i] = had;
+      w.had[i] = had, w.grown[i] = had + t;
       my_lane = lane, my_had = had, my_tokens = t;
       if (had < 0 || (int64_t)had + t > (int64_t)v.max_pages * kPageTokens) {
         atomicMin(&bad, FERRY_ECAPACITY);
@@ -340,13 +342,12 @@ __device__ inline void copy_page(const PageView& v, int layer, uint32_t from, ui
   }
 }
 
-__global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32_t* __restrict__ lanes,
-                                                 const int32_t* __restrict__ tokens, int n) {
+__global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32_t* __restrict__ lanes, int n) {
   if (!w.plan->ok) return;
   const uint32_t need = w.plan->handed ? 0 : w.plan->need, copies = w.plan->copies;
   const uint32_t step = gridDim.x * blockDim.x, at = blockIdx.x * blockDim.x + threadIdx.x;
   if (!w.plan->handed)
-    for (uint32_t i = at; i < (uint32_t)n; i += step) v.len[lanes[i]] = (int)w.had[i] + tokens[i];
+    for (uint32_t i = at; i < (uint32_t)n; i += step) v.len[lanes[i]] = (int)w.grown[i];
   // taken page r belongs to the last list place whose base is at most r
   for (uint32_t r = at; r < need; r += step) {
     int lo = 0, hi = n - 1;
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(256) void k_reserve(PageView v, Work w, const int32
     }
     const int had = (int)w.had[lo];
     const uint32_t taken = (lo + 1 < n ? w.base[lo + 1] : need) - w.base[lo];
-    const int fresh = pages_of(had + tokens[lo]) - pages_of(had);
+    const int fresh = pages_of((int)w.grown[lo]) - pages_of(had);
     const bool copy = taken > (uint32_t)fresh;
     const int col = pages_of(had) - (copy ? 1 : 0) + (int)(r - w.base[lo]);
     const uint32_t id = w.free_ids[r];
@@ -854,6 +855,21 @@ int manage(const ferry_pages* p, int n, PageView* v, Work* w) {
   return FERRY_OK;
 }
 
+// A list of n values that a managing call reads (or writes): device memory apart from what
+// the call changes, since its workgroups read the list while others already change that.
+// of_len: the call has read the list before it changes len.
+int check_list(const ferry_pages* p, const void* list, const char* name, int n, bool of_len = false) {
+  if (int rc = check_on(list, name, p->device)) return rc;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(list), to = from + (uintptr_t)n * 4;
+  auto meets = [&](const void* buf, uint64_t entries) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(buf);
+    return from < at + entries * 4 && at < to;
+  };
+  if ((!of_len && meets(p->len, p->n_lanes)) || meets(p->refs, p->n_pages) || meets(p->table, (uint64_t)p->n_lanes * p->max_pages))
+    return report(FERRY_EINVAL, std::string(name) + " is a part of the cache's own table, len or refs");
+  return FERRY_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -875,14 +891,15 @@ int ferry_pages_reserve(const ferry_pages* p, const int32_t* lanes, const int32_
     Work w;
     if (int rc = manage(p, n, &v, &w)) return rc;
     if (n == 0) return FERRY_OK;
-    if (int rc = check_all({{lanes, "lanes"}, {tokens, "tokens"}}, p->device)) return rc;
+    if (int rc = check_list(p, lanes, "lanes", n)) return rc;
+    if (int rc = check_list(p, tokens, "tokens", n, true)) return rc;
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (n <= kPlan) k_reserve_plan<true><<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
     else k_reserve_plan<false><<<1, kPlan, 0, s>>>(v, w, lanes, tokens, n);
     const int64_t most = std::min<int64_t>((int64_t)n * v.L + 64, 8l * gpu_cus(p->device));
-    k_reserve<<<(unsigned)most, 256, 0, s>>>(v, w, lanes, tokens, n);
+    k_reserve<<<(unsigned)most, 256, 0, s>>>(v, w, lanes, n);
     return launched("ferry_pages_reserve");
   });
 }
@@ -894,9 +911,10 @@ int ferry_pages_fork(const ferry_pages* p, const int32_t* src, const int32_t* ds
     Work w;
     if (int rc = manage(p, n, &v, &w)) return rc;
     if (n == 0) return FERRY_OK;
-    if (int rc = check_all({{src, "src"}, {dst, "dst"}}, p->device)) return rc;
+    if (int rc = check_list(p, src, "src", n)) return rc;
+    if (int rc = check_list(p, dst, "dst", n)) return rc;
     if (keep)
-      if (int rc = check_on(keep, "keep", p->device)) return rc;
+      if (int rc = check_list(p, keep, "keep", n, true)) return rc;
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -918,9 +936,9 @@ int ferry_pages_trim(const ferry_pages* p, const int32_t* lanes, const int32_t* 
     Work w;
     if (int rc = manage(p, n, &v, &w)) return rc;
     if (n == 0) return FERRY_OK;
-    if (int rc = check_on(lanes, "lanes", p->device)) return rc;
+    if (int rc = check_list(p, lanes, "lanes", n)) return rc;
     if (keep)
-      if (int rc = check_on(keep, "keep", p->device)) return rc;
+      if (int rc = check_list(p, keep, "keep", n)) return rc;
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -936,7 +954,7 @@ int ferry_pages_compact(const ferry_pages* p, int32_t* live, void* stream) {
     Work w;
     if (int rc = manage(p, 0, &v, &w)) return rc;
     if (live)
-      if (int rc = check_on(live, "live", p->device)) return rc;
+      if (int rc = check_list(p, live, "live", 1)) return rc;
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);

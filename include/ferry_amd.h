@@ -509,7 +509,8 @@ typedef struct ferry_pages {
 int ferry_pages_work_bytes(const ferry_pages* pages, uint64_t* bytes);
 
 /* Managing pages.  lanes, src, dst, tokens and keep are device arrays of n
- * int32 (n >= 0).  A call is made whole or not at all: a lane that is out of
+ * int32 (0 <= n <= n_lanes), and not part of table, refs or len, but that reserve's
+ * tokens and fork's keep may be len's own.  A call is made whole or not at all: a lane that is out of
  * range or named twice, or counts that do not fit, latch their error
  * (FERRY_EINVAL, FERRY_ECAPACITY) and change nothing.  A cache that contradicts
  * itself (a used table entry outside the pool, one of a page with a count of 0)

@@ -362,3 +362,33 @@ def test_tables_and_counts_that_contradict_each_other():
         p.check()
     assert e.value.code == ESTATE
     assert p.length.tolist() == [0, 0, 0, 0, 0, 50] and torch.all(p.table[4] == -1)
+
+
+def test_lists_that_are_the_cache_s_own():
+    p = F.Pages.empty(1, 1, 40, 6, 4, F.BF16)
+    p.reserve(ints([0, 1, 2]), ints([1, 2, 0]))
+    lanes = ints([5, 0, 1, 2, 3, 4])
+    for call in (lambda: p.trim(lanes, p.length), lambda: p.trim(p.length[3:]), lambda: p.reserve(p.table[0], lanes),
+                 lambda: p.reserve(p.length, lanes), lambda: p.fork(p.refs[30:31], ints([3])),
+                 lambda: p.compact(p.refs[39:])):
+        with pytest.raises(F.FerryError, match="own table, len or refs"):
+            call()
+    p.reserve(lanes, p.length)
+    assert p.length.tolist() == [1 + 2, 2 + 0, 0, 0, 0, 1]
+    p.fork(ints([0, 0]), ints([2, 3]), p.length[:2])
+    assert p.length.tolist() == [3, 2, 3, 2, 0, 1]
+    p.check()
+
+
+@pytest.mark.parametrize("n,tokens", [(5, 2000), (1500, 20)])
+def test_lanes_that_grow_by_other_lanes_lengths(n, tokens):
+    # more than the plan hands out by itself: another launch, whose workgroups write lengths
+    # and read how far lanes grow.  The list goes against the lanes' order.
+    b = Both(2 * n * (tokens // T + 3), n, 2 * tokens // T + 4, F.FP8, 1, 1)
+    order = list(range(n))[::-1]
+    first = [tokens - i % 9 for i in range(n)]
+    assert b.call("reserve", list(range(n)), first) == 0
+    b.p.reserve(ints(order), b.p.length)
+    b.l.reserve(order, first)
+    b.p.check()
+    b.same()
