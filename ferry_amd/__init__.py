@@ -712,11 +712,13 @@ class Pages:
         return _dev(t, name, n, _I32, self.device)  # says what is wrong
 
     def check(self):
-        """Raise the first error the device found since the last check
-        (synchronises)."""
+        """Raise the first error that calls on any stream found since the last check
+        (waits for the device)."""
+        torch.cuda.synchronize(self.device)
         code = int(self.error.item())
         if code:
             self.error.zero_()
+            torch.cuda.synchronize(self.device)  # before a call on another stream finds one
             raise FerryError(code, "pages", "found on the device")
 
     # ---- managing pages ---------------------------------------------------------

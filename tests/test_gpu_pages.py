@@ -392,3 +392,17 @@ def test_lanes_that_grow_by_other_lanes_lengths(n, tokens):
     b.l.reserve(order, first)
     b.p.check()
     b.same()
+
+
+def test_an_error_found_on_another_stream():
+    p = F.Pages.empty(1, 1, 8, 4, 4, F.BF16)
+    bad, s = ints([9]), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with torch.cuda.stream(s):
+            torch.cuda._sleep(20_000_000)  # still to come when the check begins
+            p.trim(bad)
+        with pytest.raises(F.FerryError) as e:
+            p.check()
+        assert e.value.code == EINVAL
+    p.check()
