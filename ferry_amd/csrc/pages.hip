@@ -846,6 +846,21 @@ void launch_append(const PageView& v, int layer, const AppendArgs& a, int pt, in
   else launch_append<XT, FERRY_FP8_E4M3>(v, layer, a, cus, s);
 }
 
+// Tokens [t, t + kLaunchTokens) of a call: a launch has a workgroup per token, and fewer
+// than 2^32 threads.
+constexpr int kLaunchTokens = 1 << 23;
+AppendArgs tokens_from(AppendArgs a, int t, int x_size, int out_size) {
+  a.n = std::min(a.n - t, kLaunchTokens);
+  if (a.lane) a.lane += t;
+  a.pos += t;
+  auto at = [&](const void* x, int64_t stride, int size) -> const void* {
+    return x ? static_cast<const uint8_t*>(x) + t * stride * size : nullptr;
+  };
+  a.q = at(a.q, a.qs[0], x_size), a.k = at(a.k, a.ks[0], x_size), a.v = at(a.v, a.vs[0], x_size);
+  a.q_out = const_cast<void*>(at(a.q_out, a.os[0], out_size));
+  return a;
+}
+
 // The common start of the managing calls.
 int manage(const ferry_pages* p, int n, PageView* v, Work* w) {
   if (int rc = page_geometry(p, v)) return rc;
@@ -1004,10 +1019,15 @@ int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* 
                  {a->v_stride[0], a->v_stride[1]}, {a->q_out_stride[0], a->q_out_stride[1]}};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int cus = gpu_cus(p->device);
-    if (a->x_dtype == FERRY_F32) launch_append<FERRY_F32>(v, layer, d, p->dtype, cus, s);
-    else if (a->x_dtype == FERRY_F16) launch_append<FERRY_F16>(v, layer, d, p->dtype, cus, s);
-    else launch_append<FERRY_BF16>(v, layer, d, p->dtype, cus, s);
-    return launched("ferry_pages_append");
+    for (int t = 0; t < a->n_tokens; t += kLaunchTokens) {
+      const AppendArgs part = tokens_from(d, t, a->x_dtype == FERRY_F32 ? 4 : 2, ot == FERRY_F32 ? 4 : 2);
+      if (a->x_dtype == FERRY_F32) launch_append<FERRY_F32>(v, layer, part, p->dtype, cus, s);
+      else if (a->x_dtype == FERRY_F16) launch_append<FERRY_F16>(v, layer, part, p->dtype, cus, s);
+      else launch_append<FERRY_BF16>(v, layer, part, p->dtype, cus, s);
+      if (int rc = launched("ferry_pages_append")) return rc;
+      if (a->n_tokens - t <= kLaunchTokens) break;
+    }
+    return FERRY_OK;
   });
 }
 

@@ -360,3 +360,22 @@ def test_no_frequencies():
     with pytest.raises(ValueError, match="inv_freq"):
         p.append(0, ints([0]), ints([0]), q=torch.zeros((1, 1, 128), device="cuda"),
                  q_out=torch.zeros((1, 1, 128), device="cuda"))
+
+
+def test_more_tokens_than_a_launch_has_workgroups():
+    # a workgroup per token, and a launch has fewer than 2^32 threads
+    n = (1 << 24) + 40
+    p = F.Pages.empty(1, 1, (1 << 20) + 3, 2, 1 << 20)
+    p.table[0] = torch.arange(1 << 20, dtype=torch.int32, device="cuda")
+    p.table[1, :3] = ints([(1 << 20) + i for i in range(3)])
+    p.length.copy_(ints([1 << 24, 40]))
+    at = torch.arange(n, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randint(1, 1 << 14, (n, 1, D), device="cuda", generator=g, dtype=torch.int16).view(torch.bfloat16)
+            for _ in range(2))
+    p.append(0, at >> 24, at & ((1 << 24) - 1), k=k, v=v,
+             inv_freq=torch.zeros(64, dtype=torch.float64, device="cuda"))  # no turn: the same bits
+    p.check()
+    for i, x in enumerate((k, v)):
+        got = p.pool[0, :, 0, i].reshape(-1, D)[:n].view(torch.int16)
+        assert torch.equal(got, x.view(torch.int16)[:, 0])
