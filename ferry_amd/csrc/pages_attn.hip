@@ -1434,15 +1434,15 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
 // ones first.  16 lanes take a row, 8 dims each; SPLIT such teams share out a row's
 // parts (16, a workgroup, where the rows are few and their parts may be many, else 1).
 // Bound by the latency of three dependent reads (where, part, write), so many rows are
-// in flight and four parts of each.
+// in flight and four parts of each.  r0: the launch's first row.
 template <int DT, int SPLIT>
-__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid) {
+__global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs a, Scratch ws, int grid, uint64_t r0) {
   constexpr int kTeams = kThreads / 16, kAhead = 4;
   __shared__ float got[SPLIT > 1 ? kTeams : 1][kPad];
   const int team = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
   const uint32_t rows = (uint32_t)a.n_tokens * a.G;
   const uint64_t all = (uint64_t)rows * v.H;
-  const uint64_t r = SPLIT > 1 ? blockIdx.x : (uint64_t)blockIdx.x * kTeams + team;
+  const uint64_t r = SPLIT > 1 ? blockIdx.x : r0 + (uint64_t)blockIdx.x * kTeams + team;
   if (r >= all) return;
   const uint32_t h = (uint32_t)(r / rows), row = (uint32_t)(r % rows);
   const int tok = token_of_row(a, (int)row);
@@ -1575,8 +1575,13 @@ void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scra
   }
   // a workgroup per row where that does not fill the GPU twice
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
-  if (all <= 2ull * grid) k_attend_join<DT, 16><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid);
-  else k_attend_join<DT, 1><<<(unsigned)((all + 15) / 16), kThreads, 0, s>>>(v, a, ws, grid);
+  if (all <= 2ull * grid) {
+    k_attend_join<DT, 16><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid, 0);
+    return;
+  }
+  constexpr uint64_t kMost = 1ull << 27;  // rows of a launch, which has fewer than 2^32 threads
+  for (uint64_t r0 = 0; r0 < all; r0 += kMost)
+    k_attend_join<DT, 1><<<(unsigned)((std::min(all - r0, kMost) + 15) / 16), kThreads, 0, s>>>(v, a, ws, grid, r0);
 }
 
 }  // namespace

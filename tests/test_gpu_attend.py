@@ -749,3 +749,36 @@ def test_a_long_tail_of_small_weights(dt, n, new):
         bound = u * want.abs() + A * (u + soft) * (1 + u) + 2.0 ** -25 + see * 2.0 ** -32 / tops * 1.5
         assert torch.all((out[row, 0].double() - want).abs() <= bound)
         assert abs(float(lse[row, 0]) - float(want_e)) <= 2 * soft + 2.0 ** -23 * abs(float(want_e))
+
+
+def test_more_rows_than_a_launch_joins():
+    # A launch of the join has fewer than 2^32 threads.  Two requests of more than 2^28 rows
+    # together: the first one's rows see next to nothing, the second's are the last and see so
+    # much that several workgroups share them.  In the queries' place: 69 GB.
+    Hq, n, len_ = 128, (1 << 21) + 1000, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = torch.randn((1, len_ // T, 1, 2, T, D), device="cuda", generator=g)
+    pool[:, :, :, 1] += 1.0
+    pool = pool.to(torch.bfloat16)
+    p = F.Pages(pool, torch.arange(len_ // T, dtype=torch.int32, device="cuda").repeat(2, 1), ints([40, len_]))
+    q = torch.full((n, Hq, D), 3.0, dtype=torch.bfloat16, device="cuda")
+    last = n - 7  # the rest: behind the last request
+    rows = torch.randn((Hq, D), device="cuda", generator=g).to(torch.bfloat16)
+    q[last - 1] = rows
+    lse = torch.zeros((n, Hq), device="cuda")
+    p.attend(0, q, q, ints([0, 1]), q_start=ints([0, last - 1, last]), lse=lse)
+    torch.cuda.synchronize()
+    p.check()
+    k, v = pool[0, :, 0, 0].reshape(-1, D).float(), pool[0, :, 0, 1].reshape(-1, D).float()
+    for h in range(0, Hq, 9):
+        s = (D ** -0.5 * (k @ rows[h].float())).double()
+        want_e = torch.logsumexp(s, 0)
+        w = torch.exp(s - want_e)
+        want, A = (w[None].float() @ v)[0].double(), (w[None].float() @ v.abs())[0].double()
+        # the bound of this file; the products above are fp32 too
+        S = float((D ** -0.5 * (k.abs() @ rows[h].float().abs())).max())
+        soft = 2 * (2 * 130 * S + len_ / 8 + 64) * 2.0 ** -24
+        assert torch.all((q[last - 1, h].double() - want).abs() <= 2.0 ** -8 * (want.abs() + 2 * A) + A * soft)
+        assert abs(float(lse[last - 1, h] - want_e)) <= 2 * soft + 2.0 ** -23 * float(want_e)
+    assert not q[:last - 41].any() and torch.all(q[last:] == 3.0)
+    assert torch.all(torch.isfinite(q[last - 41:last - 1])) and torch.all(lse[last - 41:last - 1] > -np.inf)
