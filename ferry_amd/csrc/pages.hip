@@ -933,9 +933,12 @@ int ferry_pages_fork(const ferry_pages* p, const int32_t* src, const int32_t* ds
     OnDevice on(p->device);
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    // One launch where a wavefront has at most eight 64-entry rows' worth (24 lanes of 58
-    // pages: 3.9 us, 6.4 in two launches), which bounds what the workgroup does alone.
-    if ((int64_t)n * p->max_pages <= 8192) {
+    // One launch where each of its 16 wavefronts has at most four times 64 entries of a row
+    // (24 lanes of 58 pages: 4.0 us, 5.7 in two launches); else what the workgroup does alone
+    // takes longer than a launch (128 lanes of 64 pages: 8.2 and 5.9; 1,000 of 8: 70 and 11;
+    // one of 8,192: 41 and 15).
+    const int64_t rounds = (int64_t)((n + 15) / 16) * ((p->max_pages + 63) / 64);
+    if (rounds <= 4) {
       k_fork_small<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);
     } else {
       k_fork_plan<<<1, kPlan, 0, s>>>(v, w, src, dst, keep, n);

@@ -406,3 +406,10 @@ def test_an_error_found_on_another_stream():
             p.check()
         assert e.value.code == EINVAL
     p.check()
+
+
+@pytest.mark.parametrize("n,pages", [(1, 256), (1, 257), (16, 200), (17, 129), (64, 64), (65, 64), (900, 3)])
+def test_forks_on_both_sides_of_one_launch(n, pages):
+    b = Both(3 * pages + 4, n + 3, pages, F.FP8, 1, 1)
+    assert b.call("reserve", [n, n + 1, n + 2], [16 * pages, 16 * pages - 7, 5]) == 0
+    assert b.call("fork", [n + i % 3 for i in range(n)], list(range(n))[::-1]) == 0
