@@ -1043,8 +1043,8 @@ int ferry_rope_freqs(int kind, int32_t rot_dim, double base, double stretch, dou
     if (!(base > 0.0) || !(stretch > 0.0) || !std::isfinite(base) || !std::isfinite(stretch))
       return report(FERRY_EINVAL, "base and stretch must be positive");
     if (kind == FERRY_ROPE_BASE && rot_dim < 4) return report(FERRY_EINVAL, "FERRY_ROPE_BASE needs rot_dim of 4 or more");
-    if (kind == FERRY_ROPE_PARTS && !(trained_ctx > 0.0 && fast > slow))
-      return report(FERRY_EINVAL, "FERRY_ROPE_PARTS needs trained_ctx > 0 and fast > slow");
+    if (kind == FERRY_ROPE_PARTS && !(trained_ctx > 0.0 && fast > slow && std::isfinite(trained_ctx + fast - slow)))
+      return report(FERRY_EINVAL, "FERRY_ROPE_PARTS needs trained_ctx > 0 and fast > slow, all finite");
     if (kind == FERRY_ROPE_BASE) base *= std::pow(stretch, (double)rot_dim / (rot_dim - 2));
     for (int i = 0; i < rot_dim / 2; ++i) {
       const double f = std::pow(base, -2.0 * i / rot_dim);

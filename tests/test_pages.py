@@ -103,3 +103,9 @@ def test_rope_frequencies():
 def test_rope_refusals(args):
     with pytest.raises(F.FerryError):
         F.rope_freqs(*args)
+
+
+@pytest.mark.parametrize("args", [(math.inf, 1.0, 32.0), (8192.0, -math.inf, 32.0), (8192.0, 1.0, math.inf)])
+def test_frequencies_in_parts_that_are_not_finite_are_refused(args):
+    with pytest.raises(F.FerryError, match="all finite"):
+        F.rope_freqs(F.ROPE_PARTS, 64, 1e4, 2.0, *args)
