@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kPlan) void k_reserve_plan(PageView v, Work w, cons
       atomicMin(&bad, FERRY_EINVAL);
     } else {
       const int had = v.len[lane];
-      w.had[i] = had, w.grown[i] = had + t;
+      w.had[i] = had, w.grown[i] = (uint32_t)had + (uint32_t)t;
       my_lane = lane, my_had = had, my_tokens = t;
       if (had < 0 || (int64_t)had + t > (int64_t)v.max_pages * kPageTokens) {
         atomicMin(&bad, FERRY_ECAPACITY);

@@ -546,7 +546,8 @@ int ferry_pages_compact(const ferry_pages* pages, int32_t* live, void* stream);
  * dims (even, 2..128) of q and k heads turn by pos[t] * inv_freq[i] in pairs
  * (i, i + rot_dim / 2), or (2i, 2i + 1) with `pairs` != 0, times `factor`:
  *   x_a' = factor (x_a cos - x_b sin),  x_b' = factor (x_b cos + x_a sin)
- * (angles in 64 bits, products in 32, one rounding).  Then k and v go to the
+ * (angles in 64 bits down to a part of a turn; its cosine and sine, products and
+ * sums in 32; one rounding to the stored type).  Then k and v go to the
  * lane's page in its element type; fp8 pages hold the E4M3 code of x / scale
  * with kv_scale [kv_heads][2] (K, V), which is also written beside the record:
  * all tokens of a page have to come with the same.  q goes to q_out.

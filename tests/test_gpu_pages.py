@@ -413,3 +413,11 @@ def test_forks_on_both_sides_of_one_launch(n, pages):
     b = Both(3 * pages + 4, n + 3, pages, F.FP8, 1, 1)
     assert b.call("reserve", [n, n + 1, n + 2], [16 * pages, 16 * pages - 7, 5]) == 0
     assert b.call("fork", [n + i % 3 for i in range(n)], list(range(n))[::-1]) == 0
+
+
+@pytest.mark.parametrize("n", [3, 1100])
+def test_growth_past_31_bits_is_refused(n):
+    b = Both(n + 20, n, 9, F.BF16, 1, 1)
+    assert b.call("reserve", list(range(n)), [1 + i % 16 for i in range(n)]) == 0
+    for t in (2 ** 31 - 1, 2 ** 31 - 16, 9 * 16):
+        assert b.call("reserve", [2, 1, 0] + list(range(3, n)), [0, t, 0] + [0] * (n - 3)) == ECAPACITY
