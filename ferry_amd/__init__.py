@@ -132,6 +132,28 @@ class AppendArgs(C.Structure):
     ]
 
 
+class AxesArgs(C.Structure):
+    _fields_ = [("n_axes", _i32), ("pad", _i32), ("at", _vp), ("stride", C.c_int64), ("axis", _vp)]
+
+
+class SeenArgs(C.Structure):
+    _fields_ = [("window", _i32), ("sinks", _i32), ("tree_words", _i32), ("pad", _i32), ("tree", _vp)]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [
+        ("n_req", _i32), ("n_tokens", _i32), ("tree_words", _i32), ("pad", _i32), ("lanes", _vp),
+        ("q_start", _vp), ("parent", _vp), ("tree", _vp), ("at", _vp), ("place", _vp), ("lane", _vp),
+    ]
+
+
+class AcceptArgs(C.Structure):
+    _fields_ = [
+        ("n_req", _i32), ("n_tokens", _i32), ("lanes", _vp), ("q_start", _vp), ("parent", _vp),
+        ("draft", _vp), ("chosen", _vp), ("path", _vp), ("kept", _vp), ("next", _vp),
+    ]
+
+
 class AttendArgs(C.Structure):
     _fields_ = [
         ("n_req", _i32), ("n_tokens", _i32), ("n_groups", _i32), ("q_heads", _i32),
@@ -218,10 +240,14 @@ _PROTOS = {
     "ferry_pages_fork": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _vp, _i32, _vp]),
     "ferry_pages_trim": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp, _i32, _vp]),
     "ferry_pages_compact": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp]),
-    # (args: AppendArgs / AttendArgs by reference, or packed as below)
+    # (args: structures by reference, or packed as below)
     "ferry_pages_append": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp]),
     "ferry_pages_attend_work_bytes": (C.c_int, [C.POINTER(PagesDesc), _vp, C.POINTER(C.c_uint64)]),
     "ferry_pages_attend": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp]),
+    "ferry_pages_append_axes": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp, _vp]),
+    "ferry_pages_attend_seen": (C.c_int, [C.POINTER(PagesDesc), _i32, _vp, _vp, _vp]),
+    "ferry_pages_tree": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp]),
+    "ferry_pages_accept": (C.c_int, [C.POINTER(PagesDesc), _vp, _vp]),
     "ferry_rope_freqs": (C.c_int, [C.c_int, _i32, C.c_double, C.c_double, C.c_double, C.c_double,
                                    C.c_double, _vp]),
     "ferry_refgen_selections": (C.c_int, [_i32, _i32, _i32, _i32, C.c_uint64, _vp]),
@@ -623,7 +649,13 @@ def rope_freqs(kind, rot_dim, base=10000.0, stretch=1.0, trained_ctx=0.0, slow=1
 _X_DTYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _APPEND = struct.Struct("@6ifi8P8q")  # AppendArgs, AttendArgs: packing them takes a tenth of
 _ATTEND = struct.Struct("@4ifi7P4qPQ")  # the time of filling a ctypes structure
+_AXES = struct.Struct("@2iPqP")
+_SEEN = struct.Struct("@4iP")
+_TREE = struct.Struct("@4i7P")
+_ACCEPT = struct.Struct("@2i8P")
 assert _APPEND.size == C.sizeof(AppendArgs) and _ATTEND.size == C.sizeof(AttendArgs)
+assert _AXES.size == C.sizeof(AxesArgs) and _SEEN.size == C.sizeof(SeenArgs)
+assert _TREE.size == C.sizeof(TreeArgs) and _ACCEPT.size == C.sizeof(AcceptArgs)
 _PAGE_TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16,
                FP8: torch.float8_e4m3fn}
 
@@ -763,10 +795,12 @@ class Pages:
         return t.data_ptr(), a, b
 
     def append(self, layer, lane, pos, k=None, v=None, q=None, q_out=None, inv_freq=None, factor=1.0,
-               pairs=False, kv_scale=None, stream=None):
+               pairs=False, kv_scale=None, stream=None, at=None, axis=None):
         """Rotary positions of q (into q_out) and k, and k and v into the pages:
         token t is at place pos[t] of lane[t] (int32 tensors).  inv_freq is a
-        float64 tensor of rot_dim / 2 radians per token."""
+        float64 tensor of rot_dim / 2 radians per token.  at: positions apart from the
+        places, int32 [tokens] or [axes, tokens]; pair i turns by at[axis[i]] (axis
+        int32 [rot_dim / 2], needed with several axes)."""
         n = pos.numel()
         x = q if q is not None else k
         if x is None:
@@ -790,16 +824,34 @@ class Pages:
                          factor, 0, self._list(lane, "lane", n) or 0, self._list(pos, "pos", n),
                          _dev(inv_freq, "inv_freq", 1, (torch.float64,), self.device), sp[0],
                          qp[0], kp[0], vp[0], op[0], qp[1], qp[2], kp[1], kp[2], vp[1], vp[2], op[1], op[2])
+        axes = None
+        if at is not None:
+            ap, count, stride = self._axes(at, n)
+            axes = _AXES.pack(count, 0, ap, stride, self._list(axis, "axis", inv_freq.numel()) or 0)
+        elif axis is not None:
+            raise ValueError("axis goes with at")
         if n == 0 and 0 <= layer < self._d.n_layers:
             return  # empty tensors have no address
-        _check(lib.ferry_pages_append(self._r, layer, a, self._s(stream)), "ferry_pages_append")
+        _check(lib.ferry_pages_append_axes(self._r, layer, a, axes, self._s(stream)), "ferry_pages_append")
+
+    def _axes(self, at, n):
+        """Pointer, number of axes and elements between them of positions [n] or [axes, n]."""
+        if not isinstance(at, torch.Tensor) or at.get_device() != self.device:
+            raise ValueError(f"at: expected a CUDA tensor on cuda:{self.device}")
+        if at.dtype is not torch.int32:
+            raise ValueError(f"at: dtype {at.dtype}, expected torch.int32")
+        if at.dim() not in (1, 2) or at.shape[-1] != n or (n > 1 and at.stride(-1) != 1):
+            raise ValueError(f"at: expected [{n}] or [axes, {n}], the tokens of an axis contiguous")
+        return at.data_ptr(), 1 if at.dim() == 1 else at.shape[0], 0 if at.dim() == 1 else at.stride(0)
 
     def attend(self, layer, q, out, lanes, q_start=None, group_start=None, shared=None, scale=0.0,
-               lse=None, stream=None):
+               lse=None, stream=None, window=0, sinks=0, tree=None):
         """Attention of the new query rows q [rows, q heads, 128] of lanes (all rows
         of request r are [q_start[r], q_start[r+1]); None: one row each), into
         out; requests [group_start[g], group_start[g+1]) share their first
-        shared[g] pages."""
+        shared[g] pages.  window > 0: a row sees its last `window` tokens and the lane's
+        first `sinks`.  tree: int64 [rows, words], the bits of the new tokens of its
+        request that a row sees (Pages.tree makes them)."""
         n, rows, heads, groups, sp = lanes.numel(), q.shape[0], q.shape[1], 0, None
         dt = (self.q_dtype,)
         qp, qa, qb = self._rows(q, "q", rows, 0, dt)
@@ -819,6 +871,11 @@ class Pages:
             if len(self._attend_bytes) >= 4096:
                 self._attend_bytes.clear()
             need = self._attend_bytes[shape] = b.value
+        seen, words, tp = None, 0, 0
+        if tree is not None:
+            tp, words = self._tree(tree, rows)
+        if window or sinks or words:
+            seen = _SEEN.pack(window, sinks, words, 0, tp)
         s = self._s(stream)
         if stream is None or s == self._s(None):
             work = torch.empty(need, dtype=torch.uint8, device=self.pool.device)
@@ -830,7 +887,40 @@ class Pages:
                          self._list(q_start, "q_start", n + 1) or 0,
                          self._list(group_start, "group_start", 1) or 0, sp or 0, qp, op, ep or 0,
                          qa, qb, oa, ob, work.data_ptr(), need)
-        _check(lib.ferry_pages_attend(self._r, layer, a, s), "ferry_pages_attend")
+        _check(lib.ferry_pages_attend_seen(self._r, layer, a, seen, s), "ferry_pages_attend")
+
+    # ---- drafted tokens -----------------------------------------------------------
+    def _tree(self, tree, rows):
+        """Pointer and words of a tensor of drafts' bits."""
+        if not isinstance(tree, torch.Tensor) or tree.dim() != 2 or tree.shape[0] != rows or tree.shape[1] < 1:
+            raise ValueError(f"tree: expected [{rows}, words]")
+        return _dev(tree, "tree", 1 if rows else 0, (torch.int64,), self.device), tree.shape[1]
+
+    def tree(self, lanes, parent, tree, at=None, place=None, lane=None, q_start=None, stream=None):
+        """Trees of drafted tokens from their parents [rows] (numbers within the request,
+        -1: a root): the bits of each token's ancestors and of itself into tree (int64
+        [rows, words]), its position (the depth) into at, its place in the lane and its
+        lane into place and lane, as append takes them."""
+        n, rows = lanes.numel(), parent.numel()
+        tp, words = self._tree(tree, rows)
+        a = _TREE.pack(n, rows, words, 0, self._list(lanes, "lanes", n),
+                       self._list(q_start, "q_start", n + 1) or 0, self._list(parent, "parent", rows), tp,
+                       self._list(at, "at", rows) or 0, self._list(place, "place", rows) or 0,
+                       self._list(lane, "lane", rows) or 0)
+        _check(lib.ferry_pages_tree(self._r, a, self._s(stream)), "ferry_pages_tree")
+
+    def accept(self, lanes, draft, chosen, path, kept, next, q_start=None, parent=None, stream=None):
+        """Of each request's new tokens the first stays, then the first child whose
+        draft is what the model chose after its parent, and so on: their keys and values
+        move up behind the context, the lane ends behind them.  path [rows] gets the rows
+        that stay, kept [requests] their number, next [requests] the choice after the last.
+        parent None: each token's parent is the one before it."""
+        n, rows = lanes.numel(), draft.numel()
+        a = _ACCEPT.pack(n, rows, self._list(lanes, "lanes", n), self._list(q_start, "q_start", n + 1) or 0,
+                         self._list(parent, "parent", rows) or 0, self._list(draft, "draft", rows),
+                         self._list(chosen, "chosen", rows), self._list(path, "path", rows),
+                         self._list(kept, "kept", n), self._list(next, "next", n))
+        _check(lib.ferry_pages_accept(self._r, a, self._s(stream)), "ferry_pages_accept")
 
 
 _hip = None

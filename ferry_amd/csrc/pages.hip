@@ -80,50 +80,9 @@ namespace {
 constexpr int kPlan = 1024;  // threads of the one-workgroup kernels that plan a call
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Scratch of the managing calls: a header, then arrays sized by the cache.
-struct Plan {
-  int ok;         // the call is made
-  uint32_t need;  // pages taken (reserve)
-  uint32_t copies;  // pages copied (reserve) or moved (compact)
-  int handed;     // tables, lengths and refs hold the pages taken (reserve)
-};
-struct Work {
-  Plan* plan;
-  uint32_t* free_ids;  // [n_pages] pages taken, in order (reserve); new id of each page (compact)
-  uint32_t* uses;      // [n_pages] listed lanes whose last page this is (reserve)
-  uint32_t* last;      // [n_pages] the last of them
-  uint32_t* base;      // [n_lanes] first of a listed lane's places in free_ids
-  uint32_t* had;       // [n_lanes] its tokens before the call
-  uint32_t* grown;     // [n_lanes] and after it
-  uint32_t* copy_lane;  // [n_lanes] list places whose last page is copied
-  uint32_t* copy_from;  // [n_lanes] ... and that page
-  uint32_t* from;      // [n_pages] pages moved (compact)
-};
-
-uint64_t up16(uint64_t x) { return (x + 15) & ~15ull; }
-
-Work split_work(void* w, int n_pages, int n_lanes) {
-  uint8_t* p = static_cast<uint8_t*>(w);
-  const uint64_t pg = up16((uint64_t)n_pages * 4), ln = up16((uint64_t)n_lanes * 4);
-  Work r;
-  r.plan = reinterpret_cast<Plan*>(p), p += 64;
-  r.free_ids = reinterpret_cast<uint32_t*>(p), p += pg;
-  r.uses = reinterpret_cast<uint32_t*>(p), p += pg;
-  r.last = reinterpret_cast<uint32_t*>(p), p += pg;
-  r.from = r.uses;
-  r.base = reinterpret_cast<uint32_t*>(p), p += ln;
-  r.had = reinterpret_cast<uint32_t*>(p), p += ln;
-  r.grown = reinterpret_cast<uint32_t*>(p), p += ln;
-  r.copy_lane = reinterpret_cast<uint32_t*>(p), p += ln;
-  r.copy_from = reinterpret_cast<uint32_t*>(p);
-  return r;
-}
-
 uint64_t work_bytes(int n_pages, int n_lanes) {
   return 64 + 3 * up16((uint64_t)n_pages * 4) + 5 * up16((uint64_t)n_lanes * 4);
 }
-
-__device__ inline int pages_of(int tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
 
 // Exclusive prefix sum of x over the workgroup of kPlan threads; *total gets the sum.
 __device__ inline uint64_t block_scan(uint64_t x, uint64_t* total) {
@@ -146,13 +105,6 @@ __device__ inline uint64_t block_scan(uint64_t x, uint64_t* total) {
   __syncthreads();
   *total = all;
   return before + s - x;
-}
-
-// Names each lane of the list in an LDS bitmap (n_lanes bits); false where one
-// is out of range or named twice.  The caller clears the bitmap first.
-__device__ inline bool name_lane(uint32_t* bits, int lane, int n_lanes) {
-  if (lane < 0 || lane >= n_lanes) return false;
-  return !(atomicOr(&bits[lane >> 5], 1u << (lane & 31)) >> (lane & 31) & 1u);
 }
 
 // ---- reserve -------------------------------------------------------------------
@@ -468,17 +420,7 @@ __global__ __launch_bounds__(256) void k_trim(PageView v, const int32_t* __restr
   }
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     const int lane = lanes[i], kept = keep ? keep[i] : 0, held = v.len[lane];
-    uint32_t* row = v.table + (uint64_t)lane * v.max_pages;
-    for (int e = pages_of(kept) + threadIdx.x; e < pages_of(held); e += blockDim.x) {
-      const uint32_t id = row[e];
-      row[e] = kNone;
-      if (id >= (uint32_t)v.n_pages) {
-        set_error(v.error, FERRY_ESTATE);
-      } else if ((int)atomicSub(&v.refs[id], 1u) <= 0) {  // counted as free: it stays so
-        atomicAdd(&v.refs[id], 1u);
-        set_error(v.error, FERRY_ESTATE);
-      }
-    }
+    drop_pages(v, lane, held, kept);
     __syncthreads();  // all have read the length
     if (threadIdx.x == 0) v.len[lane] = kept;
   }
@@ -575,7 +517,22 @@ struct AppendArgs {
   const void *q, *k, *v;
   void* q_out;
   int64_t qs[2], ks[2], vs[2], os[2];
+  int axes;  // positions apart from the places: their axes (0: the places are the positions)
+  const int32_t* at;    // [axes][n], at_stride between axes
+  int64_t at_stride;
+  const int32_t* axis;  // [rot / 2] (null: 0)
 };
+
+// The position that turns pair i of token t, at place pos.
+__device__ inline int position(const PageView& v, const AppendArgs& a, int i, int t, int pos) {
+  if (!a.axes) return pos;
+  int x = a.axis ? a.axis[i] : 0;
+  if ((uint32_t)x >= (uint32_t)a.axes) {
+    set_error(v.error, FERRY_ERANGE);
+    x = 0;
+  }
+  return a.at[x * a.at_stride + t];
+}
 
 // cos and sin of 2 pi t in fp32.  The part of a turn is taken in 64 bits (positions of
 // 2^24 leave 2^-30 of a turn), down to the eighth of a turn next to a quarter, so that
@@ -691,6 +648,7 @@ __global__ __launch_bounds__(256) void k_append(PageView v, int layer, AppendArg
   __shared__ __attribute__((aligned(16))) float cs[64], sn[64];
   const int t = blockIdx.x, tid = threadIdx.x, d = (tid & 15) * 8;
   const int pos = a.pos[t];
+  const int turned_by = tid < a.rot / 2 ? position(v, a, tid, t, pos) : 0;  // on its way with the page
   const int64_t page = append_page(v, a, t, pos);
   if (page < 0) return;
   const int all = a.Hq + (a.k ? 2 * v.H : 0);
@@ -719,7 +677,7 @@ __global__ __launch_bounds__(256) void k_append(PageView v, int layer, AppendArg
       first = false;
       if (tid < half) {
         float c, s;
-        turn((double)pos * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
+        turn((double)turned_by * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
         cs[tid] = c * a.factor, sn[tid] = s * a.factor;
       }
       __syncthreads();
@@ -778,7 +736,7 @@ __global__ __launch_bounds__(256) void k_append_any(PageView v, int layer, Appen
   if (page < 0) return;
   if (tid < half) {
     float c, s;
-    turn((double)pos * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
+    turn((double)position(v, a, tid, t, pos) * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
     cs[tid] = c * a.factor, sn[tid] = s * a.factor;
   }
   __syncthreads();
@@ -853,6 +811,7 @@ AppendArgs tokens_from(AppendArgs a, int t, int x_size, int out_size) {
   a.n = std::min(a.n - t, kLaunchTokens);
   if (a.lane) a.lane += t;
   a.pos += t;
+  if (a.axes) a.at += t;
   auto at = [&](const void* x, int64_t stride, int size) -> const void* {
     return x ? static_cast<const uint8_t*>(x) + t * stride * size : nullptr;
   };
@@ -861,7 +820,10 @@ AppendArgs tokens_from(AppendArgs a, int t, int x_size, int out_size) {
   return a;
 }
 
-// The common start of the managing calls.
+}  // namespace
+
+namespace ferry_amd {
+
 int manage(const ferry_pages* p, int n, PageView* v, Work* w) {
   if (int rc = page_geometry(p, v)) return rc;
   if (n < 0 || n > p->n_lanes) return report(FERRY_EINVAL, "n must be in [0, n_lanes]");
@@ -870,10 +832,7 @@ int manage(const ferry_pages* p, int n, PageView* v, Work* w) {
   return FERRY_OK;
 }
 
-// A list of n values that a managing call reads (or writes): device memory apart from what
-// the call changes, since its workgroups read the list while others already change that.
-// of_len: the call has read the list before it changes len.
-int check_list(const ferry_pages* p, const void* list, const char* name, int n, bool of_len = false) {
+int check_list(const ferry_pages* p, const void* list, const char* name, int n, bool of_len) {
   if (int rc = check_on(list, name, p->device)) return rc;
   const uintptr_t from = reinterpret_cast<uintptr_t>(list), to = from + (uintptr_t)n * 4;
   auto meets = [&](const void* buf, uint64_t entries) {
@@ -885,7 +844,7 @@ int check_list(const ferry_pages* p, const void* list, const char* name, int n, 
   return FERRY_OK;
 }
 
-}  // namespace
+}  // namespace ferry_amd
 
 extern "C" {
 
@@ -984,6 +943,11 @@ int ferry_pages_compact(const ferry_pages* p, int32_t* live, void* stream) {
 }
 
 int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* a, void* stream) {
+  return ferry_pages_append_axes(p, layer, a, nullptr, stream);
+}
+
+int ferry_pages_append_axes(const ferry_pages* p, int32_t layer, const ferry_append* a, const ferry_axes* axes,
+                            void* stream) {
   return entry([&]() -> int {
     PageView v;
     if (int rc = page_geometry(p, &v)) return rc;
@@ -994,6 +958,8 @@ int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* 
       return report(FERRY_EINVAL, "x_dtype must be F32, F16 or BF16");
     if (a->rot_dim < 2 || a->rot_dim > kPageDim || a->rot_dim % 2)
       return report(FERRY_EINVAL, "rot_dim must be even, 2..128");
+    if (axes && (axes->n_axes < 1 || axes->n_axes > 4)) return report(FERRY_EINVAL, "n_axes must be 1..4");
+    if (axes && axes->n_axes > 1 && !axes->axis) return report(FERRY_EINVAL, "several axes need axis");
     if (a->n_tokens == 0) return FERRY_OK;
     if (!a->q && !a->k) return report(FERRY_EINVAL, "neither q nor k");
     if (!a->k != !a->v) return report(FERRY_EINVAL, "k and v go together");
@@ -1002,6 +968,10 @@ int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* 
     if (a->q && (a->q_heads < 1 || a->q_heads > 65536)) return report(FERRY_EINVAL, "q_heads out of range");
     if (int rc = page_buffers(p, false)) return rc;
     if (int rc = check_all({{a->pos, "pos"}, {a->inv_freq, "inv_freq"}}, p->device)) return rc;
+    if (axes)
+      if (int rc = check_on(axes->at, "at", p->device)) return rc;
+    if (axes && axes->axis)
+      if (int rc = check_on(axes->axis, "axis", p->device)) return rc;
     if (a->k || a->lane)
       if (int rc = check_on(a->lane, "lane", p->device)) return rc;
     if (a->q)
@@ -1019,7 +989,8 @@ int ferry_pages_append(const ferry_pages* p, int32_t layer, const ferry_append* 
     AppendArgs d{a->n_tokens, a->q ? a->q_heads : 0, a->rot_dim, a->pairs != 0, ot, 0, a->factor, a->lane, a->pos,
                  a->inv_freq, a->kv_scale, a->q, a->k, a->v, a->q_out,
                  {a->q_stride[0], a->q_stride[1]}, {a->k_stride[0], a->k_stride[1]},
-                 {a->v_stride[0], a->v_stride[1]}, {a->q_out_stride[0], a->q_out_stride[1]}};
+                 {a->v_stride[0], a->v_stride[1]}, {a->q_out_stride[0], a->q_out_stride[1]}, 0, nullptr, 0, nullptr};
+    if (axes) d.axes = axes->n_axes, d.at = axes->at, d.at_stride = axes->stride, d.axis = axes->axis;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int cus = gpu_cus(p->device);
     for (int t = 0; t < a->n_tokens; t += kLaunchTokens) {

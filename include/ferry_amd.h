@@ -576,6 +576,22 @@ typedef struct ferry_append {
 int ferry_pages_append(const ferry_pages* pages, int32_t layer, const ferry_append* args,
                        void* stream);
 
+/* The same with positions apart from the places, on several axes (a picture's time,
+ * height and width, or one: the depth of a drafted token): pair i of token t turns by
+ * at[axis[i]][t] * inv_freq[i], while k and v still go to place pos[t].
+ *   at    [n_axes][n_tokens] int32, `stride` elements between axes (n_axes 1..4)
+ *   axis  [rot_dim / 2] int32, the axis of each pair; NULL with one axis.  One that is
+ *         out of range latches FERRY_ERANGE; its pairs then turn by axis 0
+ * axes NULL is ferry_pages_append. */
+typedef struct ferry_axes {
+  int32_t n_axes, pad;
+  const int32_t* at;
+  int64_t stride;
+  const int32_t* axis;
+} ferry_axes;
+int ferry_pages_append_axes(const ferry_pages* pages, int32_t layer, const ferry_append* args,
+                            const ferry_axes* axes, void* stream);
+
 /* Frequencies of rotary pairs for inv_freq, w_i = base^(-2i / rot_dim) and
  * its forms for contexts `stretch` times the trained one (host; out
  * [rot_dim / 2]):
@@ -639,6 +655,86 @@ int ferry_pages_attend_work_bytes(const ferry_pages* pages, const ferry_attend* 
                                   uint64_t* bytes);
 int ferry_pages_attend(const ferry_pages* pages, int32_t layer, const ferry_attend* args,
                        void* stream);
+
+/* The same where a row sees only a part of what is before it; seen NULL is
+ * ferry_pages_attend.  The scratch is that of ferry_pages_attend_work_bytes.
+ * window > 0: a sliding window with sinks.  The row at place i of its lane (len -
+ *   n + j for row j of n) sees the tokens t <= i with t > i - window or t < sinks.
+ *   Pages between the sinks and the window are not read.  No groups go with it.
+ * tree: a tree of drafted tokens.  With base = len - n, the row sees the tokens
+ *   before base, and of its request's n new tokens those whose bits are set in its
+ *   row of `tree` [n_tokens][tree_words] (bit c % 64 of word c / 64 is new token c,
+ *   the token at place base + c; bits from n on do not count).  A row whose
+ *   bits are all 0 sees the tokens before base only.  tree_words (1..64) holds the
+ *   longest request's tokens: a longer one latches FERRY_ERANGE, and nobody sees its
+ *   tokens from 64 tree_words on.  ferry_pages_tree makes the rows from parents.
+ * Both: the window counts by depth, i = base + (bits set) - 1, and bits count
+ *   whatever the window is. */
+typedef struct ferry_seen {
+  int32_t window, sinks;
+  int32_t tree_words;
+  int32_t pad;
+  const uint64_t* tree; /* device */
+} ferry_seen;
+int ferry_pages_attend_seen(const ferry_pages* pages, int32_t layer, const ferry_attend* args,
+                            const ferry_seen* seen, void* stream);
+
+/* Trees of drafted tokens: what append and attend need of them, from their parents.
+ * Request r is lane lanes[r] with new tokens [q_start[r], q_start[r + 1]) of the batch
+ * (q_start NULL: one each), the last of its lane, as in ferry_pages_attend.  parent
+ * [n_tokens] is the number of a token's parent among its request's (less than its
+ * own), -1 for a root.  Out, each of them but tree may be NULL:
+ *   tree   [n_tokens][tree_words] bits of a token's ancestors and of itself
+ *   at     [n_tokens] its position: tokens before the request's new ones, and ancestors
+ *   place  [n_tokens] its place in the lane, len - n + number
+ *   lane   [n_tokens] its lane
+ * Tokens of an empty request (lane -1) and of none get lane -1, place -1, position 0 and
+ * no bits: padding for ferry_pages_append.  So do those of a lane that is out of range or
+ * holds fewer tokens than the request has (FERRY_ERANGE).  A parent that is not less than its
+ * child counts as -1, bits from 64 tree_words on are left out, and both, offsets that do
+ * not ascend and a len past max_pages * 16 latch FERRY_ERANGE. */
+typedef struct ferry_tree {
+  int32_t n_req, n_tokens, tree_words, pad;
+  const int32_t* lanes;
+  const int32_t* q_start;
+  const int32_t* parent;
+  uint64_t* tree;
+  int32_t* at;
+  int32_t* place;
+  int32_t* lane;
+} ferry_tree;
+int ferry_pages_tree(const ferry_pages* pages, const ferry_tree* args, void* stream);
+
+/* Drafts that the model agrees with stay, the others go.  Requests, parents (NULL:
+ * a chain, each token's parent is the one before it) as in ferry_pages_tree.  A
+ * request's first token stays (the last step chose it); from there on the next one is
+ * the first child c of the last with draft[c] == chosen[last].  With base = len - n:
+ * the keys and values of the i-th of them, in all layers, move to place base + i,
+ * len becomes base + kept, and the pages behind are given back.
+ *   draft, chosen [n_tokens]: a token, and the model's choice after it
+ *   path [n_tokens]  out: a request's rows that stay, in their order, then -1
+ *   kept [n_req]     out: their number
+ *   next [n_req]     out: chosen[] of the last; -1 of an empty request
+ * fp8: a code that moves to a page of another scale is rounded to that scale's codes
+ * (saturating); with the same scale it is copied.  Lane -1 is an empty request, also
+ * one without tokens: it keeps none and changes nothing, but its path is -1.  A call of the kind of those that manage pages: it is made whole
+ * or not at all (path, kept and next included), a lane that is out of range or named
+ * twice, offsets that do not ascend and more new tokens than the lane holds are
+ * FERRY_EINVAL; n_req is at most n_lanes, and the results overlap neither each
+ * other nor anything that is read.  A move whose page the lane does not have, or
+ * into a page in use more than once, is left out (FERRY_ESTATE). */
+typedef struct ferry_accept {
+  int32_t n_req, n_tokens;
+  const int32_t* lanes;
+  const int32_t* q_start;
+  const int32_t* parent;
+  const int32_t* draft;
+  const int32_t* chosen;
+  int32_t* path;
+  int32_t* kept;
+  int32_t* next;
+} ferry_accept;
+int ferry_pages_accept(const ferry_pages* pages, const ferry_accept* args, void* stream);
 
 /* ---- bandwidth ceilings ----
  * Plain reads of the bytes the executor's kernels move, timed with HIP events
