@@ -524,8 +524,9 @@ struct AppendArgs {
 };
 
 // The position that turns pair i of token t, at place pos.
+template <bool AXES>
 __device__ inline int position(const PageView& v, const AppendArgs& a, int i, int t, int pos) {
-  if (!a.axes) return pos;
+  if (!AXES) return pos;
   int x = a.axis ? a.axis[i] : 0;
   if ((uint32_t)x >= (uint32_t)a.axes) {
     set_error(v.error, FERRY_ERANGE);
@@ -641,14 +642,14 @@ __device__ inline int64_t append_page(const PageView& v, const AppendArgs& a, in
 // eight too (the head's line is in the L1 cache) and all lanes of a head read before
 // one writes, which makes q_out = q safe.  Bound by memory: 18,000 tokens of 48 heads
 // (466 MB) in 87 us, 5.3 TB/s read and written (a torch copy: 4.6).
-template <int XT, int PT>
+template <int XT, int PT, bool AXES>
 __global__ __launch_bounds__(256) void k_append(PageView v, int layer, AppendArgs a) {
   constexpr int W = XT == FERRY_F32 ? 2 : 1;  // 16-byte words of 8 values
   constexpr int kAhead = 3;                   // heads of a lane on their way
   __shared__ __attribute__((aligned(16))) float cs[64], sn[64];
   const int t = blockIdx.x, tid = threadIdx.x, d = (tid & 15) * 8;
   const int pos = a.pos[t];
-  const int turned_by = tid < a.rot / 2 ? position(v, a, tid, t, pos) : 0;  // on its way with the page
+  const int turned_by = tid < a.rot / 2 ? position<AXES>(v, a, tid, t, pos) : 0;  // on its way with the page
   const int64_t page = append_page(v, a, t, pos);
   if (page < 0) return;
   const int all = a.Hq + (a.k ? 2 * v.H : 0);
@@ -727,7 +728,7 @@ __global__ __launch_bounds__(256) void k_append(PageView v, int layer, AppendArg
 
 // The same for tensors that are not 16-byte aligned and for rotated parts that do not
 // end between eights: a value per thread.
-template <int XT, int PT>
+template <int XT, int PT, bool AXES>
 __global__ __launch_bounds__(256) void k_append_any(PageView v, int layer, AppendArgs a) {
   __shared__ float cs[64], sn[64];
   const int t = blockIdx.x, tid = threadIdx.x, half = a.rot / 2;
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(256) void k_append_any(PageView v, int layer, Appen
   if (page < 0) return;
   if (tid < half) {
     float c, s;
-    turn((double)position(v, a, tid, t, pos) * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
+    turn((double)position<AXES>(v, a, tid, t, pos) * (a.inv_freq[tid] * 0.15915494309189535), &c, &s);
     cs[tid] = c * a.factor, sn[tid] = s * a.factor;
   }
   __syncthreads();
@@ -777,7 +778,7 @@ __global__ __launch_bounds__(256) void k_append_any(PageView v, int layer, Appen
   }
 }
 
-template <int XT, int PT>
+template <int XT, int PT, bool AXES>
 void launch_append(const PageView& v, int layer, AppendArgs a, int cus, hipStream_t s) {
   const int es = XT == FERRY_F32 ? 4 : 2, os = a.out_type == FERRY_F32 ? 4 : 2;
   uint64_t low = 0;
@@ -791,10 +792,15 @@ void launch_append(const PageView& v, int layer, AppendArgs a, int cus, hipStrea
     // (64 tokens: 3.6 us, 5.2 with all 48).
     const int all = a.Hq + (a.k ? 2 * v.H : 0);
     a.heads = a.n >= 4 * cus ? all : 16;
-    k_append<XT, PT><<<dim3(a.n, (all + a.heads - 1) / a.heads), 256, 0, s>>>(v, layer, a);
+    k_append<XT, PT, AXES><<<dim3(a.n, (all + a.heads - 1) / a.heads), 256, 0, s>>>(v, layer, a);
   } else {
-    k_append_any<XT, PT><<<a.n, 256, 0, s>>>(v, layer, a);
+    k_append_any<XT, PT, AXES><<<a.n, 256, 0, s>>>(v, layer, a);
   }
+}
+template <int XT, int PT>
+void launch_append(const PageView& v, int layer, const AppendArgs& a, int cus, hipStream_t s) {
+  if (a.axes) launch_append<XT, PT, true>(v, layer, a, cus, s);
+  else launch_append<XT, PT, false>(v, layer, a, cus, s);
 }
 template <int XT>
 void launch_append(const PageView& v, int layer, const AppendArgs& a, int pt, int cus, hipStream_t s) {
