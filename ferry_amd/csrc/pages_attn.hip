@@ -39,10 +39,12 @@ int attend_forms(const ferry_pages* p, const ferry_attend* a) {
 }
 
 // Workgroups of a call, and its scratch at `base` (null: sizes only).
-int plan_attend(const ferry_pages* p, const ferry_attend* a, uint8_t* base, Scratch* ws, uint64_t* bytes) {
-  const int grid = kPerCu * gpu_cus(p->device);
+// wide: of one workgroup per CU, whose tiles have up to twice the rows; its parts take
+// no more room.
+int plan_attend(const ferry_pages* p, const ferry_attend* a, bool wide, uint8_t* base, Scratch* ws, uint64_t* bytes) {
+  const int grid = (wide ? 1 : kPerCu) * gpu_cus(p->device);
   const uint64_t rows = (uint64_t)a->n_tokens * (a->q_heads / p->kv_heads), H = p->kv_heads;
-  const uint64_t tile = p->dtype == FERRY_F32 ? 16 : std::min<uint64_t>(kWide, rows);
+  const uint64_t tile = p->dtype == FERRY_F32 ? 16 : std::min<uint64_t>(wide_of(wide ? kSeenWide : kCausal), rows);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     uint8_t* r = base + at;
@@ -64,7 +66,7 @@ template <int DT>
 void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int forms, int grid,
                    hipStream_t s) {
   if (a.seen.window || a.seen.words) launch_attend_seen(v, layer, DT, a, ws, forms, grid, s);
-  else launch_forms<DT, false>(v, layer, a, ws, forms, grid, s);
+  else launch_forms<DT, kCausal>(v, layer, a, ws, forms, grid, s);
   // a workgroup per row where that does not fill the GPU twice
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
   if (all <= 2ull * grid) {
@@ -86,7 +88,7 @@ int ferry_pages_attend_work_bytes(const ferry_pages* p, const ferry_attend* a, u
     if (int rc = check_attend(p, a, nullptr, &v)) return rc;
     if (!bytes) return report(FERRY_EINVAL, "null bytes");
     Scratch ws;
-    plan_attend(p, a, nullptr, &ws, bytes);
+    plan_attend(p, a, false, nullptr, &ws, bytes);
     return FERRY_OK;
   });
 }
@@ -116,7 +118,9 @@ int ferry_pages_attend_seen(const ferry_pages* p, int32_t layer, const ferry_att
       return report(FERRY_EINVAL, "out is q with other strides");
     Scratch ws;
     uint64_t need = 0;
-    const int grid = plan_attend(p, a, static_cast<uint8_t*>(a->work), &ws, &need);
+    const int forms = attend_forms(p, a);
+    const bool partly = seen && (seen->window || seen->tree_words);
+    const int grid = plan_attend(p, a, partly && forms == 3, static_cast<uint8_t*>(a->work), &ws, &need);
     if (a->work_bytes < need) return report(FERRY_EINVAL, "work is smaller than ferry_pages_attend_work_bytes");
     if (reinterpret_cast<uintptr_t>(a->work) % 256) return report(FERRY_EINVAL, "work must be 256-byte aligned");
     OnDevice on(p->device);
@@ -133,7 +137,6 @@ int ferry_pages_attend_seen(const ferry_pages* p, int32_t layer, const ferry_att
     while (1 << (d.g_shift - 31) < d.G) ++d.g_shift;
     d.g_mul = (uint32_t)((1ull << d.g_shift) / d.G + 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int forms = attend_forms(p, a);
     if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, forms, grid, s);
     else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, forms, grid, s);
     else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, forms, grid, s);

@@ -108,9 +108,16 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
-constexpr int kStep = 4;           // pages per step
-constexpr int kWide = 128;         // rows of the widest tile
+// How a call runs: kCausal: rows see all that is before them; kSeen: a part of it;
+// kSeenWide: the same by workgroups of eight wavefronts, one per CU.
+constexpr int kCausal = 0, kSeen = 1, kSeenWide = 2;
+constexpr int threads_of(int mode) { return mode == kSeenWide ? 512 : 256; }
+constexpr int wide_of(int mode) { return mode == kSeenWide ? 256 : 128; }  // rows of the widest tile
+constexpr int kStep = 4;           // pages per step of the widest tiles
+// Pages per step of a tile: one for each wavefront where those share out the pages.
+template <int MODE>
+__host__ __device__ constexpr int step_pages(int tile) { return tile <= 32 ? threads_of(MODE) / 64 : kStep; }
+constexpr int kThreads = 256;      // of the kernel that joins
 constexpr int kGroupsInLds = 512;  // groups whose offsets are looked up in LDS
 constexpr int kPad = 132;          // floats per row of the merge buffer
 constexpr int kPerCu = 2;          // workgroups per CU
@@ -226,10 +233,10 @@ struct Seg {
 // of four wavefronts that share pages in LDS.  16 agents of 4 rows on 517 shared pages:
 // 134 us in the 128-row form, 189 in a 64-row form of the first kind; 8 agents: 181 us
 // with 32 rows, 227 in the 128-row form.  fp32 pages have the 16-row form only.
-template <int DT>
+template <int DT, int MODE>
 __device__ inline int tile_rows(int rows) {
   if (Kv<DT>::F32 || rows <= 16) return 16;
-  return rows <= 32 ? 32 : kWide;
+  return rows <= 32 ? 32 : wide_of(MODE);
 }
 
 __device__ inline int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -249,16 +256,16 @@ __device__ inline int len_of(const PageView& v, int lane) {
 // Pages that the requests [b, e) of a group attend to together: none where they have
 // a widest tile's rows each, and would read the pages once per tile in any case.  Alone,
 // their rows have one segment and need no join.
-template <int DT>
+template <int DT, int MODE>
 __device__ inline int group_pages(const PageView& v, const AttendArgs& a, int b, int e, int shared) {
-  constexpr int kRows = Kv<DT>::F32 ? 16 : kWide;
+  constexpr int kRows = Kv<DT>::F32 ? 16 : wide_of(MODE);
   const int64_t rows = (int64_t)(token_of(a, e) - token_of(a, b)) * a.G;
   return rows >= (int64_t)kRows * (e - b) ? 0 : clampi(shared, 0, v.max_pages);
 }
 
 // Shared pages of request r: those of the last group that starts at or before it,
 // if that has not ended.
-template <int DT>
+template <int DT, int MODE>
 __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int r,
                                 int* group) {
   *group = -1;
@@ -271,16 +278,16 @@ __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const in
   const int b = clampi(gs[lo], 0, a.n_req), e = clampi(gs[lo + 1], b, a.n_req);
   if (r >= e) return 0;
   *group = lo;
-  return group_pages<DT>(v, a, b, e, gp[lo]);
+  return group_pages<DT, MODE>(v, a, b, e, gp[lo]);
 }
 
 // Segment s: groups first, then requests.  gs, gp: the groups' offsets and pages.
-template <int DT, bool SEEN>
+template <int DT, int MODE>
 __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int s) {
   Seg g;
   if (s < a.n_groups) {
     const int b = clampi(gs[s], 0, a.n_req), e = clampi(gs[s + 1], b, a.n_req);
-    g.own = 0, g.req = s, g.p0 = 0, g.p1 = group_pages<DT>(v, a, b, e, gp[s]);
+    g.own = 0, g.req = s, g.p0 = 0, g.p1 = group_pages<DT, MODE>(v, a, b, e, gp[s]);
     g.lane = -1, g.base = g.len = 0;
     for (int r = b; r < e && g.lane < 0; ++r) g.lane = lane_of(v, a, r);
     const int t0 = token_of(a, b), t1 = max(t0, token_of(a, e));
@@ -291,12 +298,12 @@ __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int*
     g.own = 1, g.req = r, g.lane = lane_of(v, a, r), g.len = len_of(v, g.lane);
     g.tok0 = t0, g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G;
     g.base = g.len - (t1 - t0) + 1;
-    int shared = shared_of<DT>(v, a, gs, gp, r, &g.group);
-    if (SEEN && a.seen.words) shared = min(shared, max(0, g.base - 1) / kPageTokens);  // drafts are the request's own
+    int shared = shared_of<DT, MODE>(v, a, gs, gp, r, &g.group);
+    if (MODE && a.seen.words) shared = min(shared, max(0, g.base - 1) / kPageTokens);  // drafts are the request's own
     g.p0 = g.lane < 0 ? 0 : shared;
     g.p1 = max(g.p0, pages_of(g.len));
   }
-  g.tile = tile_rows<DT>(g.rows);
+  g.tile = tile_rows<DT, MODE>(g.rows);
   g.tiles = (g.rows + g.tile - 1) / g.tile;
   return g;
 }
@@ -327,7 +334,7 @@ __device__ inline Range tile_range(const AttendArgs& a, const Seg& g, int j) {
   if (a.seen.window) {
     r.lo_lo = clampi(from - a.seen.window, 0, g.len), r.lo_hi = clampi(to - a.seen.window, 0, g.len);
     const int ahead = pages_of(min(a.seen.sinks, g.len)), gap = r.lo_lo / kPageTokens,
-              whole = g.tile == kWide ? (ahead + kStep - 1) / kStep * kStep : ahead;
+              whole = g.tile > 32 ? (ahead + kStep - 1) / kStep * kStep : ahead;
     if (gap > whole) r.ahead = whole, r.skip = gap - whole, r.p1 -= r.skip;
   }
   return r;
@@ -335,18 +342,18 @@ __device__ inline Range tile_range(const AttendArgs& a, const Seg& g, int j) {
 
 // Steps of tile j: up to the last token its last row sees, and at least one, so
 // that every tile has a workgroup that writes its rows.
-template <bool SEEN>
+template <int MODE>
 __device__ inline int tile_steps(const AttendArgs& a, const Seg& g, int j) {
   int p1 = g.p1;
   if (g.own) {
-    if constexpr (SEEN) {
+    if constexpr (MODE != kCausal) {
       p1 = tile_range(a, g, j).p1;
     } else {
       const int last = clampi(g.base + token_of_row(a, min((j + 1) * g.tile, g.rows) - 1), 0, g.len);
       p1 = min(p1, pages_of(last));
     }
   }
-  return max(1, (p1 - g.p0 + kStep - 1) / kStep);
+  return max(1, MODE == kSeenWide && g.tile <= 32 ? (p1 - g.p0 + 7) / 8 : (p1 - g.p0 + kStep - 1) / kStep);
 }
 // Units of work: step_units() for a step, tile_units() for a tile's beginning and end.
 // Step i of a tile belongs to the workgroup whose run holds the first of its units.
@@ -359,16 +366,16 @@ __device__ constexpr int step_units(int tile) {
 }
 template <int DT>
 __device__ constexpr int tile_units(int tile) { return tile == 16 ? 26 : tile == 32 ? 35 : 65; }
-template <int DT, bool SEEN>
+template <int DT, int MODE>
 __device__ inline int tile_work(const AttendArgs& a, const Seg& g, int j) {
-  return tile_steps<SEEN>(a, g, j) * step_units<DT>(g.tile) + tile_units<DT>(g.tile);
+  return tile_steps<MODE>(a, g, j) * step_units<DT>(g.tile) + tile_units<DT>(g.tile);
 }
 // ... of all tiles of a segment, per kv head
-template <int DT, bool SEEN>
+template <int DT, int MODE>
 __device__ inline uint64_t seg_work(const AttendArgs& a, const Seg& g) {
-  if (!g.own) return (uint64_t)g.tiles * tile_work<DT, SEEN>(a, g, 0);
+  if (!g.own) return (uint64_t)g.tiles * tile_work<DT, MODE>(a, g, 0);
   uint64_t n = 0;
-  for (int j = 0; j < g.tiles; ++j) n += tile_work<DT, SEEN>(a, g, j);
+  for (int j = 0; j < g.tiles; ++j) n += tile_work<DT, MODE>(a, g, j);
   return n;
 }
 
@@ -425,8 +432,8 @@ struct SeenTile : CausalTile {
   __device__ __forceinline__ bool some(int tok) const { return tok < lim_hi && (tok >= lo_lo || tok < sinks); }
   __device__ __forceinline__ bool some(int t0, int n) const { return t0 < lim_hi && (t0 + n > lo_lo || t0 < sinks); }
 };
-template <bool SEEN>
-using Tile = std::conditional_t<SEEN, SeenTile, CausalTile>;
+template <int MODE>
+using Tile = std::conditional_t<MODE != kCausal, SeenTile, CausalTile>;
 constexpr int kNoDrafts = 0x7FFFFF00;
 
 // Bits 0 .. n - 1.
@@ -472,27 +479,30 @@ struct SegAt {
 constexpr int kListed = 32;
 
 // FORMS: 1: 16-row tiles only, 2: 32-row tiles too, 3: 128-row tiles too.
-template <int FORMS, bool SEEN>
+template <int FORMS, int MODE>
 struct Shared {
+  static constexpr int kWaves = threads_of(MODE) / 64, kWide = wide_of(MODE);
   struct Kv {
-    uint8_t k[2][kStep * 4096], v[2][kStep * 4096];
+    static constexpr int kSlots = MODE == kSeenWide ? 4 : 2;
+    uint8_t k[kSlots][kStep * 4096], v[kSlots][kStep * 4096];
   };
   struct None {};
   union {
-    float merge[4 * (FORMS == 1 ? 16 : 32) * kPad];  // [wavefront][row][dim]: accumulators to be joined
+    float merge[kWaves * (FORMS == 1 ? 16 : 32) * kPad];  // [wavefront][row][dim]: accumulators to be joined
     std::conditional_t<FORMS == 3, Kv, None> kv;     // two steps' tokens, chunks swizzled
   };
-  float ml[4][32][2];
+  float ml[kWaves][32][2];
   int lim[kWide];  // tokens that each row sees
   int lim_lo, lim_hi;
-  int odd[3];      // a step's V holds what is not finite (step s: place s % 3)
+  int odd[MODE == kSeenWide ? 8 : 3];  // a step's V holds what is not finite (step s: place s % 3, or 8)
   int left_out;    // the tile has pages that were left out for that
   int gs[kGroupsInLds + 1], gp[kGroupsInLds];
-  uint64_t sums[kThreads / 64];
+  uint64_t sums[kWaves];
   int seg;          // first segment of this workgroup's run
   int gl[kGroupsInLds];  // least number of tokens that a row of a group sees
   SegAt list[kListed];  // consecutive segments of the run
-  std::conditional_t<SEEN, int[kWide], None> lo;  // of the tokens that a row sees the first behind the sinks
+  std::conditional_t<MODE == kSeenWide, float[128][2], None> mate;  // maxima and sums of the second half
+  std::conditional_t<MODE != kCausal, int[kWide], None> lo;  // of the tokens that a row sees the first behind the sinks
 };
 
 // 8 query values of a row as two 16-bit values per dword, times the sign of the
@@ -575,9 +585,11 @@ __device__ inline void load_page(const CausalTile& t, int kv_heads, uint32_t pag
 // Bound by the pages' bytes: 32 rows take 192 matrix cycles a page and wavefront,
 // 8 KiB a page, which 256 CUs could read at 100 TB/s.  221,000 tokens of 8 kv heads
 // (906 MB), bf16: 149 us, 6.1 TB/s.
-template <int DT, int NT, bool SEEN>
+template <int DT, int NT, int MODE>
 struct Narrow {
   using K = Kv<DT>;
+  static constexpr bool SEEN = MODE != kCausal;
+  static constexpr int kStep = threads_of(MODE) / 64;  // a page per wavefront and step
   u32x4 q[NT][K::F32 ? 8 : 4];
   f32x4 o[NT][8];
   float m[NT], sum[NT];
@@ -587,7 +599,7 @@ struct Narrow {
   // whether, decided by the caller); false: left out, as one
   // does not and V or its scale holds what is not finite among those that one sees.
   template <bool MASKED, class Sh>
-  __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, const AttendArgs& a, const Tile<SEEN>& tile,
+  __device__ __forceinline__ bool consume(const PageRegs<DT>& r, int l, int t0, const AttendArgs& a, const Tile<MODE>& tile,
                                           Sh& sh, bool masked, float scale) {
     const int grp = l >> 4;
     // V rows as operand values: 8 dims of 4 tokens
@@ -710,7 +722,7 @@ struct Narrow {
 
   // The tile's steps; then sh.merge and sh.ml hold each wavefront's rows.
   template <class Sh>
-  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile<SEEN>& t, Sh& sh) {
+  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile<MODE>& t, Sh& sh) {
     const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = l & 15, grp = l >> 4;
     const float scale = a.scale * 1.4426950408889634f;
@@ -739,7 +751,6 @@ struct Narrow {
       }
     }
     // page i of this wavefront: one of each of the steps of kStep pages in [p0, p1)
-    static_assert(kStep == kThreads / 64, "a page per wavefront and step");
     const int count = (t.p1 - t.p0 + kStep - 1) / kStep;
     auto page_no = [&](int i) { return t.p0 + kStep * i + wave; };
     uint32_t ids = 0;  // lane j: the table's entry for page 64 k + j
@@ -832,15 +843,15 @@ template <int DT, int NT, class Sh>
 __device__ __forceinline__ void narrow_write(const AttendArgs& a, const CausalTile& t, Sh& sh, float* to_ml, float* to_o) {
   const int tid = this_thread();
 #pragma unroll
-  for (int r0 = 0; r0 < 16 * NT; r0 += 16) {
+  for (int r0 = 0; r0 < 16 * NT; r0 += 4 * Sh::kWaves) {
     const int row = r0 + tid / 16, d = tid % 16 * 8;
     if (row >= t.rows) continue;
     float m = -INFINITY, sum = 0.0f, x[8] = {};
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, sh.ml[w][row][0]);
+    for (int w = 0; w < Sh::kWaves; ++w) m = fmaxf(m, sh.ml[w][row][0]);
     const float ref = against(m);
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) {
+    for (int w = 0; w < Sh::kWaves; ++w) {
       const float f = exp2_fast(sh.ml[w][row][0] - ref);
       sum += f * sh.ml[w][row][1];
       const float* o = sh.merge + (w * 16 * NT + row) * kPad + d;
@@ -903,11 +914,56 @@ __device__ inline void load_lds(uint32_t to, const void* base, uint32_t at) {
                :: "s"(first_lane_i((int)to)), "v"(at), "s"(uniform(base)) : "memory");
 }
 
+// 8 codes of a column: the 16 lanes of a group name 8 tokens of 16 dims, 8 dims each.
+__device__ inline u32x2 lds_turned8(uint32_t at) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       (__attribute__((address_space(3))) i32x2*)(uintptr_t)at));
+}
+
 __device__ inline int swizzle(int tok) { return (tok & 3) << 2 | (tok >> 2 & 3); }
 
-template <int DT, bool SEEN>
+// Writes a lane's row of a wide tile: half h of each 8 dims.
+template <int DT>
+__device__ __forceinline__ void wide_write(const AttendArgs& a, const CausalTile& t, int row, int h, const f32x16 (&o)[4],
+                                           float m, float sum, int lim, float* to_ml, float* to_o) {
+  using K = Kv<DT>;
+  if (row >= t.rows) return;
+  if (to_o) {
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(to_o + (int64_t)row * kPageDim + 32 * dt + 2 * e + 4 * h) =
+            f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
+    if (h == 0) to_ml[2 * row] = m, to_ml[2 * row + 1] = sum;
+    return;
+  }
+  const float inv = lim <= 0 ? 0.0f : 1.0f / sum;
+  uint16_t* p = static_cast<uint16_t*>(a.out) + row_at(a, a.os, t.row0 + row, t.h) + 4 * h;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const u32x2 w = {pack2<K::BF>(o[dt][e] * inv, o[dt][e + 1] * inv),
+                       pack2<K::BF>(o[dt][e + 2] * inv, o[dt][e + 3] * inv)};
+      uint16_t* to = p + 32 * dt + 2 * e;
+      if (a.aligned) {
+        *reinterpret_cast<u32x2*>(to) = w;
+      } else {
+        to[0] = (uint16_t)w[0], to[1] = (uint16_t)(w[0] >> 16), to[2] = (uint16_t)w[1], to[3] = (uint16_t)(w[1] >> 16);
+      }
+    }
+  if (a.lse && h == 0) {
+    const int tok = token_of_row(a, t.row0 + row), g = t.row0 + row - tok * a.G;
+    a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+  }
+  }
+
+template <int DT, int MODE>
 struct Wide {
   using K = Kv<DT>;
+  static constexpr bool SEEN = MODE != kCausal;
   typedef std::conditional_t<K::F8, u32x2, u32x4> Word;  // 8 values
   u32x4 q[8];
   f32x16 o[4];
@@ -921,7 +977,7 @@ struct Wide {
     float c[kStep], scale;  // factor on a page's scores
     int mine;               // of the lane's tokens, in steps of 4 and gaps of 4
     u32x2 bits;             // SEEN: those tokens
-    __device__ __forceinline__ Largest(const Wide& w, const Tile<SEEN>& t, u32x2 bits, int s, int steps, int h, float scale,
+    __device__ __forceinline__ Largest(const Wide& w, const Tile<MODE>& t, u32x2 bits, int s, int steps, int h, float scale,
                                        float scales)
         : scale(scale), mine(s < steps ? w.lim - (t.p0 + kStep * s) * kPageTokens - 4 * h : 0), bits(bits) {
 #pragma unroll
@@ -954,7 +1010,7 @@ struct Wide {
   }
 
   template <class Sh>
-  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile<SEEN>& t, Sh& sh) {
+  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const Tile<MODE>& t, Sh& sh) {
     const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = l & 31, h = l >> 5, row = wave * 32 + col;
     const float scale = fabsf(a.scale) * 1.4426950408889634f;
@@ -1257,37 +1313,390 @@ struct Wide {
   }
 
   __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, float* to_ml, float* to_o) {
-    const int tid = this_thread(), l = tid & 63, h = l >> 5, row = (tid >> 6) * 32 + (l & 31);
-    if (row >= t.rows) return;
-    if (to_o) {
+    const int tid = this_thread(), l = tid & 63;
+    wide_write<DT>(a, t, (tid >> 6) * 32 + (l & 31), l >> 5, o, m, sum, lim, to_ml, to_o);
+  }
+};
+
+// A tile of up to 256 rows: eight wavefronts, as Wide's four with 32 rows each; with up to
+// 128 rows two of them (halves) take the same rows, one a step's first 32 tokens and one the
+// others, and add up in the end.  One workgroup per CU then has the pages of all its rows
+// once in LDS, in four places for a step's K and four for its V (16 KiB each; fp8 as raw
+// codes in half of that, eight places each), so that up to 96 KiB are on their way while a
+// step is computed: that hides the memory's latency where pages are read by one tile only.
+// Two workgroups of 128 rows per CU have 64 KiB on their way, and read the pages of 256 rows
+// twice.  32 x 64 drafts over 1,000 to 8,000 tokens of 8 kv heads, bf16: @@ us, 242 us so.
+// In step s the loads of V of step s + kSlots - 1 and of K of step s + kSlots begin, into the
+// places that step s - 1 has left.  A wavefront waits for its own oldest loads by their
+// count, then all meet.
+template <int DT>
+struct Wide8 {
+  using K = Kv<DT>;
+  static constexpr int kSlots = K::F8 ? 8 : 4;
+  static constexpr uint32_t kSlot = kStep * K::HALF;      // bytes of a step's K or V
+  static constexpr uint32_t kPage = K::HALF;              // ... of a page's
+  static constexpr int kLoads = kSlot / (512 * 16);       // 16-byte loads of a thread for them
+  u32x4 q[8];
+  f32x16 o[4];
+  float m, sum;
+  int lim, row;
+  bool writes;
+
+  // Where chunk c of a token is: reads of one chunk of 16 (K) or of two of 8 (V) tokens meet
+  // all banks.
+  static __device__ __forceinline__ int place(int tok) {
+    if constexpr (K::F8) return (tok >> 3 & 1) << 2 | (tok >> 1 & 1) << 1 | (tok >> 2 & 1);
+    else return swizzle(tok);
+  }
+  template <int N>
+  static __device__ __forceinline__ void wait_all_but() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  }
+  static __device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  // 8 codes -> 8 bf16 values
+  static __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
+    const u32x2 a = e4m3x4_to_bf16(lo), b = e4m3x4_to_bf16(hi);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+  static __device__ __forceinline__ bool odd_word(uint32_t w) {
+    if constexpr (K::F8) return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    else return not_finite<DT>(w);
+  }
+
+  template <class Sh>
+  __device__ __forceinline__ void run(const PageView& v, const AttendArgs& a, const SeenTile& t, Sh& sh) {
+    if (t.rows <= 128) run_tiles<1>(v, a, t, sh);
+    else run_tiles<2>(v, a, t, sh);
+  }
+  // NTT: a wavefront's token tiles of 32 of a step.
+  template <int NTT, class Sh>
+  __device__ __forceinline__ void run_tiles(const PageView& v, const AttendArgs& a, const SeenTile& t, Sh& sh) {
+    constexpr bool halves = NTT == 1;
+    const int tid = this_thread(), l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = halves ? wave & 1 : 0, group = halves ? wave >> 1 : wave;
+    const int col = l & 31, h = l >> 5;
+    row = group * 32 + col;
+    writes = half == 0;
+    const float scale = fabsf(a.scale) * 1.4426950408889634f;
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
+    const bool busy = group * 32 < t.rows;  // the others only help to load
+    lim = row < t.rows ? sh.lim[row] : 0;
+    m = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<f32x4*>(to_o + (int64_t)row * kPageDim + 32 * dt + 2 * e + 4 * h) =
-              f32x4{o[dt][e], o[dt][e + 1], o[dt][e + 2], o[dt][e + 3]};
-      if (h == 0) to_ml[2 * row] = m, to_ml[2 * row + 1] = sum;
-      return;
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int d = K::F8 ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h;
+      q[c] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned, sign) : u32x4{0u, 0u, 0u, 0u};
     }
-    const float inv = lim <= 0 ? 0.0f : 1.0f / sum;
-    uint16_t* p = static_cast<uint16_t*>(a.out) + row_at(a, a.os, t.row0 + row, t.h) + 4 * h;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const u32x2 w = {pack2<K::BF>(o[dt][e] * inv, o[dt][e + 1] * inv),
-                         pack2<K::BF>(o[dt][e + 2] * inv, o[dt][e + 3] * inv)};
-        uint16_t* to = p + 32 * dt + 2 * e;
-        if (a.aligned) {
-          *reinterpret_cast<u32x2*>(to) = w;
-        } else {
-          to[0] = (uint16_t)w[0], to[1] = (uint16_t)(w[0] >> 16), to[2] = (uint16_t)w[1], to[3] = (uint16_t)(w[1] >> 16);
-        }
+    const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
+    auto first_token = [&](int s) __attribute__((always_inline)) { return t.page(t.p0 + kStep * s) * kPageTokens; };
+    auto is_whole = [&](int s) __attribute__((always_inline)) {
+      return s < steps && t.whole(first_token(s), kStep * kPageTokens);
+    };
+    // Page ids: lane j of window w holds page 64 w + j.  Windows at, at + 1 and, on its way,
+    // at + 2; fp8: the scales of the windows of the step computed, of the next one, and
+    // of the one behind the ids' second.
+    auto read_ids = [&](int w) __attribute__((always_inline)) {
+      const int p = t.p0 + 64 * w + l;
+      return p < t.p1 ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
+    };
+    auto read_scales = [&](uint32_t ids, int w) __attribute__((always_inline)) {
+      f32x2 s = {};
+      if constexpr (K::F8) {
+        s = *reinterpret_cast<const f32x2*>(t.scales + (uint64_t)ids * (2u * v.H));
+        const int p = t.p0 + 64 * w + l;
+        if (p >= t.p1 || !t.some(t.page(p) * kPageTokens, kPageTokens)) s[1] = 0.0f;
       }
-    if (a.lse && h == 0) {
-      const int tok = token_of_row(a, t.row0 + row), g = t.row0 + row - tok * a.G;
-      a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+      return s;
+    };
+    uint32_t ids0 = checked_page(v, read_ids(0)), ids1 = checked_page(v, read_ids(1)), ids2 = read_ids(2);
+    int ids_at = 0, scales_at = 0;
+    f32x2 sc0 = read_scales(ids0, 0), sc1 = read_scales(ids1, 1), sc2 = sc1;
+    // fp8: of the scales of page i of step s
+    auto scale_of = [&](int which, int s, int i) __attribute__((always_inline)) {
+      const float x = (s >> 4) == scales_at ? sc0[which] : sc1[which];
+      return bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(x), (kStep * s + i) & 63));
+    };
+    // The thread's 16 bytes of a step in LDS: of page `mine` (and, 16 bits, two behind it)
+    // those at `unit`.
+    constexpr int kUnits = kPage / 16;  // of a page's K or V
+    const int mine = wave * 64 / kUnits, unit = tid % kUnits;
+    const int tok = unit / (K::ROW / 16);
+    const uint32_t at_word = tok * K::ROW + ((unit % (K::ROW / 16)) ^ place(tok)) * 16u;
+    const uint32_t to_k = lds_at(sh.kv.k[0]) + wave * 1024u, to_v = lds_at(sh.kv.v[0]) + wave * 1024u;
+    auto begin = [&](uint32_t to, uint32_t behind, int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int p = kStep * s + mine + 2 * j, ids = (s >> 4) == ids_at ? ids0 : ids1;
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(ids, p & 63);
+        load_lds(to + (s & kSlots - 1) * kSlot + 2 * j * kPage, t.base + (uint64_t)id * t.page_bytes + behind, at_word);
+      }
+    };
+    auto begin_k = [&](int s) __attribute__((always_inline)) { begin(to_k, 0, s); };
+    auto begin_v = [&](int s) __attribute__((always_inline)) { begin(to_v, K::HALF, s); };
+    // What no row sees of V of step s becomes zero; sets odd where it holds what is not finite.
+    auto land = [&](int s) __attribute__((always_inline)) {
+      if (s >= steps || is_whole(s)) return;
+      const int t0 = first_token(s);
+      bool bad = false;
+      if constexpr (K::F8) {  // the lanes that hold the step's V scales
+        bad = l >> 2 == (s & 15) && !finite((s >> 4) == scales_at ? sc0[1] : sc1[1]);
+      }
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int page = mine + 2 * j;
+        u32x4* word = reinterpret_cast<u32x4*>(sh.kv.v[0] + (s & kSlots - 1) * kSlot + page * kPage + unit * 16);
+        u32x4 x = *word;
+        const bool seen = t.some(t0 + kPageTokens * page + tok) && t.p0 + kStep * s + page < t.p1;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          bad |= seen && odd_word(x[w]);
+          x[w] = seen ? x[w] : 0u;
+        }
+        *word = x;
+      }
+      if (bad) sh.odd[s & 7] = 1;
+    };
+    // K: 16 bits: token col, chunk h; fp8: the same chunks, of 16 codes.
+    const uint32_t k_lane = lds_at(sh.kv.k[0]) + (32 * half + col) * K::ROW + ((h ^ place(col)) << 4);
+    // V: 16 bits: token 4 h + (l % 16) / 4, dims 16 (l / 16 % 2) + 4 (l % 4); fp8: token
+    // 4 h + i or 4 + 4 h + i of i = (l % 16) / 2, dims 16 (l / 16 % 2) + 8 (l % 2)
+    const int vt = K::F8 ? 4 * h + (l >> 1 & 3) + (l >> 3 & 1) * 8 : 4 * h + (l >> 2 & 3);
+    const uint32_t v_lane =
+        lds_at(sh.kv.v[0]) + (32 * half + vt) * K::ROW +
+        (K::F8 ? (((l >> 4 & 1) ^ place(vt)) << 4) + 8 * (l & 1)
+               : ((2 * (l >> 4 & 1) + (l >> 1 & 1) ^ place(vt)) << 4) + 8 * (l & 1));
+    // The operand of S^T's product i (token tile i % NTT, 16 dims i / NTT) from what was read.
+    typedef std::conditional_t<K::F8, u32x2, u32x4> Piece;
+    auto read_k = [&](uint32_t k_at, int i) __attribute__((always_inline)) {
+      const int c = i / NTT, tt = i % NTT;
+      if constexpr (K::F8) return lds<u32x2>((k_at ^ (c >> 1) << 5) + 32 * K::ROW * tt + 8 * (c & 1));
+      else return lds<u32x4>((k_at ^ c << 5) + 32 * K::ROW * tt);
+    };
+    // ... of O^T's product i (dims 32 (i % 4), tokens 16 (i / 4))
+    auto read_v = [&](uint32_t v_at, int i) __attribute__((always_inline)) {
+      if constexpr (K::F8) {
+        return lds_turned8((v_at ^ (i & 3) << 5) + 16 * K::ROW * (i >> 2));
+      } else {  // tokens 4 h .. + 3 and those 8 behind, whose place flips chunk bit 1
+        const u32x2 lo = lds_turned((v_at ^ (i & 3) << 6) + 16 * K::ROW * (i >> 2));
+        const u32x2 hi = lds_turned((v_at ^ (i & 3) << 6 ^ 32) + 16 * K::ROW * (i >> 2) + 8 * K::ROW);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    auto operand = [&](const Piece& x) __attribute__((always_inline)) {
+      if constexpr (K::F8) return widen(x[0], x[1]);
+      else return x;
+    };
+    auto raise_to = [&](float top, bool raise) __attribute__((always_inline)) {
+      if (__builtin_amdgcn_ballot_w64(raise)) {
+        const float to = raise ? top - K::kTop : m, f = raise ? exp2_fast(m - to) : 1.0f;
+        m = to;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= f;
+      }
+    };
+    // The tokens of step s that the lane's row sees, as bits from its first one on
+    auto bits_of = [&](int s) __attribute__((always_inline)) {
+      u32x2 bits = {0u, 0u};
+      if (s < steps && row < t.rows) {
+        const uint64_t x = seen_bits(a, t, token_of_row(a, t.row0 + row), sh.lim[row], sh.lo[row], first_token(s)) >> 4 * h;
+        bits = u32x2{(uint32_t)(x >> 32 * half), (uint32_t)(x >> 32)};
+      }
+      return bits;
+    };
+    // The largest of 4 scores from `from` on; fp8: they get their pages' scales (c); what the
+    // row does not see (`masked`) becomes -inf.
+    auto among = [&](f32x16 (&x)[NTT], int from, bool masked, u32x2 bits, const float (&c)[2 * NTT],
+                     float& top) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = from; i < from + 4; ++i) {
+        float y = x[i >> 4][i & 15];
+        if (K::F8) y *= c[i >> 3];
+        if (masked && !(bits[i >> 4] & 1u << (8 * (i >> 2 & 3) + (i & 3)))) y = -INFINITY;
+        x[i >> 4][i & 15] = y;
+        top = fmaxf(top, y);
+      }
+    };
+    auto of_row = [&](float top) __attribute__((always_inline)) {  // scaled
+      const mx_u32x2 both = pair_values<32>(top);
+      top = fmaxf(bits_f32(both[0]), bits_f32(both[1]));
+      return K::F8 ? top : top * scale;
+    };
+
+    constexpr int kProducts = 8 * NTT;  // of S^T, and of O^T
+    f32x16 x[NTT], y[NTT];
+    // Loads in the steps' order: in step s those of V of step s + kSlots - 1 and of K of s + kSlots.
+    for (int s = -kSlots; s < 0; ++s) {
+      if (s > -kSlots) begin_v(s + kSlots - 1);
+      begin_k(s + kSlots);
     }
+    constexpr int kLeft = 2 * kLoads * (kSlots - 2);  // on their way while step s ends: of steps s - kSlots + 3 .. s
+    wait_all_but<kLeft>();
+    land(0);
+    meet();
+    if (busy) {
+      uint32_t k_at = k_lane;
+      asm("" : "+v"(k_at));
+#pragma unroll
+      for (int i = 0; i < NTT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[i][e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i)
+        x[i % NTT] = mma32<K::BF>(operand(read_k(k_at, i)), q[i / NTT], x[i % NTT]);
+      const u32x2 bits = bits_of(0);
+      float c[2 * NTT], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2 * NTT; ++i) c[i] = K::F8 ? scale * scale_of(0, 0, 2 * half + i) : scale;
+#pragma unroll
+      for (int i = 0; i < 16 * NTT; i += 4) among(x, i, true, bits, c, top);
+      top = of_row(top);
+      raise_to(top, top > m + K::kMost);
+    }
+    meet();  // all have read K of step 0, which the loads of step 0 write over
+
+    // Step s, whose scores are in x, while those of step s + 1 come into y (MASKED: some row
+    // may not see them all): next to each product a part of the weights, then of the
+    // maximum, is computed and a load begun, and operands are read three products ahead.
+    auto step = [&](auto masked_, int s) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_)::value;
+      u32x2 bits = {0u, 0u};
+      if constexpr (MASKED) {  // here, where registers are free
+        bits = bits_of(s + 1);
+        asm volatile("" : "+v"(bits));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      uint32_t k_at = k_lane + (s + 1 & kSlots - 1) * kSlot, v_at = v_lane + (s & kSlots - 1) * kSlot, pop[kProducts];
+      asm("" : "+v"(k_at), "+v"(v_at));
+      Piece p[4];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) p[i] = read_k(k_at, i);
+#pragma unroll
+      for (int i = 0; i < NTT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[i][e] = 0.0f;
+      const float ref = against(m);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        p[i + 3 & 3] = i + 3 < kProducts ? read_k(k_at, i + 3) : read_v(v_at, i + 3 - kProducts);
+        y[i % NTT] = mma32<K::BF>(operand(p[i & 3]), q[i / NTT], y[i % NTT]);
+        if (i == 0) begin_v(s + kSlots - 1);
+        if (i == 2) begin_k(s + kSlots);
+        const float y0 = x[i >> 3][2 * i & 15], y1 = x[i >> 3][(2 * i & 15) + 1];
+        float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
+        float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
+        sum += p0 + p1;
+        if constexpr (K::F8) {
+          const float f = scale_of(1, s, 2 * half + (i >> 2));
+          p0 *= f, p1 *= f;
+        }
+        pop[i] = pack2<K::BF>(p0, p1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      float c[2 * NTT], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2 * NTT; ++i) c[i] = K::F8 ? scale * scale_of(0, s + 1, 2 * half + i) : scale;
+      bool raise = false;
+      constexpr int kFirst = 2;  // the product from which on scores are looked at, 4 at each
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        if (i + 3 < kProducts) p[i + 3 & 3] = read_v(v_at, i + 3);
+        o[i & 3] = mma32<K::BF>(operand(p[i & 3]), u32x4{pop[i & ~3], pop[(i & ~3) + 1], pop[(i & ~3) + 2], pop[(i & ~3) + 3]},
+                                o[i & 3]);
+        if (i >= kFirst && i < kFirst + 4 * NTT) among(y, 4 * (i - kFirst), MASKED, bits, c, top);
+        if (i == kFirst + 4 * NTT) top = of_row(top);
+        if (i == kFirst + 4 * NTT + 1) raise = top > m + K::kMost;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      raise_to(top, raise);
+#pragma unroll
+      for (int i = 0; i < NTT; ++i) x[i] = y[i];
+    };
+    // Before a step's products: the windows move on.
+    auto before = [&](int s) __attribute__((always_inline)) {
+      if (((s + kSlots - 1) >> 4) > ids_at) {
+        ++ids_at;
+        ids0 = ids1, ids1 = checked_page(v, ids2);
+        ids2 = read_ids(ids_at + 2);
+        sc2 = read_scales(ids1, ids_at + 1);
+      }
+      if ((s >> 4) > scales_at) ++scales_at, sc0 = sc1, sc1 = sc2;
+      if (tid == 0) sh.odd[(s + 2) & 7] = 0;
+    };
+    // ... and a step whose V holds what is not finite is left out.
+    auto leave_out = [&](int s) __attribute__((always_inline)) {
+      if (!first_lane_i(sh.odd[s & 7])) return;
+#pragma unroll
+      for (int i = 0; i < NTT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[i][e] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        *reinterpret_cast<u32x4*>(sh.kv.v[0] + (s & kSlots - 1) * kSlot + (mine + 2 * j) * kPage + unit * 16) = u32x4{0u, 0u, 0u, 0u};
+      if (K::F8 && l >> 2 == (s & 15)) sc0[1] = 0.0f;  // of its pages
+      if (tid == 0) sh.left_out = 1;
+      meet();
+    };
+    auto begin_step = [&](int s) __attribute__((always_inline)) { begin_v(s + kSlots - 1), begin_k(s + kSlots); };
+    for (int s = 0; s < steps;) {
+      for (; is_whole(s) && is_whole(s + 1); ++s) {
+        before(s);
+        if (busy) step(std::false_type{}, s);
+        else begin_step(s);
+        wait_all_but<kLeft>();
+        meet();
+      }
+      do {
+        before(s);
+        leave_out(s);
+        if (busy) step(std::true_type{}, s);
+        else begin_step(s);
+        ++s;
+        wait_all_but<kLeft>();
+        land(s);
+        meet();
+      } while (s < steps && !(is_whole(s) && is_whole(s + 1)));
+    }
+    wait_all_but<0>();
+    {
+      const mx_u32x2 both = pair_values<32>(sum);
+      sum = bits_f32(both[0]) + bits_f32(both[1]);
+    }
+    if (!halves) return;
+    meet();  // all is landed: the places are free
+    f32x4* mates = reinterpret_cast<f32x4*>(sh.kv.k[0]) + group * (16 * 64) + l;
+    if (half == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        mates[64 * i] = f32x4{o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]};
+      sh.mate[group * 32 + col][0] = m, sh.mate[group * 32 + col][1] = sum;  // both halves hold the same
+    }
+    meet();
+    if (half == 0) {
+      const float m1 = sh.mate[group * 32 + col][0], top = fmaxf(m, m1), ref = against(top);
+      const float f0 = exp2_fast(m - ref), f1 = exp2_fast(m1 - ref);
+      m = top;
+      sum = f0 * sum + f1 * sh.mate[group * 32 + col][1];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const f32x4 e = mates[64 * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i >> 2][4 * (i & 3) + j] = f0 * o[i >> 2][4 * (i & 3) + j] + f1 * e[j];
+      }
+    }
+  }
+
+  __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, float* to_ml, float* to_o) {
+    if (writes) wide_write<DT>(a, t, row, threadIdx.x >> 5 & 1, o, m, sum, lim, to_ml, to_o);
   }
 };
 
@@ -1315,10 +1724,11 @@ __device__ __forceinline__ void finish_row(const AttendArgs& a, int row, int h, 
 // does not see it, so here each row takes only the tokens it sees, one at a time, two
 // dims a lane.  ml, o: the tile's rows as a
 // part, which this adds to.  unit: pages that are left out together.
-template <int DT, bool SEEN, class Sh>
-__device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs& a, const Tile<SEEN>& t, int unit,
+template <int DT, int MODE, class Sh>
+__device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs& a, const Tile<MODE>& t, int unit,
                                              const Sh& sh, float* ml, float* o) {
   using K = Kv<DT>;
+  constexpr bool SEEN = MODE != kCausal;
   const int tid = this_thread(), l = tid & 63, wave = tid >> 6;
   const float scale = a.scale * 1.4426950408889634f;
   const int whole = SEEN ? 0 : max(0, t.lim_lo / kPageTokens - t.p0) / unit * unit;
@@ -1335,7 +1745,7 @@ __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs
     }
     if (!__builtin_amdgcn_ballot_w64(odd)) continue;
     const int end = t0 + min(unit, t.p1 - p) * kPageTokens;
-    for (int row = wave; row < t.rows; row += kThreads / 64) {
+    for (int row = wave; row < t.rows; row += Sh::kWaves) {
       const int lim = sh.lim[row];
       uint64_t bits = ~0ull;
       if constexpr (SEEN) bits = seen_bits(a, t, token_of_row(a, t.row0 + row), lim, sh.lo[row], t0);
@@ -1366,9 +1776,11 @@ __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs
 }
 
 // ---- the call -------------------------------------------------------------------
-template <int DT, int FORMS, bool SEEN>
-__global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
-  __shared__ __attribute__((aligned(1024))) Shared<FORMS, SEEN> sh;
+template <int DT, int FORMS, int MODE>
+__global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int layer, AttendArgs a, Scratch ws) {
+  constexpr bool SEEN = MODE != kCausal;
+  constexpr int kThreads = threads_of(MODE), kWide = wide_of(MODE);
+  __shared__ __attribute__((aligned(1024))) Shared<FORMS, MODE> sh;
   const int tid = threadIdx.x, grid = gridDim.x;
   // consecutive runs of work on one XCD (workgroups go to the 8 XCDs in turn), so
   // that tiles of the same pages meet in its L2
@@ -1390,8 +1802,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
   Seg kept;  // the thread's only segment, where it has one
   uint64_t kept_work = 0;
   for (int s = s0; s < s1; ++s) {
-    kept = segment<DT, SEEN>(v, a, gs, gp, s);
-    kept_work = seg_work<DT, SEEN>(a, kept);
+    kept = segment<DT, MODE>(v, a, gs, gp, s);
+    kept_work = seg_work<DT, MODE>(a, kept);
     mine += kept_work * v.H;
     if (kept.own && kept.group >= 0 && kept.rows > 0 && gs == sh.gs)
       atomicMin(&sh.gl[kept.group], SEEN && a.seen.words ? max(0, kept.base - 1) / kPageTokens * kPageTokens : max(0, kept.base));
@@ -1439,8 +1851,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     for (int s = s0; s < s1; ++s) {
       SegAt x;
       const bool have = decltype(first)::value && per_thread == 1;
-      x.g = have ? kept : segment<DT, SEEN>(v, a, gs, gp, s);
-      x.work = have ? kept_work : seg_work<DT, SEEN>(a, x.g);
+      x.g = have ? kept : segment<DT, MODE>(v, a, gs, gp, s);
+      x.work = have ? kept_work : seg_work<DT, MODE>(a, x.g);
       x.at = at;
       if (s >= from && s < from + kListed) sh.list[s - from] = x;
       at += x.work * v.H;
@@ -1452,7 +1864,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     int s = s0;
     if (per_thread > 1)
       for (;; ++s) {
-        at += seg_work<DT, SEEN>(a, segment<DT, SEEN>(v, a, gs, gp, s)) * v.H;
+        at += seg_work<DT, MODE>(a, segment<DT, MODE>(v, a, gs, gp, s)) * v.H;
         if (u0 < at) break;
       }
     sh.seg = s;
@@ -1484,14 +1896,14 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       tile_at = x.at + h * x.work;  // unit of the tile's first step
       j = 0;
     }
-    int work = tile_work<DT, SEEN>(a, g, j);
+    int work = tile_work<DT, MODE>(a, g, j);
     while (u >= tile_at + work) {
       tile_at += work;
       if (++j == g.tiles) j = 0, ++h;
-      work = tile_work<DT, SEEN>(a, g, j);
+      work = tile_work<DT, MODE>(a, g, j);
     }
     // this workgroup's steps [k0, k1) of the tile's `len`
-    const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps<SEEN>(a, g, j));
+    const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps<MODE>(a, g, j));
     auto steps_in = [&](int units) {  // begun within so many units
       const int n = units + per_step - 1;
       return first_lane_i(g.tile == 16 ? n / step_units<DT>(16) : g.tile == 32 ? n / step_units<DT>(32) : n / step_units<DT>(kWide));
@@ -1499,14 +1911,15 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     const int k0 = steps_in((int)(u - tile_at)), k1 = min(len, steps_in((int)min((uint64_t)work, u1 - tile_at)));
     u = tile_at + work;
     if (k0 >= k1) continue;  // the workgroup before has done them all
-    Tile<SEEN> t;
+    Tile<MODE> t;
     t.row0 = g.row0 + j * g.tile, t.rows = min(g.tile, g.rows - j * g.tile), t.h = h;
-    t.p0 = g.p0 + kStep * k0, t.p1 = min(g.p1, g.p0 + kStep * k1);
+    const int pages = MODE == kSeenWide ? step_pages<MODE>(g.tile) : kStep;
+    t.p0 = g.p0 + pages * k0, t.p1 = min(g.p1, g.p0 + pages * k1);
     if constexpr (SEEN) {
       t.ahead = t.skip = t.lo_lo = t.lo_hi = t.sinks = 0, t.before = kNoDrafts, t.len = g.len;
       if (g.own) {
         const Range r = tile_range(a, g, j);
-        t.p1 = min(r.p1, g.p0 + kStep * k1);
+        t.p1 = min(r.p1, g.p0 + pages * k1);
         t.ahead = r.ahead, t.skip = r.skip, t.lo_lo = r.lo_lo, t.lo_hi = r.lo_hi;
         t.lim_lo = r.lim_lo, t.lim_hi = r.lim_hi;
         if (a.seen.window) t.sinks = a.seen.sinks;
@@ -1539,7 +1952,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
         __syncthreads();
       }
     }
-    if (tid < 3) sh.odd[tid] = 0;
+    if (tid < (int)(sizeof(sh.odd) / sizeof(int))) sh.odd[tid] = 0;
     if (tid == 0) sh.left_out = 0;
     if (tid < t.rows) {
       const int row = t.row0 + tid, tok = token_of_row(a, row);
@@ -1608,7 +2021,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       write(ml, o);
       __threadfence_block();
       __syncthreads();
-      add_left_out<DT, SEEN>(v, a, t, unit, sh, ml, o);
+      add_left_out<DT, MODE>(v, a, t, unit, sh, ml, o);
       if (to_o) return;
       __threadfence_block();
       __syncthreads();
@@ -1619,7 +2032,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
     };
     auto narrow = [&](auto nt) __attribute__((always_inline)) {
       constexpr int NT = decltype(nt)::value;
-      Narrow<DT, NT, SEEN> x;
+      Narrow<DT, NT, MODE> x;
       x.run(v, a, t, sh);
       finish(1, [&](float* ml, float* o) __attribute__((always_inline)) { narrow_write<DT, NT>(a, t, sh, ml, o); });
     };
@@ -1631,7 +2044,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void k_attend(PageView v, int lay
       if (g.tile == 16) narrow(one);
       else if (FORMS == 2 || g.tile == 32) narrow(pair);
       else if constexpr (FORMS == 3) {
-        Wide<DT, SEEN> x;
+        std::conditional_t<MODE == kSeenWide, Wide8<DT>, Wide<DT, MODE>> x;
         x.run(v, a, t, sh);
         finish(kStep, [&](float* ml, float* o) __attribute__((always_inline)) { x.write(a, t, ml, o); });
       }
@@ -1728,12 +2141,13 @@ __global__ __launch_bounds__(kThreads) void k_attend_join(PageView v, AttendArgs
         none ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
-template <int DT, bool SEEN>
+template <int DT, int MODE>
 void launch_forms(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int forms, int grid, hipStream_t s) {
-  if (forms == 1) k_attend<DT, 1, SEEN><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+  if (forms == 1) k_attend<DT, 1, MODE><<<grid, threads_of(MODE), 0, s>>>(v, layer, a, ws);
   if constexpr (DT != FERRY_F32) {
-    if (forms == 2) k_attend<DT, 2, SEEN><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
-    if (forms == 3) k_attend<DT, 3, SEEN><<<grid, kThreads, 0, s>>>(v, layer, a, ws);
+    if (forms == 2) k_attend<DT, 2, MODE><<<grid, threads_of(MODE), 0, s>>>(v, layer, a, ws);
+    constexpr int kMode3 = MODE == kSeen ? kSeenWide : MODE;
+    if (forms == 3) k_attend<DT, 3, kMode3><<<grid, threads_of(kMode3), 0, s>>>(v, layer, a, ws);
   }
 }
 
