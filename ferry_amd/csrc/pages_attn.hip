@@ -38,6 +38,15 @@ int attend_forms(const ferry_pages* p, const ferry_attend* a) {
   return p->dtype == FERRY_F32 || rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
 }
 
+#ifndef WRULE
+#define WRULE 256
+#endif
+// Whether a call of form 3 goes to workgroups of eight wavefronts.
+bool takes_wide(const ferry_pages* p, const ferry_attend* a, const ferry_seen* seen) {
+  if (seen->tree_words) return true;
+  return seen->window && (int64_t)a->n_tokens * (a->q_heads / p->kv_heads) <= (int64_t)WRULE * a->n_req;
+}
+
 // Workgroups of a call, and its scratch at `base` (null: sizes only).
 // wide: of one workgroup per CU, whose tiles have up to twice the rows; its parts take
 // no more room.
@@ -63,13 +72,13 @@ int plan_attend(const ferry_pages* p, const ferry_attend* a, bool wide, uint8_t*
 }
 
 template <int DT>
-void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int forms, int grid,
+void launch_attend(const PageView& v, int layer, const AttendArgs& a, const Scratch& ws, int forms, bool wide, int grid,
                    hipStream_t s) {
-  if (a.seen.window || a.seen.words) launch_attend_seen(v, layer, DT, a, ws, forms, grid, s);
+  if (a.seen.window || a.seen.words) launch_attend_seen(v, layer, DT, a, ws, forms, wide, grid, s);
   else launch_forms<DT, kCausal>(v, layer, a, ws, forms, grid, s);
   // a workgroup per row where that does not fill the GPU twice
   const uint64_t all = (uint64_t)a.n_tokens * a.Hq;
-  if (all <= 2ull * grid) {
+  if (all <= 2ull * (wide ? kPerCu : 1) * grid) {
     k_attend_join<DT, 16><<<(unsigned)all, kThreads, 0, s>>>(v, a, ws, grid, 0);
     return;
   }
@@ -119,8 +128,8 @@ int ferry_pages_attend_seen(const ferry_pages* p, int32_t layer, const ferry_att
     Scratch ws;
     uint64_t need = 0;
     const int forms = attend_forms(p, a);
-    const bool partly = seen && (seen->window || seen->tree_words);
-    const int grid = plan_attend(p, a, partly && forms == 3, static_cast<uint8_t*>(a->work), &ws, &need);
+    const bool wide = forms == 3 && seen && takes_wide(p, a, seen);
+    const int grid = plan_attend(p, a, wide, static_cast<uint8_t*>(a->work), &ws, &need);
     if (a->work_bytes < need) return report(FERRY_EINVAL, "work is smaller than ferry_pages_attend_work_bytes");
     if (reinterpret_cast<uintptr_t>(a->work) % 256) return report(FERRY_EINVAL, "work must be 256-byte aligned");
     OnDevice on(p->device);
@@ -137,10 +146,10 @@ int ferry_pages_attend_seen(const ferry_pages* p, int32_t layer, const ferry_att
     while (1 << (d.g_shift - 31) < d.G) ++d.g_shift;
     d.g_mul = (uint32_t)((1ull << d.g_shift) / d.G + 1);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, forms, grid, s);
-    else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, forms, grid, s);
-    else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, forms, grid, s);
-    else launch_attend<FERRY_FP8_E4M3>(v, layer, d, ws, forms, grid, s);
+    if (p->dtype == FERRY_F32) launch_attend<FERRY_F32>(v, layer, d, ws, forms, wide, grid, s);
+    else if (p->dtype == FERRY_F16) launch_attend<FERRY_F16>(v, layer, d, ws, forms, wide, grid, s);
+    else if (p->dtype == FERRY_BF16) launch_attend<FERRY_BF16>(v, layer, d, ws, forms, wide, grid, s);
+    else launch_attend<FERRY_FP8_E4M3>(v, layer, d, ws, forms, wide, grid, s);
     return launched("ferry_pages_attend");
   });
 }

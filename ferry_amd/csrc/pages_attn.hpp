@@ -89,8 +89,8 @@ struct Scratch {
 };
 
 // The launch of k_attend with SEEN (pages_attn_seen.hip).
-void launch_attend_seen(const PageView& v, int layer, int dtype, const AttendArgs& a, const Scratch& ws, int forms, int grid,
-                        hipStream_t s);
+void launch_attend_seen(const PageView& v, int layer, int dtype, const AttendArgs& a, const Scratch& ws, int forms, bool wide,
+                        int grid, hipStream_t s);
 
 }  // namespace ferry_amd
 
@@ -281,6 +281,20 @@ __device__ inline int shared_of(const PageView& v, const AttendArgs& a, const in
   return group_pages<DT, MODE>(v, a, b, e, gp[lo]);
 }
 
+// Request r without groups: its segment.
+template <int DT, int MODE>
+__device__ inline Seg request_alone(const PageView& v, const AttendArgs& a, int r) {
+  const int t0 = token_of(a, r), t1 = max(t0, token_of(a, r + 1));
+  Seg g;
+  g.own = 1, g.req = r, g.lane = lane_of(v, a, r), g.len = len_of(v, g.lane);
+  g.tok0 = t0, g.row0 = t0 * a.G, g.rows = (t1 - t0) * a.G, g.group = -1;
+  g.base = g.len - (t1 - t0) + 1;
+  g.p0 = 0, g.p1 = pages_of(g.len);
+  g.tile = tile_rows<DT, MODE>(g.rows);
+  g.tiles = (g.rows + g.tile - 1) >> (31 - __clz(g.tile));
+  return g;
+}
+
 // Segment s: groups first, then requests.  gs, gp: the groups' offsets and pages.
 template <int DT, int MODE>
 __device__ inline Seg segment(const PageView& v, const AttendArgs& a, const int* gs, const int* gp, int s) {
@@ -373,10 +387,66 @@ __device__ inline int tile_work(const AttendArgs& a, const Seg& g, int j) {
 // ... of all tiles of a segment, per kv head
 template <int DT, int MODE>
 __device__ inline uint64_t seg_work(const AttendArgs& a, const Seg& g) {
-  if (!g.own) return (uint64_t)g.tiles * tile_work<DT, MODE>(a, g, 0);
+  if (!g.own || (MODE && a.seen.words)) return (uint64_t)g.tiles * tile_work<DT, MODE>(a, g, 0);
   uint64_t n = 0;
   for (int j = 0; j < g.tiles; ++j) n += tile_work<DT, MODE>(a, g, j);
   return n;
+}
+
+// A record of lane `from`.
+template <class T>
+__device__ inline T of_lane(const T& x, int from) {
+  static_assert(sizeof(T) % 4 == 0, "whole words");
+  int w[sizeof(T) / 4];
+  __builtin_memcpy(w, &x, sizeof(T));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 4); ++i) w[i] = __builtin_amdgcn_readlane(w[i], from);
+  T y;
+  __builtin_memcpy(&y, w, sizeof(T));
+  return y;
+}
+
+// The same by a wavefront whose lanes have a segment each (or none: g.rows 0): a thread's own
+// of few tiles, those of many tiles one after the other, a tile per lane.
+template <int DT, int MODE>
+__device__ inline uint64_t seg_work_of_all(const AttendArgs& a, const Seg& g) {
+  const bool many = g.own && !a.seen.words && g.tiles > 4;
+  uint64_t n = many ? 0 : seg_work<DT, MODE>(a, g);
+  for (uint64_t left = __builtin_amdgcn_ballot_w64(many); left; left &= left - 1) {
+    const int from = __builtin_ctzll(left);
+    const Seg x = of_lane(g, from);
+    uint64_t sum = 0;
+    for (int j = threadIdx.x & 63; j < x.tiles; j += 64) sum += tile_work<DT, MODE>(a, x, j);
+#pragma unroll
+    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == from) n = sum;
+  }
+  return n;
+}
+
+// Sum of x over the wavefront's lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ inline uint64_t moved(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xF, false) << 32 |
+         (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
+__device__ inline uint64_t sum_up_to(uint64_t x) {
+  x += moved<0x111, 0xF>(x), x += moved<0x112, 0xF>(x), x += moved<0x114, 0xF>(x), x += moved<0x118, 0xF>(x);  // within 16
+  x += moved<0x142, 0xA>(x);  // the rows' last lanes to the second and fourth row ...
+  x += moved<0x143, 0xC>(x);  // ... and of the first half to the other
+  return x;
+}
+
+// n / d of n < 2^52 (exactly; a fifth of the general division's instructions).
+__device__ inline uint64_t quotient(uint64_t n, uint32_t d) {
+  const double x = (double)(uint32_t)(n >> 32) * 4294967296.0 + (double)(uint32_t)n, y = (double)d;
+  double r = __builtin_amdgcn_rcp(y);
+  r = __builtin_fma(__builtin_fma(-y, r, 1.0), r, r);
+  double q = __builtin_floor(x * r);
+  const double rest = __builtin_fma(-q, y, x);  // exact: q is off by one at most
+  q += rest < 0.0 ? -1.0 : rest >= y ? 1.0 : 0.0;
+  const double hi = __builtin_floor(q * 0x1p-32);
+  return (uint64_t)(uint32_t)hi << 32 | (uint32_t)(q - hi * 4294967296.0);
 }
 
 // The thread's number, anew: what a tile's code derives from it is then computed for
@@ -505,19 +575,32 @@ struct Shared {
   std::conditional_t<MODE != kCausal, int[kWide], None> lo;  // of the tokens that a row sees the first behind the sinks
 };
 
-// 8 query values of a row as two 16-bit values per dword, times the sign of the
-// scale (scores are then compared before they are scaled).
-__device__ inline u32x4 load_q8(const uint16_t* p, bool aligned, uint32_t sign) {
-  u32x4 x;
+// The query values of a lane's row from p on, as N words of 8 16-bit (or 4 fp32) values at
+// dims dim(0), dim(1) ..; all on their way at once.  They get the sign of the scale (scores
+// are then compared before they are scaled); those of a row that is not `there` are 0.
+template <class E, int N, class Dim>
+__device__ __forceinline__ void load_q(u32x4 (&q)[N], const E* p, bool there, bool aligned, uint32_t sign, Dim&& dim) {
+  auto take = [&](const u32x4 (&x)[N]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < N; ++w) q[w] = there ? x[w] ^ sign : u32x4{0u, 0u, 0u, 0u};
+  };
+  u32x4 x[N];
   if (aligned) {
-    x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int w = 0; w < N; ++w) x[w] = *reinterpret_cast<const u32x4*>(p + dim(w));
+    take(x);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    for (int w = 0; w < N; ++w) {
+      const E* e = p + dim(w);
+      if constexpr (sizeof(E) == 4)
+        x[w] = u32x4{f32_bits(e[0]), f32_bits(e[1]), f32_bits(e[2]), f32_bits(e[3])};
+      else
+        x[w] = u32x4{(uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16,
+                     (uint32_t)e[4] | (uint32_t)e[5] << 16, (uint32_t)e[6] | (uint32_t)e[7] << 16};
+    }
+    take(x);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] ^= sign;
-  return x;
 }
 
 // Element offset of row `row`'s query (or output) in a tensor of strides s.
@@ -733,22 +816,11 @@ struct Narrow {
       m[nt] = -INFINITY, sum[nt] = 0.0f;
 #pragma unroll
       for (int nb = 0; nb < 8; ++nb) o[nt][nb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
-#pragma unroll
-      for (int w = 0; w < (K::F32 ? 8 : 4); ++w) {
-        u32x4 x = {0u, 0u, 0u, 0u};
-        if (row < t.rows) {
-          if constexpr (K::F32) {
-            const float* p = static_cast<const float*>(a.q) + at + 4 * (4 * w + grp);
-            if (a.aligned) x = *reinterpret_cast<const u32x4*>(p);
-            else x = u32x4{f32_bits(p[0]), f32_bits(p[1]), f32_bits(p[2]), f32_bits(p[3])};
-          } else {
-            const int d = K::F8 ? 16 * (4 * (w >> 1) + grp) + 8 * (w & 1) : 8 * (4 * w + grp);
-            x = load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned, 0u);
-          }
-        }
-        q[nt][w] = x;
-      }
+      const int64_t at = row_at(a, a.qs, t.row0 + min(row, t.rows - 1), t.h);
+      typedef std::conditional_t<K::F32, float, uint16_t> E;
+      load_q(q[nt], static_cast<const E*>(a.q) + at, row < t.rows, a.aligned, 0u, [&](int w) {
+        return K::F32 ? 4 * (4 * w + grp) : K::F8 ? 16 * (4 * (w >> 1) + grp) + 8 * (w & 1) : 8 * (4 * w + grp);
+      });
     }
     // page i of this wavefront: one of each of the steps of kStep pages in [p0, p1)
     const int count = (t.p1 - t.p0 + kStep - 1) / kStep;
@@ -1022,11 +1094,8 @@ struct Wide {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-      q[s] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + 16 * s + 8 * h, a.aligned, sign)
-                          : u32x4{0u, 0u, 0u, 0u};
+    load_q(q, static_cast<const uint16_t*>(a.q) + row_at(a, a.qs, t.row0 + min(row, t.rows - 1), t.h), row < t.rows, a.aligned,
+           sign, [&](int s) { return 16 * s + 8 * h; });
     const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
     // Page ids: lane j holds page 64 w + j of window w; the next window is read ahead.
     auto read_ids = [&](int w) __attribute__((always_inline)) {
@@ -1388,16 +1457,16 @@ struct Wide8 {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-    const int64_t at = row < t.rows ? row_at(a, a.qs, t.row0 + row, t.h) : 0;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const int d = K::F8 ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h;
-      q[c] = row < t.rows ? load_q8(static_cast<const uint16_t*>(a.q) + at + d, a.aligned, sign) : u32x4{0u, 0u, 0u, 0u};
-    }
+    load_q(q, static_cast<const uint16_t*>(a.q) + row_at(a, a.qs, t.row0 + min(row, t.rows - 1), t.h), row < t.rows, a.aligned,
+           sign, [&](int c) { return K::F8 ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h; });
     const int steps = (t.p1 - t.p0 + kStep - 1) / kStep;
     auto first_token = [&](int s) __attribute__((always_inline)) { return t.page(t.p0 + kStep * s) * kPageTokens; };
     auto is_whole = [&](int s) __attribute__((always_inline)) {
       return s < steps && t.whole(first_token(s), kStep * kPageTokens);
+    };
+    auto whole_from = [&](int s) __attribute__((always_inline)) {  // steps from s on that every row sees whole, up to 64
+      const uint64_t no = ~__builtin_amdgcn_ballot_w64(is_whole(s + l));
+      return no ? __builtin_ctzll(no) : 64;
     };
     // Page ids: lane j of window w holds page 64 w + j.  Windows at, at + 1 and, on its way,
     // at + 2; fp8: the scales of the windows of the step computed, of the next one, and
@@ -1531,6 +1600,7 @@ struct Wide8 {
     };
 
     constexpr int kProducts = 8 * NTT;  // of S^T, and of O^T
+    constexpr int kEarly = NTT == 2 ? 16 : 8;  // pairs of weights computed next to those of S^T, the others next to O^T's
     f32x16 x[NTT], y[NTT];
     // Loads in the steps' order: in step s those of V of step s + kSlots - 1 and of K of s + kSlots.
     for (int s = -kSlots; s < 0; ++s) {
@@ -1551,12 +1621,14 @@ struct Wide8 {
 #pragma unroll
       for (int i = 0; i < kProducts; ++i)
         x[i % NTT] = mma32<K::BF>(operand(read_k(k_at, i)), q[i / NTT], x[i % NTT]);
-      const u32x2 bits = bits_of(0);
+      const bool masked = !is_whole(0);
+      u32x2 bits = {0u, 0u};
+      if (masked) bits = bits_of(0);
       float c[2 * NTT], top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2 * NTT; ++i) c[i] = K::F8 ? scale * scale_of(0, 0, 2 * half + i) : scale;
 #pragma unroll
-      for (int i = 0; i < 16 * NTT; i += 4) among(x, i, true, bits, c, top);
+      for (int i = 0; i < 16 * NTT; i += 4) among(x, i, masked, bits, c, top);
       top = of_row(top);
       raise_to(top, top > m + K::kMost);
     }
@@ -1583,6 +1655,17 @@ struct Wide8 {
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[i][e] = 0.0f;
       const float ref = against(m);
+      auto weights2 = [&](int w) __attribute__((always_inline)) {
+        const float y0 = x[w >> 3][2 * w & 15], y1 = x[w >> 3][(2 * w & 15) + 1];
+        float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
+        float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
+        sum += p0 + p1;
+        if constexpr (K::F8) {
+          const float f = scale_of(1, s, 2 * half + (w >> 2));
+          p0 *= f, p1 *= f;
+        }
+        pop[w] = pack2<K::BF>(p0, p1);
+      };
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
@@ -1590,15 +1673,8 @@ struct Wide8 {
         y[i % NTT] = mma32<K::BF>(operand(p[i & 3]), q[i / NTT], y[i % NTT]);
         if (i == 0) begin_v(s + kSlots - 1);
         if (i == 2) begin_k(s + kSlots);
-        const float y0 = x[i >> 3][2 * i & 15], y1 = x[i >> 3][(2 * i & 15) + 1];
-        float p0 = exp2_fast(K::F8 ? y0 - ref : __builtin_fmaf(y0, scale, -ref));
-        float p1 = exp2_fast(K::F8 ? y1 - ref : __builtin_fmaf(y1, scale, -ref));
-        sum += p0 + p1;
-        if constexpr (K::F8) {
-          const float f = scale_of(1, s, 2 * half + (i >> 2));
-          p0 *= f, p1 *= f;
-        }
-        pop[i] = pack2<K::BF>(p0, p1);
+#pragma unroll
+        for (int w = i * kEarly / kProducts; w < (i + 1) * kEarly / kProducts; ++w) weights2(w);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
@@ -1610,6 +1686,7 @@ struct Wide8 {
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         if (i + 3 < kProducts) p[i + 3 & 3] = read_v(v_at, i + 3);
+        if (kEarly + i < kProducts) weights2(kEarly + i);
         o[i & 3] = mma32<K::BF>(operand(p[i & 3]), u32x4{pop[i & ~3], pop[(i & ~3) + 1], pop[(i & ~3) + 2], pop[(i & ~3) + 3]},
                                 o[i & 3]);
         if (i >= kFirst && i < kFirst + 4 * NTT) among(y, 4 * (i - kFirst), MASKED, bits, c, top);
@@ -1648,7 +1725,7 @@ struct Wide8 {
     };
     auto begin_step = [&](int s) __attribute__((always_inline)) { begin_v(s + kSlots - 1), begin_k(s + kSlots); };
     for (int s = 0; s < steps;) {
-      for (; is_whole(s) && is_whole(s + 1); ++s) {
+      for (const int last = s + whole_from(s) - 1; s < last; ++s) {
         before(s);
         if (busy) step(std::false_type{}, s);
         else begin_step(s);
@@ -1664,7 +1741,7 @@ struct Wide8 {
         wait_all_but<kLeft>();
         land(s);
         meet();
-      } while (s < steps && !(is_whole(s) && is_whole(s + 1)));
+      } while (s < steps && whole_from(s) < 2);
     }
     wait_all_but<0>();
     {
@@ -1798,31 +1875,57 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
   // units of this thread's segments, and their sum over all threads before it
   const int per_thread = (nseg + kThreads - 1) / kThreads, s0 = min(tid * per_thread, nseg),
             s1 = min(s0 + per_thread, nseg);
-  uint64_t mine = 0;
+  uint64_t mine = 0, before = 0, total = 0;
   Seg kept;  // the thread's only segment, where it has one
   uint64_t kept_work = 0;
+  // few requests alone: every wavefront plans by itself, a request per lane
+  const bool few = SEEN && a.n_groups == 0 && a.n_req <= 64;
+  auto misplaced = [&](const Seg& g) {
+    const int lane = a.lanes[g.req];
+    bool bad = lane < -1 || lane >= v.n_lanes || (g.lane >= 0 && v.len[g.lane] != g.len);
+    if (a.q_start)
+      bad |= a.q_start[g.req] < 0 || a.q_start[g.req] > a.q_start[g.req + 1] || a.q_start[g.req + 1] > a.n_tokens;
+    if (SEEN && a.seen.words) bad |= token_of(a, g.req + 1) - token_of(a, g.req) > 64 * a.seen.words;
+    return bad;
+  };
+  if (few) {
+    const int r = tid & 63;
+    kept = request_alone<DT, MODE>(v, a, min(r, a.n_req - 1));
+    if (r >= a.n_req) kept.rows = kept.tiles = 0;
+    kept_work = seg_work_of_all<DT, MODE>(a, kept);
+    mine = kept_work * v.H;
+    before = sum_up_to(mine);
+    total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(before >> 32), 63) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((int)before, 63);
+    before -= mine;
+    if (wg == 0 && tid < a.n_req && misplaced(kept)) set_error(v.error, FERRY_ERANGE);
+  } else {
+  if constexpr (SEEN) {
+    if (per_thread == 1) {
+      kept = segment<DT, MODE>(v, a, gs, gp, min(s0, nseg - 1));
+      if (s0 >= s1) kept.rows = kept.tiles = 0, kept.own = 0;
+      kept_work = seg_work_of_all<DT, MODE>(a, kept);
+    }
+  }
   for (int s = s0; s < s1; ++s) {
-    kept = segment<DT, MODE>(v, a, gs, gp, s);
-    kept_work = seg_work<DT, MODE>(a, kept);
+    if (!SEEN || per_thread > 1) {
+      kept = segment<DT, MODE>(v, a, gs, gp, s);
+      kept_work = seg_work<DT, MODE>(a, kept);
+    }
     mine += kept_work * v.H;
     if (kept.own && kept.group >= 0 && kept.rows > 0 && gs == sh.gs)
       atomicMin(&sh.gl[kept.group], SEEN && a.seen.words ? max(0, kept.base - 1) / kPageTokens * kPageTokens : max(0, kept.base));
     if (wg == 0) {  // what is out of range, once
       bool bad = false;
       if (kept.own) {
-        const int lane = a.lanes[kept.req];
-        bad = lane < -1 || lane >= v.n_lanes || (kept.lane >= 0 && v.len[kept.lane] != kept.len);
-        if (a.q_start)
-          bad |= a.q_start[kept.req] < 0 || a.q_start[kept.req] > a.q_start[kept.req + 1] ||
-                 a.q_start[kept.req + 1] > a.n_tokens;
-        if (SEEN && a.seen.words) bad |= token_of(a, kept.req + 1) - token_of(a, kept.req) > 64 * a.seen.words;
+        bad = misplaced(kept);
       } else {
         bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
       }
       if (bad) set_error(v.error, FERRY_ERANGE);
     }
   }
-  uint64_t before = mine;
+  before = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const uint64_t y = __shfl_up(before, d);
@@ -1830,17 +1933,20 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
   }
   if ((tid & 63) == 63) sh.sums[tid >> 6] = before;
   __syncthreads();
-  uint64_t total = 0;
   for (int i = 0; i < kThreads / 64; ++i) {
     if (i < tid >> 6) before += sh.sums[i];
     total += sh.sums[i];
   }
   before -= mine;
   total = first_lane_u64(total);
+  }
   // no run is shorter than a step, so that each one within a tile begins one
   constexpr int kMost = FORMS == 1 ? step_units<DT>(16) : 11;
   static_assert(FORMS == 1 || (step_units<DT>(16) <= kMost && step_units<DT>(32) <= kMost && step_units<DT>(kWide) <= kMost));
-  const uint64_t per = max((uint64_t)kMost, first_lane_u64((total + grid - 1) / grid));
+  uint64_t each = total + grid - 1;
+  if (SEEN && each < 1ull << 52) each = quotient(each, grid);
+  else each /= grid;
+  const uint64_t per = max((uint64_t)kMost, first_lane_u64(each));
   const uint64_t u0 = per * wg, u1 = min(total, u0 + per);
   if (u0 >= u1) return;
   const uint32_t per32 = (uint32_t)min(per, (uint64_t)0x7FFFFFFF);
@@ -1859,44 +1965,85 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
     }
     __syncthreads();
   };
-  if (u0 >= before && u0 < before + mine) {  // one thread: it has the run's first segment
-    uint64_t at = before;
-    int s = s0;
-    if (per_thread > 1)
-      for (;; ++s) {
-        at += seg_work<DT, MODE>(a, segment<DT, MODE>(v, a, gs, gp, s)) * v.H;
-        if (u0 < at) break;
-      }
-    sh.seg = s;
+  const bool has_first = u0 >= before && u0 < before + mine;  // one lane of each wavefront, or one thread
+  int s = 0, from = 0;
+  SegAt x;
+  auto listed = [&](int i) { x = few ? of_lane(SegAt{kept, before, kept_work}, i) : uniform(sh.list[i - from]); };
+  if (few) {
+    s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(has_first));
+  } else {
+    if (has_first) {
+      uint64_t at = before;
+      int s = s0;
+      if (per_thread > 1)
+        for (;; ++s) {
+          at += seg_work<DT, MODE>(a, segment<DT, MODE>(v, a, gs, gp, s)) * v.H;
+          if (u0 < at) break;
+        }
+      sh.seg = s;
+    }
+    __syncthreads();
+    s = from = first_lane_i(sh.seg);
+    list(from, std::true_type{});
   }
-  __syncthreads();
-
-  int s = first_lane_i(sh.seg), from = s;
-  list(from, std::true_type{});
   uint64_t u = u0, tile_at = 0;
   int h = -1, j = 0;
-  SegAt x;
-  auto listed = [&](int i) { x = uniform(sh.list[i]); };
-  listed(0);
+  listed(s);
   while (u < u1) {
     const int tid = this_thread();
     if (u >= x.at + x.work * v.H) {  // the next segment
-      if (++s == from + kListed) {
+      if (++s == from + kListed && !few) {
         __syncthreads();
         from = s;
         list(from, std::false_type{});
       }
-      listed(s - from);
+      listed(s);
       h = -1;
       continue;
     }
     const Seg& g = x.g;
     if (h < 0) {
-      h = u == x.at ? 0 : (int)((u - x.at) / x.work);
+      if constexpr (SEEN) {  // a guess within one
+        const uint64_t n = u - x.at;
+        h = (int)((float)n * __builtin_amdgcn_rcpf((float)x.work));
+        h = first_lane_i(h);
+        if (h * x.work > n) --h;
+        else if ((h + 1) * x.work <= n) ++h;
+      } else {
+        h = u == x.at ? 0 : (int)((u - x.at) / x.work);
+      }
       tile_at = x.at + h * x.work;  // unit of the tile's first step
       j = 0;
     }
     int work = tile_work<DT, MODE>(a, g, j);
+    if (SEEN && u >= tile_at + work && (!g.own || a.seen.words)) {  // tiles of equal work
+      if (j < g.tiles - 1) {
+        const uint64_t n = u - tile_at;
+        int skip = (int)min((float)n * __builtin_amdgcn_rcpf((float)work), (float)(g.tiles - 1 - j));
+        skip = first_lane_i(skip);
+        while (skip && (uint64_t)skip * work > n) --skip;
+        j += skip, tile_at += (uint64_t)skip * work;
+      }
+    } else if (SEEN && u >= tile_at + work) {  // a tile per lane
+      while (j < g.tiles - 1) {
+        const int l = this_thread() & 63, mine = j + l < g.tiles ? tile_work<DT, MODE>(a, g, j + l) : 0;
+        int sum = mine;  // of 64 tiles: below 2^31
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int y = __shfl_up(sum, d);
+          if (l >= d) sum += y;
+        }
+        const uint64_t over = __builtin_amdgcn_ballot_w64(tile_at + sum > u && mine > 0);
+        if (over) {
+          const int n = __builtin_ctzll(over);
+          tile_at += __builtin_amdgcn_readlane(sum - mine, n), j += n;
+          break;
+        }
+        const int n = min(63, g.tiles - 1 - j);  // the last of these is the next one's first
+        tile_at += __builtin_amdgcn_readlane(sum - mine, n), j += n;
+      }
+      work = first_lane_i(tile_work<DT, MODE>(a, g, j));
+    }
     while (u >= tile_at + work) {
       tile_at += work;
       if (++j == g.tiles) j = 0, ++h;
@@ -2146,8 +2293,7 @@ void launch_forms(const PageView& v, int layer, const AttendArgs& a, const Scrat
   if (forms == 1) k_attend<DT, 1, MODE><<<grid, threads_of(MODE), 0, s>>>(v, layer, a, ws);
   if constexpr (DT != FERRY_F32) {
     if (forms == 2) k_attend<DT, 2, MODE><<<grid, threads_of(MODE), 0, s>>>(v, layer, a, ws);
-    constexpr int kMode3 = MODE == kSeen ? kSeenWide : MODE;
-    if (forms == 3) k_attend<DT, 3, kMode3><<<grid, threads_of(kMode3), 0, s>>>(v, layer, a, ws);
+    if (forms == 3) k_attend<DT, 3, MODE><<<grid, threads_of(MODE), 0, s>>>(v, layer, a, ws);
   }
 }
 
