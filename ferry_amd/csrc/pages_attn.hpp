@@ -1032,6 +1032,48 @@ __device__ __forceinline__ void wide_write(const AttendArgs& a, const CausalTile
   }
   }
 
+// The same of a wavefront's 32 rows through LDS (the places of K and V are free), so that it
+// stores whole rows, 32 lanes a row.
+template <int DT, class Sh>
+__device__ __forceinline__ void write_rows(const AttendArgs& a, const CausalTile& t, Sh& sh, int row, const f32x16 (&o)[4],
+                                           float m, float sum, int lim, float* to_ml, float* to_o) {
+  const int l = this_thread() & 63, h = l >> 5;
+  const float inv = to_o ? 1.0f : lim <= 0 ? 0.0f : 1.0f / sum;
+  float* rows = sh.merge + (row >> 5) * (32 * kPad);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<f32x4*>(rows + (row & 31) * kPad + 32 * dt + 2 * e + 4 * h) =
+          f32x4{o[dt][e] * inv, o[dt][e + 1] * inv, o[dt][e + 2] * inv, o[dt][e + 3] * inv};
+  if (h == 0 && row < t.rows) {
+    if (to_o) {
+      to_ml[2 * row] = m, to_ml[2 * row + 1] = sum;
+    } else if (a.lse) {
+      const int tok = token_of_row(a, t.row0 + row), g = t.row0 + row - tok * a.G;
+      a.lse[(int64_t)tok * a.Hq + t.h * a.G + g] = lim <= 0 ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+    }
+  }
+  const int first = row & ~31, d = 4 * (l & 31);
+#pragma unroll 4
+  for (int i = 0; i < 32; i += 2) {
+    const int r = first + i + h;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(rows + (i + h) * kPad + d);
+    if (r >= t.rows) continue;
+    if (to_o) {
+      *reinterpret_cast<f32x4*>(to_o + (int64_t)r * kPageDim + d) = x;
+    } else {
+      uint16_t* to = static_cast<uint16_t*>(a.out) + row_at(a, a.os, t.row0 + r, t.h) + d;
+      const u32x2 w = {pack2<Kv<DT>::BF>(x[0], x[1]), pack2<Kv<DT>::BF>(x[2], x[3])};
+      if (a.aligned) {
+        *reinterpret_cast<u32x2*>(to) = w;
+      } else {
+        to[0] = (uint16_t)w[0], to[1] = (uint16_t)(w[0] >> 16), to[2] = (uint16_t)w[1], to[3] = (uint16_t)(w[1] >> 16);
+      }
+    }
+  }
+}
+
 template <int DT, int MODE>
 struct Wide {
   using K = Kv<DT>;
@@ -1349,19 +1391,20 @@ struct Wide {
     };
     int s = 0;
     if constexpr (SEEN) {  // those that some row does not see whole may come first and last
-      auto is_whole = [&](int s) __attribute__((always_inline)) {
-        return s < steps && t.whole(t.page(t.p0 + kStep * s) * kPageTokens, kStep * kPageTokens);
+      auto whole_from = [&](int s) __attribute__((always_inline)) {  // steps from s on that every row sees whole, up to 64
+        const int at = s + l;
+        const uint64_t no = ~__builtin_amdgcn_ballot_w64(at < steps && t.whole(t.page(t.p0 + kStep * at) * kPageTokens, kStep * kPageTokens));
+        return no ? __builtin_ctzll(no) : 64;
       };
-      auto two_whole = [&](int s) __attribute__((always_inline)) { return is_whole(s) && is_whole(s + 1); };
       while (s < steps) {
-        for (; two_whole(s); ++s) {
+        for (const int last = s + whole_from(s) - 1; s < last; ++s) {
           step(std::false_type{}, x, y, s);
           x[0] = y[0], x[1] = y[1];
         }
         do {
           step(std::true_type{}, x, y, s++);
           x[0] = y[0], x[1] = y[1];
-        } while (s < steps && !two_whole(s));
+        } while (s < steps && whole_from(s) < 2);
       }
     } else if constexpr (K::F8) {
       for (; s + 1 < whole; ++s) {
@@ -1381,9 +1424,11 @@ struct Wide {
     }
   }
 
-  __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, float* to_ml, float* to_o) {
-    const int tid = this_thread(), l = tid & 63;
-    wide_write<DT>(a, t, (tid >> 6) * 32 + (l & 31), l >> 5, o, m, sum, lim, to_ml, to_o);
+  template <class Sh>
+  __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, Sh& sh, float* to_ml, float* to_o) {
+    const int tid = this_thread(), l = tid & 63, row = (tid >> 6) * 32 + (l & 31);
+    if constexpr (SEEN) write_rows<DT>(a, t, sh, row, o, m, sum, lim, to_ml, to_o);
+    else wide_write<DT>(a, t, row, l >> 5, o, m, sum, lim, to_ml, to_o);
   }
 };
 
@@ -1600,7 +1645,6 @@ struct Wide8 {
     };
 
     constexpr int kProducts = 8 * NTT;  // of S^T, and of O^T
-    constexpr int kEarly = NTT == 2 ? 16 : 8;  // pairs of weights computed next to those of S^T, the others next to O^T's
     f32x16 x[NTT], y[NTT];
     // Loads in the steps' order: in step s those of V of step s + kSlots - 1 and of K of s + kSlots.
     for (int s = -kSlots; s < 0; ++s) {
@@ -1673,8 +1717,7 @@ struct Wide8 {
         y[i % NTT] = mma32<K::BF>(operand(p[i & 3]), q[i / NTT], y[i % NTT]);
         if (i == 0) begin_v(s + kSlots - 1);
         if (i == 2) begin_k(s + kSlots);
-#pragma unroll
-        for (int w = i * kEarly / kProducts; w < (i + 1) * kEarly / kProducts; ++w) weights2(w);
+        weights2(i);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
@@ -1686,7 +1729,6 @@ struct Wide8 {
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         if (i + 3 < kProducts) p[i + 3 & 3] = read_v(v_at, i + 3);
-        if (kEarly + i < kProducts) weights2(kEarly + i);
         o[i & 3] = mma32<K::BF>(operand(p[i & 3]), u32x4{pop[i & ~3], pop[(i & ~3) + 1], pop[(i & ~3) + 2], pop[(i & ~3) + 3]},
                                 o[i & 3]);
         if (i >= kFirst && i < kFirst + 4 * NTT) among(y, 4 * (i - kFirst), MASKED, bits, c, top);
@@ -1772,8 +1814,9 @@ struct Wide8 {
     }
   }
 
-  __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, float* to_ml, float* to_o) {
-    if (writes) wide_write<DT>(a, t, row, threadIdx.x >> 5 & 1, o, m, sum, lim, to_ml, to_o);
+  template <class Sh>
+  __device__ __forceinline__ void write(const AttendArgs& a, const CausalTile& t, Sh& sh, float* to_ml, float* to_o) {
+    if (writes) write_rows<DT>(a, t, sh, row, o, m, sum, lim, to_ml, to_o);
   }
 };
 
@@ -2193,7 +2236,9 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
       else if constexpr (FORMS == 3) {
         std::conditional_t<MODE == kSeenWide, Wide8<DT>, Wide<DT, MODE>> x;
         x.run(v, a, t, sh);
-        finish(kStep, [&](float* ml, float* o) __attribute__((always_inline)) { x.write(a, t, ml, o); });
+        finish(kStep, [&](float* ml, float* o) __attribute__((always_inline)) {
+          x.write(a, t, sh, ml, o);
+        });
       }
     }
   }
