@@ -892,9 +892,12 @@ class Pages:
     # ---- drafted tokens -----------------------------------------------------------
     def _tree(self, tree, rows):
         """Pointer and words of a tensor of drafts' bits."""
-        if not isinstance(tree, torch.Tensor) or tree.dim() != 2 or tree.shape[0] != rows or tree.shape[1] < 1:
+        shape = tuple(tree.shape) if isinstance(tree, torch.Tensor) else ()
+        if len(shape) != 2 or shape[0] != rows or shape[1] < 1:
             raise ValueError(f"tree: expected [{rows}, words]")
-        return _dev(tree, "tree", 1 if rows else 0, (torch.int64,), self.device), tree.shape[1]
+        if tree.dtype is torch.int64 and tree.get_device() == self.device and tree.is_contiguous():
+            return tree.data_ptr(), shape[1]
+        return _dev(tree, "tree", 0, (torch.int64,), self.device), shape[1]  # says what is wrong
 
     def tree(self, lanes, parent, tree, at=None, place=None, lane=None, q_start=None, stream=None):
         """Trees of drafted tokens from their parents [rows] (numbers within the request,

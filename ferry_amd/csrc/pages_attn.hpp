@@ -442,6 +442,7 @@ __device__ inline uint64_t quotient(uint64_t n, uint32_t d) {
   const double x = (double)(uint32_t)(n >> 32) * 4294967296.0 + (double)(uint32_t)n, y = (double)d;
   double r = __builtin_amdgcn_rcp(y);
   r = __builtin_fma(__builtin_fma(-y, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-y, r, 1.0), r, r);
   double q = __builtin_floor(x * r);
   const double rest = __builtin_fma(-q, y, x);  // exact: q is off by one at most
   q += rest < 0.0 ? -1.0 : rest >= y ? 1.0 : 0.0;

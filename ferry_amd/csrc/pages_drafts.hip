@@ -36,61 +36,79 @@ __device__ inline void no_row(const TreeArgs& a, int64_t t) {
   for (int w = 0; w < a.words; ++w) a.tree[t * a.words + w] = 0;
 }
 
-// A wavefront per request, a token per lane, 64 at a time.  Parents come before their
-// children, so of a token's ancestors those in its own 64 are found in six rounds (each
-// takes over what the ancestor reached so far has, and its reach), and those before
-// them are the row of the parent that the topmost of these has, which is written.
-// Bound by latency: per 64 tokens the read of the parents and that of the row (256
-// requests of 150 to 300 tokens write 3 MB).  The workgroup behind the last request pads
-// the tokens of none.
-__global__ __launch_bounds__(64) void k_tree(PageView v, TreeArgs a) {
-  const int r = blockIdx.x, l = threadIdx.x;
+// A workgroup per request, a token per thread (`blockDim.x` of them at a time).  Parents come
+// before their children, so of a token's ancestors those in its own 64 are found by its
+// wavefront in six rounds (each takes over what the ancestor reached so far has, and its
+// reach); the topmost of these has its parent among earlier tokens, and what that one found
+// is the next word that is not 0.  So all words of all tokens are made at once, in as many
+// steps as there are words, from LDS; only tokens behind the first blockDim.x read back
+// rows that are written.  Bound by latency: the offsets, the lane, its length and the parents
+// are dependent reads; 256 requests of 150 to 300 tokens write 3 MB in @@ us (8.0 with a
+// wavefront per request that goes on 64 by 64).  The last of the rounds pads the tokens of
+// no request.
+constexpr int kTreeThreads = 1024, kTreeGroups = 1 << 16;
+__global__ __launch_bounds__(kTreeThreads) void k_tree(PageView v, TreeArgs a) {
+  __shared__ uint64_t found[kTreeThreads];  // of a token's own 64
+  __shared__ int before[kTreeThreads];      // the parent of the topmost of these, -1: none
+  const int tid = threadIdx.x, l = tid & 63, threads = blockDim.x;
   auto token_of = [&](int r) { return a.q_start ? clampi(a.q_start[r], 0, a.n_tokens) : min(r, a.n_tokens); };
-  if (r == a.n_req) {
-    const int first = token_of(0), end = max(first, token_of(a.n_req));
-    for (int64_t i = l; i < (int64_t)first + a.n_tokens - end; i += 64)
-      no_row(a, i < first ? i : i - first + end);
-    return;
-  }
-  const int t0 = token_of(r), n = max(0, token_of(r + 1) - t0), lane = a.lanes[r];
-  const int len = lane >= 0 && lane < v.n_lanes ? v.len[lane] : 0;
-  const bool held = len >= n && len <= v.max_pages * kPageTokens;
-  const bool fine = lane >= 0 && lane < v.n_lanes && held;
-  bool bad = lane != -1 && !fine;
-  if (a.q_start) bad |= a.q_start[r] < 0 || a.q_start[r] > a.q_start[r + 1] || a.q_start[r + 1] > a.n_tokens;
-  if (n > 64 * a.words) bad = true;
-  for (int c0 = 0, k = 0; c0 < n; c0 += 64, ++k) {
-    const int c = c0 + l;
-    const int64_t t = (int64_t)t0 + c;
-    int p = c < n ? a.parent[t] : -1;
-    if (p < -1 || p >= c) {
-      if (c < n) bad = true;
-      p = -1;
+  for (int64_t r64 = blockIdx.x; r64 <= a.n_req; r64 += gridDim.x) {
+    const int r = (int)r64;
+    if (r == a.n_req) {
+      const int first = token_of(0), end = max(first, token_of(a.n_req));
+      for (int64_t i = tid; i < (int64_t)first + a.n_tokens - end; i += threads) no_row(a, i < first ? i : i - first + end);
+      break;
     }
-    uint64_t mine = 1ull << l;
-    int up = p >= c0 ? p - c0 : l;  // the ancestor reached, itself at the end
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-      mine |= __shfl(mine, up);
-      up = __shfl(up, up);
-    }
-    const int e = __shfl(p, up);  // the topmost one's parent: before these 64, or none
-    if (!fine) {
-      if (c < n) no_row(a, t);
-      continue;
-    }
-    int deep = __popcll(mine);
-    __threadfence_block();  // rows before these are read
-    if (c < n) {
-      for (int w = 0; w < a.words; ++w) {
-        const uint64_t x = w == k ? mine : w < k && e >= 0 ? a.tree[((int64_t)t0 + e) * a.words + w] : 0ull;
-        if (w < k) deep += __popcll(x);
-        a.tree[t * a.words + w] = x;
+    const int t0 = token_of(r), n = max(0, token_of(r + 1) - t0), lane = a.lanes[r];
+    const int len = lane >= 0 && lane < v.n_lanes ? v.len[lane] : 0;
+    const bool held = len >= n && len <= v.max_pages * kPageTokens;
+    const bool fine = lane >= 0 && lane < v.n_lanes && held;
+    bool bad = lane != -1 && !fine;
+    if (a.q_start) bad |= a.q_start[r] < 0 || a.q_start[r] > a.q_start[r + 1] || a.q_start[r + 1] > a.n_tokens;
+    if (n > 64 * a.words) bad = true;
+    for (int b0 = 0; b0 < n; b0 += threads) {
+      const int c = b0 + tid, c0 = c & ~63;  // (blocks are whole 64s)
+      const int64_t t = (int64_t)t0 + c;
+      if (!fine) {
+        if (c < n) no_row(a, t);
+        continue;
       }
+      int p = c < n ? a.parent[t] : -1;
+      if (p < -1 || p >= c) {
+        bad |= c < n;
+        p = -1;
+      }
+      uint64_t mine = 1ull << l;
+      int up = p >= c0 ? p - c0 : l;  // the ancestor reached, itself at the end
+#pragma unroll
+      for (int i = 0; i < 6; ++i) {
+        mine |= __shfl(mine, up);
+        up = __shfl(up, up);
+      }
+      int e = __shfl(p, up);
+      __threadfence_block();
+      __syncthreads();  // rows of the blocks before are written, what they found is read
+      found[tid] = mine, before[tid] = e;
+      __syncthreads();
+      if (c >= n) continue;
+      int deep = 0;
+      uint64_t* row = a.tree + t * a.words;
+      for (int w = c >> 6; w >= 0; --w) {  // words above are 0
+        uint64_t x = mine;
+        if (w != c >> 6) {
+          x = 0;
+          if (e >= b0 && e >> 6 == w) x = found[e - b0], e = before[e - b0];
+          else if (e >= 0 && e < b0 && w < a.words) x = a.tree[((int64_t)t0 + e) * a.words + w];
+        }
+        deep += __popcll(x);
+        if (w < a.words) row[w] = x;
+      }
+      for (int w = (c >> 6) + 1; w < a.words; ++w) row[w] = 0;
       tree_row(a, t, len - n + deep - 1, len - n + c, lane);
     }
+    if (__builtin_amdgcn_ballot_w64(bad) && l == 0) set_error(v.error, FERRY_ERANGE);
+    __syncthreads();  // the next request's tokens take the places
   }
-  if (__builtin_amdgcn_ballot_w64(bad) && l == 0) set_error(v.error, FERRY_ERANGE);
 }
 
 // ---- accept ----------------------------------------------------------------------
@@ -344,7 +362,8 @@ int ferry_pages_tree(const ferry_pages* p, const ferry_tree* a, void* stream) {
     if (!on.ok()) return report(FERRY_EHIP, "cannot use the cache's GPU");
     const TreeArgs d{a->n_req, a->n_tokens, a->tree_words, a->lanes, a->q_start, a->parent,
                      a->tree, a->at, a->place, a->lane};
-    k_tree<<<a->n_req + 1, 64, 0, static_cast<hipStream_t>(stream)>>>(v, d);
+    const int groups = (int)std::min<int64_t>((int64_t)a->n_req + 1, kTreeGroups);
+    k_tree<<<groups, std::min(64 * a->tree_words, kTreeThreads), 0, static_cast<hipStream_t>(stream)>>>(v, d);
     return launched("ferry_pages_tree");
   });
 }

@@ -49,7 +49,7 @@ def run_tree(p, lanes, parents, words, rows=None, start=None):
     return tree, at.tolist(), place.tolist(), lane.tolist()
 
 
-@pytest.mark.parametrize("sizes", [[1], [2, 0, 3], [63, 64, 65], [8] * 40, [130, 1, 700], [1000]])
+@pytest.mark.parametrize("sizes", [[1], [2, 0, 3], [63, 64, 65], [8] * 40, [130, 1, 700], [1000], [1300, 5, 4000]])
 @pytest.mark.parametrize("back", [1, 3, 40, 100000])
 def test_trees_from_parents(sizes, back):
     rng = np.random.default_rng(back + len(sizes))
