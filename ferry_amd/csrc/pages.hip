@@ -845,7 +845,8 @@ int check_list(const ferry_pages* p, const void* list, const char* name, int n, 
     const uintptr_t at = reinterpret_cast<uintptr_t>(buf);
     return from < at + entries * 4 && at < to;
   };
-  if ((!of_len && meets(p->len, p->n_lanes)) || meets(p->refs, p->n_pages) || meets(p->table, (uint64_t)p->n_lanes * p->max_pages))
+  if ((!of_len && meets(p->len, p->n_lanes)) || meets(p->refs, p->n_pages) ||
+      meets(p->table, (uint64_t)p->n_lanes * p->max_pages))
     return report(FERRY_EINVAL, std::string(name) + " is a part of the cache's own table, len or refs");
   return FERRY_OK;
 }

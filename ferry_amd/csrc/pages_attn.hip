@@ -38,13 +38,25 @@ int attend_forms(const ferry_pages* p, const ferry_attend* a) {
   return p->dtype == FERRY_F32 || rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
 }
 
-#ifndef WRULE
-#define WRULE 256
-#endif
-// Whether a call of form 3 goes to workgroups of eight wavefronts.
+// Whether a call of form 3 goes to workgroups of eight wavefronts with tiles of up to 256
+// rows, one per CU, rather than to those of four with 128, two per CU: where most tiles
+// would read their pages for a second tile of the same request.  The rule is on the rows
+// that a request has on average, as only the device knows each one's.  In us, wide and
+// not, of 8 kv heads, 32 requests over 1,000 to 8,000 tokens unless stated, bf16 (fp8):
+//   drafts, 4 heads a kv head: 12 to 24 tokens 140 and 136 (125 and 114), 16 to 32 tokens
+//   145 and 141 (136 and 119), 24 to 48 tokens 165 and 199 (176 and 182), 32 to 64 tokens
+//   175 and 229 (179 and 203); 128 requests of 12 to 24 tokens over 2,000: 189 and 166.
+//   In groups, whose shared pages meet the rows of all members: 12 to 24 tokens of 32
+//   requests over 8,000 shared tokens 1,189 and 1,471 (1,259 and 1,423), 4 to 8 tokens 544
+//   and 527.  Up to four requests have fewer parts to join: 4 x 8 tokens over 700 18.1 and
+//   19.1, 2 x 32 tokens over 131,000 175 and 178.
+//   windows of 4,096: 8 to 16 tokens 161 and 134, 24 to 48 tokens 143 and 174, 32 to 64
+//   tokens 172 and 177; of 1,000: 40 to 80 tokens 94 and 90; 4 prompts of 1,500 tokens
+//   157 and 137, as the tiles of a long request begin at other pages each.
 bool takes_wide(const ferry_pages* p, const ferry_attend* a, const ferry_seen* seen) {
-  if (seen->tree_words) return true;
-  return seen->window && (int64_t)a->n_tokens * (a->q_heads / p->kv_heads) <= (int64_t)WRULE * a->n_req;
+  const int64_t rows = (int64_t)a->n_tokens * (a->q_heads / p->kv_heads), n = a->n_req;
+  if (seen->window) return rows > 112 * n && rows <= 256 * n;
+  return a->n_groups ? rows > 32 * n : n <= 4 || rows > 112 * n;
 }
 
 // Workgroups of a call, and its scratch at `base` (null: sizes only).

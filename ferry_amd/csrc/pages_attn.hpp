@@ -8,16 +8,25 @@
 // a group with the rows of all its members, or the remaining pages of one request
 // with its own rows.  A row's output joins its (at most two) segments.
 //
-// Schedule.  A segment's rows are cut into tiles (16, 32 or 128 rows), its pages into
+// Schedule.  A segment's rows are cut into tiles (16, 32, 128 or 256 rows), its pages into
 // steps of four; a unit of work is one step of one tile of one kv head.  All units
 // of the call, in the order (segment, kv head, tile, step), are cut into equal runs,
 // one per workgroup of a grid that fills the GPU once: ragged lengths balance, and
 // a long axis is split where there are few rows.  Every workgroup finds its run from
-// the lengths by itself (a prefix sum over the segments), so nothing is planned on
-// the host and a captured call follows the lengths of its replay.  A tile that one
+// the lengths by itself (a prefix sum over the segments; where rows see a part only and up
+// to 64 requests are in no group, every wavefront by itself, a request per lane), so nothing
+// is planned on the host and a captured call follows the lengths of its replay.  A tile that one
 // workgroup finishes alone, of a row with one segment, is written out; otherwise its
 // (max, sum, output) in fp32 go to scratch, and k_attend_join adds them up in order.
 // The result depends on the lengths and on the number of CUs, not on timing.
+//
+// What rows see.  Causal rows see the tokens up to their own place: p[0] .. p[lim).  With a
+// window of w tokens and s sinks a row sees [0, s) and [lim - w, lim); its tile reads the pages of
+// [0, s) and those from the first that its first row sees, and numbers them on without the
+// gap (Tile::page), so steps are full and what lies between is not read.  Rows of a tree of drafts
+// see what was there before the drafts, and of these their ancestors: a bit each.
+// Pages that all rows of a tile see whole take no masks; others take 64 bits per row and
+// step (seen_bits), so one form of the loops serves causal ends, windows, sinks and trees.
 //
 // Softmax.  One pass with a reference m and the sum of the weights 2^(score - m) of each
 // row, in base 2.  m is raised only when a score exceeds it by kMost, and then so that this
@@ -372,7 +381,9 @@ __device__ inline int tile_steps(const AttendArgs& a, const Seg& g, int j) {
 // Units of work: step_units() for a step, tile_units() for a tile's beginning and end.
 // Step i of a tile belongs to the workgroup whose run holds the first of its units.
 // A unit is a fifth of a microsecond of a workgroup, measured in batches of all forms
-// (samples of one prompt, agents in groups, prompts in chunks) on a full GPU.
+// (samples of one prompt, agents in groups, prompts in chunks) on a full GPU.  A workgroup
+// of eight wavefronts alone on its CU takes 2.2 us for a step of 256 rows, 1.4 us for one of
+// 128 and some 14 us for a tile: the same shares.
 template <int DT>
 __device__ constexpr int step_units(int tile) {
   constexpr bool F8 = Kv<DT>::F8;
@@ -755,8 +766,8 @@ struct Narrow {
         uint32_t bits = 15u;
         if (masked) {
           const int row = nt * 16 + (l & 15);
-          bits = row < tile.rows ? (uint32_t)(seen_bits(a, tile, token_of_row(a, tile.row0 + row), sh.lim[row], sh.lo[row], t0) >> 4 * grp)
-                                 : 0u;
+          const int tok = token_of_row(a, tile.row0 + row);
+          bits = row < tile.rows ? (uint32_t)(seen_bits(a, tile, tok, sh.lim[row], sh.lo[row], t0) >> 4 * grp) : 0u;
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -855,22 +866,22 @@ struct Narrow {
         }
         if (i < mine) use(i, 0);
       } else {
-      // pages that every row sees whole, two at a time, then the others (the last of an odd
-      // number of whole ones among them, which is never left out)
-      const int seen = t.lim_lo / kPageTokens - t.p0;  // such pages of all teams
-      const int mine = clampi(seen / kStep + (seen % kStep > wave ? 1 : 0), 0, count);
-      fetch(0, 0);
-      int i = 0;
-      for (; i + 1 < mine; i += 2) {
-        fetch(i + 1, 1);
-        consume<false>(r[0], l, 0, a, t, sh, false, scale);
-        fetch(i + 2, 0);
-        consume<false>(r[1], l, 0, a, t, sh, false, scale);
-      }
-      for (; page_no(i) < t.p1; ++i) {
-        if (!consume<true>(r[0], l, page_no(i) * kPageTokens, a, t, sh, true, scale)) sh.left_out = 1;
-        fetch(i + 1, 0);
-      }
+        // pages that every row sees whole, two at a time, then the others (the last of an odd
+        // number of whole ones among them, which is never left out)
+        const int seen = t.lim_lo / kPageTokens - t.p0;  // such pages of all teams
+        const int mine = clampi(seen / kStep + (seen % kStep > wave ? 1 : 0), 0, count);
+        fetch(0, 0);
+        int i = 0;
+        for (; i + 1 < mine; i += 2) {
+          fetch(i + 1, 1);
+          consume<false>(r[0], l, 0, a, t, sh, false, scale);
+          fetch(i + 2, 0);
+          consume<false>(r[1], l, 0, a, t, sh, false, scale);
+        }
+        for (; page_no(i) < t.p1; ++i) {
+          if (!consume<true>(r[0], l, page_no(i) * kPageTokens, a, t, sh, true, scale)) sh.left_out = 1;
+          fetch(i + 1, 0);
+        }
       }
     }
     // hand over: [wavefront][row][dim]
@@ -1440,7 +1451,7 @@ struct Wide {
 // codes in half of that, eight places each), so that up to 96 KiB are on their way while a
 // step is computed: that hides the memory's latency where pages are read by one tile only.
 // Two workgroups of 128 rows per CU have 64 KiB on their way, and read the pages of 256 rows
-// twice.  32 x 64 drafts over 1,000 to 8,000 tokens of 8 kv heads, bf16: @@ us, 242 us so.
+// twice.  32 x 64 drafts over 1,000 to 8,000 tokens of 8 kv heads, bf16: 175 us, 229 us so.
 // In step s the loads of V of step s + kSlots - 1 and of K of step s + kSlots begin, into the
 // places that step s - 1 has left.  A wavefront waits for its own oldest loads by their
 // count, then all meet.
@@ -1944,49 +1955,51 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
     before -= mine;
     if (wg == 0 && tid < a.n_req && misplaced(kept)) set_error(v.error, FERRY_ERANGE);
   } else {
-  if constexpr (SEEN) {
-    if (per_thread == 1) {
-      kept = segment<DT, MODE>(v, a, gs, gp, min(s0, nseg - 1));
-      if (s0 >= s1) kept.rows = kept.tiles = 0, kept.own = 0;
-      kept_work = seg_work_of_all<DT, MODE>(a, kept);
-    }
-  }
-  for (int s = s0; s < s1; ++s) {
-    if (!SEEN || per_thread > 1) {
-      kept = segment<DT, MODE>(v, a, gs, gp, s);
-      kept_work = seg_work<DT, MODE>(a, kept);
-    }
-    mine += kept_work * v.H;
-    if (kept.own && kept.group >= 0 && kept.rows > 0 && gs == sh.gs)
-      atomicMin(&sh.gl[kept.group], SEEN && a.seen.words ? max(0, kept.base - 1) / kPageTokens * kPageTokens : max(0, kept.base));
-    if (wg == 0) {  // what is out of range, once
-      bool bad = false;
-      if (kept.own) {
-        bad = misplaced(kept);
-      } else {
-        bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
+    if constexpr (SEEN) {
+      if (per_thread == 1) {
+        kept = segment<DT, MODE>(v, a, gs, gp, min(s0, nseg - 1));
+        if (s0 >= s1) kept.rows = kept.tiles = 0, kept.own = 0;
+        kept_work = seg_work_of_all<DT, MODE>(a, kept);
       }
-      if (bad) set_error(v.error, FERRY_ERANGE);
     }
-  }
-  before = mine;
+    for (int s = s0; s < s1; ++s) {
+      if (!SEEN || per_thread > 1) {
+        kept = segment<DT, MODE>(v, a, gs, gp, s);
+        kept_work = seg_work<DT, MODE>(a, kept);
+      }
+      mine += kept_work * v.H;
+      if (kept.own && kept.group >= 0 && kept.rows > 0 && gs == sh.gs)
+        atomicMin(&sh.gl[kept.group],
+                  SEEN && a.seen.words ? max(0, kept.base - 1) / kPageTokens * kPageTokens : max(0, kept.base));
+      if (wg == 0) {  // what is out of range, once
+        bool bad = false;
+        if (kept.own) {
+          bad = misplaced(kept);
+        } else {
+          bad = gs[s] < 0 || gs[s] > gs[s + 1] || gs[s + 1] > a.n_req || gp[s] < 0 || gp[s] > v.max_pages;
+        }
+        if (bad) set_error(v.error, FERRY_ERANGE);
+      }
+    }
+    before = mine;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t y = __shfl_up(before, d);
-    if ((tid & 63) >= d) before += y;
-  }
-  if ((tid & 63) == 63) sh.sums[tid >> 6] = before;
-  __syncthreads();
-  for (int i = 0; i < kThreads / 64; ++i) {
-    if (i < tid >> 6) before += sh.sums[i];
-    total += sh.sums[i];
-  }
-  before -= mine;
-  total = first_lane_u64(total);
+    for (int d = 1; d < 64; d *= 2) {
+      const uint64_t y = __shfl_up(before, d);
+      if ((tid & 63) >= d) before += y;
+    }
+    if ((tid & 63) == 63) sh.sums[tid >> 6] = before;
+    __syncthreads();
+    for (int i = 0; i < kThreads / 64; ++i) {
+      if (i < tid >> 6) before += sh.sums[i];
+      total += sh.sums[i];
+    }
+    before -= mine;
+    total = first_lane_u64(total);
   }
   // no run is shorter than a step, so that each one within a tile begins one
   constexpr int kMost = FORMS == 1 ? step_units<DT>(16) : 11;
-  static_assert(FORMS == 1 || (step_units<DT>(16) <= kMost && step_units<DT>(32) <= kMost && step_units<DT>(kWide) <= kMost));
+  static_assert(FORMS == 1 ||
+                (step_units<DT>(16) <= kMost && step_units<DT>(32) <= kMost && step_units<DT>(kWide) <= kMost));
   uint64_t each = total + grid - 1;
   if (SEEN && each < 1ull << 52) each = quotient(each, grid);
   else each /= grid;
@@ -2019,11 +2032,12 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
     if (has_first) {
       uint64_t at = before;
       int s = s0;
-      if (per_thread > 1)
+      if (per_thread > 1) {
         for (;; ++s) {
           at += seg_work<DT, MODE>(a, segment<DT, MODE>(v, a, gs, gp, s)) * v.H;
           if (u0 < at) break;
         }
+      }
       sh.seg = s;
     }
     __syncthreads();
@@ -2097,7 +2111,9 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
     const int per_step = step_units<DT>(g.tile), len = first_lane_i(tile_steps<MODE>(a, g, j));
     auto steps_in = [&](int units) {  // begun within so many units
       const int n = units + per_step - 1;
-      return first_lane_i(g.tile == 16 ? n / step_units<DT>(16) : g.tile == 32 ? n / step_units<DT>(32) : n / step_units<DT>(kWide));
+      return first_lane_i(g.tile == 16   ? n / step_units<DT>(16)
+                          : g.tile == 32 ? n / step_units<DT>(32)
+                                         : n / step_units<DT>(kWide));
     };
     const int k0 = steps_in((int)(u - tile_at)), k1 = min(len, steps_in((int)min((uint64_t)work, u1 - tile_at)));
     u = tile_at + work;

@@ -717,8 +717,9 @@ int ferry_pages_tree(const ferry_pages* pages, const ferry_tree* args, void* str
  *   next [n_req]     out: chosen[] of the last; -1 of an empty request
  * fp8: a code that moves to a page of another scale is rounded to that scale's codes
  * (saturating); with the same scale it is copied.  Lane -1 is an empty request, also
- * one without tokens: it keeps none and changes nothing, but its path is -1.  A call of the kind of those that manage pages: it is made whole
- * or not at all (path, kept and next included), a lane that is out of range or named
+ * one without tokens: it keeps none and changes nothing, but its path is -1.  A call of
+ * the kind of those that manage pages: it is made whole or not at all (path, kept and
+ * next included), a lane that is out of range or named
  * twice, offsets that do not ascend and more new tokens than the lane holds are
  * FERRY_EINVAL; n_req is at most n_lanes, and the results overlap neither each
  * other nor anything that is read.  A move whose page the lane does not have, or

@@ -234,6 +234,18 @@ def test_many_requests(dt):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+@pytest.mark.parametrize("n", [90, 600])
+def test_many_requests_of_wide_tiles(dt, n):
+    rng = np.random.default_rng(n)
+    new = rng.integers(20, 50, n).tolist()
+    lens = [int(x + rng.integers(0, 150)) for x in new]
+    c = Seen(dt, 4, 1, lens, new, masks=[tree_of(rng, x)[1] for x in new], seed=3)
+    c.check(*c.run())
+    c = Seen(dt, 4, 1, lens, new, window=40, sinks=3, seed=4)
+    c.check(*c.run())
+
+
 def spoil(c, dt, value, rows):
     """Put `value` into K and V of tokens: rows of (request, token)."""
     raw = c.p.pool.view(torch.uint8) if dt == F.FP8 else c.p.pool
