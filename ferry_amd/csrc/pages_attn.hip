@@ -123,6 +123,7 @@ int ferry_pages_attend_seen(const ferry_pages* p, int32_t layer, const ferry_att
   return entry([&]() -> int {
     PageView v;
     if (int rc = check_attend(p, a, seen, &v)) return rc;
+    if (seen && !seen->window && !seen->tree_words) seen = nullptr;  // the causal call, its grid and scratch too
     if (layer < 0 || layer >= p->n_layers) return report(FERRY_EINVAL, "layer out of range");
     if (a->n_req == 0 || a->n_tokens == 0) return FERRY_OK;
     if (int rc = page_buffers(p, false)) return rc;

@@ -656,8 +656,8 @@ int ferry_pages_attend_work_bytes(const ferry_pages* pages, const ferry_attend* 
 int ferry_pages_attend(const ferry_pages* pages, int32_t layer, const ferry_attend* args,
                        void* stream);
 
-/* The same where a row sees only a part of what is before it; seen NULL is
- * ferry_pages_attend.  The scratch is that of ferry_pages_attend_work_bytes.
+/* The same where a row sees only a part of what is before it; seen NULL, or without
+ * a window and a tree, is ferry_pages_attend.  The scratch is that of ferry_pages_attend_work_bytes.
  * window > 0: a sliding window with sinks.  The row at place i of its lane (len -
  *   n + j for row j of n) sees the tokens t <= i with t > i - window or t < sinks.
  *   Pages between the sinks and the window are not read.  No groups go with it.

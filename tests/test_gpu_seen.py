@@ -4,6 +4,8 @@ float64 over the tokens that it sees.
 
 Tolerance: that of attention over all of a lane (test_gpu_attend), with the number
 of tokens that the row sees."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -326,6 +328,32 @@ def test_pages_before_the_window_need_not_be_there():
         c.p.table[int(c.lanes[r]), 1:(n - 128) // T] = -1
     got = c.run()  # checks that nothing was found
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dt", [F.BF16, F.FP8])
+@pytest.mark.parametrize("new", [[40, 33], [60] * 6])
+def test_a_seen_without_a_window_or_a_tree_is_the_causal_call(dt, new):
+    """Structures of zeros: the same kernels, grid and order of sums."""
+    c = Seen(dt, 32, 8, [3000 + 7 * i for i in range(len(new))], new, seed=3)
+    want = c.run()
+    n, need = len(new), C.c_uint64()
+    a = c.args()
+    d = F.AttendArgs(n_req=n, n_tokens=c.rows, q_heads=32, lanes=a["lanes"].data_ptr(), q_start=a["q_start"].data_ptr(),
+                     q=c.q.data_ptr())
+    d.q_stride[0] = d.out_stride[0] = 32 * D
+    d.q_stride[1] = d.out_stride[1] = D
+    assert F.lib.ferry_pages_attend_work_bytes(c.p._r, C.byref(d), C.byref(need)) == 0
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    d.work, d.work_bytes = work.data_ptr(), need.value
+    for seen in (None, F.SeenArgs()):
+        out, lse = torch.full_like(c.q, 9.0), torch.full((c.rows, 32), 9.0, device="cuda")
+        d.out, d.lse = out.data_ptr(), lse.data_ptr()
+        rc = F.lib.ferry_pages_attend_seen(c.p._r, 0, C.byref(d), seen and C.byref(seen),
+                                           torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        c.p.check()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 
 
 def test_requests_without_a_lane_and_rows_behind_the_last():
