@@ -340,7 +340,8 @@ struct Range {
   int lim_lo, lim_hi;  // tokens that its least and its most seeing row see, but for ...
   int lo_lo, lo_hi;    // ... those behind the sinks and before these (least, most)
 };
-// Wide tiles read whole steps, so there the pages before the gap are, too.
+// Wide tiles take whole steps, so there the gap begins at one; the pages before it that no row
+// sees (unseen) are in the steps, but are not looked up.
 __device__ inline Range tile_range(const AttendArgs& a, const Seg& g, int j) {
   Range r;
   const int first = g.base + token_of_row(a, j * g.tile),
@@ -501,6 +502,8 @@ struct CausalTile {
   __device__ __forceinline__ bool whole(int t0, int n) const { return t0 + n <= lim_lo; }
   __device__ __forceinline__ bool some(int tok) const { return tok < lim_hi; }
   __device__ __forceinline__ bool some(int t0, int) const { return t0 < lim_hi; }
+  // Whether page p of the lane's table is between the sinks and the window of every row.
+  __device__ __forceinline__ bool unseen(int) const { return false; }
 };
 struct SeenTile : CausalTile {
   int ahead, skip, lo_lo, lo_hi;  // of its Range
@@ -513,6 +516,9 @@ struct SeenTile : CausalTile {
   }
   __device__ __forceinline__ bool some(int tok) const { return tok < lim_hi && (tok >= lo_lo || tok < sinks); }
   __device__ __forceinline__ bool some(int t0, int n) const { return t0 < lim_hi && (t0 + n > lo_lo || t0 < sinks); }
+  __device__ __forceinline__ bool unseen(int p) const {
+    return (p + 1) * kPageTokens <= lo_lo && p * kPageTokens >= sinks;
+  }
 };
 template <int MODE>
 using Tile = std::conditional_t<MODE != kCausal, SeenTile, CausalTile>;
@@ -1154,7 +1160,7 @@ struct Wide {
     // Page ids: lane j holds page 64 w + j of window w; the next window is read ahead.
     auto read_ids = [&](int w) __attribute__((always_inline)) {
       const int p = t.p0 + 64 * w + l;
-      return p < t.p1 ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
+      return p < t.p1 && !t.unseen(t.page(p)) ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
     };
     uint32_t ids = checked_page(v, read_ids(0)), ids_next = 0;
     uint32_t pages[kStep];  // of the step whose K was loaded last
@@ -1175,8 +1181,8 @@ struct Wide {
         if (p >= t.p1 || !t.some(t.page(p) * kPageTokens, kPageTokens)) scales[1] = 0.0f;
       }
     };
-    // Page i of the step whose K or V is loaded next.  Pages from p1 on are page 0: they
-    // are loaded for nothing.
+    // Page i of the step whose K or V is loaded next.  Pages from p1 on, and those between the
+    // sinks and the window, are page 0: they are loaded for nothing.
     auto window = [&](int s) __attribute__((always_inline)) {  // before K of step s > 1
       if ((s - 1 & 15) == 0) k_scales = scales[0];
       if ((s - 2 & 15) == 0) v_scales = scales[1];
@@ -1530,7 +1536,7 @@ struct Wide8 {
     // of the one behind the ids' second.
     auto read_ids = [&](int w) __attribute__((always_inline)) {
       const int p = t.p0 + 64 * w + l;
-      return p < t.p1 ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
+      return p < t.p1 && !t.unseen(t.page(p)) ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
     };
     auto read_scales = [&](uint32_t ids, int w) __attribute__((always_inline)) {
       f32x2 s = {};
@@ -1869,6 +1875,7 @@ __device__ __forceinline__ void add_left_out(const PageView& v, const AttendArgs
     if (SEEN && t.whole(t0, unit * kPageTokens)) continue;
     bool odd = false;
     for (int i = 0; i < unit && p + i < t.p1; ++i) {
+      if (t.unseen(t0 / kPageTokens + i)) continue;
       const uint64_t page = checked_page(v, t.table[t0 / kPageTokens + i]);
       const uint8_t* rec = t.base + page * t.page_bytes;
       for (int e = l; e < kPageTokens * kPageDim; e += 64)

@@ -330,6 +330,42 @@ def test_pages_before_the_window_need_not_be_there():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("dt", [F.BF16, F.F16, F.FP8])
+@pytest.mark.parametrize("Hq,H", [(8, 2), (80, 2)])
+@pytest.mark.parametrize("new", [1, 9, 40])
+@pytest.mark.parametrize("sinks", [4, 20, 100])
+@pytest.mark.parametrize("gap", [1, 2, 3, 30])
+def test_pages_between_the_sinks_and_the_window_need_not_be_there(dt, Hq, H, new, sinks, gap):
+    """`gap` pages that no row sees, in tiles of all forms: their entries are not looked at."""
+    window, first = 128, (-(-sinks // T) + gap) * T  # the first row's window starts in the page behind them
+    base = first + window + 3
+    c = Seen(dt, Hq, H, [base + new, base + new + 5], [new, new], window=window, sinks=sinks, seed=gap)
+    assert not any(c.visible(r)[:, -(-sinks // T) * T:first].any() for r in range(2))
+    want = [x.clone() for x in c.run()]
+    c.check(*want)
+    hidden = [(r, t) for r in range(2) for t in range(T * -(-sinks // T), first)]
+    spoil(c, dt, float("nan"), hidden)
+    table = c.p.table.clone()
+    for lane in c.lanes:
+        c.p.table[int(lane), -(-sinks // T):first // T] = -1
+    got = c.run()  # checks that nothing was found
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if dt != F.FP8:
+        return
+    # nor where rows are done one by one, as a scale of the first page behind is not finite
+    scale = c.p.scales[c.layer, int(c.p.table[int(c.lanes[0]), first // T]), :, 1]
+    finite = scale.clone()
+    scale.fill_(float("nan"))
+    out, lse = c.run()
+    scale.copy_(finite)
+    clean = torch.ones((c.rows, 1), dtype=torch.bool, device="cuda")
+    clean[:new, 0] = torch.from_numpy(~c.visible(0)[:, first:first + T].any(1)).cuda()
+    assert torch.all(torch.isnan(out[~clean[:, 0]].float()))
+    c.p.table.copy_(table)
+    spoil(c, dt, 0.0, hidden)
+    c.check(torch.where(clean.unsqueeze(2), out, want[0]), torch.where(clean, lse, want[1]))
+
+
 @pytest.mark.parametrize("dt", [F.BF16, F.FP8])
 @pytest.mark.parametrize("new", [[40, 33], [60] * 6])
 def test_a_seen_without_a_window_or_a_tree_is_the_causal_call(dt, new):
