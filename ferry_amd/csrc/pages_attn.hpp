@@ -341,7 +341,9 @@ struct Range {
   int lo_lo, lo_hi;    // ... those behind the sinks and before these (least, most)
 };
 // Wide tiles take whole steps, so there the gap begins at one; the pages before it that no row
-// sees (unseen) are in the steps, but are not looked up.
+// sees (unseen) are in the steps, but are not looked up.  The windows of a tree's tile are
+// taken to begin where that of a row without drafts would, as the work is planned without
+// the bits; its pages before the first window of its rows are not looked up either.
 __device__ inline Range tile_range(const AttendArgs& a, const Seg& g, int j) {
   Range r;
   const int first = g.base + token_of_row(a, j * g.tile),
@@ -846,7 +848,11 @@ struct Narrow {
     uint32_t ids = 0;  // lane j: the table's entry for page 64 k + j
     auto fill_ids = [&](int i0) {
       const int p = page_no(i0 + l);
-      ids = p < t.p1 && i0 + l < count ? checked_page(v, global_at<uint32_t>(t.table, 4 * t.page(p))) : 0u;
+      ids = p < t.p1 && i0 + l < count ? global_at<uint32_t>(t.table, 4 * t.page(p)) : 0u;
+      if (ids >= (uint32_t)v.n_pages) {  // here, as it costs time before the entry is used (0.2 us of 14)
+        if (!t.unseen(t.page(p))) set_error(v.error, FERRY_ERANGE);
+        ids = 0;
+      }
     };
     auto id_of = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)ids, i & 63); };
     if (t.p0 < t.p1) {
@@ -2166,6 +2172,11 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
         __syncthreads();
       }
     }
+    const bool by_depth = SEEN && g.own && a.seen.words && a.seen.window;
+    if (by_depth) {
+      if (tid == 0) sh.lim_lo = 0x7FFFFFFF;
+      __syncthreads();
+    }
     if (tid < (int)(sizeof(sh.odd) / sizeof(int))) sh.odd[tid] = 0;
     if (tid == 0) sh.left_out = 0;
     if (tid < t.rows) {
@@ -2186,6 +2197,7 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
             end = t.before + deep;
           }
           if (a.seen.window) sh.lo[tid] = clampi(end - a.seen.window, 0, g.len);
+          if (by_depth) atomicMin(&sh.lim_lo, sh.lo[tid]);
         }
       } else if (!all_seen) {
         int lo = tok;
@@ -2211,6 +2223,10 @@ __global__ __launch_bounds__(threads_of(MODE), 2) void k_attend(PageView v, int 
     }
     __syncthreads();
     if (!g.own && !all_seen) t.lim_lo = first_lane_i(sh.lim_lo), t.lim_hi = first_lane_i(sh.lim_hi);
+    if constexpr (SEEN) {
+      // drafts are seen by their bits whatever the window is
+      if (by_depth) t.lo_lo = min(first_lane_i(sh.lim_lo), max(0, t.before));
+    }
     t = uniform(t);
     float *to_ml = nullptr, *to_o = nullptr;
     if (count > 1) {

@@ -366,6 +366,32 @@ def test_pages_between_the_sinks_and_the_window_need_not_be_there(dt, Hq, H, new
     c.check(torch.where(clean.unsqueeze(2), out, want[0]), torch.where(clean, lse, want[1]))
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("new", [1, 7, 40, 70])
+@pytest.mark.parametrize("window,sinks", [(64, 0), (64, 4), (37, 20)])
+@pytest.mark.parametrize("base", [319, 320, 326])
+def test_pages_before_the_window_of_all_drafts_need_not_be_there(dt, new, window, sinks, base):
+    """The window counts by depth: where every row has a bit, and more so where they
+    have many, tokens that a row of none would see are before all windows."""
+    rng = np.random.default_rng(base)
+    for deep in (0, 30):
+        if deep >= new:
+            continue
+        masks = [tree_of(rng, new, back=2)[1] for _ in range(2)]
+        for m in masks:
+            m[:, :deep] = True
+        c = Seen(dt, 8, 2, [base + new, base + new + 9], [new, new], window=window, sinks=sinks, masks=masks, seed=new)
+        want = [x.clone() for x in c.run()]
+        c.check(*want)
+        for r, lane in enumerate(c.lanes):
+            see = c.visible(r).any(0)
+            for page in range(-(-sinks // T), base // T):
+                if not see[page * T:(page + 1) * T].any():
+                    c.p.table[int(lane), page] = -1
+        got = c.run()  # checks that nothing was found
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("dt", [F.BF16, F.FP8])
 @pytest.mark.parametrize("new", [[40, 33], [60] * 6])
 def test_a_seen_without_a_window_or_a_tree_is_the_causal_call(dt, new):
