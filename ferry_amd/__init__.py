@@ -916,8 +916,9 @@ class Pages:
         """Of each request's new tokens the first stays, then the first child whose
         draft is what the model chose after its parent, and so on: their keys and values
         move up behind the context, the lane ends behind them.  path [rows] gets the rows
-        that stay, kept [requests] their number, next [requests] the choice after the last.
-        parent None: each token's parent is the one before it."""
+        that stay, then -1 (rows of no request are left as they are), kept [requests] their
+        number, next [requests] the choice after the last.  parent None: each token's parent
+        is the one before it."""
         n, rows = lanes.numel(), draft.numel()
         a = _ACCEPT.pack(n, rows, self._list(lanes, "lanes", n), self._list(q_start, "q_start", n + 1) or 0,
                          self._list(parent, "parent", rows) or 0, self._list(draft, "draft", rows),

@@ -660,7 +660,9 @@ int ferry_pages_attend(const ferry_pages* pages, int32_t layer, const ferry_atte
  * a window and a tree, is ferry_pages_attend.  The scratch is that of ferry_pages_attend_work_bytes.
  * window > 0: a sliding window with sinks.  The row at place i of its lane (len -
  *   n + j for row j of n) sees the tokens t <= i with t > i - window or t < sinks.
- *   Pages between the sinks and the window are not read.  No groups go with it.
+ *   Pages between the sinks and the window need not be there: their table entries may
+ *   hold anything.  No groups go with it (call without them: shared pages are then read
+ *   once per request).
  * tree: a tree of drafted tokens.  With base = len - n, the row sees the tokens
  *   before base, and of its request's n new tokens those whose bits are set in its
  *   row of `tree` [n_tokens][tree_words] (bit c % 64 of word c / 64 is new token c,
@@ -712,7 +714,8 @@ int ferry_pages_tree(const ferry_pages* pages, const ferry_tree* args, void* str
  * the keys and values of the i-th of them, in all layers, move to place base + i,
  * len becomes base + kept, and the pages behind are given back.
  *   draft, chosen [n_tokens]: a token, and the model's choice after it
- *   path [n_tokens]  out: a request's rows that stay, in their order, then -1
+ *   path [n_tokens]  out: a request's rows that stay, in their order, then -1; rows of
+ *                    no request are left as they are
  *   kept [n_req]     out: their number
  *   next [n_req]     out: chosen[] of the last; -1 of an empty request
  * fp8: a code that moves to a page of another scale is rounded to that scale's codes
