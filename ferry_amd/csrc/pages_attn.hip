@@ -42,17 +42,25 @@ int attend_forms(const ferry_pages* p, const ferry_attend* a) {
 // rows, one per CU, rather than to those of four with 128, two per CU: where most tiles
 // would read their pages for a second tile of the same request.  The rule is on the rows
 // that a request has on average, as only the device knows each one's.  In us, wide and
-// not, of 8 kv heads, 32 requests over 1,000 to 8,000 tokens unless stated, bf16 (fp8):
-//   drafts, 4 heads a kv head: 12 to 24 tokens 140 and 136 (125 and 114), 16 to 32 tokens
-//   145 and 141 (136 and 119), 24 to 48 tokens 165 and 199 (176 and 182), 32 to 64 tokens
-//   175 and 229 (179 and 203); 128 requests of 12 to 24 tokens over 2,000: 189 and 166.
-//   In groups, whose shared pages meet the rows of all members: 12 to 24 tokens of 32
-//   requests over 8,000 shared tokens 1,189 and 1,471 (1,259 and 1,423), 4 to 8 tokens 544
-//   and 527.  Up to four requests have fewer parts to join: 4 x 8 tokens over 700 18.1 and
-//   19.1, 2 x 32 tokens over 131,000 175 and 178.
-//   windows of 4,096: 8 to 16 tokens 161 and 134, 24 to 48 tokens 143 and 174, 32 to 64
-//   tokens 172 and 177; of 1,000: 40 to 80 tokens 94 and 90; 4 prompts of 1,500 tokens
-//   157 and 137, as the tiles of a long request begin at other pages each.
+// not, of 8 kv heads, 4 heads a kv head, 32 requests unless stated, bf16 (fp8):
+//   drafts over 1,000 to 8,000 tokens: 12 to 24 of them 140 and 136 (125 and 114), 16 to 32
+//   145 and 141 (136 and 119), 20 to 40 161 and 170 (173 and 160), 24 to 48 165 and 199
+//   (176 and 182), 32 to 64 175 and 229 (179 and 203); 16 and 128 requests of 12 to 24 over
+//   2,000: 47 and 42, 189 and 166 (46 and 42, 194 and 148).  In groups, whose shared pages
+//   meet the rows of all members, over 8,000 shared tokens: 4 to 8 544 and 527 (542 and 540),
+//   12 to 24 1,189 and 1,471 (1,259 and 1,423); over 1,000: 8 to 16 152 and 145 (163 and 160);
+//   four groups over 4,000: 8 to 16 557 and 663 (561 and 623).  Up to four requests have fewer
+//   parts to join: 4 x 8 over 700 18.1 and 19.1, 2 x 32 over 131,000 175 and 178.
+//   windows of 4,096: 8 to 16 tokens 161 and 134 (140 and 105), 12 to 24 117 and 133 (105 and
+//   111), 16 to 32 120 and 137 (107 and 119), 24 to 48 143 and 174 (157 and 180), 32 to 64 172
+//   and 177 (179 and 192); of 1,024: 12 to 24 50 and 54 (49 and 54); of 1,000: 40 to 80 94 and
+//   90 (107 and 101); 64 requests of 12 to 24 through 512 68 and 51, 8 of them through 4,096 53
+//   and 48; 4 prompts of 1,500 157 and 137, as the tiles of a long request begin at other
+//   pages each.
+// So the rule is not the better side everywhere: it refuses windows of 12 to 32 tokens a request,
+// where wide tiles take 5 to 14 % less if there is just one of them for each CU (32 requests
+// of 8 heads) and more if not, and takes drafts of 20 to 40 in fp8 and windows of 40 to 80,
+// at 5 to 8 % more.  It does not weigh the tiles against the CUs.
 bool takes_wide(const ferry_pages* p, const ferry_attend* a, const ferry_seen* seen) {
   const int64_t rows = (int64_t)a->n_tokens * (a->q_heads / p->kv_heads), n = a->n_req;
   if (seen->window) return rows > 112 * n && rows <= 256 * n;

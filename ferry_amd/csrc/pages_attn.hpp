@@ -385,8 +385,11 @@ __device__ inline int tile_steps(const AttendArgs& a, const Seg& g, int j) {
 // Step i of a tile belongs to the workgroup whose run holds the first of its units.
 // A unit is a fifth of a microsecond of a workgroup, measured in batches of all forms
 // (samples of one prompt, agents in groups, prompts in chunks) on a full GPU.  A workgroup
-// of eight wavefronts alone on its CU takes 2.2 us for a step of 256 rows, 1.4 us for one of
-// 128 and some 14 us for a tile: the same shares.
+// of eight wavefronts alone on its CU takes 2.2 us (11 units) for a step of 256 rows, 1.4 us
+// (7) for one of up to 128 and some 14 us for a tile, but has the units of the others, for its
+// steps of eight pages in tiles of few rows, too: where requests of unlike width meet, its
+// runs are less even (32 requests of 8 to 16 tokens through a window of 4,096, of tiles of 32 and
+// of 64 rows, 161 us; of 12 to 24, all of the wide form, 117).
 template <int DT>
 __device__ constexpr int step_units(int tile) {
   constexpr bool F8 = Kv<DT>::F8;
